@@ -447,6 +447,49 @@ int mi355_sage_sdpa_bwd_f32_grads(
  * to_bf16 != 0: src F32, dst bf16, else the other way; bases 16-byte aligned. */
 int mi355_sage_cast(int count, const void* const* src, void* const* dst, const int64_t* n, int to_bf16, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Norm and rotation of queries and keys as an operator of its own, with its gradient.  (The reference calls rms_norm,
+ * serenitymojo/ops/norm.mojo:81-114, and rope_interleaved / rope_halfsplit, ops/rope.mojo:104-165, one after the other and
+ * stores the result of each as bf16; here everything is fp32 between the rows read and the rows written.)
+ *
+ * Element types of the calls below. */
+#define MI355_SAGE_BF16 0
+#define MI355_SAGE_FP16 1
+#define MI355_SAGE_F32  2
+
+/* For every token and head:  y = x g / sqrt(mean_d x^2 + eps),  then channels [0, rot) of y are rotated by the token's angles,
+ * pairs (2i, 2i+1) or, with halfsplit, (i, i + rot/2): (a, b) -> (a cos - b sin, b cos + a sin).  Channels from rot on pass.
+ * Q [B,Hq,S,D] and K [B,Hk,S,D] through four element strides each (D stride 1, rows 16-byte aligned, so that slices of a joint
+ * projection are taken as they are), of one type: bf16, fp16 or F32; so are Q_out and K_out, which may be Q and K themselves
+ * (same base and strides), or rows of a cache; otherwise nothing written may overlap what is read.  D: a multiple of 16 up to 256.
+ * rot: a multiple of 16 up to D, 0 = no rotation (no tables needed).  Gains [D] and tables [table_rows, rot/2] (element stride
+ * table_stride between rows) of any of the three types, 16-byte aligned.  The row of the tables is positions[b*pos_stride + s]
+ * (pos_bytes 4 or 8: int32 or int64), or s without positions; where a position lies outside [0, table_rows) the token's
+ * rotated channels come out as NaN.  One launch; no workspace. */
+int mi355_sage_qk_norm_rope(
+    const void* Q, const void* K, void* Q_out, void* K_out,
+    int B, int S, int Hq, int Hk, int D, int type,
+    const int64_t* q_strides, const int64_t* k_strides, const int64_t* qo_strides, const int64_t* ko_strides,
+    int64_t q_offset_elems, int64_t k_offset_elems, int64_t qo_offset_elems, int64_t ko_offset_elems,
+    const void* q_gain, const void* k_gain, int gain_type, float eps,
+    const void* rope_cos, const void* rope_sin, int table_type, int rot, int64_t table_rows, int64_t table_stride, int halfsplit,
+    const void* positions, int64_t pos_stride, int pos_bytes, void* stream);
+
+/* Its gradient: dQ_out, dK_out (upstream), Q, K (as the forward read them) -> dQ, dK of the same type, which may be dQ_out and
+ * dK_out themselves, and d_q_gain, d_k_gain, F32 [D].  The same bits on every call (no atomics).  Workspace as in
+ * mi355_sage_sdpa_bwd_bf16. */
+size_t mi355_sage_qk_norm_rope_bwd_workspace_bytes(int B, int S, int Hq, int Hk, int D);
+int mi355_sage_qk_norm_rope_bwd(
+    const void* dQ_out, const void* dK_out, const void* Q, const void* K, void* dQ, void* dK, void* d_q_gain, void* d_k_gain,
+    int B, int S, int Hq, int Hk, int D, int type,
+    const int64_t* dqo_strides, const int64_t* dko_strides, const int64_t* q_strides, const int64_t* k_strides,
+    const int64_t* dq_strides, const int64_t* dk_strides,
+    int64_t dqo_offset_elems, int64_t dko_offset_elems, int64_t q_offset_elems, int64_t k_offset_elems,
+    int64_t dq_offset_elems, int64_t dk_offset_elems,
+    const void* q_gain, const void* k_gain, int gain_type, float eps,
+    const void* rope_cos, const void* rope_sin, int table_type, int rot, int64_t table_rows, int64_t table_stride, int halfsplit,
+    const void* positions, int64_t pos_stride, int pos_bytes, void* stream, void* workspace, size_t workspace_bytes);
+
 /* Library identification: "mi355_sage <version> gfx950". */
 const char* mi355_sage_version(void);
 

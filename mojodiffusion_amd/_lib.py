@@ -73,6 +73,11 @@ SIGNATURES = {
                               + [_vp, _vp, ctypes.c_float, _vp, _vp, _int] + [_vp] * 10 + [ctypes.c_size_t, _int, _vp]),
     "mi355_sage_quant_once_helps": (_int, [_int]),
     "mi355_sage_quant_once_takes": (_int, [_int] * 10),
+    "mi355_sage_qk_norm_rope": (_int, [_vp] * 4 + [_int] * 6 + [_i64p] * 4 + [_i64] * 4 + [_vp, _vp, _int, ctypes.c_float]
+                                + [_vp, _vp, _int, _int, _i64, _i64, _int] + [_vp, _i64, _int, _vp]),
+    "mi355_sage_qk_norm_rope_bwd_workspace_bytes": (ctypes.c_size_t, [_int] * 5),
+    "mi355_sage_qk_norm_rope_bwd": (_int, [_vp] * 8 + [_int] * 6 + [_i64p] * 6 + [_i64] * 6 + [_vp, _vp, _int, ctypes.c_float]
+                                    + [_vp, _vp, _int, _int, _i64, _i64, _int] + [_vp, _i64, _int, _vp, _vp, ctypes.c_size_t]),
     "mi355_sage_version": (ctypes.c_char_p, []),
 }
 
@@ -82,6 +87,7 @@ ROPE_INTERLEAVED = 0
 ROPE_HALFSPLIT = 1
 ROPE_TABLES_BF16 = 2
 NORM_FULL_ROW = 4
+BF16, FP16, F32 = 0, 1, 2
 
 # entry points the native host path calls, in the order of its Api struct (csrc/sage_torch.cpp)
 _HOST_ENTRIES = ("workspace_bytes", "bwd_workspace_bytes", "sdpa_bf16", "sdpa_bf16_train_fwd", "sdpa_bf16_keymask", "sdpa_bf16_mask_any",

@@ -3,6 +3,7 @@
 #include "../../include/mi355_sage.h"
 #include "../../include/mi355_sage_test.h"
 #include "sage_internal.h"
+#include "sage_window.h"
 
 #include <atomic>
 #include <chrono>
@@ -163,6 +164,16 @@ int internal_workspace(std::vector<StreamWs>& registry, size_t need, hipStream_t
         }
     }
     *out = w->p;
+    return 0;
+}
+
+// The workspace a call works in: the caller's, if it is large and aligned enough, else the library's.
+int call_workspace(const char* name, size_t need, hipStream_t stream, void** workspace, size_t bytes) {
+    if (*workspace == nullptr) return internal_workspace(g_ws, need, stream, workspace);
+    if (bytes < need || (reinterpret_cast<uintptr_t>(*workspace) & (kAlign - 1))) {
+        SAGE_LOG("%s: a workspace of %zu bytes at a 256-byte boundary needed, %zu given", name, need, bytes);
+        return MI355_SAGE_EWORKSPACE;
+    }
     return 0;
 }
 
@@ -1121,5 +1132,103 @@ int mi355_sage_sdpa_bwd_f32_grads(const void* Q, const void* K, const void* V, c
 }
 #undef SAGE_BWD_PARAMS
 #undef SAGE_BWD_ARGS
+
+
+// ---- norm and rotation of queries and keys -------------------------------------------------------
+// What both directions check and fill in.  `views`: per side input, output and (backward) upstream gradient.
+struct NormRopeView { const char* name; const void* p; const int64_t* s; int64_t off; };
+static int norm_rope_args(const NormRopeView (&q)[3], const NormRopeView (&k)[3], int views, int B, int S, int Hq, int Hk, int D, int type,
+                          const void* q_gain, const void* k_gain, int gain_type, float eps, const void* rope_cos, const void* rope_sin,
+                          int table_type, int rot, int64_t table_rows, int64_t table_stride, int halfsplit, const void* positions,
+                          int64_t pos_stride, int pos_bytes, NormRopeArgs* out) {
+    for (int i = 0; i < views; i++)
+        if (!q[i].p || !k[i].p || !q[i].s || !k[i].s) return MI355_SAGE_EINVAL;
+    if (!q_gain || !k_gain || B <= 0 || S <= 0 || Hq <= 0 || Hk <= 0 || D <= 0 || rot < 0 || rot > D || !(eps >= 0.0f)) return MI355_SAGE_EINVAL;
+    if (type < 0 || type > 2 || gain_type < 0 || gain_type > 2 || table_type < 0 || table_type > 2) return MI355_SAGE_EINVAL;
+    if (rot > 0 && (!rope_cos || !rope_sin || table_rows <= 0)) return MI355_SAGE_EINVAL;
+    if (rot > 0 && positions == nullptr && table_rows < S) { SAGE_LOG("norm_rope: %lld table rows for %d tokens", (long long)table_rows, S); return MI355_SAGE_EINVAL; }
+    if (positions != nullptr && pos_bytes != 4 && pos_bytes != 8) return MI355_SAGE_EINVAL;
+    if (D % 16 || D > 256 || rot % 16) { SAGE_LOG("norm_rope: head dim %d, %d rotated (multiples of 16 up to 256)", D, rot); return MI355_SAGE_EUNSUPPORTED; }
+    if ((int64_t)B * S > (1 << 30) / ((int64_t)Hq + Hk)) { SAGE_LOG("norm_rope: more than 2^30 rows"); return MI355_SAGE_EUNSUPPORTED; }
+    const int esz = type == MI355_SAGE_F32 ? 4 : 2, align = 16 / esz;
+    for (const NormRopeView* side : {q, k})
+        for (int i = 0; i < views; i++) {
+            const NormRopeView& v = side[i];
+            const uintptr_t at = reinterpret_cast<uintptr_t>(v.p) + (uintptr_t)(v.off * esz);
+            if (v.s[3] != 1 || (at & 15) || v.s[0] % align || v.s[1] % align || v.s[2] % align) {
+                SAGE_LOG("%s: rows must be dense and 16-byte aligned", v.name);
+                return MI355_SAGE_EUNSUPPORTED;
+            }
+        }
+    const int tsz = table_type == MI355_SAGE_F32 ? 4 : 2;
+    uintptr_t bits = reinterpret_cast<uintptr_t>(q_gain) | reinterpret_cast<uintptr_t>(k_gain);
+    if (rot > 0) bits |= reinterpret_cast<uintptr_t>(rope_cos) | reinterpret_cast<uintptr_t>(rope_sin) | (uintptr_t)(table_stride * tsz);
+    if (bits & 15) { SAGE_LOG("norm_rope: gains and table rows must be 16-byte aligned"); return MI355_SAGE_EUNSUPPORTED; }
+    NormRopeArgs a{};
+    auto fill = [&](NormRopeSide& x, const NormRopeView* v, const void* gain) {
+        auto at = [&](int i) { return const_cast<uint8_t*>(static_cast<const uint8_t*>(v[i].p)) + v[i].off * esz; };
+        x.p = at(0); x.sb = v[0].s[0]; x.sh = v[0].s[1]; x.sn = v[0].s[2];
+        x.out = at(1); x.osb = v[1].s[0]; x.osh = v[1].s[1]; x.osn = v[1].s[2];
+        if (views > 2) { x.d = at(2); x.dsb = v[2].s[0]; x.dsh = v[2].s[1]; x.dsn = v[2].s[2]; }
+        x.gain = gain;
+    };
+    fill(a.q, q, q_gain);
+    fill(a.k, k, k_gain);
+    a.B = B; a.S = S; a.Hq = Hq; a.Hk = Hk; a.D = D; a.type = type; a.gain_type = gain_type; a.table_type = table_type;
+    a.eps = eps; a.inv_d = 1.0f / D;
+    a.cos = rope_cos; a.sin = rope_sin; a.table_rows = table_rows; a.table_stride = table_stride; a.rot = rot; a.halfsplit = halfsplit != 0;
+    a.positions = positions; a.pos_sb = pos_stride; a.pos64 = pos_bytes == 8;
+    *out = a;
+    return 0;
+}
+
+int mi355_sage_qk_norm_rope(const void* Q, const void* K, void* Q_out, void* K_out, int B, int S, int Hq, int Hk, int D, int type,
+                            const int64_t* q_strides, const int64_t* k_strides, const int64_t* qo_strides, const int64_t* ko_strides,
+                            int64_t q_off, int64_t k_off, int64_t qo_off, int64_t ko_off,
+                            const void* q_gain, const void* k_gain, int gain_type, float eps,
+                            const void* rope_cos, const void* rope_sin, int table_type, int rot, int64_t table_rows, int64_t table_stride,
+                            int halfsplit, const void* positions, int64_t pos_stride, int pos_bytes, void* stream) {
+    const NormRopeView q[3] = {{"Q", Q, q_strides, q_off}, {"Q_out", Q_out, qo_strides, qo_off}, {}};
+    const NormRopeView k[3] = {{"K", K, k_strides, k_off}, {"K_out", K_out, ko_strides, ko_off}, {}};
+    NormRopeArgs a;
+    if (int rc = norm_rope_args(q, k, 2, B, S, Hq, Hk, D, type, q_gain, k_gain, gain_type, eps, rope_cos, rope_sin, table_type, rot, table_rows,
+                                table_stride, halfsplit, positions, pos_stride, pos_bytes, &a))
+        return rc;
+    SAGE_HIP(launch_norm_rope(a, static_cast<hipStream_t>(stream)));
+    return MI355_SAGE_OK;
+}
+
+size_t mi355_sage_qk_norm_rope_bwd_workspace_bytes(int B, int S, int Hq, int Hk, int D) {
+    if (B <= 0 || S <= 0 || Hq <= 0 || Hk <= 0 || D <= 0 || D % 16 || D > 256 || (int64_t)B * S > (1 << 30) / ((int64_t)Hq + Hk)) return 0;
+    int nq, nk;
+    norm_rope_bwd_split(B, S, Hq, Hk, D, &nq, &nk);
+    return align_up((size_t)(nq + nk) * D * sizeof(float));
+}
+
+int mi355_sage_qk_norm_rope_bwd(const void* dQ_out, const void* dK_out, const void* Q, const void* K, void* dQ, void* dK,
+                                void* d_q_gain, void* d_k_gain, int B, int S, int Hq, int Hk, int D, int type,
+                                const int64_t* dqo_strides, const int64_t* dko_strides, const int64_t* q_strides, const int64_t* k_strides,
+                                const int64_t* dq_strides, const int64_t* dk_strides, int64_t dqo_off, int64_t dko_off, int64_t q_off,
+                                int64_t k_off, int64_t dq_off, int64_t dk_off, const void* q_gain, const void* k_gain, int gain_type, float eps,
+                                const void* rope_cos, const void* rope_sin, int table_type, int rot, int64_t table_rows, int64_t table_stride,
+                                int halfsplit, const void* positions, int64_t pos_stride, int pos_bytes, void* stream,
+                                void* workspace, size_t workspace_bytes) {
+    if (!d_q_gain || !d_k_gain) return MI355_SAGE_EINVAL;
+    const NormRopeView q[3] = {{"Q", Q, q_strides, q_off}, {"dQ", dQ, dq_strides, dq_off}, {"dQ_out", dQ_out, dqo_strides, dqo_off}};
+    const NormRopeView k[3] = {{"K", K, k_strides, k_off}, {"dK", dK, dk_strides, dk_off}, {"dK_out", dK_out, dko_strides, dko_off}};
+    NormRopeArgs a;
+    int rc = norm_rope_args(q, k, 3, B, S, Hq, Hk, D, type, q_gain, k_gain, gain_type, eps, rope_cos, rope_sin, table_type, rot, table_rows,
+                            table_stride, halfsplit, positions, pos_stride, pos_bytes, &a);
+    if (rc) return rc;
+    const size_t need = mi355_sage_qk_norm_rope_bwd_workspace_bytes(B, S, Hq, Hk, D);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    std::lock_guard<std::mutex> together(launch_mutex(st));
+    if ((rc = call_workspace("norm_rope backward", need, st, &workspace, workspace_bytes))) return rc;
+    a.partial = static_cast<float*>(workspace);
+    a.d_gain_q = static_cast<float*>(d_q_gain);
+    a.d_gain_k = static_cast<float*>(d_k_gain);
+    SAGE_HIP(launch_norm_rope_bwd(a, st));
+    return MI355_SAGE_OK;
+}
 
 }  // extern "C"
