@@ -490,6 +490,39 @@ int mi355_sage_qk_norm_rope_bwd(
     const void* rope_cos, const void* rope_sin, int table_type, int rot, int64_t table_rows, int64_t table_stride, int halfsplit,
     const void* positions, int64_t pos_stride, int pos_bytes, void* stream, void* workspace, size_t workspace_bytes);
 
+/* ------------------------------------------------------------------------
+ * Attention over a sliding window, with a few first tokens that stay visible; bf16 or fp16 matrix products, no quantization
+ * (the reference's attention is full; windows are what long or streamed sequences and local text layers use).
+ *
+ * A query at position p sees key j (j < kv_lens[b], or < N_kv without kv_lens) when  j <= p + right  and
+ * (j >= p - left  or  j < sinks);  left or right -1: no bound on that side.  left = -1, right = 0 is causal attention.  Query i of
+ * sequence b stands at q_starts[b] + i, or q_start + i without q_starts.  A query that sees no key gets O = 0 and a
+ * statistic of -inf.  Keys at or beyond a sequence's length are never read, nor are keys that no query of a block of rows sees; a key
+ * that some query of a call sees must be finite.
+ * Q, O [B,Hq,N_q,D], K, V [B,Hk,N_kv,D], Hq a multiple of Hk: query heads h Hq/Hk .. share key head h (no expanded copies).  type
+ * MI355_SAGE_BF16 or _FP16 for all four; D 64, 128 or 256; scale > 0.  Stats (may be NULL): F32 [B,Hq,N_q] natural log-sum-exp.
+ * kv_lens, q_starts: int32 [B] on the device, or NULL; lengths outside [0, N_kv] are taken as the nearer bound.
+ * Workspace: mi355_sage_window_workspace_bytes(...) bytes, 256-byte aligned, or NULL for the library's per-stream buffer (the rules of
+ * mi355_sage_sdpa_bf16); the same bits on every call. */
+size_t mi355_sage_window_workspace_bytes(int B, int Hq, int Hk, int N_q, int N_kv, int D, int left, int right, int sinks);
+int mi355_sage_sdpa_window(
+    const void* Q, const void* K, const void* V, void* O, void* Stats,
+    int B, int Hq, int Hk, int N_q, int N_kv, int D, int type, float scale,
+    const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+    int64_t q_offset_elems, int64_t k_offset_elems, int64_t v_offset_elems, int64_t o_offset_elems, int64_t stats_offset_elems,
+    int left, int right, int sinks, const void* kv_lens, const void* q_starts, int q_start,
+    void* stream, void* workspace, size_t workspace_bytes);
+
+/* The same for the last N_q tokens of every sequence against its cache (K, V: the cache, N_kv its capacity): query i of sequence
+ * b stands at kv_lens[b] - N_q + i and sees no later key.  Sequences of fewer than N_q tokens have queries before their first, which
+ * come out as zeros.  Workspace: as above with right = 0. */
+int mi355_sage_sdpa_window_decode(
+    const void* Q, const void* K, const void* V, void* O,
+    int B, int Hq, int Hk, int N_q, int N_kv, int D, int type, float scale,
+    const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+    int64_t q_offset_elems, int64_t k_offset_elems, int64_t v_offset_elems, int64_t o_offset_elems,
+    int left, int sinks, const void* kv_lens, void* stream, void* workspace, size_t workspace_bytes);
+
 /* Library identification: "mi355_sage <version> gfx950". */
 const char* mi355_sage_version(void);
 

@@ -1,0 +1,156 @@
+"""Attention over a sliding window, with a few first tokens that stay visible: forward, training and serving forms.
+
+The reference's attention is full (serenitymojo/ops/attention.mojo:1690-1936) or masked by an additive tensor; here the mask is a rule on
+positions, and the keys it hides are not computed.  A query at position p sees key j of its sequence when
+
+    j <= p + right   and   (j >= p - left  or  j < sinks)
+
+left or right -1: no bound on that side (left=-1, right=0: causal attention).  Tensors are [B, S, H, Dh], BF16 or F16 (no
+quantization); k and v may have fewer heads than q, which then share them in order (q's heads h*Hq/Hk .. use key head h, the
+repeat_kv of models/dit/krea2_dit.mojo:703-705 without the copies).  Any strides with dense, 16-byte aligned rows.
+"""
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .attention_sage import Error
+from .norm_rope import _rows, _scratch, _strides
+
+_TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
+
+
+@dataclass
+class SdpaWindowFwd:
+    """What sdpa_window_train_fwd leaves for sdpa_window_backward; stats: F32 [B,H,S,1], the log-sum-exp of the visible scores."""
+    o: torch.Tensor
+    stats: torch.Tensor
+    q: torch.Tensor
+    k: torch.Tensor
+    v: torch.Tensor
+    scale: float
+    left: int
+    right: int
+    sinks: int
+    kv_lens: Optional[torch.Tensor]
+    q_start: int
+
+
+def _check(name, q, k, v, scale, left, right, sinks):
+    if q.dim() != 4 or k.dim() != 4:
+        raise Error("%s: q/k/v must be rank-4 [B,S,H,Dh]" % name)
+    if k.shape != v.shape:
+        raise Error("%s: k/v shape mismatch" % name)
+    if q.dtype not in _TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise Error("%s: q/k/v must be BF16 or F16, all the same" % name)
+    if q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise Error("%s: q and k/v disagree on B/Dh" % name)
+    if q.numel() == 0 or k.numel() == 0:
+        raise Error("%s: empty q or k" % name)
+    if q.shape[2] % k.shape[2]:
+        raise Error("%s: %d query heads cannot share %d key heads" % (name, q.shape[2], k.shape[2]))
+    if q.shape[3] not in (64, 128, 256):
+        raise Error("%s: Dh=%d is not supported (64, 128 or 256)" % (name, q.shape[3]))
+    if not 0.0 < scale < float("inf"):
+        raise Error("%s: scale must be positive" % name)
+    if left < -1 or right < -1 or sinks < 0:
+        raise Error("%s: left and right must be at least -1, sinks at least 0" % name)
+
+
+def _check_device(name, q, *others):
+    for t in (q, *others):
+        if t is not None and not t.is_cuda:
+            raise Error("%s: tensors must live on the GPU (no CPU fallback exists)" % name)
+        if t is not None and t.device != q.device:
+            raise Error("%s: tensors must live on one device" % name)
+
+
+def _lens(name, what, t, B):
+    """int32 [B], dense."""
+    if t is None:
+        return None
+    if t.dtype not in (torch.int32, torch.int64) or t.shape != (B,):
+        raise Error("%s: %s must be int32 or int64 [B]" % (name, what))
+    return t
+
+
+def _int32(t):
+    return None if t is None else t.to(torch.int32).contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _bound(x):
+    """The C argument for a number of keys: beyond any length all are alike."""
+    return min(int(x), 2 ** 30)
+
+
+def _forward(name, q, k, v, scale, left, right, sinks, kv_lens, q_start, want_stats):
+    _check(name, q, k, v, scale, left, right, sinks)
+    B, Sq, Hq, Dh = q.shape
+    Skv, Hk = k.shape[1], k.shape[2]
+    kv_lens = _lens(name, "kv_lens", kv_lens, B)
+    starts = _lens(name, "q_start", q_start, B) if isinstance(q_start, torch.Tensor) else None
+    start = 0 if starts is not None else int(q_start)
+    _check_device(name, q, k, v, kv_lens, starts)
+    L = _lib.lib()
+    with torch.cuda.device(q.device):
+        qi, ki, vi, lens, starts = _rows(q), _rows(k), _rows(v), _int32(kv_lens), _int32(starts)
+        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        stats = torch.empty((B, Hq, Sq, 1), dtype=torch.float32, device=q.device) if want_stats else None
+        ws = _scratch(L.mi355_sage_window_workspace_bytes(B, Hq, Hk, Sq, Skv, Dh, _bound(left), _bound(right), _bound(sinks)), o)
+        rc = L.mi355_sage_sdpa_window(
+            qi.data_ptr(), ki.data_ptr(), vi.data_ptr(), o.data_ptr(), _ptr(stats), B, Hq, Hk, Sq, Skv, Dh, _TYPES[q.dtype], float(scale),
+            _strides(qi), _strides(ki), _strides(vi), _strides(o), 0, 0, 0, 0, 0, _bound(left), _bound(right), _bound(sinks), _ptr(lens), _ptr(starts),
+            start, torch.cuda.current_stream(q.device).cuda_stream, ws.data_ptr(), ws.numel())
+    if rc != 0:
+        raise Error("%s: shim rc=%d (B=%d Sq=%d Skv=%d Hq=%d Hk=%d Dh=%d)" % (name, rc, B, Sq, Skv, Hq, Hk, Dh))
+    return o, stats, qi, ki, vi, lens
+
+
+def sdpa_window(q, k, v, scale, left, right=0, sinks=0, kv_lens=None, q_start=0):
+    """Attention of q [B,Sq,Hq,Dh] over k/v [B,Skv,Hk,Dh] through the window; returns [B,Sq,Hq,Dh] in q's type.
+
+    kv_lens: int32 or int64 [B] on the device, the sequences' lengths (keys from there on are padding: hidden, never read); None: all
+    Skv.  q_start: the position of every sequence's first query, an int or int32 / int64 [B] on the device (a
+    chunk of a prompt whose first part is already in the cache).  A query that sees no key gives zeros."""
+    return _forward("sdpa_window", q, k, v, scale, left, right, sinks, kv_lens, q_start, False)[0]
+
+
+def sdpa_window_decode(q, k_cache, v_cache, kv_lens, scale, left, sinks=0):
+    """The last Sq tokens of every sequence (one, or a few) against its cache [B,capacity,Hk,Dh]: query i of sequence b stands at
+    kv_lens[b] - Sq + i and sees keys up to itself through the window.  kv_lens counts the keys in the cache, the new tokens'
+    among them.  Queries before a sequence's first token (kv_lens[b] < Sq) give zeros."""
+    name = "sdpa_window_decode"
+    q4, k, v = q, k_cache, v_cache
+    _check(name, q4, k, v, scale, left, 0, sinks)
+    B, Sq, Hq, Dh = q.shape
+    Skv, Hk = k.shape[1], k.shape[2]
+    if kv_lens is None:
+        raise Error("%s: kv_lens must be int32 or int64 [B]" % name)
+    kv_lens = _lens(name, "kv_lens", kv_lens, B)
+    _check_device(name, q, k, v, kv_lens)
+    L = _lib.lib()
+    with torch.cuda.device(q.device):
+        qi, ki, vi, lens = _rows(q), _rows(k), _rows(v), _int32(kv_lens)
+        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ws = _scratch(L.mi355_sage_window_workspace_bytes(B, Hq, Hk, Sq, Skv, Dh, _bound(left), 0, _bound(sinks)), o)
+        rc = L.mi355_sage_sdpa_window_decode(
+            qi.data_ptr(), ki.data_ptr(), vi.data_ptr(), o.data_ptr(), B, Hq, Hk, Sq, Skv, Dh, _TYPES[q.dtype], float(scale),
+            _strides(qi), _strides(ki), _strides(vi), _strides(o), 0, 0, 0, 0, _bound(left), _bound(sinks), lens.data_ptr(),
+            torch.cuda.current_stream(q.device).cuda_stream, ws.data_ptr(), ws.numel())
+    if rc != 0:
+        raise Error("%s: shim rc=%d (B=%d Sq=%d Skv=%d Hq=%d Hk=%d Dh=%d)" % (name, rc, B, Sq, Skv, Hq, Hk, Dh))
+    return o
+
+
+def sdpa_window_train_fwd(q, k, v, scale, left, right=0, sinks=0, kv_lens=None, q_start=0):
+    """sdpa_window for a training step: the output with what the backward needs.  q_start: an int."""
+    name = "sdpa_window_train_fwd"
+    if isinstance(q_start, torch.Tensor):
+        raise Error("%s: q_start must be an int" % name)
+    o, stats, q, k, v, lens = _forward(name, q, k, v, scale, left, right, sinks, kv_lens, q_start, True)
+    return SdpaWindowFwd(o, stats, q, k, v, float(scale), left, right, sinks, lens, int(q_start))

@@ -7,6 +7,7 @@
 
 #include <atomic>
 #include <chrono>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <mutex>
@@ -1229,6 +1230,99 @@ int mi355_sage_qk_norm_rope_bwd(const void* dQ_out, const void* dK_out, const vo
     a.d_gain_k = static_cast<float*>(d_k_gain);
     SAGE_HIP(launch_norm_rope_bwd(a, st));
     return MI355_SAGE_OK;
+}
+
+
+// ---- attention over a sliding window ----------------------------------------------------------------
+// Sizes, types and the window: what all calls of this kind share.
+static int window_dims(const char* name, int B, int Hq, int Hk, int N_q, int N_kv, int D, int type, float scale, int left, int right, int sinks,
+                       int q_start, WindowArgs* a) {
+    if (B <= 0 || Hq <= 0 || Hk <= 0 || N_q <= 0 || N_kv <= 0 || D <= 0) return MI355_SAGE_EINVAL;
+    if (Hq % Hk || left < -1 || right < -1 || sinks < 0 || !(scale > 0.0f) || !(scale < INFINITY)) return MI355_SAGE_EINVAL;
+    if (type != MI355_SAGE_BF16 && type != MI355_SAGE_FP16) { SAGE_LOG("%s: bf16 or fp16", name); return MI355_SAGE_EUNSUPPORTED; }
+    if (!dims_ok(D)) { SAGE_LOG("%s: head dim %d not supported (64, 128 or 256)", name, D); return MI355_SAGE_EUNSUPPORTED; }
+    if (N_q > kWindowStart / 2 || N_kv > kWindowStart || (int64_t)N_q * (Hq / Hk) > 1 << 30 || q_start > kWindowStart || q_start < -kWindowStart) {
+        SAGE_LOG("%s: lengths or positions too large", name);
+        return MI355_SAGE_EUNSUPPORTED;
+    }
+    *a = WindowArgs{};
+    a->B = B; a->Hk = Hk; a->g = Hq / Hk; a->Sq = N_q; a->Skv = N_kv; a->D = D; a->type = type; a->scale = scale;
+    a->left = left < 0 || left > kWindowFar ? kWindowFar : left;
+    a->right = right < 0 || right > kWindowFar ? kWindowFar : right;
+    a->sinks = sinks > N_kv ? N_kv : sinks;
+    a->start = q_start;
+    return 0;
+}
+// The kernels address the rows of a block, and of a key tile, by 32-bit byte offsets from its first.
+static int window_span(const char* name, const int64_t* s, int64_t rows, int64_t heads, int D) {
+    const int64_t most = (int64_t)1 << 31;                 // elements
+    if (s[1] < 0 || s[2] < 0 || s[1] > most / heads || s[2] > most / rows || rows * s[2] + (heads - 1) * s[1] + D > most) {
+        SAGE_LOG("%s: a block's rows span more than 4 GiB, or a stride is negative", name);
+        return MI355_SAGE_EUNSUPPORTED;
+    }
+    return 0;
+}
+static int window_forward(const char* name, const void* Q, const void* K, const void* V, void* O, void* Stats, const int64_t* qs, const int64_t* ks,
+                          const int64_t* vs, const int64_t* os, int64_t q_off, int64_t k_off, int64_t v_off, int64_t o_off, int64_t stats_off,
+                          const void* kv_lens, const void* q_starts, WindowArgs& a, void* stream, void* workspace, size_t workspace_bytes) {
+    if (!Q || !K || !V || !O || !qs || !ks || !vs || !os) return MI355_SAGE_EINVAL;
+    int rc;
+    if ((rc = check_view("Q", Q, qs, q_off)) || (rc = check_view("K", K, ks, k_off)) || (rc = check_view("V", V, vs, v_off)) ||
+        (rc = check_view("O", O, os, o_off)) || (rc = window_span("Q", qs, 256 / a.g + 2, a.g, a.D)) || (rc = window_span("K", ks, 64, 1, a.D)) ||
+        (rc = window_span("V", vs, 64, 1, a.D)))
+        return rc;
+    const View q = make_view(Q, qs, q_off), k = make_view(K, ks, k_off), v = make_view(V, vs, v_off);
+    a.q = q.p; a.q_sb = q.sb; a.q_sh = q.sh; a.q_sn = q.sn;
+    a.k = k.p; a.k_sb = k.sb; a.k_sh = k.sh; a.k_sn = k.sn;
+    a.v = v.p; a.v_sb = v.sb; a.v_sh = v.sh; a.v_sn = v.sn;
+    a.o = static_cast<uint16_t*>(O) + o_off; a.o_sb = os[0]; a.o_sh = os[1]; a.o_sn = os[2];
+    a.lens = static_cast<const int32_t*>(kv_lens);
+    a.starts = static_cast<const int32_t*>(q_starts);
+    a.stats = Stats ? static_cast<float*>(Stats) + stats_off : nullptr;
+    const WindowPlan plan = window_plan(a);
+    if (!window_grid_ok(a, plan)) { SAGE_LOG("%s: too many workgroups", name); return MI355_SAGE_EUNSUPPORTED; }
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    std::lock_guard<std::mutex> together(launch_mutex(st));
+    const size_t need = window_part_bytes(a, plan);
+    if (need) {
+        if ((rc = call_workspace(name, need, st, &workspace, workspace_bytes))) return rc;
+        a.splits = plan.splits;
+        a.part = static_cast<float*>(workspace);
+        a.part_ml = a.part + need / sizeof(float) / (a.D + 2) * a.D;
+    } else {
+        a.splits = 1;
+    }
+    SAGE_HIP(launch_window(a, plan, st));
+    return MI355_SAGE_OK;
+}
+
+size_t mi355_sage_window_workspace_bytes(int B, int Hq, int Hk, int N_q, int N_kv, int D, int left, int right, int sinks) {
+    WindowArgs a;
+    if (window_dims("window", B, Hq, Hk, N_q, N_kv, D, MI355_SAGE_BF16, 1.0f, left, right, sinks, 0, &a)) return 0;
+    const size_t need = align_up(window_part_bytes(a, window_plan(a)));
+    return need ? need : kAlign;
+}
+
+int mi355_sage_sdpa_window(const void* Q, const void* K, const void* V, void* O, void* Stats, int B, int Hq, int Hk, int N_q, int N_kv, int D, int type,
+                           float scale, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+                           int64_t q_off, int64_t k_off, int64_t v_off, int64_t o_off, int64_t stats_off, int left, int right, int sinks,
+                           const void* kv_lens, const void* q_starts, int q_start, void* stream, void* workspace, size_t workspace_bytes) {
+    WindowArgs a;
+    if (int rc = window_dims("window", B, Hq, Hk, N_q, N_kv, D, type, scale, left, right, sinks, q_start, &a)) return rc;
+    return window_forward("window", Q, K, V, O, Stats, q_strides, k_strides, v_strides, o_strides, q_off, k_off, v_off, o_off, stats_off, kv_lens, q_starts,
+                          a, stream, workspace, workspace_bytes);
+}
+
+int mi355_sage_sdpa_window_decode(const void* Q, const void* K, const void* V, void* O, int B, int Hq, int Hk, int N_q, int N_kv, int D, int type,
+                                  float scale, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+                                  int64_t q_off, int64_t k_off, int64_t v_off, int64_t o_off, int left, int sinks, const void* kv_lens, void* stream,
+                                  void* workspace, size_t workspace_bytes) {
+    if (!kv_lens) return MI355_SAGE_EINVAL;
+    WindowArgs a;
+    if (int rc = window_dims("window decode", B, Hq, Hk, N_q, N_kv, D, type, scale, left, 0, sinks, 0, &a)) return rc;
+    a.at_end = 1;
+    return window_forward("window decode", Q, K, V, O, nullptr, q_strides, k_strides, v_strides, o_strides, q_off, k_off, v_off, o_off, 0, kv_lens, nullptr,
+                          a, stream, workspace, workspace_bytes);
 }
 
 }  // extern "C"

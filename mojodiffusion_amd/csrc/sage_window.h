@@ -35,4 +35,33 @@ void norm_rope_bwd_split(int B, int S, int Hq, int Hk, int D, int* wg_q, int* wg
 hipError_t launch_norm_rope(const NormRopeArgs& a, hipStream_t st);
 hipError_t launch_norm_rope_bwd(const NormRopeArgs& a, hipStream_t st);
 
+// ---- attention over a sliding window ---------------------------------------------------------------
+// A query at position p sees the keys j < len with j <= p + right and (j >= p - left or j < sinks).  Query i of sequence b stands
+// at (at_end ? len - Sq : starts ? starts[b] : start) + i.  g query heads share a key head; the rows of a workgroup are
+// (query, head of the group) pairs, heads first, so that they share one window.
+constexpr int kWindowFar = (1 << 30) - 1;        // left, right: no bound
+constexpr int kWindowStart = 1 << 29;            // positions are kept within this, so that sums with the above fit 32 bits
+struct WindowArgs {
+    const uint16_t *q, *k, *v;
+    uint16_t* o;
+    int64_t q_sb, q_sh, q_sn, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn, o_sb, o_sh, o_sn;      // strides in elements
+    int B, Hk, g, Sq, Skv, D, type;              // type: kBF16 or kF16
+    int left, right, sinks;
+    const int32_t *lens, *starts;                // [B] on the device, or null
+    int start, at_end;
+    float scale;                                 // > 0
+    float* stats;                                // [B, Hk * g, Sq] natural log-sum-exp, or null
+    // keys split over workgroups: unnormalised partial rows, their references and sums
+    int splits;
+    float *part, *part_ml;                       // [row block, split, 32, D], [row block, split, 32, 2]
+};
+struct WindowPlan {
+    int waves;                                   // > 0: workgroups of so many waves of 32 rows; 0: keys split
+    int splits;                                  // (of the latter: workgroups that share a block of 32 rows)
+};
+WindowPlan window_plan(const WindowArgs& a);
+bool window_grid_ok(const WindowArgs& a, const WindowPlan& p);
+size_t window_part_bytes(const WindowArgs& a, const WindowPlan& p);
+hipError_t launch_window(const WindowArgs& a, const WindowPlan& p, hipStream_t st);
+
 }  // namespace sage

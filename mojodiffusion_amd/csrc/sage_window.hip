@@ -1,0 +1,519 @@
+// sage_window.hip — attention over a sliding window with a few first tokens that stay visible, bf16 or fp16.
+//
+//     S_ij = scale q_i . k_j  for the keys j that query i sees,  O_i = sum_j exp(S_ij - L_i) v_j,  L_i = log sum_j exp(S_ij)
+//
+// One pass over the visible key tiles with the running reference and sum of the softmax.  A wave owns 32 rows ("x": pairs of
+// a query and a head of the group that shares keys) as the columns of its matrix products: a 32 x 32 block of scores
+// S^T = K Q^T lands with the row as the lane's column, which is the operand layout of O^T += V^T P^T, so the
+// probabilities go from registers into the next product; V^T comes from the row-major tile by the transposing LDS read.
+// Scores, reference, sum and O are fp32; P is rounded to the inputs' type as a matrix operand (an error of at most
+// half a step of each weight, unbiased over the keys), the sum is taken over the unrounded values.
+//
+// Which keys a workgroup walks follows from its rows' positions: the tiles of the first `sinks` keys, then those from the first
+// row's left edge to the last row's right edge.  Tiles that every row of a wave sees whole take no mask; a wave leaves out tiles that
+// none of its rows sees.  Rows of a tile that no row of the workgroup sees are not read at all (another key's row stands
+// in), so whatever lies there, or behind a sequence's end, cannot reach a result.
+#include "sage_grid.h"
+#include "sage_tile.h"
+#include "sage_window.h"
+
+#include <algorithm>
+
+namespace sage {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2hf __attribute__((ext_vector_type(2)));
+
+template <int T> __device__ __forceinline__ v16f product(v4i a, v4i b, v16f c) {
+    if constexpr (T == kBF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+template <int T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (T == kBF16) return pack_bf16(a, b);
+    const v2f f = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, v2hf));
+}
+// the other half-wave's value of the same column
+__device__ __forceinline__ float max_halves(float x) {
+    const v2u r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+    const v2u r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r.x) + __uint_as_float(r.y);
+}
+
+__device__ __forceinline__ int sequence_len(const WindowArgs& a, int b) { return a.lens ? max(0, min(a.lens[b], a.Skv)) : a.Skv; }
+__device__ __forceinline__ int first_position(const WindowArgs& a, int b, int len) {
+    if (a.at_end) return len - a.Sq;
+    return a.starts ? max(-kWindowStart, min(a.starts[b], kWindowStart)) : a.start;
+}
+
+// The key tiles (KT keys each) that rows at positions p_lo .. p_hi see: `first` tiles with the sinks, then those from `next` on, n in all.
+// Keys [0, s_end) and [lo, hi] are the ones that some row sees.
+struct Span {
+    int lo, hi, s_end, first, next, n;
+    __device__ int tile(int t) const { return t < first ? t : next + t - first; }
+};
+template <int KT> __device__ __forceinline__ Span key_span(const WindowArgs& a, int p_lo, int p_hi, int len) {
+    Span s;
+    s.hi = min(p_hi + a.right, len - 1);
+    s.lo = max(p_lo - a.left, 0);
+    s.s_end = max(min(a.sinks, s.hi + 1), 0);
+    s.first = (s.s_end + KT - 1) / KT;
+    s.next = max(s.lo / KT, s.first);
+    s.n = s.first + (s.hi >= s.lo ? max(s.hi / KT + 1 - s.next, 0) : 0);
+    return s;
+}
+// The key whose row is copied for row j of the tile that starts at j0: j itself where some row of the workgroup sees it, else a neighbour that one sees.
+template <int KT> __device__ __forceinline__ int copied_key(const Span& s, int j0, int j) {
+    const int gap = s.lo <= min(j0 + KT - 1, s.hi) ? s.lo : s.s_end - 1;
+    if (j >= s.s_end && j < s.lo) j = gap;
+    return min(j, s.hi);
+}
+
+// Where a lane's fragments lie in a tile: along the channels by k-step, across them by 32-channel block (rows 0-7 and 8-15; 16-row blocks are
+// + 32 * D bytes).  The XOR of the layout reaches over 16 chunks, so channels from 128 on lie 256 bytes further.
+template <int D> struct Fragments {
+    int nat[D > 128 ? 8 : D / 16], tr[D > 128 ? 4 : D / 32][2];
+    __device__ explicit Fragments(int lane) {
+        constexpr int CPR = D / 8;
+#pragma unroll
+        for (int s = 0; s < (D > 128 ? 8 : D / 16); s++) nat[s] = nat_off<CPR>(lane & 31, s * 2 + (lane >> 5));
+#pragma unroll
+        for (int d = 0; d < (D > 128 ? 4 : D / 32); d++) tr[d][0] = tr_frag_off<CPR>(lane, 0, d), tr[d][1] = tr_frag_off<CPR>(lane, 8, d);
+    }
+    __device__ v4i along(const uint8_t* tile, int s) const { return *reinterpret_cast<const v4i*>(tile + nat[s & 7] + (s >> 3) * 256); }
+    __device__ v4i across(const uint8_t* rows, int d) const { return tr_read(rows + tr[d & 3][0] + (d >> 2) * 256, rows + tr[d & 3][1] + (d >> 2) * 256); }
+};
+
+// What a lane keeps of its row, and the tile's part in it.
+template <int D> struct RowState {
+    v16f acc[D / 32];                // O^T: channels d * 32 + (i >> 2) * 8 + half * 4 + (i & 3)
+    float ref, sum;                  // reference in log2 units, and this lane's part of the sum of exp2(S - ref)
+    __device__ void clear() {
+#pragma unroll
+        for (int d = 0; d < D / 32; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
+        ref = -INFINITY;
+        sum = 0.0f;
+    }
+};
+struct RowMask { int lo, hi, sinks; };           // keys lo .. hi and [0, sinks) up to hi
+
+template <int T, int D, int KT, bool MASKED>
+__device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 16], const uint8_t* kt, const uint8_t* vt, const Fragments<D>& fr,
+                                            int j0, const RowMask& m, float c, int half) {
+    constexpr int KS = D / 16, DB = D / 32, NB = KT / 32;
+    v16f s[NB];
+#pragma unroll
+    for (int blk = 0; blk < NB; blk++) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[blk][i] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+            s[blk] = product<T>(fr.along(kt + blk * 64 * D, ks), q[ks], s[blk]);
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int blk = 0; blk < NB; blk++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            if constexpr (MASKED) {
+                const int j = j0 + blk * 32 + (i >> 2) * 8 + half * 4 + (i & 3);
+                if (!(j <= m.hi && (j >= m.lo || j < m.sinks))) s[blk][i] = -INFINITY;
+            }
+            top = fmaxf(top, s[blk][i]);
+        }
+    top = max_halves(top) * c;
+    // A new reference only where the old one lies more than 8 below: the weights stay under 2^8, and the sums have
+    // room for that; O is multiplied on few tiles instead of on most.
+    if (__any(top > st.ref + 8.0f)) {
+        const float ref = fmaxf(st.ref, top);
+        const float f = ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.ref - ref);
+        st.ref = ref;
+        st.sum *= f;
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) st.acc[d][i] *= f;
+    }
+    const float ref = MASKED && st.ref == -INFINITY ? 0.0f : st.ref;       // (no key so far: every weight is exp2(-inf))
+    uint32_t p[NB][8];
+    float part[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int blk = 0; blk < NB; blk++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[blk][i], c, -ref)), y = __builtin_amdgcn_exp2f(fmaf(s[blk][i + 1], c, -ref));
+            part[0] += x;
+            part[1] += y;
+            p[blk][i >> 1] = pack2<T>(x, y);
+        }
+    st.sum += part[0] + part[1];
+#pragma unroll
+    for (int blk = 0; blk < NB; blk++)
+#pragma unroll
+        for (int j2 = 0; j2 < 2; j2++) {
+            const v4i pb = {(int)p[blk][j2 * 4], (int)p[blk][j2 * 4 + 1], (int)p[blk][j2 * 4 + 2], (int)p[blk][j2 * 4 + 3]};
+            const uint8_t* rows = vt + (blk * 2 + j2) * 32 * D;
+#pragma unroll
+            for (int d = 0; d < DB; d++) st.acc[d] = product<T>(fr.across(rows, d), pb, st.acc[d]);
+        }
+}
+
+// A wave's view of a tile: nothing of it, all of it, or some.
+enum class Seen { kNone, kAll, kSome };
+template <int KT> __device__ __forceinline__ Seen seen(const WindowArgs& a, int p_lo, int p_hi, int len, int j0) {
+    const int j1 = j0 + KT - 1;
+    if (j0 > min(p_hi + a.right, len - 1) || (j1 < p_lo - a.left && j0 >= a.sinks)) return Seen::kNone;
+    return j1 <= min(p_lo + a.right, len - 1) && (j0 >= p_hi - a.left || j1 < a.sinks) ? Seen::kAll : Seen::kSome;
+}
+
+// 32 rows x0 .. of (query, head) pairs -> LDS at dst; rows past the last repeat it.  `base` is the first row's query.
+template <int D> __device__ __forceinline__ void query_rows_in(const WindowArgs& a, const uint16_t* base, int i_base, int x0, uint32_t dst, int lane) {
+    constexpr int CPR = D / 8, RPI = 64 / CPR;
+    const int last = a.Sq * a.g - 1;
+#pragma unroll
+    for (int n = 0; n < 32 / RPI; n++) {
+        const int r = n * RPI + lane / CPR, x = min(x0 + r, last), i = x / a.g;
+        const uint32_t off = ((uint32_t)(i - i_base) * (uint32_t)a.q_sn + (uint32_t)(x - i * a.g) * (uint32_t)a.q_sh) * 2u;
+        dma16(base, off + nat_pos<CPR>(r, lane % CPR) * 16, __builtin_amdgcn_readfirstlane(dst + n * 1024));
+    }
+}
+// The wave's finished rows: registers -> LDS (64 * D bytes at os) -> O, and the statistics.
+template <int T, int D>
+__device__ __forceinline__ void finish_rows(const WindowArgs& a, const RowState<D>& st, uint8_t* os, int b, int kvh, int x0, int lane) {
+    constexpr int CPR = D / 8, RPI = 64 / CPR, DB = D / 32;
+    const int l32 = lane & 31, half = lane >> 5, rows = a.Sq * a.g;
+    const float sum = sum_halves(st.sum);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;                     // (a row that sees no key: zeros)
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *reinterpret_cast<u32x2*>(os + nat_off<CPR>(l32, d * 4 + g) + half * 8) =
+                u32x2{pack2<T>(st.acc[d][g * 4] * inv, st.acc[d][g * 4 + 1] * inv), pack2<T>(st.acc[d][g * 4 + 2] * inv, st.acc[d][g * 4 + 3] * inv)};
+    if (a.stats != nullptr && half == 0 && x0 + l32 < rows) {
+        const int x = x0 + l32, i = x / a.g;
+        a.stats[((int64_t)b * a.Hk * a.g + kvh * a.g + (x - i * a.g)) * a.Sq + i] = sum == 0.0f ? -INFINITY : (st.ref + __builtin_amdgcn_logf(sum)) * kLn2;
+    }
+    uint16_t* o = a.o + b * a.o_sb + (int64_t)kvh * a.g * a.o_sh;
+#pragma unroll
+    for (int n = 0; n < 32 / RPI; n++) {
+        const int r = n * RPI + lane / CPR, x = x0 + r, i = x / a.g;
+        const u32x4 w = *reinterpret_cast<const u32x4*>(os + nat_off<CPR>(r, lane % CPR));
+        if (x < rows) *reinterpret_cast<u32x4*>(o + i * a.o_sn + (int64_t)(x - i * a.g) * a.o_sh + (lane % CPR) * 8) = w;
+    }
+}
+
+template <int D, int NW> struct WindowLds {
+    static constexpr int KT = D > 128 ? 32 : 64, TILE = KT * D * 2, SLOT = 2 * TILE, SLOTS = 3;
+    static constexpr int OWN = NW * 64 * D;                                // the waves' own rows: behind the first slot, and at the end
+    static constexpr int BYTES = SLOTS * SLOT > SLOT + OWN ? SLOTS * SLOT : SLOT + OWN;
+};
+
+template <int T, int D, int NW>
+__global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void window_kernel(WindowArgs a) {
+    using L = WindowLds<D, NW>;
+    constexpr int KT = L::KT, CPR = D / 8, RPW = L::TILE / 1024 / NW, KS = D / 16;
+    static_assert(L::TILE / 1024 % NW == 0, "tile copies must divide over the waves");
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
+    const int rows = a.Sq * a.g, blocks = (rows + NW * 32 - 1) / (NW * 32);
+    const int item = xcd_item((int)blockIdx.x, a.B * a.Hk * blocks);
+    const int bh = item / blocks, row0 = (blocks - 1 - item % blocks) * NW * 32;       // (the last rows first: without a left edge they see most keys)
+    const int b = bh / a.Hk, kvh = bh % a.Hk;
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int x0 = row0 + wave * 32;
+
+    const int len = sequence_len(a, b), p0 = first_position(a, b, len);
+    const int i_lo = row0 / a.g;
+    const Span span = key_span<KT>(a, p0 + i_lo, p0 + (min(row0 + NW * 32, rows) - 1) / a.g, len);
+    const int wp_lo = p0 + min(x0, rows - 1) / a.g, wp_hi = p0 + min(x0 + 31, rows - 1) / a.g;      // this wave's positions
+    const int p = p0 + min(x0 + (lane & 31), rows - 1) / a.g;
+    const RowMask mask = {p - a.left, min(p + a.right, len - 1), a.sinks};
+
+    int nat_row[RPW], nat_col[RPW];
+#pragma unroll
+    for (int i = 0; i < RPW; i++) {
+        const int P = (i * NW + wave) * 64 + lane;
+        nat_row[i] = P / CPR;
+        nat_col[i] = nat_pos<CPR>(P / CPR, P % CPR) * 16;
+    }
+    const uint32_t lds = lds_addr(smem);
+    const uint16_t* kh = a.k + b * a.k_sb + kvh * a.k_sh;
+    const uint16_t* vh = a.v + b * a.v_sb + kvh * a.v_sh;
+    const uint32_t ks_b = (uint32_t)a.k_sn * 2u, vs_b = (uint32_t)a.v_sn * 2u;
+    auto copy_tile = [&](int t, int slot) {
+        const int j0 = span.tile(t) * KT;
+        const uint16_t *kb = kh + (int64_t)j0 * a.k_sn, *vb = vh + (int64_t)j0 * a.v_sn;
+#pragma unroll
+        for (int i = 0; i < RPW; i++) {
+            const uint32_t row = (uint32_t)(copied_key<KT>(span, j0, j0 + nat_row[i]) - j0);
+            const uint32_t dst = lds + slot * L::SLOT + (i * NW + wave) * 1024;
+            dma16(kb, row * ks_b + nat_col[i], __builtin_amdgcn_readfirstlane(dst));
+            dma16(vb, row * vs_b + nat_col[i], __builtin_amdgcn_readfirstlane(dst + L::TILE));
+        }
+    };
+
+    v4i q[KS];
+    const Fragments<D> fr(lane);
+    query_rows_in<D>(a, a.q + b * a.q_sb + (int64_t)kvh * a.g * a.q_sh + (int64_t)i_lo * a.q_sn, i_lo, x0, lds + L::SLOT + wave * 64 * D, lane);
+    if (span.n > 0) copy_tile(0, 0);
+    dma_wait<0>();
+#pragma unroll
+    for (int s = 0; s < KS; s++) q[s] = fr.along(smem + L::SLOT + wave * 64 * D, s);
+#pragma unroll
+    for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));
+    __syncthreads();                     // the rows' LDS becomes the ring's other slots
+    if (span.n > 1) copy_tile(1, 1);
+
+    RowState<D> st;
+    st.clear();
+    const float c = a.scale * kLog2e;
+    int slot = 0;
+    for (int t = 0; t < span.n; t++) {
+        if (t + 1 < span.n) dma_wait<2 * RPW>();
+        else dma_wait<0>();
+        __syncthreads();                 // tile t is visible; every wave is done with the slot of tile t - 1
+        if (t + 2 < span.n) copy_tile(t + 2, slot == 0 ? 2 : slot - 1);
+        const int j0 = span.tile(t) * KT;
+        const uint8_t* kt = smem + slot * L::SLOT;
+        const Seen what = x0 < rows ? seen<KT>(a, wp_lo, wp_hi, len, j0) : Seen::kNone;
+        if (D <= 128 && what == Seen::kAll) attend_tile<T, D, KT, false>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
+        else if (what != Seen::kNone) attend_tile<T, D, KT, true>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
+        slot = slot == 2 ? 0 : slot + 1;
+    }
+    __syncthreads();                     // (no copy is in flight: the last tile's wait was for all of them)
+    if (x0 < rows) finish_rows<T, D>(a, st, smem + wave * 64 * D, b, kvh, x0, lane);
+}
+
+// ---- few rows: the keys split over waves and workgroups ---------------------------------------------------
+// A workgroup owns 32 rows; its waves take tiles of 32 keys in turn, each with two slots of its own to copy into, so no wave waits for
+// another before the end, where the waves' partial rows meet in LDS.  With several workgroups to a block of rows the partial rows go to
+// memory in fp32 and window_join_kernel adds them up, in order.  Bound by the bytes of K and V.
+template <int D> struct SplitLds {
+    static constexpr int NW = 4, KT = 32, TILE = KT * D * 2, SLOT = 2 * TILE, SLOTS = D > 128 ? 1 : 2;
+    static constexpr int RING = SLOTS * SLOT;                              // per wave
+    static constexpr int MEET = NW * 32 * (D + 4) * 4;                     // per wave 32 rows of D floats (+ 4: banks)
+    static constexpr int BYTES = NW * RING > MEET ? NW * RING : MEET;
+    static_assert(64 * D <= RING, "a wave's rows pass through its ring");
+};
+
+template <int T, int D>
+__global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
+    using L = SplitLds<D>;
+    constexpr int NW = L::NW, KT = L::KT, CPR = D / 8, RUNS = L::TILE / 1024, KS = D / 16, DB = D / 32;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
+    __shared__ float meet_ml[NW][32][2];
+    const int rows = a.Sq * a.g, blocks = (rows + 31) / 32;
+    const int split = (int)blockIdx.x % a.splits, item = (int)blockIdx.x / a.splits;
+    const int bh = item / blocks, x0 = item % blocks * 32;
+    const int b = bh / a.Hk, kvh = bh % a.Hk;
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+    const int len = sequence_len(a, b), p0 = first_position(a, b, len);
+    const int i_lo = x0 / a.g;
+    const int p_lo = p0 + i_lo, p_hi = p0 + (min(x0 + 32, rows) - 1) / a.g;
+    const Span span = key_span<KT>(a, p_lo, p_hi, len);
+    const int p = p0 + min(x0 + l32, rows - 1) / a.g;
+    const RowMask mask = {p - a.left, min(p + a.right, len - 1), a.sinks};
+    const int t0 = (int)((int64_t)span.n * split / a.splits), t1 = (int)((int64_t)span.n * (split + 1) / a.splits);
+
+    const uint32_t ring = lds_addr(smem) + wave * L::RING;
+    const uint8_t* own = smem + wave * L::RING;
+    const uint16_t* kh = a.k + b * a.k_sb + kvh * a.k_sh;
+    const uint16_t* vh = a.v + b * a.v_sb + kvh * a.v_sh;
+    const uint32_t ks_b = (uint32_t)a.k_sn * 2u, vs_b = (uint32_t)a.v_sn * 2u;
+    auto copy_tile = [&](int t, int slot) {
+        const int j0 = span.tile(t) * KT;
+        const uint16_t *kb = kh + (int64_t)j0 * a.k_sn, *vb = vh + (int64_t)j0 * a.v_sn;
+#pragma unroll
+        for (int i = 0; i < RUNS; i++) {
+            const int P = i * 64 + lane, r = P / CPR, col = nat_pos<CPR>(r, P % CPR) * 16;
+            const uint32_t row = (uint32_t)(copied_key<KT>(span, j0, j0 + r) - j0);
+            const uint32_t dst = ring + slot * L::SLOT + i * 1024;
+            dma16(kb, row * ks_b + col, __builtin_amdgcn_readfirstlane(dst));
+            dma16(vb, row * vs_b + col, __builtin_amdgcn_readfirstlane(dst + L::TILE));
+        }
+    };
+
+    v4i q[KS];
+    const Fragments<D> fr(lane);
+    query_rows_in<D>(a, a.q + b * a.q_sb + (int64_t)kvh * a.g * a.q_sh + (int64_t)i_lo * a.q_sn, i_lo, x0, ring, lane);
+    dma_wait<0>();
+#pragma unroll
+    for (int s = 0; s < KS; s++) q[s] = fr.along(own, s);
+#pragma unroll
+    for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));
+
+    RowState<D> st;
+    st.clear();
+    const float c = a.scale * kLog2e;
+    // (a slot is filled again only when the reads of what it held have come back)
+    auto reads_done = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
+    reads_done();
+    int t = t0 + wave, slot = 0;
+    if (t < t1) copy_tile(t, 0);
+    for (; t < t1; t += NW) {
+        if (L::SLOTS == 2 && t + NW < t1) {
+            reads_done();
+            copy_tile(t + NW, slot ^ 1);
+            dma_wait<2 * RUNS>();
+        } else {
+            dma_wait<0>();
+        }
+        const int j0 = span.tile(t) * KT;
+        const uint8_t* kt = own + slot * L::SLOT;
+        if (D <= 128 && seen<KT>(a, p_lo, p_hi, len, j0) == Seen::kAll) attend_tile<T, D, KT, false>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
+        else attend_tile<T, D, KT, true>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
+        if (L::SLOTS == 2) slot ^= 1;
+        else if (t + NW < t1) {
+            reads_done();
+            copy_tile(t + NW, 0);
+        }
+    }
+
+    // The waves' parts meet: every part is taken to the largest reference of its row.
+    __syncthreads();
+    const float wsum = sum_halves(st.sum);
+    if (half == 0) meet_ml[wave][l32][0] = st.ref, meet_ml[wave][l32][1] = wsum;
+    float* parts = reinterpret_cast<float*>(smem);
+    constexpr int PR = D + 4;
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *reinterpret_cast<v4f*>(parts + (wave * 32 + l32) * PR + d * 32 + g * 8 + half * 4) =
+                v4f{st.acc[d][g * 4], st.acc[d][g * 4 + 1], st.acc[d][g * 4 + 2], st.acc[d][g * 4 + 3]};
+    __syncthreads();
+    // 8 lanes to a row, D / 8 channels each
+    const int r = tid >> 3, x = x0 + r;
+    float ref = -INFINITY, sum = 0.0f, f[NW];
+#pragma unroll
+    for (int w = 0; w < NW; w++) ref = fmaxf(ref, meet_ml[w][r][0]);
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+        f[w] = ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(meet_ml[w][r][0] - ref);
+        sum = fmaf(meet_ml[w][r][1], f[w], sum);
+    }
+    if (x >= rows) return;
+    const int i = x / a.g, hg = x - i * a.g;
+    const bool last = a.splits == 1;
+    const float inv = last ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+    float* po = a.part + ((int64_t)item * a.splits + split) * 32 * D + r * D;
+    uint16_t* o = a.o + b * a.o_sb + ((int64_t)kvh * a.g + hg) * a.o_sh + i * a.o_sn;
+#pragma unroll
+    for (int n = 0; n < D / 64; n++) {
+        const int col = (n * 8 + (tid & 7)) * 8;
+        float y[8];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            v4f sumv = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
+                const v4f v = *reinterpret_cast<const v4f*>(parts + (w * 32 + r) * PR + col + h * 4);
+#pragma unroll
+                for (int e = 0; e < 4; e++) sumv[e] = fmaf(v[e], f[w], sumv[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[h * 4 + e] = sumv[e] * inv;
+        }
+        if (last) *reinterpret_cast<u32x4*>(o + col) = u32x4{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7])};
+        else {
+            *reinterpret_cast<v4f*>(po + col) = v4f{y[0], y[1], y[2], y[3]};
+            *reinterpret_cast<v4f*>(po + col + 4) = v4f{y[4], y[5], y[6], y[7]};
+        }
+    }
+    if ((tid & 7) == 0) {
+        if (!last) {
+            float* ml = a.part_ml + (((int64_t)item * a.splits + split) * 32 + r) * 2;
+            ml[0] = ref, ml[1] = sum;
+        } else if (a.stats != nullptr) {
+            a.stats[((int64_t)b * a.Hk * a.g + kvh * a.g + hg) * a.Sq + i] = sum == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(sum)) * kLn2;
+        }
+    }
+}
+
+// One wave to a row: 64 lanes of D / 64 channels each.
+template <int T, int D>
+__global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
+    constexpr int N = D / 64;
+    const int rows = a.Sq * a.g, blocks = (rows + 31) / 32;
+    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= (int64_t)a.B * a.Hk * rows) return;
+    const int lane = threadIdx.x & 63, bh = (int)(at / rows), x = (int)(at % rows), b = bh / a.Hk, kvh = bh % a.Hk;
+    const int64_t item = (int64_t)bh * blocks + x / 32;
+    const float* ml = a.part_ml + (item * a.splits * 32 + x % 32) * 2;
+    const float* part = a.part + (item * a.splits * 32 + x % 32) * D + lane * N;
+    float ref = -INFINITY, sum = 0.0f, y[N];
+    for (int s = 0; s < a.splits; s++) ref = fmaxf(ref, ml[(int64_t)s * 64]);
+#pragma unroll
+    for (int e = 0; e < N; e++) y[e] = 0.0f;
+    for (int s = 0; s < a.splits; s++) {
+        const float f = ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[(int64_t)s * 64] - ref);
+        sum = fmaf(ml[(int64_t)s * 64 + 1], f, sum);
+#pragma unroll
+        for (int e = 0; e < N; e++) y[e] = fmaf(part[(int64_t)s * 32 * D + e], f, y[e]);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int i = x / a.g, hg = x - i * a.g;
+    uint16_t* o = a.o + b * a.o_sb + ((int64_t)kvh * a.g + hg) * a.o_sh + i * a.o_sn + lane * N;
+    if constexpr (N == 1) o[0] = (uint16_t)pack2<T>(y[0] * inv, 0.0f);
+    else {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) *reinterpret_cast<uint32_t*>(o + e) = pack2<T>(y[e] * inv, y[e + 1] * inv);
+    }
+    if (a.stats != nullptr && lane == 0)
+        a.stats[((int64_t)b * a.Hk * a.g + kvh * a.g + hg) * a.Sq + i] = sum == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+int64_t row_blocks(const WindowArgs& a, int rows) { return (int64_t)a.B * a.Hk * (((int64_t)a.Sq * a.g + rows - 1) / rows); }
+
+template <int T, int D> hipError_t launch_td(const WindowArgs& a, const WindowPlan& p, hipStream_t st) {
+    if (p.waves == 8) {
+        if constexpr (D <= 128) hipLaunchKernelGGL((window_kernel<T, D, 8>), dim3((unsigned)row_blocks(a, 256)), dim3(512), 0, st, a);
+    } else if (p.waves == 4) hipLaunchKernelGGL((window_kernel<T, D, 4>), dim3((unsigned)row_blocks(a, 128)), dim3(256), 0, st, a);
+    else {
+        hipLaunchKernelGGL((window_split_kernel<T, D>), dim3((unsigned)(row_blocks(a, 32) * a.splits)), dim3(256), 0, st, a);
+        if (a.splits > 1)
+            hipLaunchKernelGGL((window_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.B * a.Hk * a.Sq * a.g + 3) / 4)), dim3(256), 0, st, a);
+    }
+    return hipGetLastError();
+}
+template <int T> hipError_t launch_t(const WindowArgs& a, const WindowPlan& p, hipStream_t st) {
+    if (a.D == 64) return launch_td<T, 64>(a, p, st);
+    if (a.D == 128) return launch_td<T, 128>(a, p, st);
+    return launch_td<T, 256>(a, p, st);
+}
+
+}  // namespace
+
+// Rows enough for half the chip: tiles shared by 4 or 8 waves.  Else the keys are split until there are four workgroups to every
+// compute unit, down to 4 tiles (one to a wave).
+WindowPlan window_plan(const WindowArgs& a) {
+    constexpr int64_t kUnits = 256;
+    if (row_blocks(a, 128) >= kUnits / 2 || a.Sq * (int64_t)a.g > 512) return WindowPlan{a.D <= 128 && row_blocks(a, 256) >= kUnits ? 8 : 4, 1};
+    const int64_t keys = a.right >= kWindowFar || a.left >= kWindowFar ? a.Skv
+                                                                       : std::min<int64_t>(a.Skv, (int64_t)a.left + a.right + 32 / a.g + 1 + a.sinks);
+    const int64_t most = std::max<int64_t>(1, keys / 128), want = (4 * kUnits + row_blocks(a, 32) - 1) / row_blocks(a, 32);
+    return WindowPlan{0, (int)std::min(most, want)};
+}
+bool window_grid_ok(const WindowArgs& a, const WindowPlan& p) {
+    return row_blocks(a, 32) * p.splits <= 0x7FFFFFFF && (int64_t)a.B * a.Hk * a.Sq * a.g <= 0x7FFFFFFF;
+}
+size_t window_part_bytes(const WindowArgs& a, const WindowPlan& p) {
+    return p.waves || p.splits == 1 ? 0 : (size_t)row_blocks(a, 32) * p.splits * 32 * (a.D + 2) * sizeof(float);
+}
+
+hipError_t launch_window(const WindowArgs& a, const WindowPlan& p, hipStream_t st) {
+    return a.type == kBF16 ? launch_t<kBF16>(a, p, st) : launch_t<kF16>(a, p, st);
+}
+
+}  // namespace sage

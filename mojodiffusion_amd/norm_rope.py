@@ -14,7 +14,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .attention_sage import Error, _workspace
+from .attention_sage import Error
 
 _TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32: _lib.F32}
 
@@ -27,17 +27,20 @@ class QkNormRopeGrads:
     d_k_norm: torch.Tensor
 
 
-def _rows(t):
-    """t, or a dense copy of it where its rows are not dense or not 16-byte aligned."""
-    per = 16 // t.element_size()
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % per == 0 for s in t.stride()[:3]):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _scratch(nbytes, like):
+    """A workspace of a call's own, from torch's allocator: calls on other streams and captured graphs (whose pool it comes from
+    under capture) never share it."""
+    return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=like.device)
 
 
 def _rows_ok(t):
     per = 16 // t.element_size()
     return t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % per == 0 for s in t.stride()[:3])
+
+
+def _rows(t):
+    """t, or a dense copy of it where its rows are not dense or not 16-byte aligned."""
+    return t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(t):
@@ -163,7 +166,7 @@ def qk_norm_rope_backward(d_q_rot, d_k_rot, q, k, q_norm, k_norm, eps, cos, sin,
     dq, dk = _out(name, None, q), _out(name, None, k)
     d_gain = torch.empty((2, Dh), dtype=torch.float32, device=q.device)
     with torch.cuda.device(q.device):
-        ws = _workspace(max(L.mi355_sage_qk_norm_rope_bwd_workspace_bytes(B, S, Hq, Hk, Dh), 256), dq)
+        ws = _scratch(L.mi355_sage_qk_norm_rope_bwd_workspace_bytes(B, S, Hq, Hk, Dh), dq)
         rc = L.mi355_sage_qk_norm_rope_bwd(
             dqi.data_ptr(), dki.data_ptr(), qi.data_ptr(), ki.data_ptr(), dq.data_ptr(), dk.data_ptr(), d_gain[0].data_ptr(),
             d_gain[1].data_ptr(), B, S, Hq, Hk, Dh, _TYPES[q.dtype], _strides(dqi), _strides(dki), _strides(qi), _strides(ki),
