@@ -523,6 +523,19 @@ int mi355_sage_sdpa_window_decode(
     int64_t q_offset_elems, int64_t k_offset_elems, int64_t v_offset_elems, int64_t o_offset_elems,
     int left, int sinks, const void* kv_lens, void* stream, void* workspace, size_t workspace_bytes);
 
+/* Gradient of mi355_sage_sdpa_window: O and Stats as the forward wrote them, dO upstream -> dQ [B,Hq,N_q,D], dK, dV [B,Hk,N_kv,D] (of a
+ * shared key head: summed over its query heads), every row written, those of keys that no query sees and of queries that see none
+ * as zeros.  D 64 or 128.  The same bits on every call (no atomics).  No output may overlap another tensor of the call. */
+size_t mi355_sage_window_bwd_workspace_bytes(int B, int Hq, int Hk, int N_q, int N_kv, int D, int left, int right, int sinks);
+int mi355_sage_sdpa_window_bwd(
+    const void* Q, const void* K, const void* V, const void* O, const void* dO, const void* Stats, void* dQ, void* dK, void* dV,
+    int B, int Hq, int Hk, int N_q, int N_kv, int D, int type, float scale,
+    const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides, const int64_t* do_strides,
+    const int64_t* dq_strides, const int64_t* dk_strides, const int64_t* dv_strides,
+    int64_t q_offset_elems, int64_t k_offset_elems, int64_t v_offset_elems, int64_t o_offset_elems, int64_t do_offset_elems,
+    int64_t stats_offset_elems, int64_t dq_offset_elems, int64_t dk_offset_elems, int64_t dv_offset_elems,
+    int left, int right, int sinks, const void* kv_lens, int q_start, void* stream, void* workspace, size_t workspace_bytes);
+
 /* Library identification: "mi355_sage <version> gfx950". */
 const char* mi355_sage_version(void);
 

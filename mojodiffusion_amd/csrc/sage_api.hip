@@ -1325,4 +1325,65 @@ int mi355_sage_sdpa_window_decode(const void* Q, const void* K, const void* V, v
                           a, stream, workspace, workspace_bytes);
 }
 
+struct WindowBwdCarve { size_t lse2, delta, part, total; };
+static WindowBwdCarve window_bwd_carve(WindowBwdArgs* a) {
+    window_bwd_plan(a);
+    a->sq_pad = (int)pad_to(a->w.Sq, 64);
+    const size_t rows = (size_t)a->w.B * a->w.Hk * a->w.g * a->sq_pad * sizeof(float);
+    WindowBwdCarve c{};
+    c.delta = align_up(rows);
+    c.part = c.delta + align_up(rows);
+    c.total = c.part + align_up((size_t)window_bwd_parts(*a) * 2 * 128 * a->w.D * sizeof(float));
+    return c;
+}
+
+size_t mi355_sage_window_bwd_workspace_bytes(int B, int Hq, int Hk, int N_q, int N_kv, int D, int left, int right, int sinks) {
+    WindowBwdArgs a{};
+    if (window_dims("window backward", B, Hq, Hk, N_q, N_kv, D, MI355_SAGE_BF16, 1.0f, left, right, sinks, 0, &a.w) || !bwd_dims_ok(D)) return 0;
+    return window_bwd_carve(&a).total;
+}
+
+int mi355_sage_sdpa_window_bwd(const void* Q, const void* K, const void* V, const void* O, const void* dO, const void* Stats, void* dQ, void* dK, void* dV,
+                               int B, int Hq, int Hk, int N_q, int N_kv, int D, int type, float scale, const int64_t* q_strides, const int64_t* k_strides,
+                               const int64_t* v_strides, const int64_t* o_strides, const int64_t* do_strides, const int64_t* dq_strides,
+                               const int64_t* dk_strides, const int64_t* dv_strides, int64_t q_off, int64_t k_off, int64_t v_off, int64_t o_off,
+                               int64_t do_off, int64_t stats_off, int64_t dq_off, int64_t dk_off, int64_t dv_off, int left, int right, int sinks,
+                               const void* kv_lens, int q_start, void* stream, void* workspace, size_t workspace_bytes) {
+    if (!Q || !K || !V || !O || !dO || !Stats || !dQ || !dK || !dV) return MI355_SAGE_EINVAL;
+    if (!q_strides || !k_strides || !v_strides || !o_strides || !do_strides || !dq_strides || !dk_strides || !dv_strides) return MI355_SAGE_EINVAL;
+    WindowBwdArgs a{};
+    int rc = window_dims("window backward", B, Hq, Hk, N_q, N_kv, D, type, scale, left, right, sinks, q_start, &a.w);
+    if (rc) return rc;
+    if (!bwd_dims_ok(D)) { SAGE_LOG("window backward: head dim %d is not supported (64 or 128)", D); return MI355_SAGE_EUNSUPPORTED; }
+    if ((rc = check_view("Q", Q, q_strides, q_off)) || (rc = check_view("K", K, k_strides, k_off)) || (rc = check_view("V", V, v_strides, v_off)) ||
+        (rc = check_view("O", O, o_strides, o_off)) || (rc = check_view("dO", dO, do_strides, do_off)) || (rc = check_view("dQ", dQ, dq_strides, dq_off)) ||
+        (rc = check_view("dK", dK, dk_strides, dk_off)) || (rc = check_view("dV", dV, dv_strides, dv_off)))
+        return rc;
+    const int64_t rows = 256 / a.w.g + 66;               // (a block of rows, or a tile of 64)
+    if ((rc = window_span("Q", q_strides, rows, a.w.g, D)) || (rc = window_span("dO", do_strides, rows, a.w.g, D)) ||
+        (rc = window_span("K", k_strides, 128, 1, D)) || (rc = window_span("V", v_strides, 128, 1, D)))
+        return rc;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    std::lock_guard<std::mutex> together(launch_mutex(st));
+    const WindowBwdCarve c = window_bwd_carve(&a);
+    if ((rc = call_workspace("window backward", c.total, st, &workspace, workspace_bytes))) return rc;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    a.lse2 = reinterpret_cast<float*>(ws);
+    a.ndelta = reinterpret_cast<float*>(ws + c.delta);
+    a.part = reinterpret_cast<float*>(ws + c.part);
+    const View q = make_view(Q, q_strides, q_off), k = make_view(K, k_strides, k_off), v = make_view(V, v_strides, v_off), d = make_view(dO, do_strides, do_off);
+    a.w.q = q.p; a.w.q_sb = q.sb; a.w.q_sh = q.sh; a.w.q_sn = q.sn;
+    a.w.k = k.p; a.w.k_sb = k.sb; a.w.k_sh = k.sh; a.w.k_sn = k.sn;
+    a.w.v = v.p; a.w.v_sb = v.sb; a.w.v_sh = v.sh; a.w.v_sn = v.sn;
+    a.w.o = const_cast<uint16_t*>(static_cast<const uint16_t*>(O)) + o_off; a.w.o_sb = o_strides[0]; a.w.o_sh = o_strides[1]; a.w.o_sn = o_strides[2];
+    a.w.stats = const_cast<float*>(static_cast<const float*>(Stats)) + stats_off;
+    a.w.lens = static_cast<const int32_t*>(kv_lens);
+    a.dout = d.p; a.do_sb = d.sb; a.do_sh = d.sh; a.do_sn = d.sn;
+    a.dq = static_cast<uint16_t*>(dQ) + dq_off; a.dq_sb = dq_strides[0]; a.dq_sh = dq_strides[1]; a.dq_sn = dq_strides[2];
+    a.dk = static_cast<uint16_t*>(dK) + dk_off; a.dk_sb = dk_strides[0]; a.dk_sh = dk_strides[1]; a.dk_sn = dk_strides[2];
+    a.dv = static_cast<uint16_t*>(dV) + dv_off; a.dv_sb = dv_strides[0]; a.dv_sh = dv_strides[1]; a.dv_sn = dv_strides[2];
+    SAGE_HIP(launch_window_bwd(a, st));
+    return MI355_SAGE_OK;
+}
+
 }  // extern "C"

@@ -64,4 +64,22 @@ bool window_grid_ok(const WindowArgs& a, const WindowPlan& p);
 size_t window_part_bytes(const WindowArgs& a, const WindowPlan& p);
 hipError_t launch_window(const WindowArgs& a, const WindowPlan& p, hipStream_t st);
 
+// Its gradient.  w: the forward's arguments (o, stats as it wrote them).
+struct WindowBwdArgs {
+    WindowArgs w;
+    const uint16_t* dout;
+    uint16_t *dq, *dk, *dv;
+    int64_t do_sb, do_sh, do_sn, dq_sb, dq_sh, dq_sn, dk_sb, dk_sh, dk_sn, dv_sb, dv_sh, dv_sn;
+    // workspace
+    float *lse2, *ndelta;                        // [B, Hk * g, sq_pad]: Stats * log2(e) (+inf: no such row, or nothing seen), -rowsum(dO * O)
+    int sq_pad;                                  // Sq rounded up to a multiple of 64
+    // How a key block's (head, query tile) pairs are dealt: `sink_blocks` blocks of 128 keys with sinks in them go to sink_chunks workgroups
+    // each, the others to chunks, of chunk_tiles pairs.
+    int sink_blocks, sink_chunks, chunks, chunk_tiles;
+    float* part;                                 // [workgroup, 2, 128, D] fp32 parts of dK and dV of blocks with several workgroups
+};
+void window_bwd_plan(WindowBwdArgs* a);          // fills in the four above from a->w
+int64_t window_bwd_parts(const WindowBwdArgs& a);        // workgroups that leave parts
+hipError_t launch_window_bwd(const WindowBwdArgs& a, hipStream_t st);
+
 }  // namespace sage

@@ -14,81 +14,13 @@
 // none of its rows sees.  Rows of a tile that no row of the workgroup sees are not read at all (another key's row stands
 // in), so whatever lies there, or behind a sequence's end, cannot reach a result.
 #include "sage_grid.h"
-#include "sage_tile.h"
-#include "sage_window.h"
+#include "sage_window_common.h"
 
 #include <algorithm>
 
 namespace sage {
 
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v2hf __attribute__((ext_vector_type(2)));
-
-template <int T> __device__ __forceinline__ v16f product(v4i a, v4i b, v16f c) {
-    if constexpr (T == kBF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
-}
-template <int T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
-    if constexpr (T == kBF16) return pack_bf16(a, b);
-    const v2f f = {a, b};
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, v2hf));
-}
-// the other half-wave's value of the same column
-__device__ __forceinline__ float max_halves(float x) {
-    const v2u r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
-}
-__device__ __forceinline__ float sum_halves(float x) {
-    const v2u r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(r.x) + __uint_as_float(r.y);
-}
-
-__device__ __forceinline__ int sequence_len(const WindowArgs& a, int b) { return a.lens ? max(0, min(a.lens[b], a.Skv)) : a.Skv; }
-__device__ __forceinline__ int first_position(const WindowArgs& a, int b, int len) {
-    if (a.at_end) return len - a.Sq;
-    return a.starts ? max(-kWindowStart, min(a.starts[b], kWindowStart)) : a.start;
-}
-
-// The key tiles (KT keys each) that rows at positions p_lo .. p_hi see: `first` tiles with the sinks, then those from `next` on, n in all.
-// Keys [0, s_end) and [lo, hi] are the ones that some row sees.
-struct Span {
-    int lo, hi, s_end, first, next, n;
-    __device__ int tile(int t) const { return t < first ? t : next + t - first; }
-};
-template <int KT> __device__ __forceinline__ Span key_span(const WindowArgs& a, int p_lo, int p_hi, int len) {
-    Span s;
-    s.hi = min(p_hi + a.right, len - 1);
-    s.lo = max(p_lo - a.left, 0);
-    s.s_end = max(min(a.sinks, s.hi + 1), 0);
-    s.first = (s.s_end + KT - 1) / KT;
-    s.next = max(s.lo / KT, s.first);
-    s.n = s.first + (s.hi >= s.lo ? max(s.hi / KT + 1 - s.next, 0) : 0);
-    return s;
-}
-// The key whose row is copied for row j of the tile that starts at j0: j itself where some row of the workgroup sees it, else a neighbour that one sees.
-template <int KT> __device__ __forceinline__ int copied_key(const Span& s, int j0, int j) {
-    const int gap = s.lo <= min(j0 + KT - 1, s.hi) ? s.lo : s.s_end - 1;
-    if (j >= s.s_end && j < s.lo) j = gap;
-    return min(j, s.hi);
-}
-
-// Where a lane's fragments lie in a tile: along the channels by k-step, across them by 32-channel block (rows 0-7 and 8-15; 16-row blocks are
-// + 32 * D bytes).  The XOR of the layout reaches over 16 chunks, so channels from 128 on lie 256 bytes further.
-template <int D> struct Fragments {
-    int nat[D > 128 ? 8 : D / 16], tr[D > 128 ? 4 : D / 32][2];
-    __device__ explicit Fragments(int lane) {
-        constexpr int CPR = D / 8;
-#pragma unroll
-        for (int s = 0; s < (D > 128 ? 8 : D / 16); s++) nat[s] = nat_off<CPR>(lane & 31, s * 2 + (lane >> 5));
-#pragma unroll
-        for (int d = 0; d < (D > 128 ? 4 : D / 32); d++) tr[d][0] = tr_frag_off<CPR>(lane, 0, d), tr[d][1] = tr_frag_off<CPR>(lane, 8, d);
-    }
-    __device__ v4i along(const uint8_t* tile, int s) const { return *reinterpret_cast<const v4i*>(tile + nat[s & 7] + (s >> 3) * 256); }
-    __device__ v4i across(const uint8_t* rows, int d) const { return tr_read(rows + tr[d & 3][0] + (d >> 2) * 256, rows + tr[d & 3][1] + (d >> 2) * 256); }
-};
 
 // What a lane keeps of its row, and the tile's part in it.
 template <int D> struct RowState {
@@ -103,12 +35,11 @@ template <int D> struct RowState {
         sum = 0.0f;
     }
 };
-struct RowMask { int lo, hi, sinks; };           // keys lo .. hi and [0, sinks) up to hi
-
 template <int T, int D, int KT, bool MASKED>
-__device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 16], const uint8_t* kt, const uint8_t* vt, const Fragments<D>& fr,
+__device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 16], const uint8_t* kt, const uint8_t* vt, const Fragments<D>& kept,
                                             int j0, const RowMask& m, float c, int half) {
     constexpr int KS = D / 16, DB = D / 32, NB = KT / 32;
+    const Fragments<D> fr = kept.fresh();
     v16f s[NB];
 #pragma unroll
     for (int blk = 0; blk < NB; blk++) {
@@ -118,15 +49,13 @@ __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 
         for (int ks = 0; ks < KS; ks++)
             s[blk] = product<T>(fr.along(kt + blk * 64 * D, ks), q[ks], s[blk]);
     }
+    const RowMask rel = m.from(j0 + half * 4);
     float top = -INFINITY;
 #pragma unroll
     for (int blk = 0; blk < NB; blk++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            if constexpr (MASKED) {
-                const int j = j0 + blk * 32 + (i >> 2) * 8 + half * 4 + (i & 3);
-                if (!(j <= m.hi && (j >= m.lo || j < m.sinks))) s[blk][i] = -INFINITY;
-            }
+            if (MASKED && !rel.sees(blk * 32 + (i >> 2) * 8 + (i & 3))) s[blk][i] = -INFINITY;
             top = fmaxf(top, s[blk][i]);
         }
     top = max_halves(top) * c;
@@ -166,49 +95,19 @@ __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 
         }
 }
 
-// A wave's view of a tile: nothing of it, all of it, or some.
-enum class Seen { kNone, kAll, kSome };
-template <int KT> __device__ __forceinline__ Seen seen(const WindowArgs& a, int p_lo, int p_hi, int len, int j0) {
-    const int j1 = j0 + KT - 1;
-    if (j0 > min(p_hi + a.right, len - 1) || (j1 < p_lo - a.left && j0 >= a.sinks)) return Seen::kNone;
-    return j1 <= min(p_lo + a.right, len - 1) && (j0 >= p_hi - a.left || j1 < a.sinks) ? Seen::kAll : Seen::kSome;
-}
-
-// 32 rows x0 .. of (query, head) pairs -> LDS at dst; rows past the last repeat it.  `base` is the first row's query.
-template <int D> __device__ __forceinline__ void query_rows_in(const WindowArgs& a, const uint16_t* base, int i_base, int x0, uint32_t dst, int lane) {
-    constexpr int CPR = D / 8, RPI = 64 / CPR;
-    const int last = a.Sq * a.g - 1;
-#pragma unroll
-    for (int n = 0; n < 32 / RPI; n++) {
-        const int r = n * RPI + lane / CPR, x = min(x0 + r, last), i = x / a.g;
-        const uint32_t off = ((uint32_t)(i - i_base) * (uint32_t)a.q_sn + (uint32_t)(x - i * a.g) * (uint32_t)a.q_sh) * 2u;
-        dma16(base, off + nat_pos<CPR>(r, lane % CPR) * 16, __builtin_amdgcn_readfirstlane(dst + n * 1024));
-    }
-}
 // The wave's finished rows: registers -> LDS (64 * D bytes at os) -> O, and the statistics.
 template <int T, int D>
 __device__ __forceinline__ void finish_rows(const WindowArgs& a, const RowState<D>& st, uint8_t* os, int b, int kvh, int x0, int lane) {
-    constexpr int CPR = D / 8, RPI = 64 / CPR, DB = D / 32;
-    const int l32 = lane & 31, half = lane >> 5, rows = a.Sq * a.g;
+    const int rows = a.Sq * a.g, x = x0 + (lane & 31);
     const float sum = sum_halves(st.sum);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;                     // (a row that sees no key: zeros)
 #pragma unroll
-    for (int d = 0; d < DB; d++)
-#pragma unroll
-        for (int g = 0; g < 4; g++)
-            *reinterpret_cast<u32x2*>(os + nat_off<CPR>(l32, d * 4 + g) + half * 8) =
-                u32x2{pack2<T>(st.acc[d][g * 4] * inv, st.acc[d][g * 4 + 1] * inv), pack2<T>(st.acc[d][g * 4 + 2] * inv, st.acc[d][g * 4 + 3] * inv)};
-    if (a.stats != nullptr && half == 0 && x0 + l32 < rows) {
-        const int x = x0 + l32, i = x / a.g;
+    for (int d = 0; d < D / 32; d++) row_put<T, D>(os, st.acc[d], d, inv, lane);
+    if (a.stats != nullptr && lane < 32 && x < rows) {
+        const int i = x / a.g;
         a.stats[((int64_t)b * a.Hk * a.g + kvh * a.g + (x - i * a.g)) * a.Sq + i] = sum == 0.0f ? -INFINITY : (st.ref + __builtin_amdgcn_logf(sum)) * kLn2;
     }
-    uint16_t* o = a.o + b * a.o_sb + (int64_t)kvh * a.g * a.o_sh;
-#pragma unroll
-    for (int n = 0; n < 32 / RPI; n++) {
-        const int r = n * RPI + lane / CPR, x = x0 + r, i = x / a.g;
-        const u32x4 w = *reinterpret_cast<const u32x4*>(os + nat_off<CPR>(r, lane % CPR));
-        if (x < rows) *reinterpret_cast<u32x4*>(o + i * a.o_sn + (int64_t)(x - i * a.g) * a.o_sh + (lane % CPR) * 8) = w;
-    }
+    query_rows_out<D>(a, os, a.o + b * a.o_sb + (int64_t)kvh * a.g * a.o_sh, a.o_sn, a.o_sh, x0, lane);
 }
 
 template <int D, int NW> struct WindowLds {
@@ -220,8 +119,7 @@ template <int D, int NW> struct WindowLds {
 template <int T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void window_kernel(WindowArgs a) {
     using L = WindowLds<D, NW>;
-    constexpr int KT = L::KT, CPR = D / 8, RPW = L::TILE / 1024 / NW, KS = D / 16;
-    static_assert(L::TILE / 1024 % NW == 0, "tile copies must divide over the waves");
+    constexpr int KT = L::KT, RPW = TilePieces<D, KT, NW>::N, KS = D / 16;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
     const int rows = a.Sq * a.g, blocks = (rows + NW * 32 - 1) / (NW * 32);
     const int item = xcd_item((int)blockIdx.x, a.B * a.Hk * blocks);
@@ -238,13 +136,7 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void window_kernel(Window
     const int p = p0 + min(x0 + (lane & 31), rows - 1) / a.g;
     const RowMask mask = {p - a.left, min(p + a.right, len - 1), a.sinks};
 
-    int nat_row[RPW], nat_col[RPW];
-#pragma unroll
-    for (int i = 0; i < RPW; i++) {
-        const int P = (i * NW + wave) * 64 + lane;
-        nat_row[i] = P / CPR;
-        nat_col[i] = nat_pos<CPR>(P / CPR, P % CPR) * 16;
-    }
+    const TilePieces<D, KT, NW> pieces(wave, lane);
     const uint32_t lds = lds_addr(smem);
     const uint16_t* kh = a.k + b * a.k_sb + kvh * a.k_sh;
     const uint16_t* vh = a.v + b * a.v_sb + kvh * a.v_sh;
@@ -254,16 +146,16 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void window_kernel(Window
         const uint16_t *kb = kh + (int64_t)j0 * a.k_sn, *vb = vh + (int64_t)j0 * a.v_sn;
 #pragma unroll
         for (int i = 0; i < RPW; i++) {
-            const uint32_t row = (uint32_t)(copied_key<KT>(span, j0, j0 + nat_row[i]) - j0);
+            const uint32_t row = (uint32_t)(copied_key<KT>(span, j0, j0 + pieces.row(i)) - j0);
             const uint32_t dst = lds + slot * L::SLOT + (i * NW + wave) * 1024;
-            dma16(kb, row * ks_b + nat_col[i], __builtin_amdgcn_readfirstlane(dst));
-            dma16(vb, row * vs_b + nat_col[i], __builtin_amdgcn_readfirstlane(dst + L::TILE));
+            dma16(kb, row * ks_b + pieces.col(i, lane), __builtin_amdgcn_readfirstlane(dst));
+            dma16(vb, row * vs_b + pieces.col(i, lane), __builtin_amdgcn_readfirstlane(dst + L::TILE));
         }
     };
 
     v4i q[KS];
     const Fragments<D> fr(lane);
-    query_rows_in<D>(a, a.q + b * a.q_sb + (int64_t)kvh * a.g * a.q_sh + (int64_t)i_lo * a.q_sn, i_lo, x0, lds + L::SLOT + wave * 64 * D, lane);
+    query_rows_in<D>(a, a.q + b * a.q_sb + (int64_t)kvh * a.g * a.q_sh + (int64_t)i_lo * a.q_sn, a.q_sn, a.q_sh, i_lo, x0, lds + L::SLOT + wave * 64 * D, lane);
     if (span.n > 0) copy_tile(0, 0);
     dma_wait<0>();
 #pragma unroll
@@ -346,7 +238,7 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
 
     v4i q[KS];
     const Fragments<D> fr(lane);
-    query_rows_in<D>(a, a.q + b * a.q_sb + (int64_t)kvh * a.g * a.q_sh + (int64_t)i_lo * a.q_sn, i_lo, x0, ring, lane);
+    query_rows_in<D>(a, a.q + b * a.q_sb + (int64_t)kvh * a.g * a.q_sh + (int64_t)i_lo * a.q_sn, a.q_sn, a.q_sh, i_lo, x0, ring, lane);
     dma_wait<0>();
 #pragma unroll
     for (int s = 0; s < KS; s++) q[s] = fr.along(own, s);

@@ -5,7 +5,7 @@ import torch
 
 from mojodiffusion_amd import attention_window as W
 from mojodiffusion_amd.attention_sage import Error
-from window_reference import check_forward, forward
+from window_reference import backward, check_backward, check_forward, forward
 
 BF, FP = torch.bfloat16, torch.float16
 
@@ -210,6 +210,123 @@ def test_streams_graphs_and_repeats():
             assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1]), i
 
 
+def grads(q, k, v, d, *window, lens=None, first=0):
+    fwd = W.sdpa_window_train_fwd(q, k, v, *window, kv_lens=lens, q_start=first)
+    g = W.sdpa_window_backward(fwd, d)
+    return fwd, (g.d_q, g.d_k, g.d_v)
+
+
+# (the forward's cases that a backward takes, sinks that many later blocks of queries see with them, windows a little over whole tiles, and key blocks
+# shared by several workgroups: few heads and long windows)
+BACKWARD = [c for c in CASES if c[5] != 256 and not isinstance(c[11], list)] + [
+    (1, 1500, 1500, 2, 1, 64, BF, 100, 0, 4, None, 0),
+    (1, 1500, 1500, 2, 1, 128, BF, 2, 0, 130, [1490], 0),
+    (2, 900, 900, 3, 3, 64, FP, 1, 1, 1, [900, 450], 0),
+    (1, 1300, 1300, 1, 1, 128, FP, -1, 0, 0, None, 0),
+    (1, 700, 1300, 4, 2, 64, BF, -1, 3, 0, [1300], 600),
+    (1, 260, 260, 2, 2, 128, BF, 2, 0, 0, None, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Sq,Skv,Hq,Hk,D,dtype,left,right,sinks,lens,first", BACKWARD)
+def test_backward(B, Sq, Skv, Hq, Hk, D, dtype, left, right, sinks, lens, first):
+    q, k, v = tensors(B, Sq, Skv, Hq, Hk, D, dtype, Sq + Skv)
+    d = torch.randn(q.shape, generator=torch.Generator().manual_seed(4)).to(dtype)
+    n = [Skv] * B if lens is None else lens
+    ref = forward(q, k, v, D ** -0.5, left, right, sinks, n, [first] * B)
+    want = backward(q, k, v, d, D ** -0.5, ref, Hq // Hk)
+    kd, vd = k.cuda(), v.cuda()
+    for b in range(B):
+        kd[b, n[b]:], vd[b, n[b]:] = float("nan"), float("inf")
+    lens = None if lens is None else torch.tensor(lens, dtype=torch.int32).cuda()
+    args = (q.cuda(), kd, vd, d.cuda(), D ** -0.5, left, right, sinks)
+    fwd, got = grads(*args, lens=lens, first=first)
+    check_backward(got, want)
+    for x, y in zip(got, grads(*args, lens=lens, first=first)[1]):
+        assert torch.equal(x, y)
+
+
+def test_the_gradient_formulas_against_central_differences():
+    B, Sq, Skv, Hq, Hk, D = 1, 9, 11, 4, 2, 8
+    g = torch.Generator().manual_seed(6)
+    q, k, v, d = (torch.randn(s, generator=g, dtype=torch.float64) for s in ((B, Sq, Hq, D), (B, Skv, Hk, D), (B, Skv, Hk, D), (B, Sq, Hq, D)))
+    args = (0.5, 3, 1, 2, [10], [1])
+    f = lambda *t: float((forward(*t, *args)[0] * d).sum())
+    got = backward(q, k, v, d, 0.5, forward(q, k, v, *args), Hq // Hk)
+    for which in range(3):
+        for i in (0, 5, 37, 70, 133):
+            t = [q.clone(), k.clone(), v.clone()]
+            t[which].view(-1)[i] += 1e-5
+            up = f(*t)
+            t[which].view(-1)[i] -= 2e-5
+            assert abs((up - f(*t)) / 2e-5 - float(got[which][0].reshape(-1)[i])) < 1e-8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_backward_of_keys_that_no_query_sees(D):
+    """Stale keys between the sinks and the window, and behind it, whatever they hold: zeros for them, the same bits for the rest."""
+    B, Sq, Skv, H = 1, 200, 900, 2
+    q, k, v = (t.cuda() for t in tensors(B, Sq, Skv, H, H, D, BF, 3))
+    d = torch.randn(q.shape, device="cuda").to(BF)
+    window = (0.1, 50, 5, 70)
+    want = grads(q, k, v, d, *window, first=500)[1]
+    k2, v2 = k.clone(), v.clone()
+    for t in (k2, v2):
+        t[:, 70:450], t[:, 705:] = float("nan"), float("inf")
+    got = grads(q, k2, v2, d, *window, first=500)[1]
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+    assert (want[1][:, 70:450] == 0).all() and (want[2][:, 705:] == 0).all()
+
+
+@pytest.mark.gpu
+def test_backward_layouts():
+    """Parts of a joint projection and an upstream gradient of other strides, as autograd hands them over."""
+    B, S, Hq, Hk, D = 2, 300, 4, 2, 128
+    joint = torch.randn((B, S, Hq + 2 * Hk, D), generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    q, k, v = joint[:, :, :Hq], joint[:, :, Hq:Hq + Hk], joint[:, :, Hq + Hk:]
+    d = torch.randn(q.shape, device="cuda").to(BF)
+    want = grads(q.contiguous(), k.contiguous(), v.contiguous(), d, 0.1, 40, 0, 4)[1]
+    for g in (d.transpose(1, 2).contiguous().transpose(1, 2), torch.empty(d.numel() + 1, dtype=BF, device="cuda")[1:].view(d.shape).copy_(d)):
+        for x, y in zip(grads(q, k, v, g, 0.1, 40, 0, 4)[1], want):
+            assert torch.equal(x, y)
+    one = d[:, :, :, :1].expand(d.shape)                               # (a broadcast gradient: rows are not dense)
+    for x, y in zip(grads(q, k, v, one, 0.1, 40)[1], grads(q, k, v, one.contiguous(), 0.1, 40)[1]):
+        assert torch.equal(x, y)
+    leaf = joint.clone().requires_grad_()
+    att = W.record_sdpa_window(leaf[:, :, :Hq], leaf[:, :, Hq:Hq + Hk], leaf[:, :, Hq + Hk:], 0.1, 40, 0, 4)
+    (g,) = torch.autograd.grad(att, leaf, d)
+    for x, y in zip((g[:, :, :Hq], g[:, :, Hq:Hq + Hk], g[:, :, Hq + Hk:]), want):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_backward_captured():
+    """A training step in a graph, replayed with other inputs and lengths and the program's own work in between."""
+    B, S, H, D = 2, 640, 2, 64
+    q, k, v = (t.cuda() for t in tensors(B, S, S, H, H, D, BF, 8))
+    d = torch.randn(q.shape, device="cuda").to(BF)
+    lens = torch.tensor([640, 300], dtype=torch.int32).cuda()
+    step = lambda: grads(q, k, v, d, 0.1, 80, 0, 3, lens=lens)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        fwd, out = step()
+    for i in range(4):
+        q.copy_(torch.randn(q.shape, device="cuda"))
+        lens.copy_(torch.tensor([640 - i, 77 * i], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, eager = step()
+        torch.cuda.synchronize()
+        assert torch.equal(fwd.o, want.o) and torch.equal(fwd.stats, want.stats)
+        for x, y in zip(out, eager):
+            assert torch.equal(x, y), i
+
+
 def test_refusals():
     q, k = torch.zeros((2, 4, 4, 64), dtype=BF), torch.zeros((2, 6, 2, 64), dtype=BF)
     lens = torch.tensor([6, 6])
@@ -229,6 +346,11 @@ def test_refusals():
                          (dict(), "must live on the GPU")):
         with pytest.raises(Error, match=text):
             W.sdpa_window_decode(**{**dec, **change})
+    fwd = W.SdpaWindowFwd(q, torch.zeros((2, 4, 4, 1)), q, k, k, 0.1, 3, 0, 0, None, 0)
+    for change, d, text in ((dict(), q.half(), "type of the forward"), (dict(), q[:, :3], "does not match"), (dict(stats=torch.zeros(3)), q, "stats must be"),
+                            (dict(q=q.repeat(1, 1, 1, 4), k=k.repeat(1, 1, 1, 4), v=k.repeat(1, 1, 1, 4)), q, "Dh=256"), (dict(), q, "must live on the GPU")):
+        with pytest.raises(Error, match=text):
+            W.sdpa_window_backward(W.SdpaWindowFwd(**{**fwd.__dict__, **change}), d)
 
 
 def test_c_refusals():
@@ -258,3 +380,15 @@ def test_c_refusals():
     assert L.mi355_sage_window_workspace_bytes(1, 4, 4, 8, 8192, 64, -1, 0, 0) > 1000
     assert L.mi355_sage_window_workspace_bytes(1, 4, 3, 8, 8192, 64, -1, 0, 0) == 0
     assert L.mi355_sage_sdpa_window_decode(A, A, A, A, 1, 4, 4, 1, 8, 64, 0, 0.1, st, st, st, st, 0, 0, 0, 0, 3, 0, None, None, None, 0) == -1
+    bwd = [A] * 9 + [1, 4, 4, 8, 8, 64, 0, 0.1] + [st] * 8 + [0] * 9 + [3, 0, 0, None, 0, None]
+    assert L.mi355_sage_sdpa_window_bwd(*bwd, A, 8) == -3
+    for at, value, code in ((0, None, -1), (8, None, -1), (17, None, -1), (14, 256, -2), (10, 5, -1), (15, 2, -2), (21, off_rows(S), -2), (24, S(0, 64, 256, 2), -2)):
+        args = list(bwd)
+        args[at] = value
+        assert L.mi355_sage_sdpa_window_bwd(*args, A, 1 << 30) == code, at
+    assert L.mi355_sage_window_bwd_workspace_bytes(1, 4, 4, 8, 8, 256, 3, 0, 0) == 0
+    assert L.mi355_sage_window_bwd_workspace_bytes(1, 4, 2, 8, 8, 64, 3, 0, 0) > 0
+
+
+def off_rows(S):
+    return S(0, 60, 256, 1)

@@ -54,3 +54,49 @@ def check_forward(o, stats, ref, dtype):
         empty = torch.isinf(L)
         assert torch.equal(torch.isinf(got), empty) and (got[empty] < 0).all()
         assert ((got - L).abs() <= E + n * 2.0 ** -24)[~empty].all()
+
+
+def backward(q, k, v, d, scale, ref, g):
+    """Gradients by the formulas and the sizes of their bounds, float64; ref: forward's result, g: query heads to a key head.
+
+    Bounds.  dS = P (dP - Delta).  P: recomputed from scores and a statistic that are off by E each (2 E relative), rounded to the type (u) for dV, handed on
+    with 11 bits (2^-10) and, as part of dS, rounded (u) for dQ and dK.  Delta is a product with the stored O, off by the forward's
+    bound: dDelta = sum |dO| bound(O).  dP and Delta are fp32 sums of D products (D 2^-24 of their sizes).  Every sum over rows or keys is fp32, and
+    the result is rounded (u); F: what fp16 loses below its normal range, 2^-25 for every P and dS."""
+    O, L, W, A, F, E = ref
+    dtype = q.dtype
+    u = torch.finfo(dtype).eps / 2
+    q, k, v, d = (t.double().cpu() for t in (q, k, v, d))
+    B, Sq, Hq, D = q.shape
+    n = max(Sq * g, k.shape[1])
+    dq, dk, dv = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    bq, bk, bv = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    e = E.transpose(1, 2).unsqueeze(-1)
+    bo = u * O.abs() + A * (1.01 * u + W.shape[3] * 2.0 ** -24 + 2.1 * e) + (F * 2.0 ** -25 if dtype == torch.float16 else 0)
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    for b in range(B):
+        for h in range(Hq):
+            w, ww = W[b, h], (W[b, h] > 0).double()
+            used = (ww.sum(0) > 0).view(-1, 1)
+            qh, dh = q[b, :, h], d[b, :, h]
+            kh, vh = k[b, :, h // g].masked_fill(~used, 0.0), v[b, :, h // g].masked_fill(~used, 0.0)
+            dp = dh @ vh.T
+            delta = (w * dp).sum(1, keepdim=True)
+            ds = w * (dp - delta)
+            dp_size = dh.abs() @ vh.abs().T + (dh.abs() * O[b, :, h].abs()).sum(1, keepdim=True)
+            d_delta = (dh.abs() * bo[b, :, h]).sum(1, keepdim=True) + D * 2.0 ** -24 * dp_size
+            p_err = (2.2 * E[b, h].view(-1, 1) + n * 2.0 ** -24) * w
+            ds_err = ds.abs() * (1.01 * u + 2.0 ** -10) + (dp - delta).abs() * (p_err + tiny) + 1.01 * (w + tiny) * d_delta + tiny * ww
+            dq[b, :, h] = scale * ds @ kh
+            bq[b, :, h] = scale * (ds_err + n * 2.0 ** -24 * ds.abs()) @ kh.abs()
+            dk[b, :, h // g] += scale * ds.T @ qh
+            bk[b, :, h // g] += scale * (ds_err + n * 2.0 ** -24 * ds.abs()).T @ qh.abs()
+            dv[b, :, h // g] += w.T @ dh
+            bv[b, :, h // g] += (w * (1.01 * u + n * 2.0 ** -24) + p_err + tiny * ww).T @ dh.abs()
+    return tuple((x, u * x.abs() + 1.01 * y + tiny) for x, y in ((dq, bq), (dk, bk), (dv, bv)))
+
+
+def check_backward(got, want):
+    for name, x, (ref, bound) in zip(("dQ", "dK", "dV"), got, want):
+        err = (x.double().cpu() - ref).abs()
+        assert torch.isfinite(x).all() and (err <= bound + 1e-30).all(), (name, float((err / (bound + 1e-30)).max()))
