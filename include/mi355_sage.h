@@ -501,12 +501,13 @@ int mi355_sage_qk_norm_rope_bwd(
  * that some query of a call sees must be finite.
  * Q, O [B,Hq,N_q,D], K, V [B,Hk,N_kv,D], Hq a multiple of Hk: query heads h Hq/Hk .. share key head h (no expanded copies).  type
  * MI355_SAGE_BF16 or _FP16 for all four; D 64, 128 or 256; scale > 0.  Stats (may be NULL): F32 [B,Hq,N_q] natural log-sum-exp.
+ * O_rest (may be NULL): what rounding to the type left of O, with O's type, strides and offset (O + O_rest is O to twice the bits), for the backward.
  * kv_lens, q_starts: int32 [B] on the device, or NULL; lengths outside [0, N_kv] are taken as the nearer bound.
  * Workspace: mi355_sage_window_workspace_bytes(...) bytes, 256-byte aligned, or NULL for the library's per-stream buffer (the rules of
  * mi355_sage_sdpa_bf16); the same bits on every call. */
 size_t mi355_sage_window_workspace_bytes(int B, int Hq, int Hk, int N_q, int N_kv, int D, int left, int right, int sinks);
 int mi355_sage_sdpa_window(
-    const void* Q, const void* K, const void* V, void* O, void* Stats,
+    const void* Q, const void* K, const void* V, void* O, void* O_rest, void* Stats,
     int B, int Hq, int Hk, int N_q, int N_kv, int D, int type, float scale,
     const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
     int64_t q_offset_elems, int64_t k_offset_elems, int64_t v_offset_elems, int64_t o_offset_elems, int64_t stats_offset_elems,
@@ -523,12 +524,13 @@ int mi355_sage_sdpa_window_decode(
     int64_t q_offset_elems, int64_t k_offset_elems, int64_t v_offset_elems, int64_t o_offset_elems,
     int left, int sinks, const void* kv_lens, void* stream, void* workspace, size_t workspace_bytes);
 
-/* Gradient of mi355_sage_sdpa_window: O and Stats as the forward wrote them, dO upstream -> dQ [B,Hq,N_q,D], dK, dV [B,Hk,N_kv,D] (of a
+/* Gradient of mi355_sage_sdpa_window: O, O_rest and Stats as the forward wrote them (O_rest may be NULL: rows that see few keys, whose O is large, then
+ * carry its rounding into dK: relative error 0.0032 for 0.0026 at a padded batch with sinks), dO upstream -> dQ [B,Hq,N_q,D], dK, dV [B,Hk,N_kv,D] (of a
  * shared key head: summed over its query heads), every row written, those of keys that no query sees and of queries that see none
  * as zeros.  D 64 or 128.  The same bits on every call (no atomics).  No output may overlap another tensor of the call. */
 size_t mi355_sage_window_bwd_workspace_bytes(int B, int Hq, int Hk, int N_q, int N_kv, int D, int left, int right, int sinks);
 int mi355_sage_sdpa_window_bwd(
-    const void* Q, const void* K, const void* V, const void* O, const void* dO, const void* Stats, void* dQ, void* dK, void* dV,
+    const void* Q, const void* K, const void* V, const void* O, const void* O_rest, const void* dO, const void* Stats, void* dQ, void* dK, void* dV,
     int B, int Hq, int Hk, int N_q, int N_kv, int D, int type, float scale,
     const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides, const int64_t* do_strides,
     const int64_t* dq_strides, const int64_t* dk_strides, const int64_t* dv_strides,

@@ -79,12 +79,12 @@ SIGNATURES = {
     "mi355_sage_qk_norm_rope_bwd": (_int, [_vp] * 8 + [_int] * 6 + [_i64p] * 6 + [_i64] * 6 + [_vp, _vp, _int, ctypes.c_float]
                                     + [_vp, _vp, _int, _int, _i64, _i64, _int] + [_vp, _i64, _int, _vp, _vp, ctypes.c_size_t]),
     "mi355_sage_window_workspace_bytes": (ctypes.c_size_t, [_int] * 9),
-    "mi355_sage_sdpa_window": (_int, [_vp] * 5 + [_int] * 7 + [ctypes.c_float] + [_i64p] * 4 + [_i64] * 5 + [_int] * 3
+    "mi355_sage_sdpa_window": (_int, [_vp] * 6 + [_int] * 7 + [ctypes.c_float] + [_i64p] * 4 + [_i64] * 5 + [_int] * 3
                                + [_vp, _vp, _int] + [_vp, _vp, ctypes.c_size_t]),
     "mi355_sage_sdpa_window_decode": (_int, [_vp] * 4 + [_int] * 7 + [ctypes.c_float] + [_i64p] * 4 + [_i64] * 4 + [_int] * 2
                                       + [_vp] + [_vp, _vp, ctypes.c_size_t]),
     "mi355_sage_window_bwd_workspace_bytes": (ctypes.c_size_t, [_int] * 9),
-    "mi355_sage_sdpa_window_bwd": (_int, [_vp] * 9 + [_int] * 7 + [ctypes.c_float] + [_i64p] * 8 + [_i64] * 9 + [_int] * 3
+    "mi355_sage_sdpa_window_bwd": (_int, [_vp] * 10 + [_int] * 7 + [ctypes.c_float] + [_i64p] * 8 + [_i64] * 9 + [_int] * 3
                                    + [_vp, _int] + [_vp, _vp, ctypes.c_size_t]),
     "mi355_sage_version": (ctypes.c_char_p, []),
 }

@@ -16,15 +16,17 @@ import torch
 
 from . import _lib
 from .attention_sage import Error, SdpaFlashGrads
-from .norm_rope import _rows, _scratch, _strides
+from .norm_rope import _rows, _rows_ok, _scratch, _strides
 
 _TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
 
 
 @dataclass
 class SdpaWindowFwd:
-    """What sdpa_window_train_fwd leaves for sdpa_window_backward; stats: F32 [B,H,S,1], the log-sum-exp of the visible scores."""
+    """What sdpa_window_train_fwd leaves for sdpa_window_backward; stats: F32 [B,H,S,1], the log-sum-exp of the visible scores; o_rest:
+    what rounding to o's type left of the output (the backward's row sums are taken with it)."""
     o: torch.Tensor
+    o_rest: torch.Tensor
     stats: torch.Tensor
     q: torch.Tensor
     k: torch.Tensor
@@ -88,7 +90,7 @@ def _bound(x):
     return min(int(x), 2 ** 30)
 
 
-def _forward(name, q, k, v, scale, left, right, sinks, kv_lens, q_start, want_stats):
+def _forward(name, q, k, v, scale, left, right, sinks, kv_lens, q_start, training):
     _check(name, q, k, v, scale, left, right, sinks)
     B, Sq, Hq, Dh = q.shape
     Skv, Hk = k.shape[1], k.shape[2]
@@ -100,15 +102,15 @@ def _forward(name, q, k, v, scale, left, right, sinks, kv_lens, q_start, want_st
     with torch.cuda.device(q.device):
         qi, ki, vi, lens, starts = _rows(q), _rows(k), _rows(v), _int32(kv_lens), _int32(starts)
         o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        stats = torch.empty((B, Hq, Sq, 1), dtype=torch.float32, device=q.device) if want_stats else None
+        rest, stats = (torch.empty_like(o), torch.empty((B, Hq, Sq, 1), dtype=torch.float32, device=q.device)) if training else (None, None)
         ws = _scratch(L.mi355_sage_window_workspace_bytes(B, Hq, Hk, Sq, Skv, Dh, _bound(left), _bound(right), _bound(sinks)), o)
         rc = L.mi355_sage_sdpa_window(
-            qi.data_ptr(), ki.data_ptr(), vi.data_ptr(), o.data_ptr(), _ptr(stats), B, Hq, Hk, Sq, Skv, Dh, _TYPES[q.dtype], float(scale),
+            qi.data_ptr(), ki.data_ptr(), vi.data_ptr(), o.data_ptr(), _ptr(rest), _ptr(stats), B, Hq, Hk, Sq, Skv, Dh, _TYPES[q.dtype], float(scale),
             _strides(qi), _strides(ki), _strides(vi), _strides(o), 0, 0, 0, 0, 0, _bound(left), _bound(right), _bound(sinks), _ptr(lens), _ptr(starts),
             start, torch.cuda.current_stream(q.device).cuda_stream, ws.data_ptr(), ws.numel())
     if rc != 0:
         raise Error("%s: shim rc=%d (B=%d Sq=%d Skv=%d Hq=%d Hk=%d Dh=%d)" % (name, rc, B, Sq, Skv, Hq, Hk, Dh))
-    return o, stats, qi, ki, vi, lens
+    return o, rest, stats, qi, ki, vi, lens
 
 
 def sdpa_window(q, k, v, scale, left, right=0, sinks=0, kv_lens=None, q_start=0):
@@ -152,36 +154,38 @@ def sdpa_window_train_fwd(q, k, v, scale, left, right=0, sinks=0, kv_lens=None, 
     name = "sdpa_window_train_fwd"
     if isinstance(q_start, torch.Tensor):
         raise Error("%s: q_start must be an int" % name)
-    o, stats, q, k, v, lens = _forward(name, q, k, v, scale, left, right, sinks, kv_lens, q_start, True)
-    return SdpaWindowFwd(o, stats, q, k, v, float(scale), left, right, sinks, lens, int(q_start))
+    o, rest, stats, q, k, v, lens = _forward(name, q, k, v, scale, left, right, sinks, kv_lens, q_start, True)
+    return SdpaWindowFwd(o, rest, stats, q, k, v, float(scale), left, right, sinks, lens, int(q_start))
 
 
 def sdpa_window_backward(fwd, d_out):
     """d_q [B,Sq,Hq,Dh], d_k, d_v [B,Skv,Hk,Dh] from a sdpa_window_train_fwd and the upstream gradient (Dh 64 or 128; the gradients of a
     shared key head are summed over its query heads; rows of padding and of keys that nothing sees are zeros)."""
     name = "sdpa_window_backward"
-    q, k, v, o, stats = fwd.q, fwd.k, fwd.v, fwd.o, fwd.stats
+    q, k, v, o, rest, stats = fwd.q, fwd.k, fwd.v, fwd.o, fwd.o_rest, fwd.stats
     _check(name, q, k, v, fwd.scale, fwd.left, fwd.right, fwd.sinks)
     if q.shape[3] == 256:
         raise Error("%s: Dh=256 is not supported by the backward kernels (64 or 128)" % name)
     if d_out.dtype != q.dtype:
         raise Error("%s: d_out must have the type of the forward output" % name)
-    if o.shape != q.shape or o.dtype != q.dtype or d_out.shape != q.shape:
+    if any(t.shape != q.shape or t.dtype != q.dtype for t in (o, rest, d_out)):
         raise Error("%s: o/d_out shape does not match q [B,S,H,Dh]" % name)
     B, Sq, Hq, Dh = q.shape
     Skv, Hk = k.shape[1], k.shape[2]
     if stats.dtype != torch.float32 or stats.numel() != B * Hq * Sq or not stats.is_contiguous():
         raise Error("%s: stats must be F32 [B,H,S,1]" % name)
     lens = _lens(name, "kv_lens", fwd.kv_lens, B)
-    _check_device(name, q, k, v, o, d_out, stats, lens)
+    _check_device(name, q, k, v, o, rest, d_out, stats, lens)
     L = _lib.lib()
     with torch.cuda.device(q.device):
-        q, k, v, o, d, lens = _rows(q), _rows(k), _rows(v), _rows(o), _rows(d_out), _int32(lens)
+        q, k, v, d, lens = _rows(q), _rows(k), _rows(v), _rows(d_out), _int32(lens)
+        if not _rows_ok(o) or o.stride() != rest.stride() or rest.data_ptr() % 16:
+            o, rest = o.clone(memory_format=torch.contiguous_format), rest.clone(memory_format=torch.contiguous_format)
         d_q = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         d_k, d_v = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2))
         ws = _scratch(L.mi355_sage_window_bwd_workspace_bytes(B, Hq, Hk, Sq, Skv, Dh, _bound(fwd.left), _bound(fwd.right), _bound(fwd.sinks)), d_q)
         rc = L.mi355_sage_sdpa_window_bwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), d.data_ptr(), stats.data_ptr(), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(),
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), rest.data_ptr(), d.data_ptr(), stats.data_ptr(), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(),
             B, Hq, Hk, Sq, Skv, Dh, _TYPES[q.dtype], fwd.scale, _strides(q), _strides(k), _strides(v), _strides(o), _strides(d), _strides(d_q),
             _strides(d_k), _strides(d_v), 0, 0, 0, 0, 0, 0, 0, 0, 0, _bound(fwd.left), _bound(fwd.right), _bound(fwd.sinks), _ptr(lens), fwd.q_start,
             torch.cuda.current_stream(q.device).cuda_stream, ws.data_ptr(), ws.numel())
@@ -196,15 +200,15 @@ class _SdpaWindowNode(torch.autograd.Function):
         if q.dim() == 4 and q.shape[3] == 256:
             raise Error("record_sdpa_window: Dh=256 is not supported by the backward kernels (64 or 128)")
         fwd = sdpa_window_train_fwd(q, k, v, scale, left, right, sinks, kv_lens, q_start)
-        ctx.save_for_backward(fwd.o, fwd.stats, fwd.q, fwd.k, fwd.v, fwd.kv_lens)
+        ctx.save_for_backward(fwd.o, fwd.o_rest, fwd.stats, fwd.q, fwd.k, fwd.v, fwd.kv_lens)
         ctx.window = (fwd.scale, left, right, sinks, fwd.q_start)
         return fwd.o
 
     @staticmethod
     def backward(ctx, g):
-        o, stats, q, k, v, lens = ctx.saved_tensors
+        o, rest, stats, q, k, v, lens = ctx.saved_tensors
         scale, left, right, sinks, q_start = ctx.window
-        grads = sdpa_window_backward(SdpaWindowFwd(o, stats, q, k, v, scale, left, right, sinks, lens, q_start), g.to(q.dtype))
+        grads = sdpa_window_backward(SdpaWindowFwd(o, rest, stats, q, k, v, scale, left, right, sinks, lens, q_start), g.to(q.dtype))
         return grads.d_q, grads.d_k, grads.d_v, None, None, None, None, None, None
 
 

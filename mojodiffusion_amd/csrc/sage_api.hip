@@ -1262,7 +1262,7 @@ static int window_span(const char* name, const int64_t* s, int64_t rows, int64_t
     }
     return 0;
 }
-static int window_forward(const char* name, const void* Q, const void* K, const void* V, void* O, void* Stats, const int64_t* qs, const int64_t* ks,
+static int window_forward(const char* name, const void* Q, const void* K, const void* V, void* O, void* O_rest, void* Stats, const int64_t* qs, const int64_t* ks,
                           const int64_t* vs, const int64_t* os, int64_t q_off, int64_t k_off, int64_t v_off, int64_t o_off, int64_t stats_off,
                           const void* kv_lens, const void* q_starts, WindowArgs& a, void* stream, void* workspace, size_t workspace_bytes) {
     if (!Q || !K || !V || !O || !qs || !ks || !vs || !os) return MI355_SAGE_EINVAL;
@@ -1275,6 +1275,8 @@ static int window_forward(const char* name, const void* Q, const void* K, const 
     a.q = q.p; a.q_sb = q.sb; a.q_sh = q.sh; a.q_sn = q.sn;
     a.k = k.p; a.k_sb = k.sb; a.k_sh = k.sh; a.k_sn = k.sn;
     a.v = v.p; a.v_sb = v.sb; a.v_sh = v.sh; a.v_sn = v.sn;
+    if (O_rest && (rc = check_view("O_rest", O_rest, os, o_off))) return rc;
+    a.rest = O_rest ? static_cast<uint16_t*>(O_rest) + o_off : nullptr;
     a.o = static_cast<uint16_t*>(O) + o_off; a.o_sb = os[0]; a.o_sh = os[1]; a.o_sn = os[2];
     a.lens = static_cast<const int32_t*>(kv_lens);
     a.starts = static_cast<const int32_t*>(q_starts);
@@ -1303,13 +1305,13 @@ size_t mi355_sage_window_workspace_bytes(int B, int Hq, int Hk, int N_q, int N_k
     return need ? need : kAlign;
 }
 
-int mi355_sage_sdpa_window(const void* Q, const void* K, const void* V, void* O, void* Stats, int B, int Hq, int Hk, int N_q, int N_kv, int D, int type,
+int mi355_sage_sdpa_window(const void* Q, const void* K, const void* V, void* O, void* O_rest, void* Stats, int B, int Hq, int Hk, int N_q, int N_kv, int D, int type,
                            float scale, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
                            int64_t q_off, int64_t k_off, int64_t v_off, int64_t o_off, int64_t stats_off, int left, int right, int sinks,
                            const void* kv_lens, const void* q_starts, int q_start, void* stream, void* workspace, size_t workspace_bytes) {
     WindowArgs a;
     if (int rc = window_dims("window", B, Hq, Hk, N_q, N_kv, D, type, scale, left, right, sinks, q_start, &a)) return rc;
-    return window_forward("window", Q, K, V, O, Stats, q_strides, k_strides, v_strides, o_strides, q_off, k_off, v_off, o_off, stats_off, kv_lens, q_starts,
+    return window_forward("window", Q, K, V, O, O_rest, Stats, q_strides, k_strides, v_strides, o_strides, q_off, k_off, v_off, o_off, stats_off, kv_lens, q_starts,
                           a, stream, workspace, workspace_bytes);
 }
 
@@ -1321,7 +1323,7 @@ int mi355_sage_sdpa_window_decode(const void* Q, const void* K, const void* V, v
     WindowArgs a;
     if (int rc = window_dims("window decode", B, Hq, Hk, N_q, N_kv, D, type, scale, left, 0, sinks, 0, &a)) return rc;
     a.at_end = 1;
-    return window_forward("window decode", Q, K, V, O, nullptr, q_strides, k_strides, v_strides, o_strides, q_off, k_off, v_off, o_off, 0, kv_lens, nullptr,
+    return window_forward("window decode", Q, K, V, O, nullptr, nullptr, q_strides, k_strides, v_strides, o_strides, q_off, k_off, v_off, o_off, 0, kv_lens, nullptr,
                           a, stream, workspace, workspace_bytes);
 }
 
@@ -1343,7 +1345,7 @@ size_t mi355_sage_window_bwd_workspace_bytes(int B, int Hq, int Hk, int N_q, int
     return window_bwd_carve(&a).total;
 }
 
-int mi355_sage_sdpa_window_bwd(const void* Q, const void* K, const void* V, const void* O, const void* dO, const void* Stats, void* dQ, void* dK, void* dV,
+int mi355_sage_sdpa_window_bwd(const void* Q, const void* K, const void* V, const void* O, const void* O_rest, const void* dO, const void* Stats, void* dQ, void* dK, void* dV,
                                int B, int Hq, int Hk, int N_q, int N_kv, int D, int type, float scale, const int64_t* q_strides, const int64_t* k_strides,
                                const int64_t* v_strides, const int64_t* o_strides, const int64_t* do_strides, const int64_t* dq_strides,
                                const int64_t* dk_strides, const int64_t* dv_strides, int64_t q_off, int64_t k_off, int64_t v_off, int64_t o_off,
@@ -1357,7 +1359,8 @@ int mi355_sage_sdpa_window_bwd(const void* Q, const void* K, const void* V, cons
     if (!bwd_dims_ok(D)) { SAGE_LOG("window backward: head dim %d is not supported (64 or 128)", D); return MI355_SAGE_EUNSUPPORTED; }
     if ((rc = check_view("Q", Q, q_strides, q_off)) || (rc = check_view("K", K, k_strides, k_off)) || (rc = check_view("V", V, v_strides, v_off)) ||
         (rc = check_view("O", O, o_strides, o_off)) || (rc = check_view("dO", dO, do_strides, do_off)) || (rc = check_view("dQ", dQ, dq_strides, dq_off)) ||
-        (rc = check_view("dK", dK, dk_strides, dk_off)) || (rc = check_view("dV", dV, dv_strides, dv_off)))
+        (rc = check_view("dK", dK, dk_strides, dk_off)) || (rc = check_view("dV", dV, dv_strides, dv_off)) ||
+        (O_rest && (rc = check_view("O_rest", O_rest, o_strides, o_off))))
         return rc;
     const int64_t rows = 256 / a.w.g + 66;               // (a block of rows, or a tile of 64)
     if ((rc = window_span("Q", q_strides, rows, a.w.g, D)) || (rc = window_span("dO", do_strides, rows, a.w.g, D)) ||
@@ -1376,6 +1379,7 @@ int mi355_sage_sdpa_window_bwd(const void* Q, const void* K, const void* V, cons
     a.w.k = k.p; a.w.k_sb = k.sb; a.w.k_sh = k.sh; a.w.k_sn = k.sn;
     a.w.v = v.p; a.w.v_sb = v.sb; a.w.v_sh = v.sh; a.w.v_sn = v.sn;
     a.w.o = const_cast<uint16_t*>(static_cast<const uint16_t*>(O)) + o_off; a.w.o_sb = o_strides[0]; a.w.o_sh = o_strides[1]; a.w.o_sn = o_strides[2];
+    a.w.rest = O_rest ? const_cast<uint16_t*>(static_cast<const uint16_t*>(O_rest)) + o_off : nullptr;
     a.w.stats = const_cast<float*>(static_cast<const float*>(Stats)) + stats_off;
     a.w.lens = static_cast<const int32_t*>(kv_lens);
     a.dout = d.p; a.do_sb = d.sb; a.do_sh = d.sh; a.do_sn = d.sn;

@@ -43,7 +43,7 @@ constexpr int kWindowFar = (1 << 30) - 1;        // left, right: no bound
 constexpr int kWindowStart = 1 << 29;            // positions are kept within this, so that sums with the above fit 32 bits
 struct WindowArgs {
     const uint16_t *q, *k, *v;
-    uint16_t* o;
+    uint16_t *o, *rest;                          // rest: what rounding left of O, in O's type and strides, or null
     int64_t q_sb, q_sh, q_sn, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn, o_sb, o_sh, o_sn;      // strides in elements
     int B, Hk, g, Sq, Skv, D, type;              // type: kBF16 or kF16
     int left, right, sinks;

@@ -35,7 +35,11 @@ template <int D> struct RowState {
         sum = 0.0f;
     }
 };
-template <int T, int D, int KT, bool MASKED>
+// MASKED: some row does not see all of the tile.  FINE: the weights enter as two operands, what rounding leaves of them in a second product: for workgroups of
+// at most kFineTiles tiles, whose rows average over too few keys for the roundings of their weights to fade (relative error of dQ, whose row sums are
+// taken from O, on a padded batch with sinks: 0.0027 without, 0.0024 with it; the products are a small part of what such a workgroup does).
+constexpr int kFineTiles = 2;
+template <int T, int D, int KT, bool MASKED, bool FINE>
 __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 16], const uint8_t* kt, const uint8_t* vt, const Fragments<D>& kept,
                                             int j0, const RowMask& m, float c, int half) {
     constexpr int KS = D / 16, DB = D / 32, NB = KT / 32;
@@ -72,7 +76,7 @@ __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 
             for (int i = 0; i < 16; i++) st.acc[d][i] *= f;
     }
     const float ref = MASKED && st.ref == -INFINITY ? 0.0f : st.ref;       // (no key so far: every weight is exp2(-inf))
-    uint32_t p[NB][8];
+    uint32_t p[NB][8], fine[FINE ? NB : 1][8];
     float part[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int blk = 0; blk < NB; blk++)
@@ -82,6 +86,7 @@ __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 
             part[0] += x;
             part[1] += y;
             p[blk][i >> 1] = pack2<T>(x, y);
+            if constexpr (FINE) fine[blk][i >> 1] = pack2<T>(rounded_off<T>(x), rounded_off<T>(y));
         }
     st.sum += part[0] + part[1];
 #pragma unroll
@@ -91,7 +96,12 @@ __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 
             const v4i pb = {(int)p[blk][j2 * 4], (int)p[blk][j2 * 4 + 1], (int)p[blk][j2 * 4 + 2], (int)p[blk][j2 * 4 + 3]};
             const uint8_t* rows = vt + (blk * 2 + j2) * 32 * D;
 #pragma unroll
-            for (int d = 0; d < DB; d++) st.acc[d] = product<T>(fr.across(rows, d), pb, st.acc[d]);
+            for (int d = 0; d < DB; d++) {
+                const v4i vf = fr.across(rows, d);
+                st.acc[d] = product<T>(vf, pb, st.acc[d]);
+                if constexpr (FINE)
+                    st.acc[d] = product<T>(vf, v4i{(int)fine[blk][j2 * 4], (int)fine[blk][j2 * 4 + 1], (int)fine[blk][j2 * 4 + 2], (int)fine[blk][j2 * 4 + 3]}, st.acc[d]);
+            }
         }
 }
 
@@ -107,7 +117,12 @@ __device__ __forceinline__ void finish_rows(const WindowArgs& a, const RowState<
         const int i = x / a.g;
         a.stats[((int64_t)b * a.Hk * a.g + kvh * a.g + (x - i * a.g)) * a.Sq + i] = sum == 0.0f ? -INFINITY : (st.ref + __builtin_amdgcn_logf(sum)) * kLn2;
     }
-    query_rows_out<D>(a, os, a.o + b * a.o_sb + (int64_t)kvh * a.g * a.o_sh, a.o_sn, a.o_sh, x0, lane);
+    const int64_t at = b * a.o_sb + (int64_t)kvh * a.g * a.o_sh;
+    query_rows_out<D>(a, os, a.o + at, a.o_sn, a.o_sh, x0, lane);
+    if (a.rest == nullptr) return;
+#pragma unroll
+    for (int d = 0; d < D / 32; d++) row_put<T, D, true>(os, st.acc[d], d, inv, lane);
+    query_rows_out<D>(a, os, a.rest + at, a.o_sn, a.o_sh, x0, lane);
 }
 
 template <int D, int NW> struct WindowLds {
@@ -177,12 +192,31 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void window_kernel(Window
         const int j0 = span.tile(t) * KT;
         const uint8_t* kt = smem + slot * L::SLOT;
         const Seen what = x0 < rows ? seen<KT>(a, wp_lo, wp_hi, len, j0) : Seen::kNone;
-        if (D <= 128 && what == Seen::kAll) attend_tile<T, D, KT, false>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
-        else if (what != Seen::kNone) attend_tile<T, D, KT, true>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
+        if (what == Seen::kNone) {
+        } else if (D <= 128 && span.n <= kFineTiles) attend_tile<T, D, KT, true, true>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
+        else if (D <= 128 && what == Seen::kAll) attend_tile<T, D, KT, false, false>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
+        else attend_tile<T, D, KT, true, false>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
         slot = slot == 2 ? 0 : slot + 1;
     }
     __syncthreads();                     // (no copy is in flight: the last tile's wait was for all of them)
     if (x0 < rows) finish_rows<T, D>(a, st, smem + wave * 64 * D, b, kvh, x0, lane);
+}
+
+// N neighbouring channels of a finished row, and what rounding left of them.
+template <int T, int N> __device__ __forceinline__ void store_row(const WindowArgs& a, int64_t at, const float (&y)[N]) {
+    auto put = [&](uint16_t* p, const float* x) {
+        if constexpr (N == 1) p[0] = (uint16_t)pack2<T>(x[0], 0.0f);
+        else if constexpr (N == 8) *reinterpret_cast<u32x4*>(p) = u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])};
+        else
+#pragma unroll
+            for (int e = 0; e < N; e += 2) *reinterpret_cast<uint32_t*>(p + e) = pack2<T>(x[e], x[e + 1]);
+    };
+    put(a.o + at, y);
+    if (a.rest == nullptr) return;
+    float r[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) r[e] = rounded_off<T>(y[e]);
+    put(a.rest + at, r);
 }
 
 // ---- few rows: the keys split over waves and workgroups ---------------------------------------------------
@@ -263,8 +297,9 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
         }
         const int j0 = span.tile(t) * KT;
         const uint8_t* kt = own + slot * L::SLOT;
-        if (D <= 128 && seen<KT>(a, p_lo, p_hi, len, j0) == Seen::kAll) attend_tile<T, D, KT, false>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
-        else attend_tile<T, D, KT, true>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
+        if (D <= 128 && span.n <= kFineTiles * 2) attend_tile<T, D, KT, true, true>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
+        else if (D <= 128 && seen<KT>(a, p_lo, p_hi, len, j0) == Seen::kAll) attend_tile<T, D, KT, false, false>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
+        else attend_tile<T, D, KT, true, false>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
         if (L::SLOTS == 2) slot ^= 1;
         else if (t + NW < t1) {
             reads_done();
@@ -300,7 +335,7 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
     const bool last = a.splits == 1;
     const float inv = last ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
     float* po = a.part + ((int64_t)item * a.splits + split) * 32 * D + r * D;
-    uint16_t* o = a.o + b * a.o_sb + ((int64_t)kvh * a.g + hg) * a.o_sh + i * a.o_sn;
+    const int64_t at = b * a.o_sb + ((int64_t)kvh * a.g + hg) * a.o_sh + i * a.o_sn;
 #pragma unroll
     for (int n = 0; n < D / 64; n++) {
         const int col = (n * 8 + (tid & 7)) * 8;
@@ -317,8 +352,9 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; e++) y[h * 4 + e] = sumv[e] * inv;
         }
-        if (last) *reinterpret_cast<u32x4*>(o + col) = u32x4{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7])};
-        else {
+        if (last) {
+            store_row<T, 8>(a, at + col, y);
+        } else {
             *reinterpret_cast<v4f*>(po + col) = v4f{y[0], y[1], y[2], y[3]};
             *reinterpret_cast<v4f*>(po + col + 4) = v4f{y[4], y[5], y[6], y[7]};
         }
@@ -356,12 +392,9 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     const int i = x / a.g, hg = x - i * a.g;
-    uint16_t* o = a.o + b * a.o_sb + ((int64_t)kvh * a.g + hg) * a.o_sh + i * a.o_sn + lane * N;
-    if constexpr (N == 1) o[0] = (uint16_t)pack2<T>(y[0] * inv, 0.0f);
-    else {
 #pragma unroll
-        for (int e = 0; e < N; e += 2) *reinterpret_cast<uint32_t*>(o + e) = pack2<T>(y[e] * inv, y[e + 1] * inv);
-    }
+    for (int e = 0; e < N; e++) y[e] *= inv;
+    store_row<T, N>(a, b * a.o_sb + ((int64_t)kvh * a.g + hg) * a.o_sh + i * a.o_sn + lane * N, y);
     if (a.stats != nullptr && lane == 0)
         a.stats[((int64_t)b * a.Hk * a.g + kvh * a.g + hg) * a.Sq + i] = sum == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(sum)) * kLn2;
 }

@@ -5,7 +5,7 @@
 //     dQ_i = scale sum_j dS_ij k_j,  dK_j = scale sum_i dS_ij q_i,  dV_j = sum_i P_ij dO_i
 // where the sums over i of a shared key head run over the queries of all its heads.  No atomics: the same bits on every call.
 //
-// Launch 1: Delta_i and L_i log2(e).  Launch 2: one grid of two kinds of workgroups, as the full backward's (sage_bwd.hip, whose
+// Launch 1: Delta_i (from O with what rounding left of it, where the caller kept that) and L_i log2(e).  Launch 2: one grid of two kinds of workgroups, as the full backward's (sage_bwd.hip, whose
 // reasons for tiles, rings and the order of the work hold here): owners of rows, that walk the key tiles their window reaches -> dQ; and owners of
 // 128 keys, that walk the (head, query tile) pairs that reach them -> dK, dV.  Blocks with sinks are reached by every later query; their
 // pairs are dealt to as many workgroups as keep the longest of them near the others, which leave fp32 parts for launch 3
@@ -41,12 +41,14 @@ __global__ __launch_bounds__(256) void window_bwd_prep_kernel(WindowBwdArgs a) {
     const bool real = i < a.w.Sq;
     float sum = 0.0f;
     if (real) {
-        const u32x4 o = *reinterpret_cast<const u32x4*>(a.w.o + b * a.w.o_sb + h * a.w.o_sh + i * a.w.o_sn + col);
+        const int64_t at = b * a.w.o_sb + h * a.w.o_sh + i * a.w.o_sn + col;
+        const u32x4 o = *reinterpret_cast<const u32x4*>(a.w.o + at);
+        const u32x4 rest = a.w.rest ? *reinterpret_cast<const u32x4*>(a.w.rest + at) : u32x4{0u, 0u, 0u, 0u};
         const u32x4 g = *reinterpret_cast<const u32x4*>(a.dout + b * a.do_sb + h * a.do_sh + i * a.do_sn + col);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const uint32_t ow = o[e >> 1], gw = g[e >> 1];
-            sum = fmaf(widen<T>(ow, e & 1), widen<T>(gw, e & 1), sum);
+            const uint32_t ow = o[e >> 1], rw = rest[e >> 1], gw = g[e >> 1];
+            sum = fmaf(widen<T>(ow, e & 1) + widen<T>(rw, e & 1), widen<T>(gw, e & 1), sum);
         }
     }
 #pragma unroll
@@ -67,13 +69,15 @@ template <int D> struct PassLds {
 // ---- dQ: owners of 32 rows per wave, key tiles ---------------------------------------------------------------
 template <int D> struct DqLds {
     static constexpr int SLOT = PassLds<D>::SLOT, OWN = kWaves<D> * 2 * 64 * D;
-    static constexpr int BYTES = 3 * SLOT > SLOT + OWN ? 3 * SLOT : SLOT + OWN;
+    static constexpr int CENTRE = 3 * SLOT, GROUPS = kWaves<D> * 64 / D;         // sums of a tile's keys, [group of rows][D] floats
+    static constexpr int BYTES = CENTRE + GROUPS * D * 4 > SLOT + OWN ? CENTRE + GROUPS * D * 4 : SLOT + OWN;
 };
 
 template <int T, int D>
 __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, int bh, int row0) {
     using L = PassLds<D>;
-    constexpr int NW = kWaves<D>, RPW = TilePieces<D, 64, NW>::N, KS = D / 16, DB = D / 32;
+    using DL = DqLds<D>;
+    constexpr int NW = kWaves<D>, CPR = D / 8, RPW = TilePieces<D, 64, NW>::N, KS = D / 16, DB = D / 32;
     const WindowArgs& w = a.w;
     const int rows = w.Sq * w.g, H = w.Hk * w.g;
     const int b = bh / w.Hk, kvh = bh % w.Hk;
@@ -136,6 +140,14 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
         const float y1 = __builtin_amdgcn_exp2f(in1 ? fmaf(s[e + 1], c, -lse) : -INFINITY) * (g[e + 1] + ndelta);
         return pack2<T>(y0, y1);
     };
+    // Rows of dS sum to zero, but for the roundings of dS and of what Delta is made of; whatever their sum is, dS K multiplies it by the
+    // keys' common offset.  So the rounded values are summed, and the sum times a vector c close to the mean key is
+    // subtracted at the end: dQ = scale dS (K - c).
+    float ds_sum = 0.0f;
+    auto add_up = [&](uint32_t w) {
+        if constexpr (T == kBF16) ds_sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w), __builtin_bit_cast(v2bf, 0x3F803F80u), ds_sum, false);
+        else ds_sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2fp, w), __builtin_bit_cast(v2fp, 0x3C003C00u), ds_sum, false);
+    };
     auto acc_step = [&](const Fragments<D>& fr, const uint8_t* kt, const uint32_t (&ds)[8], int blk, int m) {
         const int j2 = m / DB, d = m % DB;
         const v4i sb = {(int)ds[j2 * 4], (int)ds[j2 * 4 + 1], (int)ds[j2 * 4 + 2], (int)ds[j2 * 4 + 3]};
@@ -156,13 +168,13 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
         for (int ks = 0; ks < KS; ks++) {
             scores_step(f, kt, s[1], g[1], 1, ks);
 #pragma unroll
-            for (int n = ks * (8 / KS); n < (ks + 1) * (8 / KS); n++) ds[0][n] = pair(s[0], g[0], n * 2, true, true);
+            for (int n = ks * (8 / KS); n < (ks + 1) * (8 / KS); n++) add_up(ds[0][n] = pair(s[0], g[0], n * 2, true, true));
         }
 #pragma unroll
         for (int m = 0; m < 2 * DB; m++) {
             acc_step(f, kt, ds[0], 0, m);
 #pragma unroll
-            for (int n = m * (8 / (2 * DB)); n < (m + 1) * (8 / (2 * DB)); n++) ds[1][n] = pair(s[1], g[1], n * 2, true, true);
+            for (int n = m * (8 / (2 * DB)); n < (m + 1) * (8 / (2 * DB)); n++) add_up(ds[1][n] = pair(s[1], g[1], n * 2, true, true));
         }
 #pragma unroll
         for (int m = 0; m < 2 * DB; m++) acc_step(f, kt, ds[1], 1, m);
@@ -182,7 +194,7 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
 #pragma unroll
             for (int n = 0; n < 8; n++) {
                 const int e = n * 2, key = (e >> 2) * 8 + (e & 3);
-                ds[n] = pair(s, g, e, rel.sees(key), rel.sees(key + 1));
+                add_up(ds[n] = pair(s, g, e, rel.sees(key), rel.sees(key + 1)));
             }
 #pragma unroll
             for (int m = 0; m < 2 * DB; m++) acc_step(f, kt, ds, blk, m);
@@ -200,10 +212,37 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
         const uint8_t* kt = smem + slot * L::SLOT;
         if (what == Seen::kAll) whole(kt);
         else if (what == Seen::kSome) edge(kt, j0);
+        if (t == (span.n - 1) / 2) {           // c: the mean of those keys of the tile in the middle that some row here sees
+            int me = tid;
+            asm volatile("" : "+v"(me));
+            const int ch = me % D, first = me / D * (64 / DL::GROUPS);
+            float sum = 0.0f;
+#pragma unroll 1
+            for (int r = first; r < first + 64 / DL::GROUPS; r++) {
+                const float k = widen<T>(*reinterpret_cast<const uint16_t*>(kt + nat_off<CPR>(r, ch >> 3) + (ch & 7) * 2), 0);
+                sum += copied_key<64>(span, j0, j0 + r) == j0 + r ? k : 0.0f;
+            }
+            const int j1 = min(j0 + 63, span.hi), sinks = max(0, min(j1 + 1, span.s_end) - j0), others = max(0, j1 + 1 - max(max(j0, span.lo), span.s_end));
+            reinterpret_cast<float*>(smem + DL::CENTRE)[me] = sum / (float)(sinks + others);
+        }
         slot = slot == 2 ? 0 : slot + 1;
     }
     __syncthreads();
     uint8_t* os = smem + wave * 64 * D;
+    if (span.n > 0) {
+        const float rs = sum_halves(ds_sum);
+        const float* centre = reinterpret_cast<const float*>(smem + DL::CENTRE);
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                v4f c4 = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int n = 0; n < DL::GROUPS; n++) c4 += *reinterpret_cast<const v4f*>(centre + n * D + d * 32 + g * 8 + half * 4);
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[d][g * 4 + e] = fmaf(-rs, c4[e], acc[d][g * 4 + e]);
+            }
+    }
 #pragma unroll
     for (int d = 0; d < DB; d++) row_put<T, D>(os, acc[d], d, w.scale, lane);
     if (x0 < rows) query_rows_out<D>(w, os, a.dq + b * a.dq_sb + (int64_t)kvh * w.g * a.dq_sh, a.dq_sn, a.dq_sh, x0, lane);
@@ -465,18 +504,33 @@ __device__ __forceinline__ void dkdv_body(const WindowBwdArgs& a, uint8_t* smem,
 }
 
 // Head dim 128: a pair of waves shares 32 keys, the P wave with K rows and dV, the S wave, one tile behind, with V rows and dK; P crosses
-// over through LDS in fp16 (11 significant bits; see sage_bwd.hip).
-template <int D> struct PairLds {
+// over through LDS with some bits more than dS is rounded to: as fp16 pairs where that is bf16 (see sage_bwd.hip), as the upper three bytes of fp32
+// where it is fp16 (with fp16 there dK's relative error was 3.5e-4, with these 2.9e-4).
+template <int T, int D> struct PairLds {
     using L = PassLds<D>;
-    static constexpr int HAND = 4 * 2 * 2 * 64 * 16;          // [pair][32-row block][values 0-7 | 8-15][lane], fp16 pairs
+    static constexpr int WORDS = T == kBF16 ? 2 : 3;          // 16-byte words for the 16 values of a block
+    static constexpr int HAND = 4 * 2 * WORDS * 64 * 16;      // [pair][32-row block][word][lane]
     static constexpr int RING = L::ROWS + 2 * HAND, BYTES = RING + 3 * L::SLOT;
+    static_assert(BYTES <= 160 * 1024, "LDS of a compute unit");
     static_assert(8 * 64 * D <= 2 * L::SLOT, "the owner rows must fit behind the first slot");
 };
+
+// Four floats <-> the upper three bytes of each (15 bits behind the leading one).
+__device__ __forceinline__ void pack24(const float (&y)[4], uint32_t* w) {
+    const uint32_t a = __float_as_uint(y[0]), b = __float_as_uint(y[1]), c = __float_as_uint(y[2]), d = __float_as_uint(y[3]);
+    w[0] = __builtin_amdgcn_perm(b, a, 0x05030201u);
+    w[1] = __builtin_amdgcn_perm(c, b, 0x06050302u);
+    w[2] = __builtin_amdgcn_perm(d, c, 0x07060503u);
+}
+__device__ __forceinline__ float unpack24(const uint32_t* w, int i) {
+    return __uint_as_float(i == 0 ? w[0] << 8 : i == 1 ? __builtin_amdgcn_perm(w[1], w[0], 0x0504030Cu) : i == 2 ? __builtin_amdgcn_perm(w[2], w[1], 0x0403020Cu)
+                                                                                                            : w[2] & 0xFFFFFF00u);
+}
 
 template <int T, int D, int ROLE>
 __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem, int bh, const KeyWork& work, int wave, int lane) {
     using L = PassLds<D>;
-    using PL = PairLds<D>;
+    using PL = PairLds<T, D>;
     constexpr int KS = D / 16, DB = D / 32;
     const WindowArgs& w = a.w;
     const int b = bh / w.Hk, kvh = bh % w.Hk;
@@ -508,7 +562,7 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
 #pragma unroll
         for (int e = 0; e < 16; e++) acc[d][e] = 0.0f;
     const float c = w.scale * kLog2e;
-    u32x4* hand = reinterpret_cast<u32x4*>(smem + L::ROWS) + pr * 256 + lane;
+    u32x4* hand = reinterpret_cast<u32x4*>(smem + L::ROWS) + pr * 2 * PL::WORDS * 64 + lane;
 
     auto tile = [&](auto masked_tag, int pa, int mine, int turn, auto&& copy_next) {
         constexpr bool MASKED = decltype(masked_tag)::value;
@@ -517,19 +571,20 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
         const uint8_t* nt = smem + PL::RING + mine * L::SLOT + ROLE * L::TILE;
         const uint8_t* rt = smem + PL::RING + mine * L::SLOT + (1 - ROLE) * L::TILE;
         const uint8_t* rowv = smem + (mine * 2 + ROLE) * 256;
-        uint32_t hp[2][8];
+        uint32_t hp[2][4 * PL::WORDS];   // P on its way to the S wave
         if constexpr (ROLE == 1) {
 #pragma unroll
             for (int blk = 0; blk < 2; blk++)
 #pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    const u32x4 v = hand[turn * (PL::HAND / 16) + (blk * 2 + n) * 64];
+                for (int n = 0; n < PL::WORDS; n++) {
+                    const u32x4 v = hand[turn * (PL::HAND / 16) + (blk * PL::WORDS + n) * 64];
 #pragma unroll
                     for (int e = 0; e < 4; e++) hp[blk][n * 4 + e] = v[e];
                 }
         }
         v16f s[2];
-        uint32_t pk[2][8], ph[2][8];
+        uint32_t pk[2][8];
+        float last[2];
         v4f rv;
 #pragma unroll
         for (int blk = 0; blk < 2; blk++)
@@ -550,18 +605,24 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
                 if constexpr (ROLE == 0) {
                     y[e] = __builtin_amdgcn_exp2f(fmaf(s[blk][n], c, -rv[n & 3]));
                 } else {
-                    y[e] = fmaf((float)__builtin_bit_cast(v2fp, hp[blk][e0 >> 1])[e], s[blk][n], 0.0f);
+                    if constexpr (T == kBF16) y[e] = fmaf((float)__builtin_bit_cast(v2fp, hp[blk][e0 >> 1])[e], s[blk][n], 0.0f);
+                    else y[e] = unpack24(&hp[blk][(n >> 2) * 3], n & 3) * s[blk][n];
                 }
                 if (MASKED && !rel.sees(blk * 32 + (n >> 2) * 8 + (n & 3))) y[e] = 0.0f;       // (in both: a key that nothing sees may hold anything)
             }
             pk[blk][e0 >> 1] = pack2<T>(y[0], y[1]);
-            if constexpr (ROLE == 0 && T == kBF16) ph[blk][e0 >> 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[0], y[1]));
+            if constexpr (ROLE == 0) {
+                if constexpr (T == kBF16) hp[blk][e0 >> 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[0], y[1]));
+                else if (e0 & 2) pack24({last[0], last[1], y[0], y[1]}, &hp[blk][(e0 >> 2) * 3]);
+                last[0] = y[0], last[1] = y[1];
+            }
         };
         auto hand_over = [&](int blk) {
             if constexpr (ROLE == 0) {
-                const uint32_t(&r)[8] = T == kBF16 ? ph[blk] : pk[blk];
+                const auto& r = hp[blk];
 #pragma unroll
-                for (int n = 0; n < 2; n++) hand[turn * (PL::HAND / 16) + (blk * 2 + n) * 64] = u32x4{r[n * 4], r[n * 4 + 1], r[n * 4 + 2], r[n * 4 + 3]};
+                for (int n = 0; n < PL::WORDS; n++)
+                    hand[turn * (PL::HAND / 16) + (blk * PL::WORDS + n) * 64] = u32x4{r[n * 4], r[n * 4 + 1], r[n * 4 + 2], r[n * 4 + 3]};
             }
         };
         auto acc_step = [&](int blk, int m) {
@@ -621,7 +682,7 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
 template <int T, int D>
 __global__ __launch_bounds__(kWaves<D> * 64, 2) void window_bwd_kernel(WindowBwdArgs a) {
     constexpr bool PAIRED = D > 64;
-    constexpr int KV = PAIRED ? PairLds<D>::BYTES : KeyLds<D>::BYTES;
+    constexpr int KV = PAIRED ? PairLds<T, D>::BYTES : KeyLds<D>::BYTES;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[KV > DqLds<D>::BYTES ? KV : DqLds<D>::BYTES];
     const int heads = a.w.B * a.w.Hk, rows = a.w.Sq * a.w.g;
     const int tq = (rows + kRowsWg<D> - 1) / kRowsWg<D>, blocks = (a.w.Skv + kKeysWg - 1) / kKeysWg;

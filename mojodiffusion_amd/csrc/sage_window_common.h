@@ -138,13 +138,25 @@ __device__ __forceinline__ void query_rows_out(const WindowArgs& a, const uint8_
         if (x < rows) *reinterpret_cast<u32x4*>(out + i * sn + (int64_t)(x - i * a.g) * sh + (lane % CPR) * 8) = w;
     }
 }
+// what rounding to the type leaves of x
+template <int T> __device__ __forceinline__ float rounded_off(float x) {
+    if constexpr (T == kBF16) return x - (float)(__bf16)x;
+    else return x - (float)(_Float16)x;
+}
 // Channels d * 32 + g * 8 + half * 4 .. + 3 of the lane's row, an accumulator's registers times `mul` -> LDS.
-template <int T, int D> __device__ __forceinline__ void row_put(uint8_t* os, const v16f& acc, int d, float mul, int lane) {
+// REST: what rounding leaves of them.
+template <int T, int D, bool REST = false> __device__ __forceinline__ void row_put(uint8_t* os, const v16f& acc, int d, float mul, int lane) {
     asm volatile("" : "+v"(lane));
 #pragma unroll
-    for (int g = 0; g < 4; g++)
-        *reinterpret_cast<u32x2*>(os + nat_off<D / 8>(lane & 31, d * 4 + g) + (lane >> 5) * 8) =
-            u32x2{pack2<T>(acc[g * 4] * mul, acc[g * 4 + 1] * mul), pack2<T>(acc[g * 4 + 2] * mul, acc[g * 4 + 3] * mul)};
+    for (int g = 0; g < 4; g++) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            y[e] = acc[g * 4 + e] * mul;
+            if constexpr (REST) y[e] = rounded_off<T>(y[e]);
+        }
+        *reinterpret_cast<u32x2*>(os + nat_off<D / 8>(lane & 31, d * 4 + g) + (lane >> 5) * 8) = u32x2{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
+    }
 }
 
 }  // namespace

@@ -346,7 +346,7 @@ def test_refusals():
                          (dict(), "must live on the GPU")):
         with pytest.raises(Error, match=text):
             W.sdpa_window_decode(**{**dec, **change})
-    fwd = W.SdpaWindowFwd(q, torch.zeros((2, 4, 4, 1)), q, k, k, 0.1, 3, 0, 0, None, 0)
+    fwd = W.SdpaWindowFwd(q, q, torch.zeros((2, 4, 4, 1)), q, k, k, 0.1, 3, 0, 0, None, 0)
     for change, d, text in ((dict(), q.half(), "type of the forward"), (dict(), q[:, :3], "does not match"), (dict(stats=torch.zeros(3)), q, "stats must be"),
                             (dict(q=q.repeat(1, 1, 1, 4), k=k.repeat(1, 1, 1, 4), v=k.repeat(1, 1, 1, 4)), q, "Dh=256"), (dict(), q, "must live on the GPU")):
         with pytest.raises(Error, match=text):
@@ -366,7 +366,7 @@ def test_c_refusals():
 
     def call(**change):
         a = {**base, **change}
-        return L.mi355_sage_sdpa_window(a["q"], a["k"], a["v"], a["o"], None, a["B"], a["Hq"], a["Hk"], a["Nq"], a["Nkv"], a["D"], a["type"], a["scale"],
+        return L.mi355_sage_sdpa_window(a["q"], a["k"], a["v"], a["o"], None, None, a["B"], a["Hq"], a["Hk"], a["Nq"], a["Nkv"], a["D"], a["type"], a["scale"],
                                         a["qs"], a["ks"], a["vs"], a["os"], *a["off"], 0, a["left"], a["right"], a["sinks"], None, None, a["start"], None,
                                         a["ws"], a["nws"])
     for change in (dict(q=None), dict(o=None), dict(vs=None), dict(B=0), dict(Hk=0), dict(Hq=6), dict(Nq=0), dict(Nkv=-1), dict(scale=0.0), dict(scale=float("inf")),
@@ -380,9 +380,9 @@ def test_c_refusals():
     assert L.mi355_sage_window_workspace_bytes(1, 4, 4, 8, 8192, 64, -1, 0, 0) > 1000
     assert L.mi355_sage_window_workspace_bytes(1, 4, 3, 8, 8192, 64, -1, 0, 0) == 0
     assert L.mi355_sage_sdpa_window_decode(A, A, A, A, 1, 4, 4, 1, 8, 64, 0, 0.1, st, st, st, st, 0, 0, 0, 0, 3, 0, None, None, None, 0) == -1
-    bwd = [A] * 9 + [1, 4, 4, 8, 8, 64, 0, 0.1] + [st] * 8 + [0] * 9 + [3, 0, 0, None, 0, None]
+    bwd = [A] * 10 + [1, 4, 4, 8, 8, 64, 0, 0.1] + [st] * 8 + [0] * 9 + [3, 0, 0, None, 0, None]
     assert L.mi355_sage_sdpa_window_bwd(*bwd, A, 8) == -3
-    for at, value, code in ((0, None, -1), (8, None, -1), (17, None, -1), (14, 256, -2), (10, 5, -1), (15, 2, -2), (21, off_rows(S), -2), (24, S(0, 64, 256, 2), -2)):
+    for at, value, code in ((0, None, -1), (9, None, -1), (18, None, -1), (15, 256, -2), (11, 5, -1), (16, 2, -2), (22, off_rows(S), -2), (25, S(0, 64, 256, 2), -2)):
         args = list(bwd)
         args[at] = value
         assert L.mi355_sage_sdpa_window_bwd(*args, A, 1 << 30) == code, at

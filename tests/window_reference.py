@@ -60,9 +60,9 @@ def backward(q, k, v, d, scale, ref, g):
     """Gradients by the formulas and the sizes of their bounds, float64; ref: forward's result, g: query heads to a key head.
 
     Bounds.  dS = P (dP - Delta).  P: recomputed from scores and a statistic that are off by E each (2 E relative), rounded to the type (u) for dV, handed on
-    with 11 bits (2^-10) and, as part of dS, rounded (u) for dQ and dK.  Delta is a product with the stored O, off by the forward's
-    bound: dDelta = sum |dO| bound(O).  dP and Delta are fp32 sums of D products (D 2^-24 of their sizes).  Every sum over rows or keys is fp32, and
-    the result is rounded (u); F: what fp16 loses below its normal range, 2^-25 for every P and dS."""
+    with 11 bits (2^-10) and, as part of dS, rounded (u) for dQ and dK.  Delta is a product with O, stored to twice the type's bits and else off
+    by the forward's bound: dDelta = sum |dO| bound(O).  dP and Delta are fp32 sums of D products (D 2^-24 of their sizes).  Every sum over rows or keys is fp32, and
+    the result is rounded (u).  dQ is taken as scale dS (K - c), c a mean of keys: an error of dS meets |k| + |c|, and |c| is no larger than a key.  F: what fp16 loses below its normal range, 2^-25 for every P and dS."""
     O, L, W, A, F, E = ref
     dtype = q.dtype
     u = torch.finfo(dtype).eps / 2
@@ -72,7 +72,7 @@ def backward(q, k, v, d, scale, ref, g):
     dq, dk, dv = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
     bq, bk, bv = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
     e = E.transpose(1, 2).unsqueeze(-1)
-    bo = u * O.abs() + A * (1.01 * u + W.shape[3] * 2.0 ** -24 + 2.1 * e) + (F * 2.0 ** -25 if dtype == torch.float16 else 0)
+    bo = 2 * u * u * O.abs() + A * (1.01 * u + W.shape[3] * 2.0 ** -24 + 2.1 * e) + (F * 2.0 ** -25 if dtype == torch.float16 else 0)
     tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
     for b in range(B):
         for h in range(Hq):
@@ -88,7 +88,7 @@ def backward(q, k, v, d, scale, ref, g):
             p_err = (2.2 * E[b, h].view(-1, 1) + n * 2.0 ** -24) * w
             ds_err = ds.abs() * (1.01 * u + 2.0 ** -10) + (dp - delta).abs() * (p_err + tiny) + 1.01 * (w + tiny) * d_delta + tiny * ww
             dq[b, :, h] = scale * ds @ kh
-            bq[b, :, h] = scale * (ds_err + n * 2.0 ** -24 * ds.abs()) @ kh.abs()
+            bq[b, :, h] = scale * (ds_err + n * 2.0 ** -24 * ds.abs()) @ (kh.abs() + kh.abs().amax(0))
             dk[b, :, h // g] += scale * ds.T @ qh
             bk[b, :, h // g] += scale * (ds_err + n * 2.0 ** -24 * ds.abs()).T @ qh.abs()
             dv[b, :, h // g] += w.T @ dh
