@@ -99,7 +99,9 @@ BF16, FP16, F32 = 0, 1, 2
 
 # entry points the native host path calls, in the order of its Api struct (csrc/sage_torch.cpp)
 _HOST_ENTRIES = ("workspace_bytes", "bwd_workspace_bytes", "sdpa_bf16", "sdpa_bf16_train_fwd", "sdpa_bf16_keymask", "sdpa_bf16_mask_any",
-                 "sdpa_bf16_norm_rope", "sdpa_bf16_norm_rope_train_fwd", "sdpa_bwd_bf16", "sdpa_bwd_f32_grads", "cast")
+                 "sdpa_bf16_norm_rope", "sdpa_bf16_norm_rope_train_fwd", "sdpa_bwd_bf16", "sdpa_bwd_f32_grads", "cast", "qk_norm_rope",
+                 "qk_norm_rope_bwd_workspace_bytes", "qk_norm_rope_bwd", "window_workspace_bytes", "sdpa_window", "sdpa_window_decode",
+                 "window_bwd_workspace_bytes", "sdpa_window_bwd")
 
 _lib = None
 _host = None

@@ -19,6 +19,8 @@ from .attention_sage import Error, SdpaFlashGrads
 from .norm_rope import _rows, _rows_ok, _scratch, _strides
 
 _TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
+# Calls that meet every check go through the native host path (_lib.host(), csrc/sage_torch.cpp), which returns None for the others;
+# those continue below, where the checks are stated.
 
 
 @dataclass
@@ -91,6 +93,9 @@ def _bound(x):
 
 
 def _forward(name, q, k, v, scale, left, right, sinks, kv_lens, q_start, training):
+    r = _lib.host().window(q, k, v, scale, left, right, sinks, kv_lens, q_start, int(training))
+    if r is not None:
+        return (*r, q, k, v, kv_lens) if training else (r,)
     _check(name, q, k, v, scale, left, right, sinks)
     B, Sq, Hq, Dh = q.shape
     Skv, Hk = k.shape[1], k.shape[2]
@@ -126,9 +131,12 @@ def sdpa_window_decode(q, k_cache, v_cache, kv_lens, scale, left, sinks=0):
     """The last Sq tokens of every sequence (one, or a few) against its cache [B,capacity,Hk,Dh]: query i of sequence b stands at
     kv_lens[b] - Sq + i and sees keys up to itself through the window.  kv_lens counts the keys in the cache, the new tokens'
     among them.  Queries before a sequence's first token (kv_lens[b] < Sq) give zeros."""
+    o = _lib.host().window_decode(q, k_cache, v_cache, kv_lens, scale, left, sinks)
+    if o is not None:
+        return o
     name = "sdpa_window_decode"
-    q4, k, v = q, k_cache, v_cache
-    _check(name, q4, k, v, scale, left, 0, sinks)
+    k, v = k_cache, v_cache
+    _check(name, q, k, v, scale, left, 0, sinks)
     B, Sq, Hq, Dh = q.shape
     Skv, Hk = k.shape[1], k.shape[2]
     if kv_lens is None:
@@ -162,6 +170,9 @@ def sdpa_window_backward(fwd, d_out):
     """d_q [B,Sq,Hq,Dh], d_k, d_v [B,Skv,Hk,Dh] from a sdpa_window_train_fwd and the upstream gradient (Dh 64 or 128; the gradients of a
     shared key head are summed over its query heads; rows of padding and of keys that nothing sees are zeros)."""
     name = "sdpa_window_backward"
+    r = _lib.host().window_bwd(fwd.q, fwd.k, fwd.v, fwd.o, fwd.o_rest, d_out, fwd.stats, fwd.scale, fwd.left, fwd.right, fwd.sinks, fwd.kv_lens, fwd.q_start)
+    if r is not None:
+        return SdpaFlashGrads(*r)
     q, k, v, o, rest, stats = fwd.q, fwd.k, fwd.v, fwd.o, fwd.o_rest, fwd.stats
     _check(name, q, k, v, fwd.scale, fwd.left, fwd.right, fwd.sinks)
     if q.shape[3] == 256:

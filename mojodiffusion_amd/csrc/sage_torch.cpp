@@ -34,6 +34,14 @@ struct Api {
     decltype(&mi355_sage_sdpa_bwd_bf16) bwd;
     decltype(&mi355_sage_sdpa_bwd_f32_grads) bwd_f32;
     decltype(&mi355_sage_cast) cast;
+    decltype(&mi355_sage_qk_norm_rope) rope;
+    decltype(&mi355_sage_qk_norm_rope_bwd_workspace_bytes) rope_bwd_workspace_bytes;
+    decltype(&mi355_sage_qk_norm_rope_bwd) rope_bwd;
+    decltype(&mi355_sage_window_workspace_bytes) window_workspace_bytes;
+    decltype(&mi355_sage_sdpa_window) window;
+    decltype(&mi355_sage_sdpa_window_decode) window_decode;
+    decltype(&mi355_sage_window_bwd_workspace_bytes) window_bwd_workspace_bytes;
+    decltype(&mi355_sage_sdpa_window_bwd) window_bwd;
 } api;
 constexpr int kApiEntries = sizeof(Api) / sizeof(void*);
 static_assert(sizeof(Api) == kApiEntries * sizeof(void*), "one pointer per entry");
@@ -387,6 +395,236 @@ PyObject* py_record(PyObject* const* a, Py_ssize_t n) {
     return THPVariable_Wrap(std::move(out));
 }
 
+// ---- norm and rotation, windowed attention (norm_rope.py, attention_window.py) ---------------------------
+// Views of dense, 16-byte aligned rows are taken as they are; anything else goes to the Python path, which copies or refuses.
+bool dense_rows(const at::Tensor& t) {
+    if (t.dim() != 4 || !t.is_cuda() || t.stride(3) != 1 || !aligned16(t)) return false;
+    const int64_t per = 16 / t.element_size();
+    return t.stride(0) % per == 0 && t.stride(1) % per == 0 && t.stride(2) % per == 0;
+}
+Strides bhsd(const at::Tensor& t) { return Strides{{t.stride(0), t.stride(2), t.stride(1), 1}}; }
+bool fits(int64_t x) { return x > 0 && x <= 0x7FFFFFFF; }
+at::Tensor fresh(at::IntArrayRef sizes, const at::Tensor& like, at::ScalarType type) {
+    return at::empty(sizes, at::TensorOptions().dtype(type).device(like.device()));
+}
+int element_type(at::ScalarType t) {
+    return t == at::kBFloat16 ? MI355_SAGE_BF16 : t == at::kHalf ? MI355_SAGE_FP16 : t == at::kFloat ? MI355_SAGE_F32 : -1;
+}
+
+struct RopeCall {
+    const at::Tensor *q, *k, *gq, *gk, *cs = nullptr, *sn = nullptr, *pos = nullptr;
+    double eps;
+    int halfsplit, type, gain_type, table_type = 0, rot = 0, pos_bytes = 0;
+    int64_t table_rows = 0, table_stride = 0, pos_stride = 0;
+};
+// a[0..8]: q, k, q_norm, k_norm, eps, cos, sin, halfsplit, positions
+bool rope_args(PyObject* const* a, RopeCall& c) {
+    if (!tensor_arg(a[0], c.q) || !tensor_arg(a[1], c.k) || !tensor_arg(a[2], c.gq) || !tensor_arg(a[3], c.gk) || !double_arg(a[4], c.eps) || !(c.eps >= 0.0) ||
+        (a[7] != Py_True && a[7] != Py_False))
+        return false;
+    c.halfsplit = a[7] == Py_True;
+    const at::Tensor &q = *c.q, &k = *c.k;
+    if (!dense_rows(q) || !dense_rows(k) || q.device() != k.device() || q.scalar_type() != k.scalar_type() || (c.type = element_type(q.scalar_type())) < 0) return false;
+    if (q.size(0) != k.size(0) || q.size(1) != k.size(1) || q.size(3) != k.size(3) || q.numel() == 0 || k.numel() == 0) return false;
+    const int64_t B = q.size(0), S = q.size(1), D = q.size(3);
+    if (!fits(B) || !fits(S) || !fits(q.size(2)) || !fits(k.size(2)) || D % 16 || D > 256) return false;
+    if ((c.gain_type = element_type(c.gq->scalar_type())) < 0) return false;
+    for (const at::Tensor* g : {c.gq, c.gk})
+        if (g->dim() != 1 || g->numel() != D || !g->is_contiguous() || !aligned16(*g) || g->scalar_type() != c.gq->scalar_type() || g->device() != q.device()) return false;
+    if ((a[5] == Py_None) != (a[6] == Py_None) || (a[8] != Py_None && a[5] == Py_None)) return false;
+    if (a[5] != Py_None) {
+        if (!tensor_arg(a[5], c.cs) || !tensor_arg(a[6], c.sn) || c.cs->dim() != 2 || c.cs->sizes() != c.sn->sizes() || c.cs->strides() != c.sn->strides()) return false;
+        if ((c.table_type = element_type(c.cs->scalar_type())) < 0 || c.sn->scalar_type() != c.cs->scalar_type()) return false;
+        c.table_rows = c.cs->size(0);
+        c.table_stride = c.cs->stride(0);
+        c.rot = c.cs->size(1) * 2 > D ? -1 : (int)c.cs->size(1) * 2;
+        if (c.rot <= 0 || c.rot % 16 || c.table_rows < 1 || c.cs->stride(1) != 1 || (c.table_stride * (int64_t)c.cs->element_size()) % 16 || !aligned16(*c.cs) || !aligned16(*c.sn) ||
+            c.cs->device() != q.device() || c.sn->device() != q.device() || (a[8] == Py_None && c.table_rows < S))
+            return false;
+    }
+    if (a[8] != Py_None) {
+        if (!tensor_arg(a[8], c.pos) || (c.pos->scalar_type() != at::kInt && c.pos->scalar_type() != at::kLong) || c.pos->device() != q.device()) return false;
+        const at::Tensor& p = *c.pos;
+        if (!(p.dim() == 2 && (p.size(0) == B || p.size(0) == 1) && p.size(1) == S) && !(p.dim() == 1 && p.size(0) == S)) return false;
+        if (p.stride(-1) != 1) return false;
+        c.pos_bytes = (int)p.element_size();
+        c.pos_stride = p.dim() == 1 || p.size(0) == 1 ? 0 : p.stride(0);
+    }
+    return true;
+}
+const void* data_or_null(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
+
+// rope(q, k, q_norm, k_norm, eps, cos, sin, halfsplit, positions) -> (q_rot, k_rot) or None
+PyObject* py_rope(PyObject* const* a, Py_ssize_t n) {
+    RopeCall c;
+    if (intercepted() || n != 9 || !rope_args(a, c)) Py_RETURN_NONE;
+    at::Tensor out[2];
+    const int rc = without_gil([&] {
+        const at::Tensor &q = *c.q, &k = *c.k;
+        const c10::DeviceGuard guard(q.device());
+        out[0] = fresh(q.sizes(), q, q.scalar_type());
+        out[1] = fresh(k.sizes(), k, k.scalar_type());
+        const Strides qs = bhsd(q), ks = bhsd(k), qo = bhsd(out[0]), ko = bhsd(out[1]);
+        return api.rope(q.data_ptr(), k.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), q.size(0), q.size(1), q.size(2), k.size(2), q.size(3), c.type, qs.s, ks.s,
+                        qo.s, ko.s, 0, 0, 0, 0, c.gq->data_ptr(), c.gk->data_ptr(), c.gain_type, (float)c.eps, data_or_null(c.cs), data_or_null(c.sn), c.table_type,
+                        c.rot, c.table_rows, c.table_stride, c.halfsplit, data_or_null(c.pos), c.pos_stride, c.pos_bytes, stream_of(q));
+    });
+    if (rc != 0) Py_RETURN_NONE;
+    PyObject* t = PyTuple_New(2);
+    for (int i = 0; i < 2; i++) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(std::move(out[i])));
+    return t;
+}
+
+// rope_bwd(d_q_rot, d_k_rot, q, k, q_norm, k_norm, eps, cos, sin, halfsplit, positions) -> (d_q, d_k, d_q_norm, d_k_norm) or None
+PyObject* py_rope_bwd(PyObject* const* a, Py_ssize_t n) {
+    RopeCall c;
+    const at::Tensor *dq, *dk;
+    if (intercepted() || n != 11 || !tensor_arg(a[0], dq) || !tensor_arg(a[1], dk) || !rope_args(a + 2, c)) Py_RETURN_NONE;
+    for (auto [d, x] : {std::pair{dq, c.q}, std::pair{dk, c.k}})
+        if (!dense_rows(*d) || d->sizes() != x->sizes() || d->scalar_type() != x->scalar_type() || d->device() != x->device()) Py_RETURN_NONE;
+    at::Tensor out[4];
+    const int rc = without_gil([&] {
+        const at::Tensor &q = *c.q, &k = *c.k;
+        const int B = q.size(0), S = q.size(1), Hq = q.size(2), Hk = k.size(2), D = q.size(3);
+        const size_t need = api.rope_bwd_workspace_bytes(B, S, Hq, Hk, D);
+        if (need == 0) return MI355_SAGE_EUNSUPPORTED;
+        const c10::DeviceGuard guard(q.device());
+        out[0] = fresh(q.sizes(), q, q.scalar_type());
+        out[1] = fresh(k.sizes(), k, k.scalar_type());
+        for (int i = 2; i < 4; i++) out[i] = fresh({D}, q, at::kFloat);
+        const at::Tensor ws = fresh({(int64_t)need}, q, at::kByte);        // (a call's own: see norm_rope.py)
+        const Strides gqs = bhsd(*dq), gks = bhsd(*dk), qs = bhsd(q), ks = bhsd(k), qo = bhsd(out[0]), ko = bhsd(out[1]);
+        return api.rope_bwd(dq->data_ptr(), dk->data_ptr(), q.data_ptr(), k.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(), B, S,
+                            Hq, Hk, D, c.type, gqs.s, gks.s, qs.s, ks.s, qo.s, ko.s, 0, 0, 0, 0, 0, 0, c.gq->data_ptr(), c.gk->data_ptr(), c.gain_type, (float)c.eps,
+                            data_or_null(c.cs), data_or_null(c.sn), c.table_type, c.rot, c.table_rows, c.table_stride, c.halfsplit, data_or_null(c.pos), c.pos_stride,
+                            c.pos_bytes, stream_of(q), ws.data_ptr(), need);
+    });
+    if (rc != 0) Py_RETURN_NONE;
+    PyObject* t = PyTuple_New(4);
+    for (int i = 0; i < 4; i++) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(std::move(out[i])));
+    return t;
+}
+
+struct WindowCall {
+    const at::Tensor *q, *k, *v, *lens = nullptr;
+    double scale;
+    int left, right = 0, sinks, type;
+};
+bool window_shapes(const WindowCall& c) {
+    const at::Tensor &q = *c.q, &k = *c.k, &v = *c.v;
+    if (!dense_rows(q) || !dense_rows(k) || !dense_rows(v) || k.sizes() != v.sizes() || q.device() != k.device() || q.device() != v.device()) return false;
+    if (q.scalar_type() != k.scalar_type() || q.scalar_type() != v.scalar_type() || c.type < 0 || c.type == MI355_SAGE_F32) return false;
+    if (q.size(0) != k.size(0) || q.size(3) != k.size(3) || q.numel() == 0 || k.numel() == 0 || q.size(2) % k.size(2)) return false;
+    if (!fits(q.size(0)) || !fits(q.size(1)) || !fits(q.size(2)) || !fits(k.size(1)) || q.size(3) > 256) return false;
+    if (!(c.scale > 0.0) || c.left < -1 || c.right < -1 || c.sinks < 0) return false;
+    return c.lens == nullptr || (c.lens->dim() == 1 && c.lens->size(0) == q.size(0) && c.lens->scalar_type() == at::kInt && c.lens->is_contiguous() &&
+                                 c.lens->device() == q.device());
+}
+// a workspace of the call's own, if it needs one
+at::Tensor window_scratch(size_t need, const at::Tensor& like) { return need > 256 ? fresh({(int64_t)need}, like, at::kByte) : at::Tensor(); }
+
+// window(q, k, v, scale, left, right, sinks, kv_lens, q_start, training) -> o, (o, rest, stats) with training, or None
+PyObject* py_window(PyObject* const* a, Py_ssize_t n) {
+    WindowCall c;
+    int start, training;
+    if (intercepted() || n != 10 || !tensor_arg(a[0], c.q) || !tensor_arg(a[1], c.k) || !tensor_arg(a[2], c.v) || !double_arg(a[3], c.scale) || !int_arg(a[4], c.left) ||
+        !int_arg(a[5], c.right) || !int_arg(a[6], c.sinks) || !int_arg(a[8], start) || !int_arg(a[9], training))
+        Py_RETURN_NONE;
+    if (a[7] != Py_None && !tensor_arg(a[7], c.lens)) Py_RETURN_NONE;
+    c.type = element_type(c.q->scalar_type());
+    if (!window_shapes(c)) Py_RETURN_NONE;
+    at::Tensor o, rest, stats;
+    const int rc = without_gil([&] {
+        const at::Tensor &q = *c.q, &k = *c.k, &v = *c.v;
+        const int B = q.size(0), Sq = q.size(1), Hq = q.size(2), D = q.size(3), Skv = k.size(1), Hk = k.size(2);
+        const size_t need = api.window_workspace_bytes(B, Hq, Hk, Sq, Skv, D, c.left, c.right, c.sinks);
+        if (need == 0) return MI355_SAGE_EUNSUPPORTED;
+        const c10::DeviceGuard guard(q.device());
+        o = fresh(q.sizes(), q, q.scalar_type());
+        if (training) {
+            rest = fresh(q.sizes(), q, q.scalar_type());
+            stats = fresh({B, Hq, Sq, 1}, q, at::kFloat);
+        }
+        const at::Tensor ws = window_scratch(need, q);
+        const Strides qs = bhsd(q), ks = bhsd(k), vs = bhsd(v), os = bhsd(o);
+        return api.window(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), training ? rest.data_ptr() : nullptr, training ? stats.data_ptr() : nullptr, B, Hq, Hk, Sq,
+                          Skv, D, c.type, (float)c.scale, qs.s, ks.s, vs.s, os.s, 0, 0, 0, 0, 0, c.left, c.right, c.sinks, data_or_null(c.lens), nullptr, start, stream_of(q),
+                          ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0);
+    });
+    if (rc != 0) Py_RETURN_NONE;
+    if (!training) return THPVariable_Wrap(std::move(o));
+    PyObject* t = PyTuple_New(3);
+    PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(std::move(o)));
+    PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(std::move(rest)));
+    PyTuple_SET_ITEM(t, 2, THPVariable_Wrap(std::move(stats)));
+    return t;
+}
+
+// window_decode(q, k, v, kv_lens, scale, left, sinks) -> o or None
+PyObject* py_window_decode(PyObject* const* a, Py_ssize_t n) {
+    WindowCall c;
+    if (intercepted() || n != 7 || !tensor_arg(a[0], c.q) || !tensor_arg(a[1], c.k) || !tensor_arg(a[2], c.v) || !tensor_arg(a[3], c.lens) || !double_arg(a[4], c.scale) ||
+        !int_arg(a[5], c.left) || !int_arg(a[6], c.sinks))
+        Py_RETURN_NONE;
+    c.type = element_type(c.q->scalar_type());
+    if (!window_shapes(c)) Py_RETURN_NONE;
+    at::Tensor o;
+    const int rc = without_gil([&] {
+        const at::Tensor &q = *c.q, &k = *c.k, &v = *c.v;
+        const int B = q.size(0), Sq = q.size(1), Hq = q.size(2), D = q.size(3), Skv = k.size(1), Hk = k.size(2);
+        const size_t need = api.window_workspace_bytes(B, Hq, Hk, Sq, Skv, D, c.left, 0, c.sinks);
+        if (need == 0) return MI355_SAGE_EUNSUPPORTED;
+        const c10::DeviceGuard guard(q.device());
+        o = fresh(q.sizes(), q, q.scalar_type());
+        const at::Tensor ws = window_scratch(need, q);
+        const Strides qs = bhsd(q), ks = bhsd(k), vs = bhsd(v), os = bhsd(o);
+        return api.window_decode(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), B, Hq, Hk, Sq, Skv, D, c.type, (float)c.scale, qs.s, ks.s, vs.s, os.s, 0, 0, 0, 0,
+                                 c.left, c.sinks, c.lens->data_ptr(), stream_of(q), ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0);
+    });
+    if (rc != 0) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(o));
+}
+
+// window_bwd(q, k, v, o, rest, d_out, stats, scale, left, right, sinks, kv_lens, q_start) -> (d_q, d_k, d_v) or None
+PyObject* py_window_bwd(PyObject* const* a, Py_ssize_t n) {
+    WindowCall c;
+    const at::Tensor *o, *rest, *d, *stats;
+    int start;
+    if (intercepted() || n != 13 || !tensor_arg(a[0], c.q) || !tensor_arg(a[1], c.k) || !tensor_arg(a[2], c.v) || !tensor_arg(a[3], o) || !tensor_arg(a[4], rest) ||
+        !tensor_arg(a[5], d) || !tensor_arg(a[6], stats) || !double_arg(a[7], c.scale) || !int_arg(a[8], c.left) || !int_arg(a[9], c.right) || !int_arg(a[10], c.sinks) ||
+        !int_arg(a[12], start))
+        Py_RETURN_NONE;
+    if (a[11] != Py_None && !tensor_arg(a[11], c.lens)) Py_RETURN_NONE;
+    c.type = element_type(c.q->scalar_type());
+    if (!window_shapes(c)) Py_RETURN_NONE;
+    const at::Tensor& q = *c.q;
+    for (const at::Tensor* t : {o, rest, d})
+        if (!dense_rows(*t) || t->sizes() != q.sizes() || t->scalar_type() != q.scalar_type() || t->device() != q.device()) Py_RETURN_NONE;
+    if (o->strides() != rest->strides() || stats->scalar_type() != at::kFloat || stats->device() != q.device() || !stats->is_contiguous() ||
+        stats->numel() != q.size(0) * q.size(1) * q.size(2))
+        Py_RETURN_NONE;
+    at::Tensor g[3];
+    const int rc = without_gil([&] {
+        const at::Tensor &k = *c.k, &v = *c.v;
+        const int B = q.size(0), Sq = q.size(1), Hq = q.size(2), D = q.size(3), Skv = k.size(1), Hk = k.size(2);
+        const size_t need = api.window_bwd_workspace_bytes(B, Hq, Hk, Sq, Skv, D, c.left, c.right, c.sinks);
+        if (need == 0) return MI355_SAGE_EUNSUPPORTED;
+        const c10::DeviceGuard guard(q.device());
+        g[0] = fresh(q.sizes(), q, q.scalar_type());
+        g[1] = fresh(k.sizes(), q, q.scalar_type());
+        g[2] = fresh(v.sizes(), q, q.scalar_type());
+        const at::Tensor ws = fresh({(int64_t)need}, q, at::kByte);
+        const Strides qs = bhsd(q), ks = bhsd(k), vs = bhsd(v), os = bhsd(*o), ds = bhsd(*d), dqs = bhsd(g[0]), dks = bhsd(g[1]), dvs = bhsd(g[2]);
+        return api.window_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o->data_ptr(), rest->data_ptr(), d->data_ptr(), stats->data_ptr(), g[0].data_ptr(), g[1].data_ptr(),
+                              g[2].data_ptr(), B, Hq, Hk, Sq, Skv, D, c.type, (float)c.scale, qs.s, ks.s, vs.s, os.s, ds.s, dqs.s, dks.s, dvs.s, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                              c.left, c.right, c.sinks, data_or_null(c.lens), start, stream_of(q), ws.data_ptr(), need);
+    });
+    if (rc != 0) Py_RETURN_NONE;
+    PyObject* t = PyTuple_New(3);
+    for (int i = 0; i < 3; i++) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(std::move(g[i])));
+    return t;
+}
+
 // workspace(nbytes, tensor) -> this (device, stream)'s buffer
 PyObject* py_workspace(PyObject* const* a, Py_ssize_t n) {
     if (n != 2 || !PyLong_Check(a[0]) || !THPVariable_Check(a[1])) {
@@ -418,7 +656,8 @@ PyObject* py_bind(PyObject* const* a, Py_ssize_t n) {
 }
 
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(entry<py_##name>)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(fwd), METHOD(bias), METHOD(norm_rope), METHOD(bwd), METHOD(record), METHOD(workspace), METHOD(bind), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {METHOD(fwd), METHOD(bias), METHOD(norm_rope), METHOD(bwd), METHOD(record), METHOD(workspace), METHOD(bind),
+                         METHOD(rope), METHOD(rope_bwd), METHOD(window), METHOD(window_decode), METHOD(window_bwd), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_sage_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -16,6 +16,8 @@ import torch
 from . import _lib
 from .attention_sage import Error
 
+# Calls that meet every check go through the native host path (_lib.host(), csrc/sage_torch.cpp), which returns None for the others;
+# those continue below, where the checks are stated.
 _TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32: _lib.F32}
 
 
@@ -135,6 +137,10 @@ def qk_norm_rope(q, k, q_norm, k_norm, eps, cos, sin, halfsplit=False, positions
     Dh: the other channels pass.  halfsplit: pairs (i, i + rot/2) instead of (2i, 2i+1).  positions: int32 or int64
     [B,S] or [S], rows of the tables by token (a token whose position is not in the tables comes out as NaN);
     without it token s takes row s.  q_out/k_out: where to write, e.g. rows of a cache; q and k themselves are allowed."""
+    if q_out is None and k_out is None:
+        r = _lib.host().rope(q, k, q_norm, k_norm, eps, cos, sin, halfsplit, positions)
+        if r is not None:
+            return r
     name = "qk_norm_rope"
     gq, gk, table, pos, keep = _check(name, q, k, q_norm, k_norm, eps, cos, sin, positions)
     B, S, Hq, Dh = q.shape
@@ -154,6 +160,9 @@ def qk_norm_rope(q, k, q_norm, k_norm, eps, cos, sin, halfsplit=False, positions
 def qk_norm_rope_backward(d_q_rot, d_k_rot, q, k, q_norm, k_norm, eps, cos, sin, halfsplit=False, positions=None):
     """Gradients of qk_norm_rope from the upstream gradients of its two results and the inputs it was called with: d_q and d_k in
     q's type, the gains' in F32 (sums over every token and head; the same bits on every call)."""
+    r = _lib.host().rope_bwd(d_q_rot, d_k_rot, q, k, q_norm, k_norm, eps, cos, sin, halfsplit, positions)
+    if r is not None:
+        return QkNormRopeGrads(*r)
     name = "qk_norm_rope_backward"
     gq, gk, table, pos, keep = _check(name, q, k, q_norm, k_norm, eps, cos, sin, positions)
     for d, x in ((d_q_rot, q), (d_k_rot, k)):
