@@ -34,6 +34,16 @@ template <int D> struct RowState {
         ref = -INFINITY;
         sum = 0.0f;
     }
+    // A new reference (log2 units), where `top` lies above the old one.
+    __device__ void raise(float top) {
+        const float r = fmaxf(ref, top), f = r == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - r);
+        ref = r;
+        sum *= f;
+#pragma unroll
+        for (int d = 0; d < D / 32; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) acc[d][i] *= f;
+    }
 };
 // MASKED: some row does not see all of the tile.  FINE: the weights enter as two operands, what rounding leaves of them in a second product: for workgroups of
 // at most kFineTiles tiles, whose rows average over too few keys for the roundings of their weights to fade (relative error of dQ, whose row sums are
@@ -65,16 +75,7 @@ __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 
     top = max_halves(top) * c;
     // A new reference only where the old one lies more than 8 below: the weights stay under 2^8, and the sums have
     // room for that; O is multiplied on few tiles instead of on most.
-    if (__any(top > st.ref + 8.0f)) {
-        const float ref = fmaxf(st.ref, top);
-        const float f = ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.ref - ref);
-        st.ref = ref;
-        st.sum *= f;
-#pragma unroll
-        for (int d = 0; d < DB; d++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) st.acc[d][i] *= f;
-    }
+    if (__any(top > st.ref + 8.0f)) st.raise(top);
     const float ref = MASKED && st.ref == -INFINITY ? 0.0f : st.ref;       // (no key so far: every weight is exp2(-inf))
     uint32_t p[NB][8], fine[FINE ? NB : 1][8];
     float part[2] = {0.0f, 0.0f};
@@ -177,26 +178,120 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void window_kernel(Window
     for (int s = 0; s < KS; s++) q[s] = fr.along(smem + L::SLOT + wave * 64 * D, s);
 #pragma unroll
     for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));
-    __syncthreads();                     // the rows' LDS becomes the ring's other slots
-    if (span.n > 1) copy_tile(1, 1);
+    // (the barrier in front of tile 0 also stands in front of what is copied over the rows)
 
     RowState<D> st;
     st.clear();
     const float c = a.scale * kLog2e;
-    int slot = 0;
-    for (int t = 0; t < span.n; t++) {
-        if (t + 1 < span.n) dma_wait<2 * RPW>();
-        else dma_wait<0>();
-        __syncthreads();                 // tile t is visible; every wave is done with the slot of tile t - 1
-        if (t + 2 < span.n) copy_tile(t + 2, slot == 0 ? 2 : slot - 1);
-        const int j0 = span.tile(t) * KT;
-        const uint8_t* kt = smem + slot * L::SLOT;
-        const Seen what = x0 < rows ? seen<KT>(a, wp_lo, wp_hi, len, j0) : Seen::kNone;
-        if (what == Seen::kNone) {
-        } else if (D <= 128 && span.n <= kFineTiles) attend_tile<T, D, KT, true, true>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
-        else if (D <= 128 && what == Seen::kAll) attend_tile<T, D, KT, false, false>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
-        else attend_tile<T, D, KT, true, false>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
-        slot = slot == 2 ? 0 : slot + 1;
+    if (D <= 128 && span.n <= kFineTiles) {
+        for (int t = 0; t < span.n; t++) {
+            dma_wait<0>();
+            __syncthreads();             // tile t is visible
+            if (t + 1 < span.n) copy_tile(t + 1, t + 1);
+            const int j0 = span.tile(t) * KT;
+            const uint8_t* kt = smem + t * L::SLOT;
+            if (x0 < rows && seen<KT>(a, wp_lo, wp_hi, len, j0) != Seen::kNone)
+                attend_tile<T, D, KT, true, true>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
+        }
+    } else {
+        // Blocks of 32 keys, one after the other: the scores of the next block are taken while this one's weights are formed, so that matrix and vector
+        // instructions of a wave overlap; what a block costs either pipe is about the same.  Where a wave takes part in only one of the
+        // two, the other runs on rows that are there anyway, with weights of zero or scores that are dropped: one path, so that O stays where it is.
+        constexpr int NK = KS < 8 ? KS : 8, NV = D < 128 ? D / 32 : 4;
+        uint32_t ka[NK], va[NV][2];      // where the fragments of the tiles in work lie
+        auto keys_at = [&](int slot) {
+            const Fragments<D> f = fr.fresh();
+            const uint32_t at = lds + slot * L::SLOT;
+#pragma unroll
+            for (int s = 0; s < NK; s++) ka[s] = at + (f.nat ^ (s << 5));
+#pragma unroll
+            for (int s = 0; s < NK; s++) asm volatile("" : "+v"(ka[s]));
+        };
+        auto values_at = [&](int slot) {
+            const Fragments<D> f = fr.fresh();
+            const uint32_t at = lds + slot * L::SLOT + L::TILE;
+#pragma unroll
+            for (int d = 0; d < NV; d++) va[d][0] = at + (f.tr[0] ^ (d << 6)), va[d][1] = at + (f.tr[1] ^ (d << 6));
+#pragma unroll
+            for (int d = 0; d < NV; d++) asm volatile("" : "+v"(va[d][0]), "+v"(va[d][1]));
+        };
+        auto step = [&](const v16f& x, bool now, int rows_now, v16f& y, Seen next, int rows_next, int j0) {
+            if (next == Seen::kAll) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) y[i] = 0.0f;
+            } else {                     // (scores that are not seen start, and stay, at -inf)
+                const RowMask rel = next == Seen::kNone ? RowMask{1, -1, 0} : mask.from(j0 + half * 4);
+#pragma unroll
+                for (int i = 0; i < 16; i++) y[i] = rel.sees((i >> 2) * 8 + (i & 3)) ? 0.0f : -INFINITY;
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) y = product<T>(lds_read(ka[ks & 7] + rows_next * 64 * D + (ks >> 3) * 256), q[ks], y);
+            uint32_t w[8];
+            float part[2] = {0.0f, 0.0f};
+            const float ref = !now ? INFINITY : st.ref == -INFINITY ? 0.0f : st.ref;       // (no key so far: every weight is exp2(-inf))
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const float u = __builtin_amdgcn_exp2f(fmaf(x[i], c, -ref)), v = __builtin_amdgcn_exp2f(fmaf(x[i + 1], c, -ref));
+                part[0] += u;
+                part[1] += v;
+                w[i >> 1] = pack2<T>(u, v);
+            }
+            st.sum += part[0] + part[1];
+#pragma unroll
+            for (int j2 = 0; j2 < 2; j2++)
+#pragma unroll
+                for (int d = 0; d < D / 32; d++) {
+                    const int at = (rows_now * 2 + j2) * 32 * D + (d >> 2) * 256;
+                    st.acc[d] = product<T>(lds_read_across(va[d & 3][0] + at, va[d & 3][1] + at),
+                                           v4i{(int)w[j2 * 4], (int)w[j2 * 4 + 1], (int)w[j2 * 4 + 2], (int)w[j2 * 4 + 3]}, st.acc[d]);
+                }
+            float top = y[0];
+#pragma unroll
+            for (int i = 1; i < 16; i++) top = fmaxf(top, y[i]);
+            top = max_halves(top) * c;
+            if (__any(top > st.ref + 8.0f)) st.raise(top);
+        };
+        v16f s[2];
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[0][i] = s[1][i] = -INFINITY;
+        auto seen_at = [&](int t) { return t < span.n && x0 < rows ? seen<KT>(a, wp_lo, wp_hi, len, span.tile(t) * KT) : Seen::kNone; };
+        Seen now = Seen::kNone, next;
+        int slot = 0;                    // of tile t + 1
+        auto arrive = [&](int t) {       // tile t + 1 becomes visible, the slot of tile t - 1 is filled again
+            if (t + 1 < span.n) dma_wait<0>();
+            __syncthreads();
+            if (t + 2 < span.n) copy_tile(t + 2, slot == 2 ? 0 : slot + 1);
+            next = seen_at(t + 1);
+        };
+        auto before = [](int slot) { return slot == 0 ? 2 : slot - 1; };
+        // The wave's second operands where it has none of its own: the other tile's.
+        auto cross = [&](const v16f& x, v16f& y, int rows_now, int t) {
+            const bool has = now != Seen::kNone;
+            if (has || next != Seen::kNone) {
+                keys_at(next != Seen::kNone ? slot : before(slot));
+                if (KT == 32 || !has) values_at(has ? before(slot) : slot);
+                step(x, has, rows_now, y, next, 0, t + 1 < span.n ? span.tile(t + 1) * KT : 0);
+            }
+            now = next;
+            slot = slot == 2 ? 0 : slot + 1;
+        };
+        if constexpr (KT == 64) {
+            for (int t = -1; t < span.n; t++) {
+                if (now != Seen::kNone) {
+                    values_at(before(slot));
+                    step(s[0], true, 0, s[1], now, 1, span.tile(t) * KT + 32);
+                }
+                arrive(t);
+                cross(s[1], s[0], 1, t);
+            }
+        } else {
+            for (int t = -1; t < span.n; t += 2) {           // (a tile past the last: nothing is seen, nothing copied)
+                arrive(t);
+                cross(s[0], s[1], 0, t);
+                arrive(t + 1);
+                cross(s[1], s[0], 0, t + 1);
+            }
+        }
     }
     __syncthreads();                     // (no copy is in flight: the last tile's wait was for all of them)
     if (x0 < rows) finish_rows<T, D>(a, st, smem + wave * 64 * D, b, kvh, x0, lane);

@@ -22,6 +22,14 @@ template <int T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const v2f f = {a, b};
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, v2hf));
 }
+// fragments by their LDS address
+__device__ __forceinline__ v4i lds_read(uint32_t at) { return *(const __attribute__((address_space(3))) v4i*)(uintptr_t)at; }
+__device__ __forceinline__ v4i lds_read_across(uint32_t lo, uint32_t hi) {
+    using lds_v4s = __attribute__((address_space(3))) v4s;
+    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)lo));
+    const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)hi));
+    return v4i{(int)a.x, (int)a.y, (int)b.x, (int)b.y};
+}
 // the other half-wave's value of the same column
 __device__ __forceinline__ float max_halves(float x) {
     const v2u r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
