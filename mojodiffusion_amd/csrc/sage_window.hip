@@ -157,15 +157,24 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void window_kernel(Window
     const uint16_t* kh = a.k + b * a.k_sb + kvh * a.k_sh;
     const uint16_t* vh = a.v + b * a.v_sb + kvh * a.v_sh;
     const uint32_t ks_b = (uint32_t)a.k_sn * 2u, vs_b = (uint32_t)a.v_sn * 2u;
+    uint32_t k_off[RPW], v_off[RPW];     // of this lane's pieces of a tile whose rows are all copied as they are
+#pragma unroll
+    for (int i = 0; i < RPW; i++) k_off[i] = pieces.row(i) * ks_b + pieces.col(i, lane), v_off[i] = pieces.row(i) * vs_b + pieces.col(i, lane);
     auto copy_tile = [&](int t, int slot) {
         const int j0 = span.tile(t) * KT;
         const uint16_t *kb = kh + (int64_t)j0 * a.k_sn, *vb = vh + (int64_t)j0 * a.v_sn;
+        const bool whole = j0 + KT - 1 <= span.hi && (j0 >= span.lo || j0 + KT <= span.s_end);
 #pragma unroll
         for (int i = 0; i < RPW; i++) {
-            const uint32_t row = (uint32_t)(copied_key<KT>(span, j0, j0 + pieces.row(i)) - j0);
+            uint32_t ko = k_off[i], vo = v_off[i];
+            if (!whole) {
+                const uint32_t row = (uint32_t)(copied_key<KT>(span, j0, j0 + pieces.row(i)) - j0);
+                ko = row * ks_b + pieces.col(i, lane);
+                vo = row * vs_b + pieces.col(i, lane);
+            }
             const uint32_t dst = lds + slot * L::SLOT + (i * NW + wave) * 1024;
-            dma16(kb, row * ks_b + pieces.col(i, lane), __builtin_amdgcn_readfirstlane(dst));
-            dma16(vb, row * vs_b + pieces.col(i, lane), __builtin_amdgcn_readfirstlane(dst + L::TILE));
+            dma16(kb, ko, __builtin_amdgcn_readfirstlane(dst));
+            dma16(vb, vo, __builtin_amdgcn_readfirstlane(dst + L::TILE));
         }
     };
 
@@ -216,19 +225,21 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void window_kernel(Window
             for (int d = 0; d < NV; d++) asm volatile("" : "+v"(va[d][0]), "+v"(va[d][1]));
         };
         auto step = [&](const v16f& x, bool now, int rows_now, v16f& y, Seen next, int rows_next, int j0) {
+            const v4i first = lds_read(ka[0] + rows_next * 64 * D);
             if (next == Seen::kAll) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) y[i] = 0.0f;
+                y = product<T>(first, q[0], v16f{});
             } else {                     // (scores that are not seen start, and stay, at -inf)
                 const RowMask rel = next == Seen::kNone ? RowMask{1, -1, 0} : mask.from(j0 + half * 4);
 #pragma unroll
                 for (int i = 0; i < 16; i++) y[i] = rel.sees((i >> 2) * 8 + (i & 3)) ? 0.0f : -INFINITY;
+                y = product<T>(first, q[0], y);
             }
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) y = product<T>(lds_read(ka[ks & 7] + rows_next * 64 * D + (ks >> 3) * 256), q[ks], y);
+            for (int ks = 1; ks < KS; ks++) y = product<T>(lds_read(ka[ks & 7] + rows_next * 64 * D + (ks >> 3) * 256), q[ks], y);
             uint32_t w[8];
             float part[2] = {0.0f, 0.0f};
-            const float ref = !now ? INFINITY : st.ref == -INFINITY ? 0.0f : st.ref;       // (no key so far: every weight is exp2(-inf))
+            // (no key so far: every weight is exp2(-inf); no block now: likewise, by a reference of +inf, without a branch in the middle)
+            const float ref = (st.ref == -INFINITY ? 0.0f : st.ref) + __uint_as_float(0x7F800000u & ((uint32_t)now - 1u));
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
                 const float u = __builtin_amdgcn_exp2f(fmaf(x[i], c, -ref)), v = __builtin_amdgcn_exp2f(fmaf(x[i + 1], c, -ref));
