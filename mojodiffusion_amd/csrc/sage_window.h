@@ -56,8 +56,7 @@ struct WindowArgs {
     float *part, *part_ml;                       // [row block, split, 32, D], [row block, split, 32, 2]
 };
 struct WindowPlan {
-    int waves;                                   // > 0: workgroups of so many waves of 32 rows; 0: keys split
-    int splits;                                  // (of the latter: workgroups that share a block of 32 rows)
+    int splits;                                  // 0: tiles shared by the waves of a workgroup; else the keys split, so many workgroups to a block of 32 rows
 };
 WindowPlan window_plan(const WindowArgs& a);
 bool window_grid_ok(const WindowArgs& a, const WindowPlan& p);

@@ -46,9 +46,9 @@ template <int D> struct RowState {
     }
 };
 // MASKED: some row does not see all of the tile.  FINE: the weights enter as two operands, what rounding leaves of them in a second product: for workgroups of
-// at most kFineTiles tiles, whose rows average over too few keys for the roundings of their weights to fade (relative error of dQ, whose row sums are
+// at most kFineKeys keys, whose rows average over too few keys for the roundings of their weights to fade (relative error of dQ, whose row sums are
 // taken from O, on a padded batch with sinks: 0.0027 without, 0.0024 with it; the products are a small part of what such a workgroup does).
-constexpr int kFineTiles = 2;
+constexpr int kFineKeys = 128;
 template <int T, int D, int KT, bool MASKED, bool FINE>
 __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 16], const uint8_t* kt, const uint8_t* vt, const Fragments<D>& kept,
                                             int j0, const RowMask& m, float c, int half) {
@@ -126,16 +126,29 @@ __device__ __forceinline__ void finish_rows(const WindowArgs& a, const RowState<
     query_rows_out<D>(a, os, a.rest + at, a.o_sn, a.o_sh, x0, lane);
 }
 
-template <int D, int NW> struct WindowLds {
-    static constexpr int KT = D > 128 ? 32 : 64, TILE = KT * D * 2, SLOT = 2 * TILE, SLOTS = 3;
-    static constexpr int OWN = NW * 64 * D;                                // the waves' own rows: behind the first slot, and at the end
-    static constexpr int BYTES = SLOTS * SLOT > SLOT + OWN ? SLOTS * SLOT : SLOT + OWN;
+struct Range {
+    int first;
+    unsigned n;
+    __device__ bool has(int t) const { return (unsigned)(t - first) < n; }
 };
 
-template <int T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void window_kernel(WindowArgs a) {
-    using L = WindowLds<D, NW>;
-    constexpr int KT = L::KT, RPW = TilePieces<D, KT, NW>::N, KS = D / 16;
+// Tiles of 32 keys, two slots for K and two for V, which is needed one step later.  (A third of each: 1620 -> 1662 us at [1,16896,48 on 12,128], 287 -> 320 for one
+// token of 32 sequences: less LDS, more workgroups.)  The waves' own rows lie over all slots but K's first at the start, and over the
+// front again at the end.
+template <int D> struct WindowLds {
+    static constexpr int NW = 4, KT = 32, TILE = KT * D * 2, OWN = NW * 64 * D;
+    static constexpr int K0 = 3 * TILE > OWN ? 3 * TILE : OWN, BYTES = K0 + TILE;
+    static __device__ int keys(int t) { return t & 1 ? 2 * TILE : K0; }
+    static __device__ int values(int t) { return (t & 1) * TILE; }
+};
+
+// Workgroups of four waves, 128 rows: two or more share a compute unit and meet no common barrier, so that one's matrix instructions run
+// beside another's vector instructions (128 channels, us: 8 waves with tiles of 64 keys -> this form: [1,16896,48 on 12] window 4096 + 4 1683 -> 1673, a
+// step of [2,1248,30] window +-256 201 -> 190, one token of 32 sequences against 8192 keys 361 -> 287).
+template <int T, int D>
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void window_kernel(WindowArgs a) {
+    using L = WindowLds<D>;
+    constexpr int NW = L::NW, KT = L::KT, RPW = TilePieces<D, KT, NW>::N, KS = D / 16;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
     const int rows = a.Sq * a.g, blocks = (rows + NW * 32 - 1) / (NW * 32);
     const int item = xcd_item((int)blockIdx.x, a.B * a.Hk * blocks);
@@ -154,157 +167,174 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void window_kernel(Window
 
     const TilePieces<D, KT, NW> pieces(wave, lane);
     const uint32_t lds = lds_addr(smem);
-    const uint16_t* kh = a.k + b * a.k_sb + kvh * a.k_sh;
-    const uint16_t* vh = a.v + b * a.v_sb + kvh * a.v_sh;
-    const uint32_t ks_b = (uint32_t)a.k_sn * 2u, vs_b = (uint32_t)a.v_sn * 2u;
-    uint32_t k_off[RPW], v_off[RPW];     // of this lane's pieces of a tile whose rows are all copied as they are
+    // What every tile of a walk asks is answered ahead, for the tiles of the window: which of them are copied whole, which this wave sees all of.
+    auto tiles_within = [&](int lo, int hi) {        // those whose keys all lie in lo .. hi, as (index of the first, number)
+        const int t0 = max((max(lo, 0) + KT - 1) / KT, span.next), t1 = hi + 1 < KT ? span.next : (hi + 1) / KT;
+        return Range{t0 - span.next + span.first, (unsigned)max(t1 - t0, 0)};
+    };
+    const Range whole = tiles_within(span.lo, span.hi);
+    const Range all = tiles_within(wp_hi - a.left, x0 < rows ? min(wp_lo + a.right, len - 1) : -1);
+    struct Rows {                        // K or V: the tile to be copied next, and its lane's pieces where it is copied whole
+        const uint16_t* at;
+        int64_t tile;
+        uint32_t sn, off[RPW];
+    };
+    auto rows_of = [&](const uint16_t* head, int64_t sn) {
+        Rows r;
+        r.at = head + (int64_t)span.tile(0) * KT * sn;
+        r.tile = KT * sn;
+        r.sn = (uint32_t)sn * 2u;
 #pragma unroll
-    for (int i = 0; i < RPW; i++) k_off[i] = pieces.row(i) * ks_b + pieces.col(i, lane), v_off[i] = pieces.row(i) * vs_b + pieces.col(i, lane);
-    auto copy_tile = [&](int t, int slot) {
-        const int j0 = span.tile(t) * KT;
-        const uint16_t *kb = kh + (int64_t)j0 * a.k_sn, *vb = vh + (int64_t)j0 * a.v_sn;
-        const bool whole = j0 + KT - 1 <= span.hi && (j0 >= span.lo || j0 + KT <= span.s_end);
+        for (int i = 0; i < RPW; i++) r.off[i] = pieces.row(i) * r.sn + pieces.col(i, lane);
+        return r;
+    };
+    Rows k = rows_of(a.k + b * a.k_sb + kvh * a.k_sh, a.k_sn), v = rows_of(a.v + b * a.v_sb + kvh * a.v_sh, a.v_sn);
+    auto copy = [&](Rows& r, int t, int to) {
 #pragma unroll
         for (int i = 0; i < RPW; i++) {
-            uint32_t ko = k_off[i], vo = v_off[i];
-            if (!whole) {
-                const uint32_t row = (uint32_t)(copied_key<KT>(span, j0, j0 + pieces.row(i)) - j0);
-                ko = row * ks_b + pieces.col(i, lane);
-                vo = row * vs_b + pieces.col(i, lane);
+            uint32_t off = r.off[i];
+            if (!whole.has(t)) {
+                const int j0 = span.tile(t) * KT;
+                off = (uint32_t)(copied_key<KT>(span, j0, j0 + pieces.row(i)) - j0) * r.sn + pieces.col(i, lane);
             }
-            const uint32_t dst = lds + slot * L::SLOT + (i * NW + wave) * 1024;
-            dma16(kb, ko, __builtin_amdgcn_readfirstlane(dst));
-            dma16(vb, vo, __builtin_amdgcn_readfirstlane(dst + L::TILE));
+            dma16(r.at, off, __builtin_amdgcn_readfirstlane(lds + to + (i * NW + wave) * 1024));
         }
+        r.at += (t + 1 == span.first ? span.next - t : 1) * r.tile;      // (from the tiles with sinks to the window's)
     };
 
     v4i q[KS];
     const Fragments<D> fr(lane);
-    query_rows_in<D>(a, a.q + b * a.q_sb + (int64_t)kvh * a.g * a.q_sh + (int64_t)i_lo * a.q_sn, a.q_sn, a.q_sh, i_lo, x0, lds + L::SLOT + wave * 64 * D, lane);
-    if (span.n > 0) copy_tile(0, 0);
+    query_rows_in<D>(a, a.q + b * a.q_sb + (int64_t)kvh * a.g * a.q_sh + (int64_t)i_lo * a.q_sn, a.q_sn, a.q_sh, i_lo, x0, lds + wave * 64 * D, lane);
+    if (span.n > 0) copy(k, 0, L::keys(0));
     dma_wait<0>();
 #pragma unroll
-    for (int s = 0; s < KS; s++) q[s] = fr.along(smem + L::SLOT + wave * 64 * D, s);
+    for (int s = 0; s < KS; s++) q[s] = fr.along(smem + wave * 64 * D, s);
 #pragma unroll
-    for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));
-    // (the barrier in front of tile 0 also stands in front of what is copied over the rows)
+    for (int s = 0; s < KS; s++) {
+        if constexpr (D > 128) asm volatile("" : "+a"(q[s]));          // (room among the vector registers: the products read them there too)
+        else asm volatile("" : "+v"(q[s]));
+    }
+    __syncthreads();                     // the rows' LDS becomes the rings' slots
 
     RowState<D> st;
     st.clear();
     const float c = a.scale * kLog2e;
-    if (D <= 128 && span.n <= kFineTiles) {
+    if (D <= 128 && span.n * KT <= kFineKeys) {
         for (int t = 0; t < span.n; t++) {
+            if (t > 0) {
+                __syncthreads();         // every wave is done with tile t - 1
+                copy(k, t, L::keys(0));
+            }
+            copy(v, t, L::values(0));
             dma_wait<0>();
-            __syncthreads();             // tile t is visible
-            if (t + 1 < span.n) copy_tile(t + 1, t + 1);
+            __syncthreads();
             const int j0 = span.tile(t) * KT;
-            const uint8_t* kt = smem + t * L::SLOT;
             if (x0 < rows && seen<KT>(a, wp_lo, wp_hi, len, j0) != Seen::kNone)
-                attend_tile<T, D, KT, true, true>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
+                attend_tile<T, D, KT, true, true>(st, q, smem + L::keys(0), smem + L::values(0), fr, j0, mask, c, half);
         }
     } else {
-        // Blocks of 32 keys, one after the other: the scores of the next block are taken while this one's weights are formed, so that matrix and vector
-        // instructions of a wave overlap; what a block costs either pipe is about the same.  Where a wave takes part in only one of the
-        // two, the other runs on rows that are there anyway, with weights of zero or scores that are dropped: one path, so that O stays where it is.
+        // One tile after the other: the scores of the next are taken while this one's weights are formed, so that matrix and vector instructions of a
+        // wave overlap; what a tile costs either pipe is about the same.  Where a wave takes part in only one of the two, the other runs on
+        // rows that are there anyway, with weights of zero or scores that are dropped: one path, so that O stays where it is.
         constexpr int NK = KS < 8 ? KS : 8, NV = D < 128 ? D / 32 : 4;
-        uint32_t ka[NK], va[NV][2];      // where the fragments of the tiles in work lie
-        auto keys_at = [&](int slot) {
+        auto step = [&](const v16f& x, bool now, uint32_t values, v16f& y, Seen next, uint32_t keys, int j0) {
             const Fragments<D> f = fr.fresh();
-            const uint32_t at = lds + slot * L::SLOT;
+            uint32_t ka[NK], va[NV][2];  // where the fragments lie
 #pragma unroll
-            for (int s = 0; s < NK; s++) ka[s] = at + (f.nat ^ (s << 5));
+            for (int s = 0; s < NK; s++) ka[s] = keys + (f.nat ^ (s << 5));
 #pragma unroll
-            for (int s = 0; s < NK; s++) asm volatile("" : "+v"(ka[s]));
-        };
-        auto values_at = [&](int slot) {
-            const Fragments<D> f = fr.fresh();
-            const uint32_t at = lds + slot * L::SLOT + L::TILE;
+            for (int d = 0; d < NV; d++) va[d][0] = values + (f.tr[0] ^ (d << 6)), va[d][1] = values + (f.tr[1] ^ (d << 6));
+            // Products in groups of four, the operands of a group requested a group ahead; the scheduler keeps to the groups where there is no second
+            // wave on the SIMD to run meanwhile (256 channels: 207 -> 162 us at [1,4429,18,256] window +-511).
+            constexpr int NG = KS / 4, DB = D / 32, NP = 2 * DB / 4;
+            constexpr bool ALONE = D > 128;
+            v4i f4[2][4];
+            auto request_k = [&](int g) {
 #pragma unroll
-            for (int d = 0; d < NV; d++) va[d][0] = at + (f.tr[0] ^ (d << 6)), va[d][1] = at + (f.tr[1] ^ (d << 6));
+                for (int i = 0; i < 4; i++) f4[g & 1][i] = lds_read(ka[(g * 4 + i) & 7] + (g >> 1) * 256);
+            };
+            auto request_v = [&](int g) {
 #pragma unroll
-            for (int d = 0; d < NV; d++) asm volatile("" : "+v"(va[d][0]), "+v"(va[d][1]));
-        };
-        auto step = [&](const v16f& x, bool now, int rows_now, v16f& y, Seen next, int rows_next, int j0) {
-            const v4i first = lds_read(ka[0] + rows_next * 64 * D);
+                for (int i = 0; i < 4; i++) {
+                    const int j2 = (g * 4 + i) / DB, d = (g * 4 + i) % DB, at = j2 * 32 * D + (d >> 2) * 256;
+                    f4[(NG + g) & 1][i] = lds_read_across(va[d & 3][0] + at, va[d & 3][1] + at);
+                }
+            };
+            auto group_ends = [] {
+                if constexpr (ALONE) __builtin_amdgcn_sched_barrier(0);
+            };
+            request_k(0);
             if (next == Seen::kAll) {
-                y = product<T>(first, q[0], v16f{});
+                y = product<T>(f4[0][0], q[0], v16f{});
             } else {                     // (scores that are not seen start, and stay, at -inf)
                 const RowMask rel = next == Seen::kNone ? RowMask{1, -1, 0} : mask.from(j0 + half * 4);
 #pragma unroll
                 for (int i = 0; i < 16; i++) y[i] = rel.sees((i >> 2) * 8 + (i & 3)) ? 0.0f : -INFINITY;
-                y = product<T>(first, q[0], y);
+                y = product<T>(f4[0][0], q[0], y);
             }
-#pragma unroll
-            for (int ks = 1; ks < KS; ks++) y = product<T>(lds_read(ka[ks & 7] + rows_next * 64 * D + (ks >> 3) * 256), q[ks], y);
             uint32_t w[8];
             float part[2] = {0.0f, 0.0f};
-            // (no key so far: every weight is exp2(-inf); no block now: likewise, by a reference of +inf, without a branch in the middle)
+            // (no key so far: every weight is exp2(-inf); no tile now: likewise, by a reference of +inf, without a branch in the middle)
             const float ref = (st.ref == -INFINITY ? 0.0f : st.ref) + __uint_as_float(0x7F800000u & ((uint32_t)now - 1u));
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float u = __builtin_amdgcn_exp2f(fmaf(x[i], c, -ref)), v = __builtin_amdgcn_exp2f(fmaf(x[i + 1], c, -ref));
-                part[0] += u;
-                part[1] += v;
-                w[i >> 1] = pack2<T>(u, v);
+            for (int g = 0; g < NG; g++) {
+                if (g + 1 < NG) request_k(g + 1);
+                else request_v(0);
+#pragma unroll
+                for (int i = g == 0; i < 4; i++) y = product<T>(f4[g & 1][i], q[g * 4 + i], y);
+#pragma unroll
+                for (int i = g * (16 / NG); i < (g + 1) * (16 / NG); i += 2) {
+                    const float u = __builtin_amdgcn_exp2f(fmaf(x[i], c, -ref)), v = __builtin_amdgcn_exp2f(fmaf(x[i + 1], c, -ref));
+                    part[0] += u;
+                    part[1] += v;
+                    w[i >> 1] = pack2<T>(u, v);
+                }
+                group_ends();
             }
             st.sum += part[0] + part[1];
-#pragma unroll
-            for (int j2 = 0; j2 < 2; j2++)
-#pragma unroll
-                for (int d = 0; d < D / 32; d++) {
-                    const int at = (rows_now * 2 + j2) * 32 * D + (d >> 2) * 256;
-                    st.acc[d] = product<T>(lds_read_across(va[d & 3][0] + at, va[d & 3][1] + at),
-                                           v4i{(int)w[j2 * 4], (int)w[j2 * 4 + 1], (int)w[j2 * 4 + 2], (int)w[j2 * 4 + 3]}, st.acc[d]);
-                }
             float top = y[0];
 #pragma unroll
-            for (int i = 1; i < 16; i++) top = fmaxf(top, y[i]);
+            for (int g = 0; g < NP; g++) {
+                if (g + 1 < NP) request_v(g + 1);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int j2 = (g * 4 + i) / DB, d = (g * 4 + i) % DB;
+                    st.acc[d] = product<T>(f4[(NG + g) & 1][i], v4i{(int)w[j2 * 4], (int)w[j2 * 4 + 1], (int)w[j2 * 4 + 2], (int)w[j2 * 4 + 3]}, st.acc[d]);
+                }
+                if (g == NP - 1) {
+#pragma unroll
+                    for (int i = 1; i < 16; i++) top = fmaxf(top, y[i]);
+                }
+                group_ends();
+            }
             top = max_halves(top) * c;
             if (__any(top > st.ref + 8.0f)) st.raise(top);
         };
         v16f s[2];
 #pragma unroll
         for (int i = 0; i < 16; i++) s[0][i] = s[1][i] = -INFINITY;
-        auto seen_at = [&](int t) { return t < span.n && x0 < rows ? seen<KT>(a, wp_lo, wp_hi, len, span.tile(t) * KT) : Seen::kNone; };
-        Seen now = Seen::kNone, next;
-        int slot = 0;                    // of tile t + 1
-        auto arrive = [&](int t) {       // tile t + 1 becomes visible, the slot of tile t - 1 is filled again
-            if (t + 1 < span.n) dma_wait<0>();
-            __syncthreads();
-            if (t + 2 < span.n) copy_tile(t + 2, slot == 2 ? 0 : slot + 1);
-            next = seen_at(t + 1);
-        };
-        auto before = [](int slot) { return slot == 0 ? 2 : slot - 1; };
-        // The wave's second operands where it has none of its own: the other tile's.
-        auto cross = [&](const v16f& x, v16f& y, int rows_now, int t) {
-            const bool has = now != Seen::kNone;
-            if (has || next != Seen::kNone) {
-                keys_at(next != Seen::kNone ? slot : before(slot));
-                if (KT == 32 || !has) values_at(has ? before(slot) : slot);
-                step(x, has, rows_now, y, next, 0, t + 1 < span.n ? span.tile(t + 1) * KT : 0);
+        Seen now = Seen::kNone;
+        auto tile = [&](const v16f& x, v16f& y, int t) {
+            dma_wait<0>();
+            __syncthreads();             // K of tile t + 1 and V of tile t are visible; every wave is done with K of t and V of t - 1
+            if (t + 2 < span.n) copy(k, t + 2, L::keys(t));
+            if (t + 1 < span.n) copy(v, t + 1, L::values(t + 1));
+            Seen next = Seen::kNone;
+            if (all.has(t + 1)) next = Seen::kAll;
+            else if (t + 1 < span.n && x0 < rows) next = seen<KT>(a, wp_lo, wp_hi, len, span.tile(t + 1) * KT);
+            const bool has = now != Seen::kNone, comes = next != Seen::kNone;
+            if (has || comes) {
+                const uint32_t keys = lds + L::keys(t + 1), values = lds + L::values(t);
+                step(x, has, has ? values : keys, y, next, comes ? keys : values, comes ? span.tile(t + 1) * KT : 0);
             }
             now = next;
-            slot = slot == 2 ? 0 : slot + 1;
         };
-        if constexpr (KT == 64) {
-            for (int t = -1; t < span.n; t++) {
-                if (now != Seen::kNone) {
-                    values_at(before(slot));
-                    step(s[0], true, 0, s[1], now, 1, span.tile(t) * KT + 32);
-                }
-                arrive(t);
-                cross(s[1], s[0], 1, t);
-            }
-        } else {
-            for (int t = -1; t < span.n; t += 2) {           // (a tile past the last: nothing is seen, nothing copied)
-                arrive(t);
-                cross(s[0], s[1], 0, t);
-                arrive(t + 1);
-                cross(s[1], s[0], 0, t + 1);
-            }
+        for (int t = -1; t < span.n; t += 2) {               // (a tile past the last: nothing is seen, nothing copied)
+            tile(s[0], s[1], t);
+            tile(s[1], s[0], t + 1);
         }
     }
-    __syncthreads();                     // (no copy is in flight: the last tile's wait was for all of them)
+    __syncthreads();                     // (no copy is in flight: the last step's wait was for all of them)
     if (x0 < rows) finish_rows<T, D>(a, st, smem + wave * 64 * D, b, kvh, x0, lane);
 }
 
@@ -403,7 +433,7 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
         }
         const int j0 = span.tile(t) * KT;
         const uint8_t* kt = own + slot * L::SLOT;
-        if (D <= 128 && span.n <= kFineTiles * 2) attend_tile<T, D, KT, true, true>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
+        if (D <= 128 && span.n * KT <= kFineKeys) attend_tile<T, D, KT, true, true>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
         else if (D <= 128 && seen<KT>(a, p_lo, p_hi, len, j0) == Seen::kAll) attend_tile<T, D, KT, false, false>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
         else attend_tile<T, D, KT, true, false>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
         if (L::SLOTS == 2) slot ^= 1;
@@ -508,9 +538,7 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
 int64_t row_blocks(const WindowArgs& a, int rows) { return (int64_t)a.B * a.Hk * (((int64_t)a.Sq * a.g + rows - 1) / rows); }
 
 template <int T, int D> hipError_t launch_td(const WindowArgs& a, const WindowPlan& p, hipStream_t st) {
-    if (p.waves == 8) {
-        if constexpr (D <= 128) hipLaunchKernelGGL((window_kernel<T, D, 8>), dim3((unsigned)row_blocks(a, 256)), dim3(512), 0, st, a);
-    } else if (p.waves == 4) hipLaunchKernelGGL((window_kernel<T, D, 4>), dim3((unsigned)row_blocks(a, 128)), dim3(256), 0, st, a);
+    if (!p.splits) hipLaunchKernelGGL((window_kernel<T, D>), dim3((unsigned)row_blocks(a, 128)), dim3(256), 0, st, a);
     else {
         hipLaunchKernelGGL((window_split_kernel<T, D>), dim3((unsigned)(row_blocks(a, 32) * a.splits)), dim3(256), 0, st, a);
         if (a.splits > 1)
@@ -526,21 +554,21 @@ template <int T> hipError_t launch_t(const WindowArgs& a, const WindowPlan& p, h
 
 }  // namespace
 
-// Rows enough for half the chip: tiles shared by 4 or 8 waves.  Else the keys are split until there are four workgroups to every
+// Rows enough for half the chip, or too many of them: tiles shared by four waves.  Else the keys are split until there are four workgroups to every
 // compute unit, down to 4 tiles (one to a wave).
 WindowPlan window_plan(const WindowArgs& a) {
     constexpr int64_t kUnits = 256;
-    if (row_blocks(a, 128) >= kUnits / 2 || a.Sq * (int64_t)a.g > 512) return WindowPlan{a.D <= 128 && row_blocks(a, 256) >= kUnits ? 8 : 4, 1};
+    if (row_blocks(a, 128) >= kUnits / 2 || a.Sq * (int64_t)a.g > 512) return WindowPlan{0};
     const int64_t keys = a.right >= kWindowFar || a.left >= kWindowFar ? a.Skv
                                                                        : std::min<int64_t>(a.Skv, (int64_t)a.left + a.right + 32 / a.g + 1 + a.sinks);
     const int64_t most = std::max<int64_t>(1, keys / 128), want = (4 * kUnits + row_blocks(a, 32) - 1) / row_blocks(a, 32);
-    return WindowPlan{0, (int)std::min(most, want)};
+    return WindowPlan{(int)std::min(most, want)};
 }
 bool window_grid_ok(const WindowArgs& a, const WindowPlan& p) {
-    return row_blocks(a, 32) * p.splits <= 0x7FFFFFFF && (int64_t)a.B * a.Hk * a.Sq * a.g <= 0x7FFFFFFF;
+    return row_blocks(a, 32) * std::max(p.splits, 1) <= 0x7FFFFFFF && (int64_t)a.B * a.Hk * a.Sq * a.g <= 0x7FFFFFFF;
 }
 size_t window_part_bytes(const WindowArgs& a, const WindowPlan& p) {
-    return p.waves || p.splits == 1 ? 0 : (size_t)row_blocks(a, 32) * p.splits * 32 * (a.D + 2) * sizeof(float);
+    return p.splits <= 1 ? 0 : (size_t)row_blocks(a, 32) * p.splits * 32 * (a.D + 2) * sizeof(float);
 }
 
 hipError_t launch_window(const WindowArgs& a, const WindowPlan& p, hipStream_t st) {
