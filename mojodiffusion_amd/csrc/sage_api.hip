@@ -1241,7 +1241,7 @@ static int window_dims(const char* name, int B, int Hq, int Hk, int N_q, int N_k
     if (Hq % Hk || left < -1 || right < -1 || sinks < 0 || !(scale > 0.0f) || !(scale < INFINITY)) return MI355_SAGE_EINVAL;
     if (type != MI355_SAGE_BF16 && type != MI355_SAGE_FP16) { SAGE_LOG("%s: bf16 or fp16", name); return MI355_SAGE_EUNSUPPORTED; }
     if (!dims_ok(D)) { SAGE_LOG("%s: head dim %d not supported (64, 128 or 256)", name, D); return MI355_SAGE_EUNSUPPORTED; }
-    if (N_q > kWindowStart / 2 || N_kv > kWindowStart || (int64_t)N_q * (Hq / Hk) > 1 << 30 || q_start > kWindowStart || q_start < -kWindowStart) {
+    if (N_q > kWindowStart / 2 || N_kv > kWindowStart || (int64_t)B * Hq * pad_to(N_q, 64) > 1 << 29 || (int64_t)N_q * (Hq / Hk) > 1 << 30 || q_start > kWindowStart || q_start < -kWindowStart) {
         SAGE_LOG("%s: lengths or positions too large", name);
         return MI355_SAGE_EUNSUPPORTED;
     }
@@ -1335,7 +1335,7 @@ static WindowBwdCarve window_bwd_carve(WindowBwdArgs* a) {
     WindowBwdCarve c{};
     c.delta = align_up(rows);
     c.part = c.delta + align_up(rows);
-    c.total = c.part + align_up((size_t)window_bwd_parts(*a) * 2 * 128 * a->w.D * sizeof(float));
+    c.total = c.part + align_up((size_t)window_bwd_parts(*a) * 2 * kWindowBwdKeys * a->w.D * sizeof(float));
     return c;
 }
 

@@ -126,12 +126,6 @@ __device__ __forceinline__ void finish_rows(const WindowArgs& a, const RowState<
     query_rows_out<D>(a, os, a.rest + at, a.o_sn, a.o_sh, x0, lane);
 }
 
-struct Range {
-    int first;
-    unsigned n;
-    __device__ bool has(int t) const { return (unsigned)(t - first) < n; }
-};
-
 // Tiles of 32 keys, two slots for K and two for V, which is needed one step later.  (A third of each: 1620 -> 1662 us at [1,16896,48 on 12,128], 287 -> 320 for one
 // token of 32 sequences: less LDS, more workgroups.)  The waves' own rows lie over all slots but K's first at the start, and over the
 // front again at the end.
@@ -148,7 +142,7 @@ template <int D> struct WindowLds {
 template <int T, int D>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void window_kernel(WindowArgs a) {
     using L = WindowLds<D>;
-    constexpr int NW = L::NW, KT = L::KT, RPW = TilePieces<D, KT, NW>::N, KS = D / 16;
+    constexpr int NW = L::NW, KT = L::KT, KS = D / 16;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
     const int rows = a.Sq * a.g, blocks = (rows + NW * 32 - 1) / (NW * 32);
     const int item = xcd_item((int)blockIdx.x, a.B * a.Hk * blocks);
@@ -165,47 +159,15 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void window_kernel(WindowArgs
     const int p = p0 + min(x0 + (lane & 31), rows - 1) / a.g;
     const RowMask mask = {p - a.left, min(p + a.right, len - 1), a.sinks};
 
-    const TilePieces<D, KT, NW> pieces(wave, lane);
     const uint32_t lds = lds_addr(smem);
-    // What every tile of a walk asks is answered ahead, for the tiles of the window: which of them are copied whole, which this wave sees all of.
-    auto tiles_within = [&](int lo, int hi) {        // those whose keys all lie in lo .. hi, as (index of the first, number)
-        const int t0 = max((max(lo, 0) + KT - 1) / KT, span.next), t1 = hi + 1 < KT ? span.next : (hi + 1) / KT;
-        return Range{t0 - span.next + span.first, (unsigned)max(t1 - t0, 0)};
-    };
-    const Range whole = tiles_within(span.lo, span.hi);
-    const Range all = tiles_within(wp_hi - a.left, x0 < rows ? min(wp_lo + a.right, len - 1) : -1);
-    struct Rows {                        // K or V: the tile to be copied next, and its lane's pieces where it is copied whole
-        const uint16_t* at;
-        int64_t tile;
-        uint32_t sn, off[RPW];
-    };
-    auto rows_of = [&](const uint16_t* head, int64_t sn) {
-        Rows r;
-        r.at = head + (int64_t)span.tile(0) * KT * sn;
-        r.tile = KT * sn;
-        r.sn = (uint32_t)sn * 2u;
-#pragma unroll
-        for (int i = 0; i < RPW; i++) r.off[i] = pieces.row(i) * r.sn + pieces.col(i, lane);
-        return r;
-    };
-    Rows k = rows_of(a.k + b * a.k_sb + kvh * a.k_sh, a.k_sn), v = rows_of(a.v + b * a.v_sb + kvh * a.v_sh, a.v_sn);
-    auto copy = [&](Rows& r, int t, int to) {
-#pragma unroll
-        for (int i = 0; i < RPW; i++) {
-            uint32_t off = r.off[i];
-            if (!whole.has(t)) {
-                const int j0 = span.tile(t) * KT;
-                off = (uint32_t)(copied_key<KT>(span, j0, j0 + pieces.row(i)) - j0) * r.sn + pieces.col(i, lane);
-            }
-            dma16(r.at, off, __builtin_amdgcn_readfirstlane(lds + to + (i * NW + wave) * 1024));
-        }
-        r.at += (t + 1 == span.first ? span.next - t : 1) * r.tile;      // (from the tiles with sinks to the window's)
-    };
+    const KeyTiles<D, NW> tiles(span, lds, wave, lane);
+    const Range all = tiles.within(wp_hi - a.left, x0 < rows ? min(wp_lo + a.right, len - 1) : -1);       // which this wave sees all of
+    auto k = tiles.rows(a.k + b * a.k_sb + kvh * a.k_sh, a.k_sn), v = tiles.rows(a.v + b * a.v_sb + kvh * a.v_sh, a.v_sn);
 
     v4i q[KS];
     const Fragments<D> fr(lane);
     query_rows_in<D>(a, a.q + b * a.q_sb + (int64_t)kvh * a.g * a.q_sh + (int64_t)i_lo * a.q_sn, a.q_sn, a.q_sh, i_lo, x0, lds + wave * 64 * D, lane);
-    if (span.n > 0) copy(k, 0, L::keys(0));
+    if (span.n > 0) tiles.copy(k, 0, L::keys(0));
     dma_wait<0>();
 #pragma unroll
     for (int s = 0; s < KS; s++) q[s] = fr.along(smem + wave * 64 * D, s);
@@ -223,9 +185,9 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void window_kernel(WindowArgs
         for (int t = 0; t < span.n; t++) {
             if (t > 0) {
                 __syncthreads();         // every wave is done with tile t - 1
-                copy(k, t, L::keys(0));
+                tiles.copy(k, t, L::keys(0));
             }
-            copy(v, t, L::values(0));
+            tiles.copy(v, t, L::values(0));
             dma_wait<0>();
             __syncthreads();
             const int j0 = span.tile(t) * KT;
@@ -317,8 +279,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void window_kernel(WindowArgs
         auto tile = [&](const v16f& x, v16f& y, int t) {
             dma_wait<0>();
             __syncthreads();             // K of tile t + 1 and V of tile t are visible; every wave is done with K of t and V of t - 1
-            if (t + 2 < span.n) copy(k, t + 2, L::keys(t));
-            if (t + 1 < span.n) copy(v, t + 1, L::values(t + 1));
+            if (t + 2 < span.n) tiles.copy(k, t + 2, L::keys(t));
+            if (t + 1 < span.n) tiles.copy(v, t + 1, L::values(t + 1));
             Seen next = Seen::kNone;
             if (all.has(t + 1)) next = Seen::kAll;
             else if (t + 1 < span.n && x0 < rows) next = seen<KT>(a, wp_lo, wp_hi, len, span.tile(t + 1) * KT);

@@ -7,7 +7,7 @@
 //
 // Launch 1: Delta_i (from O with what rounding left of it, where the caller kept that) and L_i log2(e).  Launch 2: one grid of two kinds of workgroups, as the full backward's (sage_bwd.hip, whose
 // reasons for tiles, rings and the order of the work hold here): owners of rows, that walk the key tiles their window reaches -> dQ; and owners of
-// 128 keys, that walk the (head, query tile) pairs that reach them -> dK, dV.  Blocks with sinks are reached by every later query; their
+// 64 keys, that walk the (head, query tile) pairs that reach them -> dK, dV.  Blocks with sinks are reached by every later query; their
 // pairs are dealt to as many workgroups as keep the longest of them near the others, which leave fp32 parts for launch 3
 // to add up in order.  The same where there are too few key blocks to fill the chip.
 #include "sage_grid.h"
@@ -22,9 +22,8 @@ namespace {
 
 typedef __fp16 v2fp __attribute__((ext_vector_type(2)));
 
-template <int D> constexpr int kWaves = D > 64 ? 8 : 4;
-constexpr int kKeysWg = 128;
-template <int D> constexpr int kRowsWg = kWaves<D> * 32;
+constexpr int kWaves = 4, kRowsWg = kWaves * 32;
+constexpr int kKeysWg = kWindowBwdKeys;                          // (pairs of waves share 32 keys)
 
 template <int T> __device__ __forceinline__ float widen(uint32_t w, int i) {
     if constexpr (T == kBF16) return __uint_as_float(i ? w & 0xFFFF0000u : w << 16);
@@ -60,58 +59,48 @@ __global__ __launch_bounds__(256) void window_bwd_prep_kernel(WindowBwdArgs a) {
     }
 }
 
-// What the two passes see of a tile of y rows.
-template <int D> struct PassLds {
-    static constexpr int TILE = 64 * D * 2, SLOT = 2 * TILE, SLOTS = 3;
-    static constexpr int ROWS = 2048;                // [slot][lse | -Delta][64], of query tiles
-};
+// Both passes walk tiles of 32 rows, one after the other, and scores of pairs that do not see each other start, and stay, at -inf.  What hides the
+// latencies of a tile (scores, exponentials, products, each waiting for the one before) is other workgroups' waves on the same SIMD: four of them at
+// 64 channels, two at 128, where a wave's operands and sums alone are 128 and more registers.  (64 channels, [2,8192,24 on 8] window 1024 + 4, forward
+// and backward, us: two waves with the next tile's scores taken beside this one's exponentials 732; three 645; four, with the pairs below, 635.)
 
-// ---- dQ: owners of 32 rows per wave, key tiles ---------------------------------------------------------------
+// ---- dQ: owners of rows, key tiles ------------------------------------------------------------------------------
+// Two slots of K and V.  The owners' rows lie over the second at the start, and on their way out over the front.
 template <int D> struct DqLds {
-    static constexpr int SLOT = PassLds<D>::SLOT, OWN = kWaves<D> * 2 * 64 * D;
-    static constexpr int CENTRE = 3 * SLOT, GROUPS = kWaves<D> * 64 / D;         // sums of a tile's keys, [group of rows][D] floats
-    static constexpr int BYTES = CENTRE + GROUPS * D * 4 > SLOT + OWN ? CENTRE + GROUPS * D * 4 : SLOT + OWN;
+    static constexpr int TILE = 32 * D * 2, OWN = kWaves * 2 * 64 * D;
+    static constexpr int CENTRE = 4 * TILE, GROUPS = kWaves * 64 / D;       // sums of a tile's keys, [group of rows][D] floats
+    static constexpr int BYTES = OWN + 2 * TILE;
+    static __device__ int keys(int t) { return t & 1 ? 0 : OWN; }
+    static __device__ int values(int t) { return keys(t) + TILE; }
+    static_assert(CENTRE + GROUPS * D * 4 <= OWN && kWaves * 64 * D <= CENTRE, "the centre lies behind the second slot and behind the rows on their way out");
 };
 
 template <int T, int D>
 __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, int bh, int row0) {
-    using L = PassLds<D>;
-    using DL = DqLds<D>;
-    constexpr int NW = kWaves<D>, CPR = D / 8, RPW = TilePieces<D, 64, NW>::N, KS = D / 16, DB = D / 32;
+    using L = DqLds<D>;
+    constexpr int NW = kWaves, CPR = D / 8, KS = D / 16, DB = D / 32;
     const WindowArgs& w = a.w;
     const int rows = w.Sq * w.g, H = w.Hk * w.g;
     const int b = bh / w.Hk, kvh = bh % w.Hk;
-    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l32 = lane & 31;
+    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int x0 = row0 + wave * 32, x = min(x0 + l32, rows - 1), i = x / w.g, hg = x - i * w.g;
     const int len = sequence_len(w, b), p0 = first_position(w, b, len);
     const int i_lo = row0 / w.g;
-    const Span span = key_span<64>(w, p0 + i_lo, p0 + (min(row0 + NW * 32, rows) - 1) / w.g, len);
+    const Span span = key_span<32>(w, p0 + i_lo, p0 + (min(row0 + NW * 32, rows) - 1) / w.g, len);
     const int wp_lo = p0 + min(x0, rows - 1) / w.g, wp_hi = p0 + min(x0 + 31, rows - 1) / w.g;
     const RowMask mask = {p0 + i - w.left, min(p0 + i + w.right, len - 1), w.sinks};
 
-    const TilePieces<D, 64, NW> pieces(wave, lane);
     const uint32_t lds = lds_addr(smem);
-    const uint16_t* kh = w.k + b * w.k_sb + kvh * w.k_sh;
-    const uint16_t* vh = w.v + b * w.v_sb + kvh * w.v_sh;
-    const uint32_t ks_b = (uint32_t)w.k_sn * 2u, vs_b = (uint32_t)w.v_sn * 2u;
-    auto copy_tile = [&](int t, int slot) {
-        const int j0 = span.tile(t) * 64;
-        const uint16_t *kb = kh + (int64_t)j0 * w.k_sn, *vb = vh + (int64_t)j0 * w.v_sn;
-#pragma unroll
-        for (int n = 0; n < RPW; n++) {
-            const uint32_t row = (uint32_t)(copied_key<64>(span, j0, j0 + pieces.row(n)) - j0);
-            const uint32_t dst = lds + slot * L::SLOT + (n * NW + wave) * 1024;
-            dma16(kb, row * ks_b + pieces.col(n, lane), __builtin_amdgcn_readfirstlane(dst));
-            dma16(vb, row * vs_b + pieces.col(n, lane), __builtin_amdgcn_readfirstlane(dst + L::TILE));
-        }
-    };
+    const KeyTiles<D, NW> tiles(span, lds, wave, lane);
+    const Range all = tiles.within(wp_hi - w.left, x0 < rows ? min(wp_lo + w.right, len - 1) : -1);
+    auto k = tiles.rows(w.k + b * w.k_sb + kvh * w.k_sh, w.k_sn), v = tiles.rows(w.v + b * w.v_sb + kvh * w.v_sh, w.v_sn);
     const Fragments<D> fr(lane);
     v4i b1[KS], b2[KS];
-    const uint32_t own = L::SLOT + wave * 2 * 64 * D;
+    const uint32_t own = wave * 2 * 64 * D;
     query_rows_in<D>(w, w.q + b * w.q_sb + (int64_t)kvh * w.g * w.q_sh + (int64_t)i_lo * w.q_sn, w.q_sn, w.q_sh, i_lo, x0, lds + own, lane);
     query_rows_in<D>(w, a.dout + b * a.do_sb + (int64_t)kvh * w.g * a.do_sh + (int64_t)i_lo * a.do_sn, a.do_sn, a.do_sh, i_lo, x0, lds + own + 64 * D, lane);
-    if (span.n > 0) copy_tile(0, 0);
+    if (span.n > 0) tiles.copy(k, 0, L::keys(0)), tiles.copy(v, 0, L::values(0));
     const int64_t at = ((int64_t)b * H + kvh * w.g + hg) * a.sq_pad + i;
     float lse = a.lse2[at], ndelta = a.ndelta[at];
     dma_wait<0>();
@@ -120,8 +109,6 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
 #pragma unroll
     for (int s = 0; s < KS; s++) asm volatile("" : "+v"(b1[s]), "+v"(b2[s]));
     asm volatile("" : "+v"(lse), "+v"(ndelta));
-    __syncthreads();
-    if (span.n > 1) copy_tile(1, 1);
 
     v16f acc[DB];
 #pragma unroll
@@ -129,153 +116,112 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
 #pragma unroll
         for (int e = 0; e < 16; e++) acc[d][e] = 0.0f;
     const float c = w.scale * kLog2e;
-
-    // A block of 32 keys: scores S = K Q^T and G = V dO^T, then dS, then dQ^T += K^T dS.
-    auto scores_step = [&](const Fragments<D>& fr, const uint8_t* kt, v16f& s, v16f& g, int blk, int ks) {
-        s = product<T>(fr.along(kt + blk * 64 * D, ks), b1[ks], s);
-        g = product<T>(fr.along(kt + L::TILE + blk * 64 * D, ks), b2[ks], g);
-    };
-    auto pair = [&](const v16f& s, const v16f& g, int e, bool in0, bool in1) {
-        const float y0 = __builtin_amdgcn_exp2f(in0 ? fmaf(s[e], c, -lse) : -INFINITY) * (g[e] + ndelta);
-        const float y1 = __builtin_amdgcn_exp2f(in1 ? fmaf(s[e + 1], c, -lse) : -INFINITY) * (g[e + 1] + ndelta);
-        return pack2<T>(y0, y1);
-    };
     // Rows of dS sum to zero, but for the roundings of dS and of what Delta is made of; whatever their sum is, dS K multiplies it by the
     // keys' common offset.  So the rounded values are summed, and the sum times a vector c close to the mean key is
     // subtracted at the end: dQ = scale dS (K - c).
     float ds_sum = 0.0f;
-    auto add_up = [&](uint32_t w) {
-        if constexpr (T == kBF16) ds_sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w), __builtin_bit_cast(v2bf, 0x3F803F80u), ds_sum, false);
-        else ds_sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2fp, w), __builtin_bit_cast(v2fp, 0x3C003C00u), ds_sum, false);
+
+    // c: the mean of a tile's keys that some row here sees, of the first or of one from the window's middle, whichever has more of them.  (Of the
+    // middle of all tiles, which may hold a single key: dQ's relative error 8% higher, [2,12456,2 on 1,128] window 36 + 77.)
+    auto keys_of = [&](int t) {
+        const int j0 = span.tile(t) * 32, j1 = min(j0 + 31, span.hi);
+        return max(0, min(j1 + 1, span.s_end) - j0) + max(0, j1 + 1 - max(max(j0, span.lo), span.s_end));
     };
-    auto acc_step = [&](const Fragments<D>& fr, const uint8_t* kt, const uint32_t (&ds)[8], int blk, int m) {
-        const int j2 = m / DB, d = m % DB;
-        const v4i sb = {(int)ds[j2 * 4], (int)ds[j2 * 4 + 1], (int)ds[j2 * 4 + 2], (int)ds[j2 * 4 + 3]};
-        acc[d] = product<T>(fr.across(kt + (blk * 2 + j2) * 32 * D, d), sb, acc[d]);
-    };
-    // A whole tile, its two blocks overlapped: scores(0) | scores(1) + dS(0) | products(0) + dS(1) | products(1).
-    auto whole = [&](const uint8_t* kt) {
-        const Fragments<D> f = fr.fresh();
-        v16f s[2], g[2];
-        uint32_t ds[2][8];
-#pragma unroll
-        for (int blk = 0; blk < 2; blk++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) s[blk][e] = g[blk][e] = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) scores_step(f, kt, s[0], g[0], 0, ks);
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            scores_step(f, kt, s[1], g[1], 1, ks);
-#pragma unroll
-            for (int n = ks * (8 / KS); n < (ks + 1) * (8 / KS); n++) add_up(ds[0][n] = pair(s[0], g[0], n * 2, true, true));
-        }
-#pragma unroll
-        for (int m = 0; m < 2 * DB; m++) {
-            acc_step(f, kt, ds[0], 0, m);
-#pragma unroll
-            for (int n = m * (8 / (2 * DB)); n < (m + 1) * (8 / (2 * DB)); n++) add_up(ds[1][n] = pair(s[1], g[1], n * 2, true, true));
-        }
-#pragma unroll
-        for (int m = 0; m < 2 * DB; m++) acc_step(f, kt, ds[1], 1, m);
-    };
-    // A tile on the window's edge, block by block (the registers that the mask takes).
-    auto edge = [&](const uint8_t* kt, int j0) {
-#pragma unroll 1
-        for (int blk = 0; blk < 2; blk++) {
+    int centre = 0;
+    for (int n = 0; n < 2; n++) {
+        const int t = span.first + (span.n - span.first - n) / 2;
+        if (t >= 0 && t < span.n && keys_of(t) > keys_of(centre)) centre = t;
+    }
+    for (int t = 0; t < span.n; t++) {
+        dma_wait<0>();
+        __syncthreads();                 // tile t is visible; every wave is done with tile t - 1
+        if (t + 1 < span.n) tiles.copy(k, t + 1, L::keys(t + 1)), tiles.copy(v, t + 1, L::values(t + 1));
+        const uint32_t keys = lds + L::keys(t), values = lds + L::values(t);
+        const int j0 = span.tile(t) * 32;
+        const Seen what = all.has(t) ? Seen::kAll : x0 < rows ? seen<32>(w, wp_lo, wp_hi, len, j0) : Seen::kNone;
+        if (what != Seen::kNone) {
             const Fragments<D> f = fr.fresh();
-            const RowMask rel = mask.from(j0 + blk * 32 + half * 4);
             v16f s, g;
+            if (what == Seen::kAll) {
+                s = product<T>(lds_read(keys + f.nat), b1[0], v16f{});
+            } else {
+                const RowMask rel = mask.from(j0 + (lane_here() >> 5) * 4);
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[e] = rel.sees((e >> 2) * 8 + (e & 3)) ? 0.0f : -INFINITY;
+                s = product<T>(lds_read(keys + f.nat), b1[0], s);
+            }
+            g = product<T>(lds_read(values + f.nat), b2[0], v16f{});
+#pragma unroll
+            for (int ks = 1; ks < KS; ks++) {
+                s = product<T>(lds_read(keys + (f.nat ^ (ks << 5))), b1[ks], s);
+                g = product<T>(lds_read(values + (f.nat ^ (ks << 5))), b2[ks], g);
+            }
             uint32_t ds[8];
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[e] = g[e] = 0.0f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) scores_step(f, kt, s, g, blk, ks);
-#pragma unroll
-            for (int n = 0; n < 8; n++) {
-                const int e = n * 2, key = (e >> 2) * 8 + (e & 3);
-                add_up(ds[n] = pair(s, g, e, rel.sees(key), rel.sees(key + 1)));
+            for (int e = 0; e < 16; e += 2) {
+                const float y0 = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse)) * (g[e] + ndelta), y1 = __builtin_amdgcn_exp2f(fmaf(s[e + 1], c, -lse)) * (g[e + 1] + ndelta);
+                const uint32_t y = ds[e >> 1] = pack2<T>(y0, y1);
+                if constexpr (T == kBF16) ds_sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, y), __builtin_bit_cast(v2bf, 0x3F803F80u), ds_sum, false);
+                else ds_sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2fp, y), __builtin_bit_cast(v2fp, 0x3C003C00u), ds_sum, false);
             }
 #pragma unroll
-            for (int m = 0; m < 2 * DB; m++) acc_step(f, kt, ds, blk, m);
+            for (int m = 0; m < 2 * DB; m++) {
+                const int j2 = m / DB, d = m % DB;
+                acc[d] = product<T>(lds_read_across(keys + (f.tr[0] ^ (d << 6)) + j2 * 32 * D, keys + (f.tr[1] ^ (d << 6)) + j2 * 32 * D),
+                                    v4i{(int)ds[j2 * 4], (int)ds[j2 * 4 + 1], (int)ds[j2 * 4 + 2], (int)ds[j2 * 4 + 3]}, acc[d]);
+            }
         }
-    };
-
-    int slot = 0;
-    for (int t = 0; t < span.n; t++) {
-        if (t + 1 < span.n) dma_wait<2 * RPW>();
-        else dma_wait<0>();
-        __syncthreads();
-        if (t + 2 < span.n) copy_tile(t + 2, slot == 0 ? 2 : slot - 1);
-        const int j0 = span.tile(t) * 64;
-        const Seen what = x0 < rows ? seen<64>(w, wp_lo, wp_hi, len, j0) : Seen::kNone;
-        const uint8_t* kt = smem + slot * L::SLOT;
-        if (what == Seen::kAll) whole(kt);
-        else if (what == Seen::kSome) edge(kt, j0);
-        if (t == (span.n - 1) / 2) {           // c: the mean of those keys of the tile in the middle that some row here sees
-            int me = tid;
-            asm volatile("" : "+v"(me));
-            const int ch = me % D, first = me / D * (64 / DL::GROUPS);
+        if (t == centre) {
+            const int me = wave * 64 + lane_here(), ch = me % D, first = me / D * (32 / L::GROUPS);
+            const uint8_t* kt = smem + L::keys(t);
             float sum = 0.0f;
 #pragma unroll 1
-            for (int r = first; r < first + 64 / DL::GROUPS; r++) {
-                const float k = widen<T>(*reinterpret_cast<const uint16_t*>(kt + nat_off<CPR>(r, ch >> 3) + (ch & 7) * 2), 0);
-                sum += copied_key<64>(span, j0, j0 + r) == j0 + r ? k : 0.0f;
+            for (int r = first; r < first + 32 / L::GROUPS; r++) {
+                const float key = widen<T>(*reinterpret_cast<const uint16_t*>(kt + nat_off<CPR>(r, ch >> 3) + (ch & 7) * 2), 0);
+                sum += copied_key<32>(span, j0, j0 + r) == j0 + r ? key : 0.0f;
             }
-            const int j1 = min(j0 + 63, span.hi), sinks = max(0, min(j1 + 1, span.s_end) - j0), others = max(0, j1 + 1 - max(max(j0, span.lo), span.s_end));
-            reinterpret_cast<float*>(smem + DL::CENTRE)[me] = sum / (float)(sinks + others);
+            reinterpret_cast<float*>(smem + L::CENTRE)[me] = sum / (float)keys_of(t);
         }
-        slot = slot == 2 ? 0 : slot + 1;
     }
     __syncthreads();
     uint8_t* os = smem + wave * 64 * D;
+    const int end_lane = lane_here(), end_half = end_lane >> 5;
     if (span.n > 0) {
         const float rs = sum_halves(ds_sum);
-        const float* centre = reinterpret_cast<const float*>(smem + DL::CENTRE);
+        const float* centre = reinterpret_cast<const float*>(smem + L::CENTRE);
 #pragma unroll
         for (int d = 0; d < DB; d++)
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
+            for (int q = 0; q < 4; q++) {
                 v4f c4 = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int n = 0; n < DL::GROUPS; n++) c4 += *reinterpret_cast<const v4f*>(centre + n * D + d * 32 + g * 8 + half * 4);
+                for (int n = 0; n < L::GROUPS; n++) c4 += *reinterpret_cast<const v4f*>(centre + n * D + d * 32 + q * 8 + end_half * 4);
 #pragma unroll
-                for (int e = 0; e < 4; e++) acc[d][g * 4 + e] = fmaf(-rs, c4[e], acc[d][g * 4 + e]);
+                for (int e = 0; e < 4; e++) acc[d][q * 4 + e] = fmaf(-rs, c4[e], acc[d][q * 4 + e]);
             }
     }
 #pragma unroll
-    for (int d = 0; d < DB; d++) row_put<T, D>(os, acc[d], d, w.scale, lane);
-    if (x0 < rows) query_rows_out<D>(w, os, a.dq + b * a.dq_sb + (int64_t)kvh * w.g * a.dq_sh, a.dq_sn, a.dq_sh, x0, lane);
+    for (int d = 0; d < DB; d++) row_put<T, D>(os, acc[d], d, w.scale, end_lane);
+    if (x0 < rows) query_rows_out<D>(w, os, a.dq + b * a.dq_sb + (int64_t)kvh * w.g * a.dq_sh, a.dq_sn, a.dq_sh, x0, end_lane);
 }
 
-// ---- dK, dV: owners of keys, (head, query tile) pairs -----------------------------------------------------------
-// The query tiles that reach keys k0 .. of a block: indices t0 .. t0 + nt - 1 of every head of the group.
+// ---- dK, dV: owners of keys, (head, query tile) pairs --------------------------------------------------------------
+// The tiles of 32 queries that reach `keys` keys from k0 on: indices t0 .. t0 + nt - 1 of every head of the group.
 struct QuerySpan { int t0, nt; };
-__device__ __forceinline__ QuerySpan query_span(const WindowArgs& w, int k0, int p0, int len) {
-    const int k1 = min(k0 + kKeysWg, len) - 1;
+__device__ __forceinline__ QuerySpan query_span(const WindowArgs& w, int k0, int keys, int p0, int len) {
+    const int k1 = min(k0 + keys, len) - 1;
     const int64_t lo = (int64_t)k0 - w.right - p0;
     const int64_t hi = k0 < w.sinks ? (int64_t)w.Sq - 1 : (int64_t)k1 + w.left - p0;
     const int i0 = (int)(lo < 0 ? 0 : lo > w.Sq ? w.Sq : lo), i1 = (int)(hi < -1 ? -1 : hi > w.Sq - 1 ? w.Sq - 1 : hi);
     if (k1 < k0 || i1 < i0) return QuerySpan{0, 0};
-    return QuerySpan{i0 >> 6, (i1 >> 6) - (i0 >> 6) + 1};
+    return QuerySpan{i0 >> 5, (i1 >> 5) - (i0 >> 5) + 1};
 }
-// Which of the queries at positions pa .. pb a wave's keys x0 .. x1 are seen by.
+// Which of the queries at positions pa .. pb a wave's keys x0 .. x0 + 31 are seen by.
 __device__ __forceinline__ Seen seen_by(const WindowArgs& w, int x0, int len, int pa, int pb) {
     const int x1 = x0 + 31;
     if (x0 >= len || x0 > pb + w.right || (x1 < pa - w.left && x0 >= w.sinks)) return Seen::kNone;
     return x1 < len && x1 <= pa + w.right && (x0 >= pb - w.left || x1 < w.sinks) ? Seen::kAll : Seen::kSome;
 }
-// Which rows of a workgroup's share: the walk over heads and tiles, one pair after the other.
-struct Walk {
-    int t0, nt, hg, qt;
-    __device__ Walk(const QuerySpan& q, int first) : t0(q.t0), nt(q.nt), hg(0), qt(0) {
-        if (nt > 0) hg = first / nt, qt = first - hg * nt;
-    }
-    __device__ void next() {
-        if (++qt == nt) qt = 0, hg++;
-    }
-    __device__ int tile() const { return t0 + qt; }
-};
 // Positions of queries p that see the lane's key: lo <= p <= hi.  (Up to the last query: the padding of its tile stands at further ones.)
 struct KeyMask {
     int lo, hi;
@@ -287,14 +233,14 @@ __device__ __forceinline__ KeyMask key_mask(const WindowArgs& w, int j, int len,
 
 // What a workgroup of this kind does: block of keys, chunk of its pairs, and where its result goes.
 struct KeyWork { int k0, first, count; int64_t part; };          // part: index of its fp32 part, -1: straight to dK and dV
-__device__ __forceinline__ KeyWork key_work(const WindowBwdArgs& a, int bh, int r, int total_blocks) {
+template <int D> __device__ __forceinline__ KeyWork key_work(const WindowBwdArgs& a, int bh, int r, int total_blocks) {
     const int sink_wgs = a.sink_blocks * a.sink_chunks;
     int block, chunk;
     KeyWork k;
     k.part = -1;
     if (r < sink_wgs) {
         block = r / a.sink_chunks, chunk = r % a.sink_chunks;
-        if (a.sink_chunks > 1) k.part = (int64_t)bh * ((a.sink_chunks > 1 ? sink_wgs : 0) + (a.chunks > 1 ? (total_blocks - a.sink_blocks) * a.chunks : 0)) + r;
+        if (a.sink_chunks > 1) k.part = (int64_t)bh * (sink_wgs + (a.chunks > 1 ? (total_blocks - a.sink_blocks) * a.chunks : 0)) + r;
     } else {
         r -= sink_wgs;
         block = a.sink_blocks + r / a.chunks, chunk = r % a.chunks;
@@ -333,186 +279,108 @@ __device__ __forceinline__ void key_rows_out(const WindowBwdArgs& a, const v16f 
         if (x0 + r < a.w.Skv) *reinterpret_cast<u32x4*>(out + (int64_t)(x0 + r) * sn + (lane % CPR) * 8) = v;
     }
 }
+// A wave's 32 keys from x0 on of the block at k0 -> LDS.  Keys that no query sees are not read: another row of the block stands in, whose gradient
+// is dropped by probabilities of zero.  (`span`: of all queries.  A block that nothing sees reads some row and uses none.)
 template <int D>
-__device__ __forceinline__ void key_rows_in(const uint16_t* head, int64_t sn, int k0, int x0, int last, uint32_t dst, int lane) {
+__device__ __forceinline__ void key_rows_in(const Span& span, const uint16_t* head, int64_t sn, int k0, int x0, uint32_t dst, int lane) {
     constexpr int CPR = D / 8, RPI = 64 / CPR;
-    const uint16_t* base = head + (int64_t)k0 * sn;          // (k0 <= last, or nothing of it is used)
+    const int base = max(min(k0, span.hi), 0);
+    const uint16_t* at = head + (int64_t)base * sn;
 #pragma unroll
     for (int n = 0; n < 32 / RPI; n++) {
         const int r = n * RPI + lane / CPR;
-        dma16(base, (uint32_t)(max(min(x0 + r, last), k0) - k0) * (uint32_t)(sn * 2) + nat_pos<CPR>(r, lane % CPR) * 16, __builtin_amdgcn_readfirstlane(dst + n * 1024));
+        const int j = min(max(copied_key<kKeysWg>(span, k0, x0 + r), base), base + kKeysWg - 1);
+        dma16(at, (uint32_t)(max(min(j, span.hi), base) - base) * (uint32_t)(sn * 2) + nat_pos<CPR>(r, lane % CPR) * 16, __builtin_amdgcn_readfirstlane(dst + n * 1024));
     }
 }
 
-// A query tile's copies: 64 rows of Q and of dO of one head, and their statistics.
-template <int T, int D, int NW> struct QueryTiles {
-    using L = PassLds<D>;
-    static constexpr int RPW = TilePieces<D, 64, NW>::N;
-    const WindowBwdArgs& a;
-    int b, kvh, wave, lane;
-    TilePieces<D, 64, NW> pieces;
-    uint32_t rows_at, ring_at;
-    __device__ QueryTiles(const WindowBwdArgs& a_, int b_, int kvh_, int wave_, int lane_, uint32_t rows_at_, uint32_t ring_at_)
-        : a(a_), b(b_), kvh(kvh_), wave(wave_), lane(lane_), pieces(wave_, lane_), rows_at(rows_at_), ring_at(ring_at_) {}
-    __device__ void copy(int hg, int qt, int slot) const {
-        const WindowArgs& w = a.w;
-        const int h = kvh * w.g + hg, i0 = qt * 64;
-        const uint16_t* qb = w.q + b * w.q_sb + h * w.q_sh + (int64_t)i0 * w.q_sn;
-        const uint16_t* gb = a.dout + b * a.do_sb + h * a.do_sh + (int64_t)i0 * a.do_sn;
-        const int64_t row = ((int64_t)b * w.Hk * w.g + h) * a.sq_pad + i0;
-        // (first, so that a wait for the copies below covers them)
-        if (wave == 0) dma4(a.lse2 + row, lane * 4, __builtin_amdgcn_readfirstlane(rows_at + (slot * 2 + 0) * 256));
-        if (wave == 1) dma4(a.ndelta + row, lane * 4, __builtin_amdgcn_readfirstlane(rows_at + (slot * 2 + 1) * 256));
+// Q or dO on its way into LDS: tiles of 32 queries of one head after the other, then the next head's.
+template <int D> struct QueryRows {
+    using Pieces = TilePieces<D, 32, kWaves>;
+    const uint16_t* at;                  // of the tile to be copied next
+    int64_t tile, turn;                  // from a tile to the next, from a head's last to the next head's first
+    uint32_t sn, off[Pieces::N];
+    int qt, nt, t0;
+    __device__ QueryRows(const Pieces& p, const uint16_t* head, int64_t sh, int64_t sn_, const QuerySpan& q, int first, int lane) {
+        const int hg = q.nt > 0 ? first / q.nt : 0;
+        nt = q.nt;
+        t0 = q.t0;
+        qt = first - hg * nt;
+        at = head + hg * sh + (int64_t)(t0 + qt) * 32 * sn_;
+        tile = 32 * sn_;
+        turn = sh - (nt - 1) * tile;
+        sn = (uint32_t)sn_ * 2u;
 #pragma unroll
-        for (int n = 0; n < RPW; n++) {
-            const uint32_t r = (uint32_t)min(pieces.row(n), w.Sq - 1 - i0);
-            const uint32_t dst = ring_at + slot * L::SLOT + (n * NW + wave) * 1024;
-            dma16(qb, r * (uint32_t)(w.q_sn * 2) + pieces.col(n, lane), __builtin_amdgcn_readfirstlane(dst));
-            dma16(gb, r * (uint32_t)(a.do_sn * 2) + pieces.col(n, lane), __builtin_amdgcn_readfirstlane(dst + L::TILE));
+        for (int n = 0; n < Pieces::N; n++) off[n] = p.row(n) * sn + p.col(n, lane);
+    }
+    __device__ void copy(const Pieces& p, int Sq, uint32_t to, int wave, int lane) {
+        const int left = Sq - (t0 + qt) * 32;            // (rows behind the last query repeat it)
+#pragma unroll
+        for (int n = 0; n < Pieces::N; n++) {
+            uint32_t o = off[n];
+            if (left < 32) o = (uint32_t)min(p.row(n), left - 1) * sn + p.col(n, lane);
+            dma16(at, o, __builtin_amdgcn_readfirstlane(to + (n * kWaves + wave) * 1024));
         }
+        const bool last = qt == nt - 1;
+        at += last ? turn : tile;
+        qt = last ? 0 : qt + 1;
+    }
+};
+// The statistics of the same tiles: 32 log-sum-exps and 32 -Delta, side by side.
+struct QueryStats {
+    const float* at;
+    int64_t turn;
+    uint32_t off;
+    int qt, nt;
+    __device__ QueryStats(const WindowBwdArgs& a, int64_t head, const QuerySpan& q, int first, int lane) {
+        const int hg = q.nt > 0 ? first / q.nt : 0;
+        nt = q.nt;
+        qt = first - hg * nt;
+        at = a.lse2 + (head + hg) * a.sq_pad + (q.t0 + qt) * 32;
+        turn = a.sq_pad - (nt - 1) * 32;
+        off = (uint32_t)(lane & 31) * 4u + (lane < 32 ? 0u : (uint32_t)((a.ndelta - a.lse2) * 4));
+    }
+    __device__ void copy(uint32_t to) {
+        dma4(at, off, __builtin_amdgcn_readfirstlane(to));
+        const bool last = qt == nt - 1;
+        at += last ? turn : 32;
+        qt = last ? 0 : qt + 1;
+    }
+};
+// Positions of the tiles' first queries.
+struct QueryWalk {
+    int p, qt, nt, p_first;
+    __device__ QueryWalk(const QuerySpan& q, int first, int p0) {
+        nt = q.nt;
+        qt = nt > 0 ? first % nt : 0;
+        p_first = p0 + q.t0 * 32;
+        p = p_first + qt * 32;
+    }
+    __device__ void next() {
+        const bool last = qt == nt - 1;
+        p = last ? p_first : p + 32;
+        qt = last ? 0 : qt + 1;
     }
 };
 
-// Head dim 64: a wave carries both products of its 32 keys.
-template <int D> struct KeyLds {
-    using L = PassLds<D>;
-    static constexpr int OWN = kWaves<D> * 2 * 64 * D;
-    static constexpr int BYTES = L::ROWS + (3 * L::SLOT > L::SLOT + OWN ? 3 * L::SLOT : L::SLOT + OWN);
-};
-
-template <int T, int D>
-__device__ __forceinline__ void dkdv_body(const WindowBwdArgs& a, uint8_t* smem, int bh, const KeyWork& work) {
-    using L = PassLds<D>;
-    constexpr int NW = kWaves<D>, KS = D / 16, DB = D / 32, RPW = QueryTiles<T, D, NW>::RPW;
-    static_assert(NW * 32 == kKeysWg, "a wave owns 32 keys");
-    const WindowArgs& w = a.w;
-    const int b = bh / w.Hk, kvh = bh % w.Hk;
-    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l32 = lane & 31;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int x0 = work.k0 + wave * 32, j = x0 + l32;
-    const int len = sequence_len(w, b), p0 = first_position(w, b, len);
-    const QuerySpan qs = query_span(w, work.k0, p0, len);
-    const int n_tiles = max(0, min(qs.nt * w.g - work.first, work.count));
-    const KeyMask mask = key_mask(w, j, len, p0);
-    const uint32_t lds = lds_addr(smem);
-    const QueryTiles<T, D, NW> tiles(a, b, kvh, wave, lane, lds, lds + L::ROWS);
-    Walk ahead(qs, work.first), here = ahead;
-
-    const Fragments<D> kept(lane);
-    v4i b1[KS], b2[KS];
-    const uint32_t own = L::ROWS + L::SLOT + wave * 2 * 64 * D;
-    key_rows_in<D>(w.k + b * w.k_sb + kvh * w.k_sh, w.k_sn, min(work.k0, max(len - 1, 0)), x0, max(len - 1, 0), lds + own, lane);
-    key_rows_in<D>(w.v + b * w.v_sb + kvh * w.v_sh, w.v_sn, min(work.k0, max(len - 1, 0)), x0, max(len - 1, 0), lds + own + 64 * D, lane);
-    if (n_tiles > 0) tiles.copy(ahead.hg, ahead.tile(), 0), ahead.next();
-    dma_wait<0>();
+// Scores of a tile of queries with the lane's key, where they start.
+__device__ __forceinline__ void start_scores(v16f& s, const KeyMask& mask, Seen what, int pa, int half) {
+    const KeyMask rel = what == Seen::kNone ? KeyMask{1, 0} : KeyMask{mask.lo - pa - half * 4, mask.hi - pa - half * 4};
 #pragma unroll
-    for (int s = 0; s < KS; s++) b1[s] = kept.along(smem + own, s), b2[s] = kept.along(smem + own + 64 * D, s);
-#pragma unroll
-    for (int s = 0; s < KS; s++) asm volatile("" : "+v"(b1[s]), "+v"(b2[s]));
-    __syncthreads();
-    if (n_tiles > 1) tiles.copy(ahead.hg, ahead.tile(), 1), ahead.next();
-
-    v16f dk[DB], dv[DB];
-#pragma unroll
-    for (int d = 0; d < DB; d++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) dk[d][e] = dv[d][e] = 0.0f;
-    const float c = w.scale * kLog2e;
-
-    auto tile = [&](auto masked_tag, int pa, int slot) {
-        constexpr bool MASKED = decltype(masked_tag)::value;
-        const KeyMask rel = {mask.lo - pa - half * 4, mask.hi - pa - half * 4};
-        const Fragments<D> fr = kept.fresh();
-        const uint8_t* qt = smem + L::ROWS + slot * L::SLOT;
-        const uint8_t* gt = qt + L::TILE;
-        const uint8_t* rows = smem + slot * 512;
-        v16f s[2], g[2];
-        uint32_t pp[2][8], ds[2][8];
-#pragma unroll
-        for (int blk = 0; blk < 2; blk++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const v4f nd = *reinterpret_cast<const v4f*>(rows + 256 + (blk * 32 + q * 8 + half * 4) * 4);
-#pragma unroll
-                for (int e = 0; e < 4; e++) s[blk][q * 4 + e] = 0.0f, g[blk][q * 4 + e] = nd[e];
-            }
-        auto scores_step = [&](int blk, int ks) {
-            s[blk] = product<T>(fr.along(qt + blk * 64 * D, ks), b1[ks], s[blk]);
-            g[blk] = product<T>(fr.along(gt + blk * 64 * D, ks), b2[ks], g[blk]);
-        };
-        v4f lse;
-        auto pair = [&](int blk, int e0) {
-            if ((e0 & 3) == 0) lse = *reinterpret_cast<const v4f*>(rows + (blk * 32 + (e0 >> 2) * 8 + half * 4) * 4);
-            float y[2], z[2];
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int n = e0 + e;
-                y[e] = __builtin_amdgcn_exp2f(fmaf(s[blk][n], c, -lse[n & 3]));
-                z[e] = y[e] * g[blk][n];
-                if constexpr (MASKED) {
-                    const bool in = rel.sees(blk * 32 + (n >> 2) * 8 + (n & 3));
-                    y[e] = in ? y[e] : 0.0f;
-                    z[e] = in ? z[e] : 0.0f;             // (a key that nothing sees may hold anything)
-                }
-            }
-            pp[blk][e0 >> 1] = pack2<T>(y[0], y[1]);
-            ds[blk][e0 >> 1] = pack2<T>(z[0], z[1]);
-        };
-        auto acc_step = [&](int blk, int m) {
-            const int which = m / (2 * DB), j2 = (m / DB) & 1, d = m % DB;
-            const int at = (blk * 2 + j2) * 32 * D;
-            const uint32_t(&r)[8] = which == 0 ? ds[blk] : pp[blk];
-            const v4i sb = {(int)r[j2 * 4], (int)r[j2 * 4 + 1], (int)r[j2 * 4 + 2], (int)r[j2 * 4 + 3]};
-            if (which == 0) dk[d] = product<T>(fr.across(qt + at, d), sb, dk[d]);
-            else dv[d] = product<T>(fr.across(gt + at, d), sb, dv[d]);
-        };
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) scores_step(0, ks);
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            scores_step(1, ks);
-#pragma unroll
-            for (int n = 0; n < 8 / KS; n++) pair(0, (ks * (8 / KS) + n) * 2);
-        }
-#pragma unroll
-        for (int m = 0; m < 4 * DB; m++) {
-            acc_step(0, m);
-#pragma unroll
-            for (int n = 0; n < 8 / (4 * DB); n++) pair(1, (m * (8 / (4 * DB)) + n) * 2);
-        }
-#pragma unroll
-        for (int m = 0; m < 4 * DB; m++) acc_step(1, m);
-    };
-
-    int slot = 0;
-    for (int t = 0; t < n_tiles; t++) {
-        if (t + 1 < n_tiles) dma_wait<2 * RPW>();
-        else dma_wait<0>();
-        __syncthreads();
-        if (t + 2 < n_tiles) tiles.copy(ahead.hg, ahead.tile(), slot == 0 ? 2 : slot - 1), ahead.next();
-        const int pa = p0 + here.tile() * 64;
-        here.next();
-        const Seen what = seen_by(w, x0, len, pa, min(pa + 63, p0 + w.Sq - 1));
-        if (what == Seen::kAll) tile(std::false_type{}, pa, slot);
-        else if (what == Seen::kSome) tile(std::true_type{}, pa, slot);
-        slot = slot == 2 ? 0 : slot + 1;
-    }
-    __syncthreads();
-    uint8_t* os = smem + L::ROWS + wave * 64 * D;
-    key_rows_out<T, D>(a, dk, w.scale, os, work.part, 0, a.dk + b * a.dk_sb + kvh * a.dk_sh, a.dk_sn, x0, work.k0, lane);
-    key_rows_out<T, D>(a, dv, 1.0f, os, work.part, 1, a.dv + b * a.dv_sb + kvh * a.dv_sh, a.dv_sn, x0, work.k0, lane);
+    for (int e = 0; e < 16; e++) s[e] = rel.sees((e >> 2) * 8 + (e & 3)) ? 0.0f : -INFINITY;
 }
 
-// Head dim 128: a pair of waves shares 32 keys, the P wave with K rows and dV, the S wave, one tile behind, with V rows and dK; P crosses
+// A pair of waves shares 32 keys, the P wave with K rows and dV, the S wave, one tile behind, with V rows and dK; P crosses
 // over through LDS with some bits more than dS is rounded to: as fp16 pairs where that is bf16 (see sage_bwd.hip), as the upper three bytes of fp32
-// where it is fp16 (with fp16 there dK's relative error was 3.5e-4, with these 2.9e-4).
+// where it is fp16 (with fp16 there dK's relative error was 3.5e-4, with these 2.9e-4).  In step t the P wave takes the scores of tile t + 1 and the
+// weights of t, the S wave the products with dO of t and dS of t - 1: four slots of Q, two of dO and of the statistics.
 template <int T, int D> struct PairLds {
-    using L = PassLds<D>;
-    static constexpr int WORDS = T == kBF16 ? 2 : 3;          // 16-byte words for the 16 values of a block
-    static constexpr int HAND = 4 * 2 * WORDS * 64 * 16;      // [pair][32-row block][word][lane]
-    static constexpr int RING = L::ROWS + 2 * HAND, BYTES = RING + 3 * L::SLOT;
-    static_assert(BYTES <= 160 * 1024, "LDS of a compute unit");
-    static_assert(8 * 64 * D <= 2 * L::SLOT, "the owner rows must fit behind the first slot");
+    static constexpr int TILE = 32 * D * 2, WORDS = T == kBF16 ? 2 : 3;      // 16-byte words for the 16 values of a lane
+    static constexpr int HAND = 2 * WORDS * 64 * 16;                          // [pair][word][lane]
+    static constexpr int NONE = 512, ROWS = 768, RING = ROWS + 2 * HAND, OWN = kWaves * 64 * D;
+    static constexpr int FIRST = RING + (OWN > 5 * TILE ? OWN : 5 * TILE), BYTES = FIRST + TILE;
+    static __device__ int q(int t) { return (t & 3) == 0 ? FIRST : RING + ((t & 3) - 1) * TILE; }
+    static __device__ int d(int t) { return RING + (3 + (t & 1)) * TILE; }
 };
 
 // Four floats <-> the upper three bytes of each (15 bits behind the leading one).
@@ -529,178 +397,164 @@ __device__ __forceinline__ float unpack24(const uint32_t* w, int i) {
 
 template <int T, int D, int ROLE>
 __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem, int bh, const KeyWork& work, int wave, int lane) {
-    using L = PassLds<D>;
-    using PL = PairLds<T, D>;
+    using L = PairLds<T, D>;
     constexpr int KS = D / 16, DB = D / 32;
+    static_assert(kWaves * 16 == kKeysWg, "a pair of waves owns 32 keys");
     const WindowArgs& w = a.w;
     const int b = bh / w.Hk, kvh = bh % w.Hk;
-    const int pr = wave & 3, half = lane >> 5, l32 = lane & 31;
+    const int pr = wave & 1, half = lane >> 5, l32 = lane & 31;
     const int x0 = work.k0 + pr * 32, j = x0 + l32;
-    const int len = sequence_len(w, b), p0 = first_position(w, b, len);
-    const QuerySpan qs = query_span(w, work.k0, p0, len);
+    const int len = sequence_len(w, b), p0 = first_position(w, b, len), p_last = p0 + w.Sq - 1;
+    const QuerySpan qs = query_span(w, work.k0, kKeysWg, p0, len);
     const int n_tiles = max(0, min(qs.nt * w.g - work.first, work.count));
     const KeyMask mask = key_mask(w, j, len, p0);
     const uint32_t lds = lds_addr(smem);
-    const QueryTiles<T, D, 8> tiles(a, b, kvh, wave, lane, lds, lds + PL::RING);
-    Walk ahead(qs, work.first), here = ahead;
+    const typename QueryRows<D>::Pieces pieces(wave, lane);
+    QueryRows<D> q(pieces, w.q + b * w.q_sb + (int64_t)kvh * w.g * w.q_sh, w.q_sh, w.q_sn, qs, work.first, lane);
+    QueryRows<D> d(pieces, a.dout + b * a.do_sb + (int64_t)kvh * w.g * a.do_sh, a.do_sh, a.do_sn, qs, work.first, lane);
+    QueryStats st(a, (int64_t)b * w.Hk * w.g + kvh * w.g, qs, work.first, lane);
+    QueryWalk walk(qs, work.first, p0);
 
-    const Fragments<D> kept(lane);
+    const Fragments<D> fr(lane);
     v4i bx[KS];
-    const uint32_t own = PL::RING + L::SLOT + wave * 64 * D;
-    key_rows_in<D>(ROLE == 0 ? w.k + b * w.k_sb + kvh * w.k_sh : w.v + b * w.v_sb + kvh * w.v_sh, ROLE == 0 ? w.k_sn : w.v_sn, min(work.k0, max(len - 1, 0)), x0,
-                   max(len - 1, 0), lds + own, lane);
-    if (n_tiles > 0) tiles.copy(ahead.hg, ahead.tile(), 0), ahead.next();
+    const uint32_t own = L::RING + wave * 64 * D;
+    const Span keys_seen = key_span<32>(w, p0, p_last, len);
+    key_rows_in<D>(keys_seen, ROLE == 0 ? w.k + b * w.k_sb + kvh * w.k_sh : w.v + b * w.v_sb + kvh * w.v_sh, ROLE == 0 ? w.k_sn : w.v_sn, work.k0, x0, lds + own, lane);
+    if (n_tiles > 0) q.copy(pieces, w.Sq, lds + L::q(0), wave, lane);
+    if (wave == 0) *reinterpret_cast<float*>(smem + L::NONE + lane * 4) = lane < 32 ? INFINITY : 0.0f;        // (statistics where there is no tile: probabilities of zero)
     dma_wait<0>();
 #pragma unroll
-    for (int s = 0; s < KS; s++) bx[s] = kept.along(smem + own, s);
+    for (int s = 0; s < KS; s++) bx[s] = fr.along(smem + own, s);
 #pragma unroll
     for (int s = 0; s < KS; s++) asm volatile("" : "+v"(bx[s]));
 
-    v16f acc[DB];
+    v16f acc[DB], s[2];
 #pragma unroll
-    for (int d = 0; d < DB; d++)
+    for (int n = 0; n < DB; n++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) acc[d][e] = 0.0f;
+        for (int e = 0; e < 16; e++) acc[n][e] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; e++) s[0][e] = s[1][e] = ROLE == 0 ? -INFINITY : 0.0f;
     const float c = w.scale * kLog2e;
-    u32x4* hand = reinterpret_cast<u32x4*>(smem + L::ROWS) + pr * 2 * PL::WORDS * 64 + lane;
+    u32x4* hand = reinterpret_cast<u32x4*>(smem + L::ROWS) + pr * L::WORDS * 64 + lane;
 
-    auto tile = [&](auto masked_tag, int pa, int mine, int turn, auto&& copy_next) {
-        constexpr bool MASKED = decltype(masked_tag)::value;
-        const KeyMask rel = {mask.lo - pa - half * 4, mask.hi - pa - half * 4};
-        const Fragments<D> fr = kept.fresh();
-        const uint8_t* nt = smem + PL::RING + mine * L::SLOT + ROLE * L::TILE;
-        const uint8_t* rt = smem + PL::RING + mine * L::SLOT + (1 - ROLE) * L::TILE;
-        const uint8_t* rowv = smem + (mine * 2 + ROLE) * 256;
-        uint32_t hp[2][4 * PL::WORDS];   // P on its way to the S wave
-        if constexpr (ROLE == 1) {
+    // `score`: the tile whose scores (P wave: Q K^T, S wave: dO V^T) are taken; `rows`: the one whose rows (dO, Q) the products take; stats: of tile t.
+    auto step = [&](const v16f& s, bool now, uint32_t rows, v16f& sn, Seen next, uint32_t score, int pa, int t) {
+        const Fragments<D> f = fr.fresh();
+        const uint8_t* stats = smem + ((ROLE == 0 ? now : next != Seen::kNone) ? (t & 1) * 256 : L::NONE) + half * 16;
+        if (ROLE == 0 && next == Seen::kAll) {
+            sn = product<T>(lds_read(score + f.nat), bx[0], v16f{});
+        } else {
+            if constexpr (ROLE == 0) {
+                start_scores(sn, mask, next, pa, half);
+            } else {
 #pragma unroll
-            for (int blk = 0; blk < 2; blk++)
+                for (int n = 0; n < 4; n++) {
+                    const v4f nd = *reinterpret_cast<const v4f*>(stats + 128 + n * 32);
 #pragma unroll
-                for (int n = 0; n < PL::WORDS; n++) {
-                    const u32x4 v = hand[turn * (PL::HAND / 16) + (blk * PL::WORDS + n) * 64];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) hp[blk][n * 4 + e] = v[e];
+                    for (int e = 0; e < 4; e++) sn[n * 4 + e] = nd[e];
                 }
-        }
-        v16f s[2];
-        uint32_t pk[2][8];
-        float last[2];
-        v4f rv;
-#pragma unroll
-        for (int blk = 0; blk < 2; blk++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                v4f nd = {0.0f, 0.0f, 0.0f, 0.0f};
-                if constexpr (ROLE == 1) nd = *reinterpret_cast<const v4f*>(rowv + (blk * 32 + q * 8 + half * 4) * 4);
-#pragma unroll
-                for (int e = 0; e < 4; e++) s[blk][q * 4 + e] = nd[e];
             }
-        auto scores_step = [&](int blk, int ks) { s[blk] = product<T>(fr.along(nt + blk * 64 * D, ks), bx[ks], s[blk]); };
-        auto pair = [&](int blk, int e0) {
-            if (ROLE == 0 && (e0 & 3) == 0) rv = *reinterpret_cast<const v4f*>(rowv + (blk * 32 + (e0 >> 2) * 8 + half * 4) * 4);
-            float y[2];
+            sn = product<T>(lds_read(score + f.nat), bx[0], sn);
+        }
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int n = e0 + e;
-                if constexpr (ROLE == 0) {
-                    y[e] = __builtin_amdgcn_exp2f(fmaf(s[blk][n], c, -rv[n & 3]));
+        for (int ks = 1; ks < KS; ks++) sn = product<T>(lds_read(score + (f.nat ^ (ks << 5))), bx[ks], sn);
+        uint32_t pk[8], hp[4 * L::WORDS];
+        if constexpr (ROLE == 0) {
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                const v4f lse = *reinterpret_cast<const v4f*>(stats + n * 32);
+                float y[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = __builtin_amdgcn_exp2f(fmaf(s[n * 4 + e], c, -lse[e]));
+                pk[n * 2] = pack2<T>(y[0], y[1]);
+                pk[n * 2 + 1] = pack2<T>(y[2], y[3]);
+                if constexpr (T == kBF16) {
+                    hp[n * 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[0], y[1]));
+                    hp[n * 2 + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[2], y[3]));
                 } else {
-                    if constexpr (T == kBF16) y[e] = fmaf((float)__builtin_bit_cast(v2fp, hp[blk][e0 >> 1])[e], s[blk][n], 0.0f);
-                    else y[e] = unpack24(&hp[blk][(n >> 2) * 3], n & 3) * s[blk][n];
+                    pack24(y, &hp[n * 3]);
                 }
-                if (MASKED && !rel.sees(blk * 32 + (n >> 2) * 8 + (n & 3))) y[e] = 0.0f;       // (in both: a key that nothing sees may hold anything)
             }
-            pk[blk][e0 >> 1] = pack2<T>(y[0], y[1]);
-            if constexpr (ROLE == 0) {
-                if constexpr (T == kBF16) hp[blk][e0 >> 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[0], y[1]));
-                else if (e0 & 2) pack24({last[0], last[1], y[0], y[1]}, &hp[blk][(e0 >> 2) * 3]);
-                last[0] = y[0], last[1] = y[1];
+#pragma unroll
+            for (int n = 0; n < L::WORDS; n++) hand[(t & 1) * (L::HAND / 16) + n * 64] = u32x4{hp[n * 4], hp[n * 4 + 1], hp[n * 4 + 2], hp[n * 4 + 3]};
+        } else {
+#pragma unroll
+            for (int n = 0; n < L::WORDS; n++) {
+                const u32x4 v = now ? hand[((t - 1) & 1) * (L::HAND / 16) + n * 64] : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int e = 0; e < 4; e++) hp[n * 4 + e] = v[e];
             }
-        };
-        auto hand_over = [&](int blk) {
-            if constexpr (ROLE == 0) {
-                const auto& r = hp[blk];
 #pragma unroll
-                for (int n = 0; n < PL::WORDS; n++)
-                    hand[turn * (PL::HAND / 16) + (blk * PL::WORDS + n) * 64] = u32x4{r[n * 4], r[n * 4 + 1], r[n * 4 + 2], r[n * 4 + 3]};
+            for (int n = 0; n < 16; n += 2) {
+                float y[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    // (as a multiply-add: one instruction with the fp16 operand's conversion in it)
+                    if constexpr (T == kBF16) y[e] = fmaf((float)__builtin_bit_cast(v2fp, hp[n >> 1])[e], s[n + e], 0.0f);
+                    else y[e] = unpack24(&hp[(n >> 2) * 3], (n & 3) + e) * s[n + e];
+                }
+                pk[n >> 1] = pack2<T>(y[0], y[1]);
             }
-        };
-        auto acc_step = [&](int blk, int m) {
-            const int j2 = m / DB, d = m % DB;
-            const v4i sb = {(int)pk[blk][j2 * 4], (int)pk[blk][j2 * 4 + 1], (int)pk[blk][j2 * 4 + 2], (int)pk[blk][j2 * 4 + 3]};
-            acc[d] = product<T>(fr.across(rt + (blk * 2 + j2) * 32 * D, d), sb, acc[d]);
-        };
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) scores_step(0, ks);
-        copy_next();
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            scores_step(1, ks);
-#pragma unroll
-            for (int n = 0; n < 8 / KS; n++) pair(0, (ks * (8 / KS) + n) * 2);
         }
-        hand_over(0);
 #pragma unroll
         for (int m = 0; m < 2 * DB; m++) {
-            acc_step(0, m);
-#pragma unroll
-            for (int n = 0; n < 8 / (2 * DB); n++) pair(1, (m * (8 / (2 * DB)) + n) * 2);
+            const int j2 = m / DB, d = m % DB;
+            const uint32_t lo = (f.tr[0] ^ (d << 6)) + j2 * 32 * D, hi = (f.tr[1] ^ (d << 6)) + j2 * 32 * D;
+            acc[d] = product<T>(lds_read_across(rows + lo, rows + hi), v4i{(int)pk[j2 * 4], (int)pk[j2 * 4 + 1], (int)pk[j2 * 4 + 2], (int)pk[j2 * 4 + 3]}, acc[d]);
         }
-        hand_over(1);
-#pragma unroll
-        for (int m = 0; m < 2 * DB; m++) acc_step(1, m);
     };
-
-    // iteration `it`: the P wave works on tile it, the S wave on tile it - 1
-    int slot = 0;                        // it % 3
-    for (int it = 0; n_tiles > 0 && it <= n_tiles; it++) {
+    // What the keys are seen by in tiles t + 1, t, t - 1.
+    Seen ahead = Seen::kNone, here = Seen::kNone, behind = Seen::kNone;
+    auto tile = [&](const v16f& s, v16f& sn, int t) {
         dma_wait<0>();
-        __syncthreads();                 // this iteration's tile and the previous one's P are visible; the slot of tile it - 2 is free
-        const int next = slot == 2 ? 0 : slot + 1;
-        const int mine = ROLE == 0 ? slot : slot == 0 ? 2 : slot - 1;
-        slot = next;
-        bool copied = it + 1 >= n_tiles;
-        auto copy_next = [&] {
-            if (!copied) tiles.copy(ahead.hg, ahead.tile(), next), ahead.next();
-            copied = true;
-        };
-        if (ROLE == 0 ? it < n_tiles : it > 0) {
-            const int pa = p0 + here.tile() * 64, turn = (ROLE == 0 ? it : it - 1) & 1;
-            here.next();
-            const Seen what = seen_by(w, x0, len, pa, min(pa + 63, p0 + w.Sq - 1));
-            if (what == Seen::kAll) tile(std::false_type{}, pa, mine, turn, copy_next);
-            else if (what == Seen::kSome) tile(std::true_type{}, pa, mine, turn, copy_next);
+        __syncthreads();                 // Q of tile t + 1, dO and statistics of t and P of t - 1 are visible; every wave is done with Q of t - 2, dO of t - 1
+        if (t + 2 < n_tiles) q.copy(pieces, w.Sq, lds + L::q(t + 2), wave, lane);
+        if (t + 1 < n_tiles) {
+            d.copy(pieces, w.Sq, lds + L::d(t + 1), wave, lane);
+            if (wave == 0) st.copy(lds + ((t + 1) & 1) * 256);
         }
-        copy_next();
+        const int pa = walk.p;
+        behind = here, here = ahead;
+        ahead = t + 1 < n_tiles ? seen_by(w, x0, len, pa, min(pa + 31, p_last)) : Seen::kNone;
+        walk.next();
+        if constexpr (ROLE == 0) {
+            const bool has = here != Seen::kNone, comes = ahead != Seen::kNone;
+            const uint32_t rows = lds + L::d(t), score = lds + L::q(t + 1);
+            if (has || comes) step(s, has, has ? rows : score, sn, ahead, comes ? score : rows, pa, t);
+        } else {
+            const bool has = behind != Seen::kNone, comes = here != Seen::kNone;
+            const uint32_t rows = lds + L::q(t - 1), score = lds + L::d(t);
+            if (has || comes) step(s, has, has ? rows : score, sn, here, comes ? score : rows, 0, t);
+        }
+    };
+    for (int t = -1; n_tiles > 0 && t <= n_tiles; t += 2) {
+        tile(s[0], s[1], t);
+        tile(s[1], s[0], t + 1);
     }
     __syncthreads();                     // (every copy has landed, every tile has been read: the ring takes the output rows)
-    uint8_t* os = smem + PL::RING + wave * 64 * D;
+    uint8_t* os = smem + L::RING + wave * 64 * D;
     if constexpr (ROLE == 0) key_rows_out<T, D>(a, acc, 1.0f, os, work.part, 1, a.dv + b * a.dv_sb + kvh * a.dv_sh, a.dv_sn, x0, work.k0, lane);
     else key_rows_out<T, D>(a, acc, w.scale, os, work.part, 0, a.dk + b * a.dk_sb + kvh * a.dk_sh, a.dk_sn, x0, work.k0, lane);
 }
 
 template <int T, int D>
-__global__ __launch_bounds__(kWaves<D> * 64, 2) void window_bwd_kernel(WindowBwdArgs a) {
-    constexpr bool PAIRED = D > 64;
-    constexpr int KV = PAIRED ? PairLds<T, D>::BYTES : KeyLds<D>::BYTES;
+__global__ __launch_bounds__(kWaves * 64, D > 64 ? 2 : 4) void window_bwd_kernel(WindowBwdArgs a) {
+    constexpr int KV = PairLds<T, D>::BYTES;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[KV > DqLds<D>::BYTES ? KV : DqLds<D>::BYTES];
     const int heads = a.w.B * a.w.Hk, rows = a.w.Sq * a.w.g;
-    const int tq = (rows + kRowsWg<D> - 1) / kRowsWg<D>, blocks = (a.w.Skv + kKeysWg - 1) / kKeysWg;
+    const int tq = (rows + kRowsWg - 1) / kRowsWg, blocks = (a.w.Skv + kKeysWg - 1) / kKeysWg;
     const int id = (int)blockIdx.x, nq = heads * tq;
     if (id < nq) {
         const int item = xcd_item(id, nq);
-        dq_body<T, D>(a, smem, item / tq, (tq - 1 - item % tq) * kRowsWg<D>);
+        dq_body<T, D>(a, smem, item / tq, (tq - 1 - item % tq) * kRowsWg);
         return;
     }
     const int tk = a.sink_blocks * a.sink_chunks + (blocks - a.sink_blocks) * a.chunks, item = xcd_item(id - nq, heads * tk);
-    const KeyWork work = key_work(a, item / tk, item % tk, blocks);
-    if constexpr (PAIRED) {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-        if (wave < 4) dkdv_role<T, D, 0>(a, smem, item / tk, work, wave, lane);
-        else dkdv_role<T, D, 1>(a, smem, item / tk, work, wave, lane);
-    } else {
-        dkdv_body<T, D>(a, smem, item / tk, work);
-    }
+    const KeyWork work = key_work<D>(a, item / tk, item % tk, blocks);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    if (wave < 2) dkdv_role<T, D, 0>(a, smem, item / tk, work, wave, lane);
+    else dkdv_role<T, D, 1>(a, smem, item / tk, work, wave, lane);
 }
 
 // Launch 3: dK and dV of the blocks that several workgroups share, their parts added in order.  8 channels to a thread.
@@ -735,12 +589,12 @@ __global__ __launch_bounds__(256) void window_bwd_join_kernel(WindowBwdArgs a) {
 template <int T, int D> hipError_t launch_td(const WindowBwdArgs& a, hipStream_t st) {
     const int64_t heads = (int64_t)a.w.B * a.w.Hk, rows = (int64_t)a.w.Sq * a.w.g, blocks = (a.w.Skv + kKeysWg - 1) / kKeysWg;
     const int64_t prep = (heads * a.w.g * a.sq_pad * (D / 8) + 255) / 256;
-    const int64_t grid = heads * ((rows + kRowsWg<D> - 1) / kRowsWg<D> + a.sink_blocks * a.sink_chunks + (blocks - a.sink_blocks) * a.chunks);
+    const int64_t grid = heads * ((rows + kRowsWg - 1) / kRowsWg + a.sink_blocks * a.sink_chunks + (blocks - a.sink_blocks) * a.chunks);
     const int64_t shared = (a.sink_chunks > 1 ? a.sink_blocks : 0) + (a.chunks > 1 ? blocks - a.sink_blocks : 0);
     const int64_t join = (heads * shared * 2 * kKeysWg * (D / 8) + 255) / 256;
     if (prep > 0x7FFFFFFF || grid > 0x7FFFFFFF || join > 0x7FFFFFFF) return hipErrorInvalidValue;
     hipLaunchKernelGGL((window_bwd_prep_kernel<T, D>), dim3((unsigned)prep), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((window_bwd_kernel<T, D>), dim3((unsigned)grid), dim3(kWaves<D> * 64), 0, st, a);
+    hipLaunchKernelGGL((window_bwd_kernel<T, D>), dim3((unsigned)grid), dim3(kWaves * 64), 0, st, a);
     if (join > 0) hipLaunchKernelGGL((window_bwd_join_kernel<T, D>), dim3((unsigned)join), dim3(256), 0, st, a);
     return hipGetLastError();
 }
@@ -748,20 +602,21 @@ template <int T, int D> hipError_t launch_td(const WindowBwdArgs& a, hipStream_t
 }  // namespace
 
 // A key block's pairs without sinks: as many as its window spans.  They are dealt to several workgroups where whole blocks would leave the chip
-// partly empty (two to a compute unit are wanted), down to 8 pairs; a block with sinks to as many as give each about that share too.
+// partly empty (four to a compute unit are wanted), down to 16 pairs; a block with sinks to as many as give each about that share too.
 void window_bwd_plan(WindowBwdArgs* a) {
     const WindowArgs& w = a->w;
-    const int64_t all = (w.Sq + 63) / 64, blocks = (w.Skv + kKeysWg - 1) / kKeysWg, heads = (int64_t)w.B * w.Hk;
-    const int64_t tiles = std::min<int64_t>(all, ((int64_t)w.left + w.right + kKeysWg + 62) / 64 + 1), pairs = tiles * w.g;
-    const int64_t want = std::max<int64_t>(1, 512 / (blocks * heads)), most = std::max<int64_t>(1, pairs / 8);
+    const int64_t keys = kWindowBwdKeys;
+    const int64_t all = (w.Sq + 31) / 32, blocks = (w.Skv + keys - 1) / keys, heads = (int64_t)w.B * w.Hk;
+    const int64_t tiles = std::min<int64_t>(all, ((int64_t)w.left + w.right + keys + 30) / 32 + 1), pairs = tiles * w.g;
+    const int64_t want = std::max<int64_t>(1, 1024 / (blocks * heads)), most = std::max<int64_t>(1, pairs / 16);
     const int64_t chunks = std::min(want, most), per = (pairs + chunks - 1) / chunks;
     a->chunks = (int)((pairs + per - 1) / per);
     a->chunk_tiles = (int)per;
-    a->sink_blocks = tiles < all ? (w.sinks + kKeysWg - 1) / kKeysWg : 0;
+    a->sink_blocks = tiles < all ? (int)((w.sinks + keys - 1) / keys) : 0;
     a->sink_chunks = (int)((all * w.g + per - 1) / per);
 }
 int64_t window_bwd_parts(const WindowBwdArgs& a) {
-    const int64_t blocks = (a.w.Skv + kKeysWg - 1) / kKeysWg;
+    const int64_t keys = kWindowBwdKeys, blocks = (a.w.Skv + keys - 1) / keys;
     return (int64_t)a.w.B * a.w.Hk * ((a.sink_chunks > 1 ? a.sink_blocks * a.sink_chunks : 0) + (a.chunks > 1 ? (blocks - a.sink_blocks) * a.chunks : 0));
 }
 

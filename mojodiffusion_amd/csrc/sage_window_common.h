@@ -76,6 +76,13 @@ struct RowMask {
     __device__ bool sees(int j) const { return j <= hi && (j >= lo || j < sinks); }
 };
 
+// The lane's number, formed where it is used: not kept in a register through a loop for what follows it.
+__device__ __forceinline__ int lane_here() {
+    uint32_t all = 0xFFFFFFFFu;
+    asm volatile("" : "+s"(all));
+    return (int)__builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0u));
+}
+
 // A wave's view of a tile: nothing of it, all of it, or some.
 enum class Seen { kNone, kAll, kSome };
 template <int KT> __device__ __forceinline__ Seen seen(const WindowArgs& a, int p_lo, int p_hi, int len, int j0) {
@@ -119,6 +126,54 @@ template <int D, int KT, int NW> struct TilePieces {
     }
     __device__ int row(int n) const { return row0 + n * PASS; }
     __device__ uint32_t col(int n, int lane) const { return (uint32_t)(PASS % 16 == 0 ? col0 : nat_pos<CPR>(row(n), lane % CPR) * 16); }
+};
+
+// Tiles of 32 keys of one head on their way into LDS: K and V each walk the tiles of a span, copied by NW waves.
+struct Range {
+    int first;
+    unsigned n;
+    __device__ bool has(int t) const { return (unsigned)(t - first) < n; }
+};
+template <int D, int NW> struct KeyTiles {
+    static constexpr int KT = 32;
+    using Pieces = TilePieces<D, KT, NW>;
+    Span span;
+    Pieces pieces;
+    uint32_t lds;
+    int wave, lane;
+    Range whole;                         // which tiles of the window are copied as they are
+    __device__ KeyTiles(const Span& s, uint32_t lds_, int wave_, int lane_) : span(s), pieces(wave_, lane_), lds(lds_), wave(wave_), lane(lane_) { whole = within(s.lo, s.hi); }
+    // The tiles of the window whose keys all lie in lo .. hi: what every tile of a walk would ask, answered once.
+    __device__ Range within(int lo, int hi) const {
+        const int t0 = max((max(lo, 0) + KT - 1) / KT, span.next), t1 = hi + 1 < KT ? span.next : (hi + 1) / KT;
+        return Range{t0 - span.next + span.first, (unsigned)max(t1 - t0, 0)};
+    }
+    struct Rows {                        // K or V: the tile to be copied next, and the lane's pieces where it is copied whole
+        const uint16_t* at;
+        int64_t tile;
+        uint32_t sn, off[Pieces::N];
+    };
+    __device__ Rows rows(const uint16_t* head, int64_t sn) const {
+        Rows r;
+        r.at = head + (int64_t)span.tile(0) * KT * sn;
+        r.tile = KT * sn;
+        r.sn = (uint32_t)sn * 2u;
+#pragma unroll
+        for (int i = 0; i < Pieces::N; i++) r.off[i] = pieces.row(i) * r.sn + pieces.col(i, lane);
+        return r;
+    }
+    __device__ void copy(Rows& r, int t, int to) const {
+#pragma unroll
+        for (int i = 0; i < Pieces::N; i++) {
+            uint32_t off = r.off[i];
+            if (!whole.has(t)) {
+                const int j0 = span.tile(t) * KT;
+                off = (uint32_t)(copied_key<KT>(span, j0, j0 + pieces.row(i)) - j0) * r.sn + pieces.col(i, lane);
+            }
+            dma16(r.at, off, __builtin_amdgcn_readfirstlane(lds + to + (i * NW + wave) * 1024));
+        }
+        r.at += (t + 1 == span.first ? span.next - t : 1) * r.tile;        // (from the tiles with sinks to the window's)
+    }
 };
 
 // 32 rows x0 .. of (query, head) pairs -> LDS at dst; rows past the last repeat it.  `base` is query i_base's row of the group's first head.
