@@ -17,6 +17,7 @@
 #include "sage_window_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace sage {
 
@@ -348,7 +349,7 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
     const Span span = key_span<KT>(a, p_lo, p_hi, len);
     const int p = p0 + min(x0 + l32, rows - 1) / a.g;
     const RowMask mask = {p - a.left, min(p + a.right, len - 1), a.sinks};
-    const int t0 = (int)((int64_t)span.n * split / a.splits), t1 = (int)((int64_t)span.n * (split + 1) / a.splits);
+    const int share = span.n / a.splits, over = span.n - share * a.splits, t0 = share * split + min(split, over), t1 = t0 + share + (split < over ? 1 : 0);
 
     const uint32_t ring = lds_addr(smem) + wave * L::RING;
     const uint8_t* own = smem + wave * L::RING;
@@ -371,7 +372,14 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
     v4i q[KS];
     const Fragments<D> fr(lane);
     query_rows_in<D>(a, a.q + b * a.q_sb + (int64_t)kvh * a.g * a.q_sh + (int64_t)i_lo * a.q_sn, a.q_sn, a.q_sh, i_lo, x0, ring, lane);
-    dma_wait<0>();
+    // (the first tile travels beside the rows where there is a slot for it)
+    int t = t0 + wave, slot = L::SLOTS - 1;
+    if (L::SLOTS == 2 && t < t1) {
+        copy_tile(t, 1);
+        dma_wait<2 * RUNS>();
+    } else {
+        dma_wait<0>();
+    }
 #pragma unroll
     for (int s = 0; s < KS; s++) q[s] = fr.along(own, s);
 #pragma unroll
@@ -383,8 +391,7 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
     // (a slot is filled again only when the reads of what it held have come back)
     auto reads_done = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
     reads_done();
-    int t = t0 + wave, slot = 0;
-    if (t < t1) copy_tile(t, 0);
+    if (L::SLOTS == 1 && t < t1) copy_tile(t, 0);
     for (; t < t1; t += NW) {
         if (L::SLOTS == 2 && t + NW < t1) {
             reads_done();
@@ -467,26 +474,79 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
     }
 }
 
-// One wave to a row: 64 lanes of D / 64 channels each.
-template <int T, int D>
+// 64 lanes of D / 64 channels each to a row; WAVES of them share a row's parts and meet in LDS: four where there are more than eight parts, one else.
+// What this launch takes is latencies (4 us of the 10 of one token against 1024 keys of 12 heads), so a wave requests eight parts (four, where
+// no more are left) at a time, their statistics with them, and adds them up as the tiles are, by a running maximum.
+constexpr int kJoinParts = 8;
+template <int T, int D, int WAVES>
 __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
     constexpr int N = D / 64;
+    typedef float vnf __attribute__((ext_vector_type(N)));
     const int rows = a.Sq * a.g, blocks = (rows + 31) / 32;
-    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= (int64_t)a.B * a.Hk * rows) return;
-    const int lane = threadIdx.x & 63, bh = (int)(at / rows), x = (int)(at % rows), b = bh / a.Hk, kvh = bh % a.Hk;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const uint32_t at = WAVES > 1 ? blockIdx.x : blockIdx.x * 4u + (uint32_t)wave;
+    if (at >= (uint32_t)(a.B * a.Hk * rows)) return;
+    const int lane = threadIdx.x & 63, bh = (int)(at / (uint32_t)rows), x = (int)at - bh * rows, b = bh / a.Hk, kvh = bh % a.Hk;
     const int64_t item = (int64_t)bh * blocks + x / 32;
     const float* ml = a.part_ml + (item * a.splits * 32 + x % 32) * 2;
     const float* part = a.part + (item * a.splits * 32 + x % 32) * D + lane * N;
     float ref = -INFINITY, sum = 0.0f, y[N];
-    for (int s = 0; s < a.splits; s++) ref = fmaxf(ref, ml[(int64_t)s * 64]);
 #pragma unroll
     for (int e = 0; e < N; e++) y[e] = 0.0f;
-    for (int s = 0; s < a.splits; s++) {
-        const float f = ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[(int64_t)s * 64] - ref);
-        sum = fmaf(ml[(int64_t)s * 64 + 1], f, sum);
+    auto take = [&](auto count, int s0) {
+        constexpr int AT_ONCE = decltype(count)::value;
+        vnf v[AT_ONCE];
+        float m[AT_ONCE], l[AT_ONCE], top = ref;
 #pragma unroll
-        for (int e = 0; e < N; e++) y[e] = fmaf(part[(int64_t)s * 32 * D + e], f, y[e]);
+        for (int u = 0; u < AT_ONCE; u++) {
+            const int64_t s = min(s0 + u, a.splits - 1);
+            m[u] = ml[s * 64];
+            l[u] = ml[s * 64 + 1];
+            v[u] = *reinterpret_cast<const vnf*>(part + s * 32 * D);
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++) top = fmaxf(top, m[u]);
+        if (top == -INFINITY) return;
+        const float f0 = __builtin_amdgcn_exp2f(ref - top);
+        ref = top;
+        sum *= f0;
+#pragma unroll
+        for (int e = 0; e < N; e++) y[e] *= f0;
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++) {
+            if (s0 + u >= a.splits) return;
+            const float f = __builtin_amdgcn_exp2f(m[u] - ref);
+            sum = fmaf(l[u], f, sum);
+#pragma unroll
+            for (int e = 0; e < N; e++) y[e] = fmaf(v[u][e], f, y[e]);
+        }
+    };
+    for (int s0 = WAVES > 1 ? wave * kJoinParts : 0; s0 < a.splits; s0 += WAVES * kJoinParts) {
+        if (a.splits - s0 > kJoinParts / 2) take(std::integral_constant<int, kJoinParts>{}, s0);
+        else take(std::integral_constant<int, kJoinParts / 2>{}, s0);
+    }
+    if constexpr (WAVES > 1) {
+        __shared__ float meet[WAVES][N + 2][64];
+        meet[wave][N][lane] = ref, meet[wave][N + 1][lane] = sum;
+#pragma unroll
+        for (int e = 0; e < N; e++) meet[wave][e][lane] = y[e];
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int n = 1; n < WAVES; n++) ref = fmaxf(ref, meet[n][N][lane]);
+        const float top = ref;
+        sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; e++) y[e] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < WAVES; n++) {
+            const float m = meet[n][N][lane];
+            if (m == -INFINITY) continue;
+            const float f = __builtin_amdgcn_exp2f(m - top);
+            sum = fmaf(meet[n][N + 1][lane], f, sum);
+#pragma unroll
+            for (int e = 0; e < N; e++) y[e] = fmaf(meet[n][e][lane], f, y[e]);
+        }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     const int i = x / a.g, hg = x - i * a.g;
@@ -503,8 +563,9 @@ template <int T, int D> hipError_t launch_td(const WindowArgs& a, const WindowPl
     if (!p.splits) hipLaunchKernelGGL((window_kernel<T, D>), dim3((unsigned)row_blocks(a, 128)), dim3(256), 0, st, a);
     else {
         hipLaunchKernelGGL((window_split_kernel<T, D>), dim3((unsigned)(row_blocks(a, 32) * a.splits)), dim3(256), 0, st, a);
-        if (a.splits > 1)
-            hipLaunchKernelGGL((window_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.B * a.Hk * a.Sq * a.g + 3) / 4)), dim3(256), 0, st, a);
+        const int64_t rows = (int64_t)a.B * a.Hk * a.Sq * a.g;
+        if (a.splits > kJoinParts) hipLaunchKernelGGL((window_join_kernel<T, D, 4>), dim3((unsigned)rows), dim3(256), 0, st, a);
+        else if (a.splits > 1) hipLaunchKernelGGL((window_join_kernel<T, D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
     }
     return hipGetLastError();
 }
@@ -516,15 +577,21 @@ template <int T> hipError_t launch_t(const WindowArgs& a, const WindowPlan& p, h
 
 }  // namespace
 
-// Rows enough for half the chip, or too many of them: tiles shared by four waves.  Else the keys are split until there are four workgroups to every
-// compute unit, down to 4 tiles (one to a wave).
+// Blocks of 128 rows for half the chip: tiles shared by four waves.  (96 such blocks at 128 channels: 30 us, split 27; 192: 30, split 40.)  One token a
+// sequence gains nothing from the sharing: there as many blocks as compute units are asked for (128 blocks of 8192 keys: 197 us, split 104; 512 of 2048: 97,
+// split 99).  Else the keys are split, until the chip is full once: a workgroup's LDS leaves room for two on a compute unit at 64 channels, one above.
+// Down to 128 keys (one tile to a wave), counted as a row sees them on the average; and to the root of their number, since the join's time
+// grows with the parts (one head against 65536 keys, us: 512 parts 37, 90 parts 16; 2048 keys: 9).
 WindowPlan window_plan(const WindowArgs& a) {
     constexpr int64_t kUnits = 256;
-    if (row_blocks(a, 128) >= kUnits / 2 || a.Sq * (int64_t)a.g > 512) return WindowPlan{0};
-    const int64_t keys = a.right >= kWindowFar || a.left >= kWindowFar ? a.Skv
-                                                                       : std::min<int64_t>(a.Skv, (int64_t)a.left + a.right + 32 / a.g + 1 + a.sinks);
-    const int64_t most = std::max<int64_t>(1, keys / 128), want = (4 * kUnits + row_blocks(a, 32) - 1) / row_blocks(a, 32);
-    return WindowPlan{(int)std::min(most, want)};
+    if (row_blocks(a, 128) >= (a.Sq * (int64_t)a.g > 32 ? kUnits / 2 : kUnits)) return WindowPlan{0};
+    int64_t keys = a.right >= kWindowFar || a.left >= kWindowFar ? a.Skv
+                                                                 : std::min<int64_t>(a.Skv, (int64_t)a.left + a.right + 32 / a.g + 1 + a.sinks);
+    if (a.right < kWindowFar) keys -= std::min<int64_t>(a.Sq, keys) / 2;
+    const int64_t room = (a.D > 64 ? kUnits : 2 * kUnits) / row_blocks(a, 32);
+    int64_t splits = std::max<int64_t>(1, std::min(room, keys / 128));
+    while (splits * splits > std::max<int64_t>(1, keys / 8)) splits--;
+    return WindowPlan{(int)splits};
 }
 bool window_grid_ok(const WindowArgs& a, const WindowPlan& p) {
     return row_blocks(a, 32) * std::max(p.splits, 1) <= 0x7FFFFFFF && (int64_t)a.B * a.Hk * a.Sq * a.g <= 0x7FFFFFFF;

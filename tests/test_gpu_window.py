@@ -17,7 +17,7 @@ def tensors(B, Sq, Skv, Hq, Hk, D, dtype, seed=0):
     return make(B, Sq, Hq, D).to(dtype), k.to(dtype), make(B, Skv, Hk, D).to(dtype)
 
 
-# Few rows (keys split over waves and workgroups) and many (shared tiles of 4 and of 8 waves); one query, one key; windows of one key, of whole
+# Few rows (keys split over waves and workgroups) and many (tiles shared by a workgroup's waves); one query, one key; windows of one key, of whole
 # tiles and one more or less; sinks inside, at and behind a tile's end, more than there are keys; right edges; no left edge, no edge at all;
 # sequences of length 0, 1 and others; queries before the first key and behind the last; odd groups of heads.
 CASES = [
@@ -44,10 +44,23 @@ CASES = [
     (2, 2100, 2100, 20, 5, 64, FP, 90, 0, 4, [2100, 1500], 0),
     (1, 600, 600, 2, 2, 128, BF, 5, 0, 3, [600], [10]),
 ]
+# ... and with rows enough for shared tiles
+MANY = [
+    (8, 33, 33, 32, 16, 64, BF, 7, 0, 4, None, 0),
+    (8, 100, 100, 16, 16, 256, FP, 16, 16, 0, None, 0),
+    (8, 65, 200, 48, 16, 128, BF, 63, 0, 64, [200, 0, 1, 64, 65, 128, 199, 37], 120),
+    (4, 150, 150, 60, 12, 64, BF, -1, 0, 0, None, 0),
+    (8, 40, 129, 16, 16, 128, BF, -1, -1, 0, [129, 64, 0, 1, 33, 32, 31, 100], 0),
+    (8, 70, 300, 32, 16, 128, FP, 20, 3, 500, None, 250),
+    (8, 9, 150, 32, 32, 64, FP, 4, 0, 2, [150] * 8, [-3, 48, -20, 190, 0, 1, 149, 140]),
+    (4, 270, 270, 16, 16, 256, BF, 100, 10, 33, [270, 3, 0, 200], 0),
+    (64, 1, 200, 8, 4, 128, BF, 50, 0, 4, [200 - 3 * i for i in range(64)], 130),
+    (1, 140, 140, 64, 64, 128, BF, 0, 0, 0, None, 0),
+]
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("B,Sq,Skv,Hq,Hk,D,dtype,left,right,sinks,lens,first", CASES)
+@pytest.mark.parametrize("B,Sq,Skv,Hq,Hk,D,dtype,left,right,sinks,lens,first", CASES + MANY)
 def test_forward(B, Sq, Skv, Hq, Hk, D, dtype, left, right, sinks, lens, first):
     q, k, v = tensors(B, Sq, Skv, Hq, Hk, D, dtype, Sq + Skv)
     n = [Skv] * B if lens is None else lens
@@ -82,6 +95,10 @@ DECODE = [
     (5, 1, 64, 12, 12, 128, BF, 10, 64, [64, 1, 2, 30, 11]),
     (2, 1, 200, 2, 2, 64, BF, 8, 3, [500, -4]),
     (1, 2, 9000, 16, 1, 256, FP, 8191, 4, [8999]),
+    (1, 1, 6000, 8, 1, 64, FP, -1, 3, [5990]),
+    (2, 1, 1500, 4, 2, 64, BF, -1, 0, [1500, 12]),
+    (64, 1, 90, 8, 4, 128, FP, 40, 3, [90 - i for i in range(64)]),
+    (128, 3, 70, 2, 2, 256, BF, -1, 0, [i % 71 for i in range(128)]),
 ]
 
 
@@ -102,10 +119,10 @@ def test_decode(B, Sq, cap, Hq, Hk, D, dtype, left, sinks, lens):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("Sq,first", [(40, 960), (640, 300)])
-def test_keys_that_no_query_sees_are_not_read(Sq, first):
+@pytest.mark.parametrize("Sq,first,H", [(40, 960, 2), (640, 300, 2), (300, 500, 32)])
+def test_keys_that_no_query_sees_are_not_read(Sq, first, H):
     """Between the sinks and the window's left edge, behind its right edge and behind the length: whatever lies there, the same bits."""
-    B, Skv, H, D, left, right, sinks, n = 2, 1100, 2, 128, 50, 5, 70, 1090
+    B, Skv, D, left, right, sinks, n = 2, 1100, 128, 50, 5, 70, 1090
     q, k, v = (t.cuda() for t in tensors(B, Sq, Skv, H, H, D, BF, 3))
     lens = torch.tensor([n, n], dtype=torch.int32).cuda()
     args = dict(scale=0.1, left=left, right=right, sinks=sinks, kv_lens=lens, q_start=first)
@@ -120,9 +137,10 @@ def test_keys_that_no_query_sees_are_not_read(Sq, first):
 
 
 @pytest.mark.gpu
-def test_extreme_scores():
+@pytest.mark.parametrize("S,H,D", [(600, 1, 64), (130, 64, 64), (130, 64, 128)])
+def test_extreme_scores(S, H, D):
     """Scores of +-1e4 and more, rising along the keys and falling, equal ones, and masked keys whose scores would be the largest."""
-    B, S, H, D = 1, 600, 1, 64
+    B = 1
     q, k, v = tensors(B, S, S, H, H, D, BF, 5)
     rise = torch.linspace(-30, 30, S).view(1, S, 1, 1)
     for kk, qq in ((k * 0 + rise, q * 0 + 4), (k * 0 - rise, q * 0 + 4), (k * 0, q), (k * 40, q * 40)):
@@ -169,6 +187,9 @@ def test_offsets_beyond_32_bits():
     q = torch.randn((1, 600, 4, D)).to(BF)
     ref = forward(q, k[:, 39000:], v[:, 39000:], 0.125, 20, 0, 0, [1000], [300])
     check_forward(W.sdpa_window(q.cuda(), k, v, 0.125, 20, 0, 0, q_start=39300), None, ref, BF)
+    q = torch.randn((1, 4200, 4, D)).to(BF).cuda()
+    window = (0.125, 20, 0, 4, None, 35000)
+    assert torch.equal(W.sdpa_window(q, k, v, *window), W.sdpa_window(q, k.contiguous(), v.contiguous(), *window))
 
 
 @pytest.mark.gpu
