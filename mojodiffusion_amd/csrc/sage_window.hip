@@ -46,64 +46,52 @@ template <int D> struct RowState {
             for (int i = 0; i < 16; i++) acc[d][i] *= f;
     }
 };
-// MASKED: some row does not see all of the tile.  FINE: the weights enter as two operands, what rounding leaves of them in a second product: for workgroups of
+// FINE: the weights enter as two operands, what rounding leaves of them in a second product: for workgroups of
 // at most kFineKeys keys, whose rows average over too few keys for the roundings of their weights to fade (relative error of dQ, whose row sums are
 // taken from O, on a padded batch with sinks: 0.0027 without, 0.0024 with it; the products are a small part of what such a workgroup does).
 constexpr int kFineKeys = 128;
-template <int T, int D, int KT, bool MASKED, bool FINE>
-__device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 16], const uint8_t* kt, const uint8_t* vt, const Fragments<D>& kept,
-                                            int j0, const RowMask& m, float c, int half) {
-    constexpr int KS = D / 16, DB = D / 32, NB = KT / 32;
-    const Fragments<D> fr = kept.fresh();
-    v16f s[NB];
+template <int T, int D, bool FINE>
+__device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 16], uint32_t kt, uint32_t vt, const Fragments<D>& kept,
+                                            Seen what, int j0, const RowMask& m, float c) {
+    constexpr int KS = D / 16, DB = D / 32;
+    const Fragments<D> f = kept.fresh();
+    auto key = [&](int ks) { return lds_read(kt + (f.nat ^ ((ks & 7) << 5)) + (ks >> 3) * 256); };
+    v16f s = product<T>(key(0), q[0], v16f{});
 #pragma unroll
-    for (int blk = 0; blk < NB; blk++) {
+    for (int ks = 1; ks < KS; ks++) s = product<T>(key(ks), q[ks], s);
+    if (what != Seen::kAll) {
+        const RowMask rel = m.from(j0 + (lane_here() >> 5) * 4);
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[blk][i] = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++)
-            s[blk] = product<T>(fr.along(kt + blk * 64 * D, ks), q[ks], s[blk]);
+        for (int i = 0; i < 16; i++) s[i] = rel.sees((i >> 2) * 8 + (i & 3)) ? s[i] : -INFINITY;
     }
-    const RowMask rel = m.from(j0 + half * 4);
-    float top = -INFINITY;
+    float top = s[0];
 #pragma unroll
-    for (int blk = 0; blk < NB; blk++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            if (MASKED && !rel.sees(blk * 32 + (i >> 2) * 8 + (i & 3))) s[blk][i] = -INFINITY;
-            top = fmaxf(top, s[blk][i]);
-        }
+    for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
     top = max_halves(top) * c;
     // A new reference only where the old one lies more than 8 below: the weights stay under 2^8, and the sums have
     // room for that; O is multiplied on few tiles instead of on most.
     if (__any(top > st.ref + 8.0f)) st.raise(top);
-    const float ref = MASKED && st.ref == -INFINITY ? 0.0f : st.ref;       // (no key so far: every weight is exp2(-inf))
-    uint32_t p[NB][8], fine[FINE ? NB : 1][8];
+    const float ref = st.ref == -INFINITY ? 0.0f : st.ref;       // (no key so far: every weight is exp2(-inf))
+    uint32_t p[8], fine[FINE ? 8 : 1];
     float part[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int blk = 0; blk < NB; blk++)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-            const float x = __builtin_amdgcn_exp2f(fmaf(s[blk][i], c, -ref)), y = __builtin_amdgcn_exp2f(fmaf(s[blk][i + 1], c, -ref));
-            part[0] += x;
-            part[1] += y;
-            p[blk][i >> 1] = pack2<T>(x, y);
-            if constexpr (FINE) fine[blk][i >> 1] = pack2<T>(rounded_off<T>(x), rounded_off<T>(y));
-        }
+    for (int i = 0; i < 16; i += 2) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ref)), y = __builtin_amdgcn_exp2f(fmaf(s[i + 1], c, -ref));
+        part[0] += x;
+        part[1] += y;
+        p[i >> 1] = pack2<T>(x, y);
+        if constexpr (FINE) fine[i >> 1] = pack2<T>(rounded_off<T>(x), rounded_off<T>(y));
+    }
     st.sum += part[0] + part[1];
 #pragma unroll
-    for (int blk = 0; blk < NB; blk++)
+    for (int j2 = 0; j2 < 2; j2++)
 #pragma unroll
-        for (int j2 = 0; j2 < 2; j2++) {
-            const v4i pb = {(int)p[blk][j2 * 4], (int)p[blk][j2 * 4 + 1], (int)p[blk][j2 * 4 + 2], (int)p[blk][j2 * 4 + 3]};
-            const uint8_t* rows = vt + (blk * 2 + j2) * 32 * D;
-#pragma unroll
-            for (int d = 0; d < DB; d++) {
-                const v4i vf = fr.across(rows, d);
-                st.acc[d] = product<T>(vf, pb, st.acc[d]);
-                if constexpr (FINE)
-                    st.acc[d] = product<T>(vf, v4i{(int)fine[blk][j2 * 4], (int)fine[blk][j2 * 4 + 1], (int)fine[blk][j2 * 4 + 2], (int)fine[blk][j2 * 4 + 3]}, st.acc[d]);
-            }
+        for (int d = 0; d < DB; d++) {
+            const uint32_t at = vt + j2 * 32 * D + (d >> 2) * 256;
+            const v4i vf = lds_read_across(at + (f.tr[0] ^ ((d & 3) << 6)), at + (f.tr[1] ^ ((d & 3) << 6)));
+            st.acc[d] = product<T>(vf, v4i{(int)p[j2 * 4], (int)p[j2 * 4 + 1], (int)p[j2 * 4 + 2], (int)p[j2 * 4 + 3]}, st.acc[d]);
+            if constexpr (FINE)
+                st.acc[d] = product<T>(vf, v4i{(int)fine[j2 * 4], (int)fine[j2 * 4 + 1], (int)fine[j2 * 4 + 2], (int)fine[j2 * 4 + 3]}, st.acc[d]);
         }
 }
 
@@ -127,9 +115,7 @@ __device__ __forceinline__ void finish_rows(const WindowArgs& a, const RowState<
     query_rows_out<D>(a, os, a.rest + at, a.o_sn, a.o_sh, x0, lane);
 }
 
-// Tiles of 32 keys, two slots for K and two for V, which is needed one step later.  (A third of each: 1620 -> 1662 us at [1,16896,48 on 12,128], 287 -> 320 for one
-// token of 32 sequences: less LDS, more workgroups.)  The waves' own rows lie over all slots but K's first at the start, and over the
-// front again at the end.
+// Tiles of 32 keys, two slots.  The waves' own rows lie over all of them but K's first at the start, and over the front again at the end.
 template <int D> struct WindowLds {
     static constexpr int NW = 4, KT = 32, TILE = KT * D * 2, OWN = NW * 64 * D;
     static constexpr int K0 = 3 * TILE > OWN ? 3 * TILE : OWN, BYTES = K0 + TILE;
@@ -137,11 +123,12 @@ template <int D> struct WindowLds {
     static __device__ int values(int t) { return (t & 1) * TILE; }
 };
 
-// Workgroups of four waves, 128 rows: two or more share a compute unit and meet no common barrier, so that one's matrix instructions run
-// beside another's vector instructions (128 channels, us: 8 waves with tiles of 64 keys -> this form: [1,16896,48 on 12] window 4096 + 4 1683 -> 1673, a
-// step of [2,1248,30] window +-256 201 -> 190, one token of 32 sequences against 8192 keys 361 -> 287).
+// Workgroups of four waves, 128 rows.  A wave's step from scores to exponentials to products is one chain; what fills the gaps is the waves of other
+// workgroups on the same SIMD, which meet no common barrier with it: five at 64 channels, three at 128, two at 256 (by registers: O, Q and one
+// tile's scores are 64, 112, 208 of them).  The next tile's scores taken beside this one's weights, with a wave less, was slower: [1,16896,48 on 12,128]
+// window 4096 + 4 1615 us, this form 1553; a training step of [2,1248,30,128] +-256 180, 175.  Two waves of this form at 128 channels: 1950.
 template <int T, int D>
-__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void window_kernel(WindowArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 5 : D == 128 ? 3 : 2) void window_kernel(WindowArgs a) {
     using L = WindowLds<D>;
     constexpr int NW = L::NW, KT = L::KT, KS = D / 16;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
@@ -149,7 +136,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void window_kernel(WindowArgs
     const int item = xcd_item((int)blockIdx.x, a.B * a.Hk * blocks);
     const int bh = item / blocks, row0 = (blocks - 1 - item % blocks) * NW * 32;       // (the last rows first: without a left edge they see most keys)
     const int b = bh / a.Hk, kvh = bh % a.Hk;
-    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int x0 = row0 + wave * 32;
 
@@ -174,129 +161,26 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void window_kernel(WindowArgs
     for (int s = 0; s < KS; s++) q[s] = fr.along(smem + wave * 64 * D, s);
 #pragma unroll
     for (int s = 0; s < KS; s++) {
-        if constexpr (D > 128) asm volatile("" : "+a"(q[s]));          // (room among the vector registers: the products read them there too)
-        else asm volatile("" : "+v"(q[s]));
+        asm volatile("" : "+v"(q[s]));
     }
     __syncthreads();                     // the rows' LDS becomes the rings' slots
+    if (span.n > 0) tiles.copy(v, 0, L::values(0));
 
     RowState<D> st;
     st.clear();
     const float c = a.scale * kLog2e;
-    if (D <= 128 && span.n * KT <= kFineKeys) {
+    auto walk = [&](auto fine) {
         for (int t = 0; t < span.n; t++) {
-            if (t > 0) {
-                __syncthreads();         // every wave is done with tile t - 1
-                tiles.copy(k, t, L::keys(0));
-            }
-            tiles.copy(v, t, L::values(0));
             dma_wait<0>();
-            __syncthreads();
+            __syncthreads();             // tile t is visible; every wave is done with tile t - 1
+            if (t + 1 < span.n) tiles.copy(k, t + 1, L::keys(t + 1)), tiles.copy(v, t + 1, L::values(t + 1));
             const int j0 = span.tile(t) * KT;
-            if (x0 < rows && seen<KT>(a, wp_lo, wp_hi, len, j0) != Seen::kNone)
-                attend_tile<T, D, KT, true, true>(st, q, smem + L::keys(0), smem + L::values(0), fr, j0, mask, c, half);
+            const Seen what = all.has(t) ? Seen::kAll : x0 < rows ? seen<KT>(a, wp_lo, wp_hi, len, j0) : Seen::kNone;
+            if (what != Seen::kNone) attend_tile<T, D, decltype(fine)::value>(st, q, lds + L::keys(t), lds + L::values(t), fr, what, j0, mask, c);
         }
-    } else {
-        // One tile after the other: the scores of the next are taken while this one's weights are formed, so that matrix and vector instructions of a
-        // wave overlap; what a tile costs either pipe is about the same.  Where a wave takes part in only one of the two, the other runs on
-        // rows that are there anyway, with weights of zero or scores that are dropped: one path, so that O stays where it is.
-        constexpr int NK = KS < 8 ? KS : 8, NV = D < 128 ? D / 32 : 4;
-        auto step = [&](const v16f& x, bool now, uint32_t values, v16f& y, Seen next, uint32_t keys, int j0) {
-            const Fragments<D> f = fr.fresh();
-            uint32_t ka[NK], va[NV][2];  // where the fragments lie
-#pragma unroll
-            for (int s = 0; s < NK; s++) ka[s] = keys + (f.nat ^ (s << 5));
-#pragma unroll
-            for (int d = 0; d < NV; d++) va[d][0] = values + (f.tr[0] ^ (d << 6)), va[d][1] = values + (f.tr[1] ^ (d << 6));
-            // Products in groups of four, the operands of a group requested a group ahead; the scheduler keeps to the groups where there is no second
-            // wave on the SIMD to run meanwhile (256 channels: 207 -> 162 us at [1,4429,18,256] window +-511).
-            constexpr int NG = KS / 4, DB = D / 32, NP = 2 * DB / 4;
-            constexpr bool ALONE = D > 128;
-            v4i f4[2][4];
-            auto request_k = [&](int g) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) f4[g & 1][i] = lds_read(ka[(g * 4 + i) & 7] + (g >> 1) * 256);
-            };
-            auto request_v = [&](int g) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int j2 = (g * 4 + i) / DB, d = (g * 4 + i) % DB, at = j2 * 32 * D + (d >> 2) * 256;
-                    f4[(NG + g) & 1][i] = lds_read_across(va[d & 3][0] + at, va[d & 3][1] + at);
-                }
-            };
-            auto group_ends = [] {
-                if constexpr (ALONE) __builtin_amdgcn_sched_barrier(0);
-            };
-            request_k(0);
-            if (next == Seen::kAll) {
-                y = product<T>(f4[0][0], q[0], v16f{});
-            } else {                     // (scores that are not seen start, and stay, at -inf)
-                const RowMask rel = next == Seen::kNone ? RowMask{1, -1, 0} : mask.from(j0 + half * 4);
-#pragma unroll
-                for (int i = 0; i < 16; i++) y[i] = rel.sees((i >> 2) * 8 + (i & 3)) ? 0.0f : -INFINITY;
-                y = product<T>(f4[0][0], q[0], y);
-            }
-            uint32_t w[8];
-            float part[2] = {0.0f, 0.0f};
-            // (no key so far: every weight is exp2(-inf); no tile now: likewise, by a reference of +inf, without a branch in the middle)
-            const float ref = (st.ref == -INFINITY ? 0.0f : st.ref) + __uint_as_float(0x7F800000u & ((uint32_t)now - 1u));
-#pragma unroll
-            for (int g = 0; g < NG; g++) {
-                if (g + 1 < NG) request_k(g + 1);
-                else request_v(0);
-#pragma unroll
-                for (int i = g == 0; i < 4; i++) y = product<T>(f4[g & 1][i], q[g * 4 + i], y);
-#pragma unroll
-                for (int i = g * (16 / NG); i < (g + 1) * (16 / NG); i += 2) {
-                    const float u = __builtin_amdgcn_exp2f(fmaf(x[i], c, -ref)), v = __builtin_amdgcn_exp2f(fmaf(x[i + 1], c, -ref));
-                    part[0] += u;
-                    part[1] += v;
-                    w[i >> 1] = pack2<T>(u, v);
-                }
-                group_ends();
-            }
-            st.sum += part[0] + part[1];
-            float top = y[0];
-#pragma unroll
-            for (int g = 0; g < NP; g++) {
-                if (g + 1 < NP) request_v(g + 1);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int j2 = (g * 4 + i) / DB, d = (g * 4 + i) % DB;
-                    st.acc[d] = product<T>(f4[(NG + g) & 1][i], v4i{(int)w[j2 * 4], (int)w[j2 * 4 + 1], (int)w[j2 * 4 + 2], (int)w[j2 * 4 + 3]}, st.acc[d]);
-                }
-                if (g == NP - 1) {
-#pragma unroll
-                    for (int i = 1; i < 16; i++) top = fmaxf(top, y[i]);
-                }
-                group_ends();
-            }
-            top = max_halves(top) * c;
-            if (__any(top > st.ref + 8.0f)) st.raise(top);
-        };
-        v16f s[2];
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[0][i] = s[1][i] = -INFINITY;
-        Seen now = Seen::kNone;
-        auto tile = [&](const v16f& x, v16f& y, int t) {
-            dma_wait<0>();
-            __syncthreads();             // K of tile t + 1 and V of tile t are visible; every wave is done with K of t and V of t - 1
-            if (t + 2 < span.n) tiles.copy(k, t + 2, L::keys(t));
-            if (t + 1 < span.n) tiles.copy(v, t + 1, L::values(t + 1));
-            Seen next = Seen::kNone;
-            if (all.has(t + 1)) next = Seen::kAll;
-            else if (t + 1 < span.n && x0 < rows) next = seen<KT>(a, wp_lo, wp_hi, len, span.tile(t + 1) * KT);
-            const bool has = now != Seen::kNone, comes = next != Seen::kNone;
-            if (has || comes) {
-                const uint32_t keys = lds + L::keys(t + 1), values = lds + L::values(t);
-                step(x, has, has ? values : keys, y, next, comes ? keys : values, comes ? span.tile(t + 1) * KT : 0);
-            }
-            now = next;
-        };
-        for (int t = -1; t < span.n; t += 2) {               // (a tile past the last: nothing is seen, nothing copied)
-            tile(s[0], s[1], t);
-            tile(s[1], s[0], t + 1);
-        }
-    }
+    };
+    if (D <= 128 && span.n * KT <= kFineKeys) walk(std::bool_constant<D <= 128>{});
+    else walk(std::false_type{});
     __syncthreads();                     // (no copy is in flight: the last step's wait was for all of them)
     if (x0 < rows) finish_rows<T, D>(a, st, smem + wave * 64 * D, b, kvh, x0, lane);
 }
@@ -401,10 +285,10 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
             dma_wait<0>();
         }
         const int j0 = span.tile(t) * KT;
-        const uint8_t* kt = own + slot * L::SLOT;
-        if (D <= 128 && span.n * KT <= kFineKeys) attend_tile<T, D, KT, true, true>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
-        else if (D <= 128 && seen<KT>(a, p_lo, p_hi, len, j0) == Seen::kAll) attend_tile<T, D, KT, false, false>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
-        else attend_tile<T, D, KT, true, false>(st, q, kt, kt + L::TILE, fr, j0, mask, c, half);
+        const uint32_t kt = ring + slot * L::SLOT;
+        const Seen what = seen<KT>(a, p_lo, p_hi, len, j0);
+        if (D <= 128 && span.n * KT <= kFineKeys) attend_tile<T, D, D <= 128>(st, q, kt, kt + L::TILE, fr, what, j0, mask, c);
+        else attend_tile<T, D, false>(st, q, kt, kt + L::TILE, fr, what, j0, mask, c);
         if (L::SLOTS == 2) slot ^= 1;
         else if (t + NW < t1) {
             reads_done();

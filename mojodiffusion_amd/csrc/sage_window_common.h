@@ -109,9 +109,6 @@ template <int D> struct Fragments {
         return f;
     }
     __device__ v4i along(const uint8_t* tile, int s) const { return *reinterpret_cast<const v4i*>(tile + (nat ^ ((s & 7) << 5)) + (s >> 3) * 256); }
-    __device__ v4i across(const uint8_t* rows, int d) const {
-        return tr_read(rows + (tr[0] ^ ((d & 3) << 6)) + (d >> 2) * 256, rows + (tr[1] ^ ((d & 3) << 6)) + (d >> 2) * 256);
-    }
 };
 
 // The pieces of a [KT][D] tile that a lane of NW waves copies: piece n is 16 bytes of row(n).  Rows a multiple of 16 apart are laid out alike,
