@@ -461,7 +461,7 @@ int mi355_sage_cast(int count, const void* const* src, void* const* dst, const i
  * pairs (2i, 2i+1) or, with halfsplit, (i, i + rot/2): (a, b) -> (a cos - b sin, b cos + a sin).  Channels from rot on pass.
  * Q [B,Hq,S,D] and K [B,Hk,S,D] through four element strides each (D stride 1, rows 16-byte aligned, so that slices of a joint
  * projection are taken as they are), of one type: bf16, fp16 or F32; so are Q_out and K_out, which may be Q and K themselves
- * (same base and strides), or rows of a cache; otherwise nothing written may overlap what is read.  D: a multiple of 16 up to 256.
+ * (same base and strides), or rows of a cache; otherwise nothing written may overlap what is read, nor rows of an output each other.  D: a multiple of 16 up to 256.
  * rot: a multiple of 16 up to D, 0 = no rotation (no tables needed).  Gains [D] and tables [table_rows, rot/2] (element stride
  * table_stride between rows) of any of the three types, 16-byte aligned.  The row of the tables is positions[b*pos_stride + s]
  * (pos_bytes 4 or 8: int32 or int64), or s without positions; where a position lies outside [0, table_rows) the token's

@@ -216,6 +216,7 @@ class _SdpaWindowNode(torch.autograd.Function):
         return fwd.o
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         o, rest, stats, q, k, v, lens = ctx.saved_tensors
         scale, left, right, sinks, q_start = ctx.window

@@ -1138,6 +1138,14 @@ int mi355_sage_sdpa_bwd_f32_grads(const void* Q, const void* K, const void* V, c
 // ---- norm and rotation of queries and keys -------------------------------------------------------
 // What both directions check and fill in.  `views`: per side input, output and (backward) upstream gradient.
 struct NormRopeView { const char* name; const void* p; const int64_t* s; int64_t off; };
+// Rows that are written must be told apart by their strides: a broadcast tensor cannot be an output.
+static int distinct_rows(const char* name, const int64_t* s, int B, int H, int N) {
+    if ((B > 1 && s[0] == 0) || (H > 1 && s[1] == 0) || (N > 1 && s[2] == 0)) {
+        SAGE_LOG("%s: an output's rows must lie apart", name);
+        return MI355_SAGE_EINVAL;
+    }
+    return 0;
+}
 static int norm_rope_args(const NormRopeView (&q)[3], const NormRopeView (&k)[3], int views, int B, int S, int Hq, int Hk, int D, int type,
                           const void* q_gain, const void* k_gain, int gain_type, float eps, const void* rope_cos, const void* rope_sin,
                           int table_type, int rot, int64_t table_rows, int64_t table_stride, int halfsplit, const void* positions,
@@ -1151,6 +1159,8 @@ static int norm_rope_args(const NormRopeView (&q)[3], const NormRopeView (&k)[3]
     if (positions != nullptr && pos_bytes != 4 && pos_bytes != 8) return MI355_SAGE_EINVAL;
     if (D % 16 || D > 256 || rot % 16) { SAGE_LOG("norm_rope: head dim %d, %d rotated (multiples of 16 up to 256)", D, rot); return MI355_SAGE_EUNSUPPORTED; }
     if ((int64_t)B * S > (1 << 30) / ((int64_t)Hq + Hk)) { SAGE_LOG("norm_rope: more than 2^30 rows"); return MI355_SAGE_EUNSUPPORTED; }
+    if (int rc = distinct_rows(q[1].name, q[1].s, B, Hq, S)) return rc;
+    if (int rc = distinct_rows(k[1].name, k[1].s, B, Hk, S)) return rc;
     const int esz = type == MI355_SAGE_F32 ? 4 : 2, align = 16 / esz;
     for (const NormRopeView* side : {q, k})
         for (int i = 0; i < views; i++) {
@@ -1268,7 +1278,7 @@ static int window_forward(const char* name, const void* Q, const void* K, const 
     if (!Q || !K || !V || !O || !qs || !ks || !vs || !os) return MI355_SAGE_EINVAL;
     int rc;
     if ((rc = check_view("Q", Q, qs, q_off)) || (rc = check_view("K", K, ks, k_off)) || (rc = check_view("V", V, vs, v_off)) ||
-        (rc = check_view("O", O, os, o_off)) || (rc = window_span("Q", qs, 256 / a.g + 2, a.g, a.D)) || (rc = window_span("K", ks, 64, 1, a.D)) ||
+        (rc = check_view("O", O, os, o_off)) || (rc = distinct_rows("O", os, a.B, a.Hk * a.g, a.Sq)) || (rc = window_span("Q", qs, 256 / a.g + 2, a.g, a.D)) || (rc = window_span("K", ks, 64, 1, a.D)) ||
         (rc = window_span("V", vs, 64, 1, a.D)))
         return rc;
     const View q = make_view(Q, qs, q_off), k = make_view(K, ks, k_off), v = make_view(V, vs, v_off);
@@ -1360,7 +1370,8 @@ int mi355_sage_sdpa_window_bwd(const void* Q, const void* K, const void* V, cons
     if ((rc = check_view("Q", Q, q_strides, q_off)) || (rc = check_view("K", K, k_strides, k_off)) || (rc = check_view("V", V, v_strides, v_off)) ||
         (rc = check_view("O", O, o_strides, o_off)) || (rc = check_view("dO", dO, do_strides, do_off)) || (rc = check_view("dQ", dQ, dq_strides, dq_off)) ||
         (rc = check_view("dK", dK, dk_strides, dk_off)) || (rc = check_view("dV", dV, dv_strides, dv_off)) ||
-        (O_rest && (rc = check_view("O_rest", O_rest, o_strides, o_off))))
+        (O_rest && (rc = check_view("O_rest", O_rest, o_strides, o_off))) || (rc = distinct_rows("dQ", dq_strides, B, Hq, N_q)) ||
+        (rc = distinct_rows("dK", dk_strides, B, Hk, N_kv)) || (rc = distinct_rows("dV", dv_strides, B, Hk, N_kv)))
         return rc;
     const int64_t rows = 256 / a.w.g + 66;               // (a block of rows, or a tile of 64)
     if ((rc = window_span("Q", q_strides, rows, a.w.g, D)) || (rc = window_span("dO", do_strides, rows, a.w.g, D)) ||

@@ -124,6 +124,8 @@ def _out(name, out, like):
         raise Error("%s: an output must have the shape, type and device of its input" % name)
     if not _rows_ok(out):
         raise Error("%s: rows of an output must be dense and 16-byte aligned" % name)
+    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        raise Error("%s: rows of an output must lie apart" % name)
     return out
 
 
@@ -195,6 +197,7 @@ class _QkNormRopeNode(torch.autograd.Function):
         return qo, ko
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, g_q, g_k):
         q, k, q_norm, k_norm, cos, sin, positions = ctx.saved_tensors
         g = qk_norm_rope_backward(g_q.to(q.dtype), g_k.to(k.dtype), q, k, q_norm, k_norm, ctx.eps, cos, sin, ctx.halfsplit, positions)

@@ -318,6 +318,7 @@ def test_c_refusals():
     st = _lib.strides_bhnd(8, 4, 64)
     bad = (ctypes.c_int64 * 4)(8 * 4 * 64, 64, 4 * 64, 2)
     off = (ctypes.c_int64 * 4)(8 * 4 * 64, 60, 4 * 64, 1)
+    flat = (ctypes.c_int64 * 4)(8 * 4 * 64, 0, 4 * 64, 1)
     base = dict(q=A, k=A, qo=A, ko=A, B=1, S=8, Hq=4, Hk=4, D=64, type=0, qs=st, ks=st, qos=st, kos=st, o=(0, 0, 0, 0), gq=A, gk=A, gt=2,
                 eps=1e-6, c=A, s=A, tt=2, rot=64, rows=8, stride=32, half=0, pos=None, ps=0, pb=0)
 
@@ -327,7 +328,8 @@ def test_c_refusals():
                                          a["qos"], a["kos"], *a["o"], a["gq"], a["gk"], a["gt"], a["eps"], a["c"], a["s"], a["tt"], a["rot"],
                                          a["rows"], a["stride"], a["half"], a["pos"], a["ps"], a["pb"], None)
     for change in (dict(q=None), dict(ko=None), dict(gq=None), dict(qs=None), dict(B=0), dict(S=-1), dict(Hk=0), dict(type=3), dict(gt=-1), dict(tt=5),
-                   dict(rot=80), dict(rot=-16), dict(c=None), dict(rows=7), dict(rows=0, pos=A, pb=4), dict(pos=A, pb=2), dict(eps=-1.0)):
+                   dict(rot=80), dict(rot=-16), dict(c=None), dict(rows=7), dict(rows=0, pos=A, pb=4), dict(pos=A, pb=2), dict(eps=-1.0),
+                   dict(kos=flat), dict(qos=flat)):
         assert fwd(**change) == -1, change
     for change in (dict(D=72, rot=32), dict(D=272), dict(rot=24), dict(qs=bad), dict(kos=off), dict(q=A + 8), dict(o=(4, 0, 0, 0)), dict(gk=A + 4),
                    dict(stride=33), dict(B=1 << 15, S=1 << 15, rows=1 << 15)):

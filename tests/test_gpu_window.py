@@ -391,7 +391,7 @@ def test_c_refusals():
                                         a["qs"], a["ks"], a["vs"], a["os"], *a["off"], 0, a["left"], a["right"], a["sinks"], None, None, a["start"], None,
                                         a["ws"], a["nws"])
     for change in (dict(q=None), dict(o=None), dict(vs=None), dict(B=0), dict(Hk=0), dict(Hq=6), dict(Nq=0), dict(Nkv=-1), dict(scale=0.0), dict(scale=float("inf")),
-                   dict(scale=float("nan")), dict(left=-2), dict(right=-2), dict(sinks=-1)):
+                   dict(scale=float("nan")), dict(left=-2), dict(right=-2), dict(sinks=-1), dict(os=S(0, 0, 64, 1)), dict(os=S(0, 512, 0, 1))):
         assert call(**change) == -1, change
     for change in (dict(D=96), dict(type=2), dict(Nq=1 << 29), dict(Nkv=(1 << 29) + 1), dict(start=(1 << 29) + 1), dict(ks=S(0, 64, 256, 2)),
                    dict(qs=S(0, 60, 256, 1)), dict(k=A + 8), dict(off=(0, 0, 4, 0)), dict(ks=S(0, 64, 1 << 26, 1)), dict(vs=S(0, 64, -64, 1)),
@@ -403,7 +403,8 @@ def test_c_refusals():
     assert L.mi355_sage_sdpa_window_decode(A, A, A, A, 1, 4, 4, 1, 8, 64, 0, 0.1, st, st, st, st, 0, 0, 0, 0, 3, 0, None, None, None, 0) == -1
     bwd = [A] * 10 + [1, 4, 4, 8, 8, 64, 0, 0.1] + [st] * 8 + [0] * 9 + [3, 0, 0, None, 0, None]
     assert L.mi355_sage_sdpa_window_bwd(*bwd, A, 8) == -3
-    for at, value, code in ((0, None, -1), (9, None, -1), (18, None, -1), (15, 256, -2), (11, 5, -1), (16, 2, -2), (22, off_rows(S), -2), (25, S(0, 64, 256, 2), -2)):
+    for at, value, code in ((0, None, -1), (9, None, -1), (18, None, -1), (15, 256, -2), (11, 5, -1), (16, 2, -2), (22, off_rows(S), -2), (25, S(0, 64, 256, 2), -2),
+                            (23, S(0, 0, 64, 1), -1), (24, S(0, 64, 0, 1), -1), (25, S(0, 0, 64, 1), -1)):
         args = list(bwd)
         args[at] = value
         assert L.mi355_sage_sdpa_window_bwd(*args, A, 1 << 30) == code, at
