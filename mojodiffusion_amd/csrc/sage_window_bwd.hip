@@ -63,6 +63,7 @@ __global__ __launch_bounds__(256) void window_bwd_prep_kernel(WindowBwdArgs a) {
 // latencies of a tile (scores, exponentials, products, each waiting for the one before) is other workgroups' waves on the same SIMD: four of them at
 // 64 channels, two at 128, where a wave's operands and sums alone are 128 and more registers.  (64 channels, [2,8192,24 on 8] window 1024 + 4, forward
 // and backward, us: two waves with the next tile's scores taken beside this one's exponentials 732; three 645; four, with the pairs below, 635.)
+// Half of a SIMD's issue slots there are vector instructions, a third matrix instructions; slots that are known at compile time save a tenth of the former.
 
 // ---- dQ: owners of rows, key tiles ------------------------------------------------------------------------------
 // Two slots of K and V.  The owners' rows lie over the second at the start, and on their way out over the front.
@@ -132,15 +133,15 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
         const int t = span.first + (span.n - span.first - n) / 2;
         if (t >= 0 && t < span.n && keys_of(t) > keys_of(centre)) centre = t;
     }
-    for (int t = 0; t < span.n; t++) {
+    auto tile = [&](int t, int slot) {
         dma_wait<0>();
         __syncthreads();                 // tile t is visible; every wave is done with tile t - 1
-        if (t + 1 < span.n) tiles.copy(k, t + 1, L::keys(t + 1)), tiles.copy(v, t + 1, L::values(t + 1));
-        const uint32_t keys = lds + L::keys(t), values = lds + L::values(t);
+        if (t + 1 < span.n) tiles.copy(k, t + 1, L::keys(slot + 1)), tiles.copy(v, t + 1, L::values(slot + 1));
+        const uint32_t keys = lds + L::keys(slot), values = lds + L::values(slot);
         const int j0 = span.tile(t) * 32;
         const Seen what = all.has(t) ? Seen::kAll : x0 < rows ? seen<32>(w, wp_lo, wp_hi, len, j0) : Seen::kNone;
         if (what != Seen::kNone) {
-            const Fragments<D> f = fr.fresh();
+            const Fragments<D> f = D > 64 ? fr.fresh() : fr;
             v16f s, g;
             if (what == Seen::kAll) {
                 s = product<T>(lds_read(keys + f.nat), b1[0], v16f{});
@@ -173,7 +174,7 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
         }
         if (t == centre) {
             const int me = wave * 64 + lane_here(), ch = me % D, first = me / D * (32 / L::GROUPS);
-            const uint8_t* kt = smem + L::keys(t);
+            const uint8_t* kt = smem + L::keys(slot);
             float sum = 0.0f;
 #pragma unroll 1
             for (int r = first; r < first + 32 / L::GROUPS; r++) {
@@ -181,6 +182,14 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
                 sum += copied_key<32>(span, j0, j0 + r) == j0 + r ? key : 0.0f;
             }
             reinterpret_cast<float*>(smem + L::CENTRE)[me] = sum / (float)keys_of(t);
+        }
+    };
+    if constexpr (D > 64) {
+        for (int t = 0; t < span.n; t++) tile(t, t & 1);
+    } else {                             // (slots known ahead: addresses stay in registers, the slots in the reads' offsets)
+        for (int t = 0; t < span.n; t += 2) {
+            tile(t, 0);
+            if (t + 1 < span.n) tile(t + 1, 1);
         }
     }
     __syncthreads();
@@ -364,23 +373,23 @@ struct QueryWalk {
 };
 
 // Scores of a tile of queries with the lane's key, where they start.
-__device__ __forceinline__ void start_scores(v16f& s, const KeyMask& mask, Seen what, int pa, int half) {
-    const KeyMask rel = what == Seen::kNone ? KeyMask{1, 0} : KeyMask{mask.lo - pa - half * 4, mask.hi - pa - half * 4};
+__device__ __forceinline__ void start_scores(v16f& s, const KeyMask& mask, int pa, int half) {
+    const KeyMask rel = {mask.lo - pa - half * 4, mask.hi - pa - half * 4};
 #pragma unroll
     for (int e = 0; e < 16; e++) s[e] = rel.sees((e >> 2) * 8 + (e & 3)) ? 0.0f : -INFINITY;
 }
 
 // A pair of waves shares 32 keys, the P wave with K rows and dV, the S wave, one tile behind, with V rows and dK; P crosses
 // over through LDS with some bits more than dS is rounded to: as fp16 pairs where that is bf16 (see sage_bwd.hip), as the upper three bytes of fp32
-// where it is fp16 (with fp16 there dK's relative error was 3.5e-4, with these 2.9e-4).  In step t the P wave takes the scores of tile t + 1 and the
-// weights of t, the S wave the products with dO of t and dS of t - 1: four slots of Q, two of dO and of the statistics.
+// where it is fp16 (with fp16 there dK's relative error was 3.5e-4, with these 2.9e-4).  Three slots of Q, dO and their statistics: the tile on its way
+// in, the P wave's and the S wave's.
 template <int T, int D> struct PairLds {
     static constexpr int TILE = 32 * D * 2, WORDS = T == kBF16 ? 2 : 3;      // 16-byte words for the 16 values of a lane
     static constexpr int HAND = 2 * WORDS * 64 * 16;                          // [pair][word][lane]
-    static constexpr int NONE = 512, ROWS = 768, RING = ROWS + 2 * HAND, OWN = kWaves * 64 * D;
-    static constexpr int FIRST = RING + (OWN > 5 * TILE ? OWN : 5 * TILE), BYTES = FIRST + TILE;
-    static __device__ int q(int t) { return (t & 3) == 0 ? FIRST : RING + ((t & 3) - 1) * TILE; }
-    static __device__ int d(int t) { return RING + (3 + (t & 1)) * TILE; }
+    static constexpr int ROWS = 768, RING = ROWS + 2 * HAND, BYTES = RING + 6 * TILE;
+    static __device__ int q(int slot) { return RING + (slot == 0 ? 4 : slot * 2 - 2) * TILE; }
+    static __device__ int d(int slot) { return q(slot) + TILE; }
+    static_assert(kWaves * 64 * D == 4 * TILE, "the owners' rows lie over all slots but the first, and over the front on their way out");
 };
 
 // Four floats <-> the upper three bytes of each (15 bits behind the leading one).
@@ -420,46 +429,48 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
     const uint32_t own = L::RING + wave * 64 * D;
     const Span keys_seen = key_span<32>(w, p0, p_last, len);
     key_rows_in<D>(keys_seen, ROLE == 0 ? w.k + b * w.k_sb + kvh * w.k_sh : w.v + b * w.v_sb + kvh * w.v_sh, ROLE == 0 ? w.k_sn : w.v_sn, work.k0, x0, lds + own, lane);
-    if (n_tiles > 0) q.copy(pieces, w.Sq, lds + L::q(0), wave, lane);
-    if (wave == 0) *reinterpret_cast<float*>(smem + L::NONE + lane * 4) = lane < 32 ? INFINITY : 0.0f;        // (statistics where there is no tile: probabilities of zero)
+    auto copy = [&](int slot) {
+        if (wave == 0) st.copy(lds + slot * 256);
+        q.copy(pieces, w.Sq, lds + L::q(slot), wave, lane);
+        d.copy(pieces, w.Sq, lds + L::d(slot), wave, lane);
+    };
+    if (n_tiles > 0) copy(0);
     dma_wait<0>();
 #pragma unroll
     for (int s = 0; s < KS; s++) bx[s] = fr.along(smem + own, s);
 #pragma unroll
     for (int s = 0; s < KS; s++) asm volatile("" : "+v"(bx[s]));
 
-    v16f acc[DB], s[2];
+    v16f acc[DB];
 #pragma unroll
     for (int n = 0; n < DB; n++)
 #pragma unroll
         for (int e = 0; e < 16; e++) acc[n][e] = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 16; e++) s[0][e] = s[1][e] = ROLE == 0 ? -INFINITY : 0.0f;
     const float c = w.scale * kLog2e;
     u32x4* hand = reinterpret_cast<u32x4*>(smem + L::ROWS) + pr * L::WORDS * 64 + lane;
 
-    // `score`: the tile whose scores (P wave: Q K^T, S wave: dO V^T) are taken; `rows`: the one whose rows (dO, Q) the products take; stats: of tile t.
-    auto step = [&](const v16f& s, bool now, uint32_t rows, v16f& sn, Seen next, uint32_t score, int pa, int t) {
-        const Fragments<D> f = fr.fresh();
-        const uint8_t* stats = smem + ((ROLE == 0 ? now : next != Seen::kNone) ? (t & 1) * 256 : L::NONE) + half * 16;
-        if (ROLE == 0 && next == Seen::kAll) {
-            sn = product<T>(lds_read(score + f.nat), bx[0], v16f{});
+    // One tile of this wave's: scores (P wave: Q K^T, S wave: dO V^T - Delta), then the product with the rows (dO, Q) of the same tile.
+    auto step = [&](Seen what, int pa, int slot, int parity) {
+        const Fragments<D> f = D > 64 ? fr.fresh() : fr;
+        const uint32_t score = lds + (ROLE == 0 ? L::q(slot) : L::d(slot)), rows = lds + (ROLE == 0 ? L::d(slot) : L::q(slot));
+        const uint8_t* stats = smem + slot * 256 + ROLE * 128 + half * 16;
+        v16f s;
+        if constexpr (ROLE == 0) {
+            if (what != Seen::kAll) start_scores(s, mask, pa, half);
+            s = what == Seen::kAll ? product<T>(lds_read(score + f.nat), bx[0], v16f{}) : product<T>(lds_read(score + f.nat), bx[0], s);
         } else {
-            if constexpr (ROLE == 0) {
-                start_scores(sn, mask, next, pa, half);
-            } else {
 #pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    const v4f nd = *reinterpret_cast<const v4f*>(stats + 128 + n * 32);
+            for (int n = 0; n < 4; n++) {
+                const v4f nd = *reinterpret_cast<const v4f*>(stats + n * 32);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) sn[n * 4 + e] = nd[e];
-                }
+                for (int e = 0; e < 4; e++) s[n * 4 + e] = nd[e];
             }
-            sn = product<T>(lds_read(score + f.nat), bx[0], sn);
+            s = product<T>(lds_read(score + f.nat), bx[0], s);
         }
 #pragma unroll
-        for (int ks = 1; ks < KS; ks++) sn = product<T>(lds_read(score + (f.nat ^ (ks << 5))), bx[ks], sn);
+        for (int ks = 1; ks < KS; ks++) s = product<T>(lds_read(score + (f.nat ^ (ks << 5))), bx[ks], s);
         uint32_t pk[8], hp[4 * L::WORDS];
+        u32x4* mine = hand + parity * (L::HAND / 16);
         if constexpr (ROLE == 0) {
 #pragma unroll
             for (int n = 0; n < 4; n++) {
@@ -477,11 +488,11 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
                 }
             }
 #pragma unroll
-            for (int n = 0; n < L::WORDS; n++) hand[(t & 1) * (L::HAND / 16) + n * 64] = u32x4{hp[n * 4], hp[n * 4 + 1], hp[n * 4 + 2], hp[n * 4 + 3]};
+            for (int n = 0; n < L::WORDS; n++) mine[n * 64] = u32x4{hp[n * 4], hp[n * 4 + 1], hp[n * 4 + 2], hp[n * 4 + 3]};
         } else {
 #pragma unroll
             for (int n = 0; n < L::WORDS; n++) {
-                const u32x4 v = now ? hand[((t - 1) & 1) * (L::HAND / 16) + n * 64] : u32x4{0u, 0u, 0u, 0u};
+                const u32x4 v = mine[n * 64];
 #pragma unroll
                 for (int e = 0; e < 4; e++) hp[n * 4 + e] = v[e];
             }
@@ -504,33 +515,26 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
             acc[d] = product<T>(lds_read_across(rows + lo, rows + hi), v4i{(int)pk[j2 * 4], (int)pk[j2 * 4 + 1], (int)pk[j2 * 4 + 2], (int)pk[j2 * 4 + 3]}, acc[d]);
         }
     };
-    // What the keys are seen by in tiles t + 1, t, t - 1.
-    Seen ahead = Seen::kNone, here = Seen::kNone, behind = Seen::kNone;
-    auto tile = [&](const v16f& s, v16f& sn, int t) {
+    auto tile = [&](int t, int slot) {   // slot: t % 3
         dma_wait<0>();
-        __syncthreads();                 // Q of tile t + 1, dO and statistics of t and P of t - 1 are visible; every wave is done with Q of t - 2, dO of t - 1
-        if (t + 2 < n_tiles) q.copy(pieces, w.Sq, lds + L::q(t + 2), wave, lane);
-        if (t + 1 < n_tiles) {
-            d.copy(pieces, w.Sq, lds + L::d(t + 1), wave, lane);
-            if (wave == 0) st.copy(lds + ((t + 1) & 1) * 256);
-        }
+        __syncthreads();                 // tile t and P of t - 1 are visible; every wave is done with tile t - 2
+        if (t + 1 < n_tiles) copy(slot == 2 ? 0 : slot + 1);
+        if (ROLE == 0 ? t >= n_tiles : t == 0) return;
         const int pa = walk.p;
-        behind = here, here = ahead;
-        ahead = t + 1 < n_tiles ? seen_by(w, x0, len, pa, min(pa + 31, p_last)) : Seen::kNone;
+        const Seen what = seen_by(w, x0, len, pa, min(pa + 31, p_last));
         walk.next();
-        if constexpr (ROLE == 0) {
-            const bool has = here != Seen::kNone, comes = ahead != Seen::kNone;
-            const uint32_t rows = lds + L::d(t), score = lds + L::q(t + 1);
-            if (has || comes) step(s, has, has ? rows : score, sn, ahead, comes ? score : rows, pa, t);
-        } else {
-            const bool has = behind != Seen::kNone, comes = here != Seen::kNone;
-            const uint32_t rows = lds + L::q(t - 1), score = lds + L::d(t);
-            if (has || comes) step(s, has, has ? rows : score, sn, here, comes ? score : rows, 0, t);
-        }
+        if (what != Seen::kNone) step(what, pa, ROLE == 0 ? slot : slot == 0 ? 2 : slot - 1, (t - ROLE) & 1);
     };
-    for (int t = -1; n_tiles > 0 && t <= n_tiles; t += 2) {
-        tile(s[0], s[1], t);
-        tile(s[1], s[0], t + 1);
+    if (n_tiles > 0) {
+        if constexpr (D > 64) {
+            for (int t = 0, slot = 0; t <= n_tiles; t++, slot = slot == 2 ? 0 : slot + 1) tile(t, slot);
+        } else {                         // (slots known ahead, as above)
+            for (int t = 0; t <= n_tiles; t += 3) {
+                tile(t, 0);
+                if (t + 1 <= n_tiles) tile(t + 1, 1);
+                if (t + 2 <= n_tiles) tile(t + 2, 2);
+            }
+        }
     }
     __syncthreads();                     // (every copy has landed, every tile has been read: the ring takes the output rows)
     uint8_t* os = smem + L::RING + wave * 64 * D;
