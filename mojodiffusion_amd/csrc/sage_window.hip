@@ -470,18 +470,29 @@ template <int T> hipError_t launch_t(const WindowArgs& a, const WindowPlan& p, h
 }  // namespace
 
 // Blocks of 128 rows for half the chip: tiles shared by four waves.  (96 such blocks at 128 channels: 30 us, split 27; 192: 30, split 40.)  One token a
-// sequence gains nothing from the sharing: there as many blocks as compute units are asked for (128 blocks of 8192 keys: 197 us, split 104; 512 of 2048: 97,
-// split 99).  Else the keys are split, until the chip is full once: a workgroup's LDS leaves room for two on a compute unit at 64 channels, one above.
+// sequence gains nothing from the sharing: there it takes as many blocks as compute units (128 blocks of 8192 keys: 197 us, split 104), and at 128
+// channels, from 1024 keys on, the keys are split where that leaves the last round of workgroups full or nearly, since four waves with two tiles each on
+// their way keep more bytes in flight (256 blocks of 8192 keys: 218 us, split 180; of 1024: 31, split 24; 384 of up to 8192: 291, in two parts 278; but 264
+// of 1024: 32, in four parts 40; at 64 channels 512 of 2048 39, split 45, at 256 512 of 1024 96, split 105).
+// Split: until the chip is full once, a workgroup's LDS leaving room for two on a compute unit at 64 channels, for one above.
 // Down to 128 keys (one tile to a wave), counted as a row sees them on the average; and to the root of their number, since the join's time
 // grows with the parts (one head against 65536 keys, us: 512 parts 37, 90 parts 16; 2048 keys: 9).
 WindowPlan window_plan(const WindowArgs& a) {
     constexpr int64_t kUnits = 256;
-    if (row_blocks(a, 128) >= (a.Sq * (int64_t)a.g > 32 ? kUnits / 2 : kUnits)) return WindowPlan{0};
     int64_t keys = a.right >= kWindowFar || a.left >= kWindowFar ? a.Skv
                                                                  : std::min<int64_t>(a.Skv, (int64_t)a.left + a.right + 32 / a.g + 1 + a.sinks);
     if (a.right < kWindowFar) keys -= std::min<int64_t>(a.Sq, keys) / 2;
-    const int64_t room = (a.D > 64 ? kUnits : 2 * kUnits) / row_blocks(a, 32);
-    int64_t splits = std::max<int64_t>(1, std::min(room, keys / 128));
+    const int64_t room = a.D > 64 ? kUnits : 2 * kUnits, blocks = row_blocks(a, 32);
+    int64_t splits = room / blocks;
+    if (a.Sq * (int64_t)a.g > 32) {
+        if (row_blocks(a, 128) >= kUnits / 2) return WindowPlan{0};
+    } else if (blocks >= kUnits) {
+        if (a.D != 128 || keys < 1024) return WindowPlan{0};
+        auto full = [&](int64_t n) { const int64_t last = blocks * n % room; return last == 0 || last >= room * 3 / 4; };
+        for (splits = 1; !full(splits); splits++)
+            if (splits == 3) return WindowPlan{0};
+    }
+    splits = std::max<int64_t>(1, std::min(splits, keys / 128));
     while (splits * splits > std::max<int64_t>(1, keys / 8)) splits--;
     return WindowPlan{(int)splits};
 }

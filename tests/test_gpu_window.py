@@ -99,6 +99,9 @@ DECODE = [
     (2, 1, 1500, 4, 2, 64, BF, -1, 0, [1500, 12]),
     (64, 1, 90, 8, 4, 128, FP, 40, 3, [90 - i for i in range(64)]),
     (128, 3, 70, 2, 2, 256, BF, -1, 0, [i % 71 for i in range(128)]),
+    (32, 1, 1100, 32, 8, 128, BF, -1, 0, [1100 - 37 * i for i in range(32)]),
+    (96, 1, 1500, 8, 4, 128, FP, 1200, 4, [1500 - 15 * i for i in range(96)]),
+    (33, 1, 1030, 8, 8, 128, BF, -1, 0, [1030 - 31 * i for i in range(33)]),
 ]
 
 
