@@ -160,9 +160,7 @@ __global__ __launch_bounds__(256, D == 64 ? 5 : D == 128 ? 3 : 2) void window_ke
 #pragma unroll
     for (int s = 0; s < KS; s++) q[s] = fr.along(smem + wave * 64 * D, s);
 #pragma unroll
-    for (int s = 0; s < KS; s++) {
-        asm volatile("" : "+v"(q[s]));
-    }
+    for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));
     __syncthreads();                     // the rows' LDS becomes the rings' slots
     if (span.n > 0) tiles.copy(v, 0, L::values(0));
 

@@ -63,6 +63,7 @@ __global__ __launch_bounds__(256) void window_bwd_prep_kernel(WindowBwdArgs a) {
 // latencies of a tile (scores, exponentials, products, each waiting for the one before) is other workgroups' waves on the same SIMD: four of them at
 // 64 channels, two at 128, where a wave's operands and sums alone are 128 and more registers.  (64 channels, [2,8192,24 on 8] window 1024 + 4, forward
 // and backward, us: two waves with the next tile's scores taken beside this one's exponentials 732; three 645; four, with the pairs below, 635.)
+// (Pairs for dQ as well, 64 rows to a workgroup, three waves to a SIMD at 128 channels: 114 -> 114 us at [2,1248,30,128] +-256, 452 -> 466 here; not kept.)
 // Half of a SIMD's issue slots there are vector instructions, a third matrix instructions; slots that are known at compile time save a tenth of the former.
 
 // ---- dQ: owners of rows, key tiles ------------------------------------------------------------------------------
