@@ -43,6 +43,9 @@ CASES = [
     (16, 160, 160, 16, 16, 128, BF, 40, 0, 1, None, 0),
     (2, 2100, 2100, 20, 5, 64, FP, 90, 0, 4, [2100, 1500], 0),
     (1, 600, 600, 2, 2, 128, BF, 5, 0, 3, [600], [10]),
+    (1, 50, 50, 71, 1, 64, BF, 9, 2, 1, None, 0),
+    (2, 3, 130, 128, 1, 128, FP, 60, 0, 4, [130, 40], 100),
+    (1, 35, 90, 300, 2, 64, BF, -1, 0, 0, None, 55),
 ]
 # ... and with rows enough for shared tiles
 MANY = [
@@ -99,6 +102,8 @@ DECODE = [
     (2, 1, 1500, 4, 2, 64, BF, -1, 0, [1500, 12]),
     (64, 1, 90, 8, 4, 128, FP, 40, 3, [90 - i for i in range(64)]),
     (128, 3, 70, 2, 2, 256, BF, -1, 0, [i % 71 for i in range(128)]),
+    (3, 1, 700, 96, 1, 128, BF, 300, 2, [700, 299, 1]),
+    (2, 2, 400, 65, 1, 256, FP, -1, 0, [400, 1]),
     (32, 1, 1100, 32, 8, 128, BF, -1, 0, [1100 - 37 * i for i in range(32)]),
     (96, 1, 1500, 8, 4, 128, FP, 1200, 4, [1500 - 15 * i for i in range(96)]),
     (33, 1, 1030, 8, 8, 128, BF, -1, 0, [1030 - 31 * i for i in range(33)]),
