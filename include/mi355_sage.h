@@ -498,7 +498,7 @@ int mi355_sage_qk_norm_rope_bwd(
  * (j >= p - left  or  j < sinks);  left or right -1: no bound on that side.  left = -1, right = 0 is causal attention.  Query i of
  * sequence b stands at q_starts[b] + i, or q_start + i without q_starts.  A query that sees no key gets O = 0 and a
  * statistic of -inf.  Keys at or beyond a sequence's length are never read, nor are keys that no query of a block of rows sees; a key
- * that some query of a call sees must be finite.
+ * that some query of a call sees must be finite.  A query that is not gives a row of NaN, unless it sees no key, and touches no other row.
  * Q, O [B,Hq,N_q,D], K, V [B,Hk,N_kv,D], Hq a multiple of Hk: query heads h Hq/Hk .. share key head h (no expanded copies).  type
  * MI355_SAGE_BF16 or _FP16 for all four; D 64, 128 or 256; scale > 0.  Stats (may be NULL): F32 [B,Hq,N_q] natural log-sum-exp.
  * O_rest (may be NULL): what rounding to the type left of O, with O's type, strides and offset (O + O_rest is O to twice the bits), for the backward.

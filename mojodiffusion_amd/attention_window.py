@@ -123,7 +123,8 @@ def sdpa_window(q, k, v, scale, left, right=0, sinks=0, kv_lens=None, q_start=0)
 
     kv_lens: int32 or int64 [B] on the device, the sequences' lengths (keys from there on are padding: hidden, never read); None: all
     Skv.  q_start: the position of every sequence's first query, an int or int32 / int64 [B] on the device (a
-    chunk of a prompt whose first part is already in the cache).  A query that sees no key gives zeros."""
+    chunk of a prompt whose first part is already in the cache).  A query that sees no key gives zeros; one that sees some and holds a NaN or an
+    infinity gives NaN in its own row."""
     return _forward("sdpa_window", q, k, v, scale, left, right, sinks, kv_lens, q_start, False)[0]
 
 

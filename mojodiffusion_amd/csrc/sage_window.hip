@@ -95,12 +95,20 @@ __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 
         }
 }
 
+// What a row's weighted sum is multiplied by.  A sum of zero is that of a row that sees no key, which gives zeros, or one whose scores are
+// all -inf, which gives what exp(-inf + inf) is; the mask tells them apart.  (A NaN among the scores is in the sum.)
+__device__ __forceinline__ float weight_of(const WindowArgs& a, float sum, int b, int i) {
+    if (sum != 0.0f) return 1.0f / sum;
+    const int len = sequence_len(a, b);
+    return seeing(a, first_position(a, b, len), len).has(i) ? __builtin_nanf("") : 0.0f;
+}
+
 // The wave's finished rows: registers -> LDS (64 * D bytes at os) -> O, and the statistics.
 template <int T, int D>
 __device__ __forceinline__ void finish_rows(const WindowArgs& a, const RowState<D>& st, uint8_t* os, int b, int kvh, int x0, int lane) {
     const int rows = a.Sq * a.g, x = x0 + (lane & 31);
     const float sum = sum_halves(st.sum);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;                     // (a row that sees no key: zeros)
+    const float inv = weight_of(a, sum, b, min(x, rows - 1) / a.g);
 #pragma unroll
     for (int d = 0; d < D / 32; d++) row_put<T, D>(os, st.acc[d], d, inv, lane);
     if (a.stats != nullptr && lane < 32 && x < rows) {
@@ -328,7 +336,7 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
     if (x >= rows) return;
     const int i = x / a.g, hg = x - i * a.g;
     const bool last = a.splits == 1;
-    const float inv = last ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+    const float inv = last ? weight_of(a, sum, b, i) : 1.0f;
     float* po = a.part + ((int64_t)item * a.splits + split) * 32 * D + r * D;
     const int64_t at = b * a.o_sb + ((int64_t)kvh * a.g + hg) * a.o_sh + i * a.o_sn;
 #pragma unroll
@@ -396,8 +404,8 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
         }
 #pragma unroll
         for (int u = 0; u < AT_ONCE; u++) top = fmaxf(top, m[u]);
-        if (top == -INFINITY) return;
-        const float f0 = __builtin_amdgcn_exp2f(ref - top);
+        // (no reference yet: parts that saw nothing, whose sums are zero, and parts whose scores were NaN, whose sums are: they pass as they are)
+        const float f0 = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - top);
         ref = top;
         sum *= f0;
 #pragma unroll
@@ -405,7 +413,7 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
 #pragma unroll
         for (int u = 0; u < AT_ONCE; u++) {
             if (s0 + u >= a.splits) return;
-            const float f = __builtin_amdgcn_exp2f(m[u] - ref);
+            const float f = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[u] - ref);
             sum = fmaf(l[u], f, sum);
 #pragma unroll
             for (int e = 0; e < N; e++) y[e] = fmaf(v[u][e], f, y[e]);
@@ -430,16 +438,14 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
         for (int e = 0; e < N; e++) y[e] = 0.0f;
 #pragma unroll
         for (int n = 0; n < WAVES; n++) {
-            const float m = meet[n][N][lane];
-            if (m == -INFINITY) continue;
-            const float f = __builtin_amdgcn_exp2f(m - top);
+            const float f = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(meet[n][N][lane] - top);
             sum = fmaf(meet[n][N + 1][lane], f, sum);
 #pragma unroll
             for (int e = 0; e < N; e++) y[e] = fmaf(meet[n][e][lane], f, y[e]);
         }
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     const int i = x / a.g, hg = x - i * a.g;
+    const float inv = weight_of(a, sum, b, i);
 #pragma unroll
     for (int e = 0; e < N; e++) y[e] *= inv;
     store_row<T, N>(a, b * a.o_sb + ((int64_t)kvh * a.g + hg) * a.o_sh + i * a.o_sn + lane * N, y);

@@ -46,6 +46,15 @@ __device__ __forceinline__ int first_position(const WindowArgs& a, int b, int le
     return a.starts ? max(-kWindowStart, min(a.starts[b], kWindowStart)) : a.start;
 }
 
+// The queries of a sequence that see a key: lo <= i <= hi.
+struct Seeing {
+    int lo, hi;
+    __device__ bool has(int i) const { return i >= lo && i <= hi; }
+};
+__device__ __forceinline__ Seeing seeing(const WindowArgs& a, int p0, int len) {
+    return Seeing{max(0, -a.right - p0), len == 0 ? -1 : a.sinks > 0 ? a.Sq - 1 : min(a.Sq - 1, len - 1 + a.left - p0)};
+}
+
 // The key tiles (KT keys each) that rows at positions p_lo .. p_hi see: `first` tiles with the sinks, then those from `next` on, n in all.
 // Keys [0, s_end) and [lo, hi] are the ones that some row sees.
 struct Span {
