@@ -73,11 +73,11 @@ struct WindowBwdArgs {
     float *lse2, *ndelta;                        // [B, Hk * g, sq_pad]: Stats * log2(e) (+inf: no such row, or nothing seen), -rowsum(dO * O)
     int sq_pad;                                  // Sq rounded up to a multiple of 64
     // How a key block's (head, query tile) pairs are dealt: `sink_blocks` blocks of kWindowBwdKeys keys with sinks in them go to sink_chunks workgroups
-    // each, the others to chunks, of chunk_tiles pairs.
-    int sink_blocks, sink_chunks, chunks, chunk_tiles;
+    // each, of sink_tiles pairs, the others to chunks, of chunk_tiles pairs.
+    int sink_blocks, sink_chunks, sink_tiles, chunks, chunk_tiles;
     float* part;                                 // [workgroup, 2, kWindowBwdKeys, D] fp32 parts of dK and dV of blocks with several workgroups
 };
-void window_bwd_plan(WindowBwdArgs* a);          // fills in the four above from a->w
+void window_bwd_plan(WindowBwdArgs* a);          // fills in the five above from a->w
 constexpr int kWindowBwdKeys = 64;               // keys of a workgroup
 int64_t window_bwd_parts(const WindowBwdArgs& a);        // workgroups that leave parts
 hipError_t launch_window_bwd(const WindowBwdArgs& a, hipStream_t st);

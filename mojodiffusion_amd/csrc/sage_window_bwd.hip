@@ -8,7 +8,7 @@
 // Launch 1: Delta_i (from O with what rounding left of it, where the caller kept that) and L_i log2(e).  Launch 2: one grid of two kinds of workgroups, as the full backward's (sage_bwd.hip, whose
 // reasons for tiles, rings and the order of the work hold here): owners of rows, that walk the key tiles their window reaches -> dQ; and owners of
 // 64 keys, that walk the (head, query tile) pairs that reach them -> dK, dV.  Blocks with sinks are reached by every later query; their
-// pairs are dealt to as many workgroups as keep the longest of them near the others, which leave fp32 parts for launch 3
+// pairs are dealt to several workgroups (window_bwd_plan), which leave fp32 parts for launch 3
 // to add up in order.  The same where there are too few key blocks to fill the chip.
 #include "sage_grid.h"
 #include "sage_window_common.h"
@@ -250,18 +250,19 @@ template <int D> __device__ __forceinline__ KeyWork key_work(const WindowBwdArgs
     k.part = -1;
     if (r < sink_wgs) {
         block = r / a.sink_chunks, chunk = r % a.sink_chunks;
+        k.count = a.sink_tiles;
         if (a.sink_chunks > 1) k.part = (int64_t)bh * (sink_wgs + (a.chunks > 1 ? (total_blocks - a.sink_blocks) * a.chunks : 0)) + r;
     } else {
         r -= sink_wgs;
         block = a.sink_blocks + r / a.chunks, chunk = r % a.chunks;
+        k.count = a.chunk_tiles;
         if (a.chunks > 1) {
             const int mine = a.sink_chunks > 1 ? sink_wgs : 0;
             k.part = (int64_t)bh * (mine + (total_blocks - a.sink_blocks) * a.chunks) + mine + r;
         }
     }
     k.k0 = block * kKeysWg;
-    k.first = chunk * a.chunk_tiles;
-    k.count = a.chunk_tiles;
+    k.first = chunk * k.count;
     return k;
 }
 
@@ -562,7 +563,8 @@ __global__ __launch_bounds__(kWaves * 64, D > 64 ? 2 : 4) void window_bwd_kernel
     else dkdv_role<T, D, 1>(a, smem, item / tk, work, wave, lane);
 }
 
-// Launch 3: dK and dV of the blocks that several workgroups share, their parts added in order.  8 channels to a thread.
+// Launch 3: dK and dV of the blocks that several workgroups share, their parts added in order.  8 channels to a thread, which
+// requests eight parts at a time (one after the other, each is a trip to memory).
 template <int T, int D>
 __global__ __launch_bounds__(256) void window_bwd_join_kernel(WindowBwdArgs a) {
     constexpr int CPR = D / 8;
@@ -580,10 +582,20 @@ __global__ __launch_bounds__(256) void window_bwd_join_kernel(WindowBwdArgs a) {
     const int64_t part = bh * wgs + (sink ? (int64_t)n * a.sink_chunks : sink_wgs + (int64_t)(n - sink_parts) * a.chunks);
     const float* p = a.part + ((part * 2 + which) * kKeysWg + key) * D + col;
     float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int c = 0; c < chunks; c++) {
-        const v4f u = *reinterpret_cast<const v4f*>(p + (int64_t)c * 2 * kKeysWg * D), v = *reinterpret_cast<const v4f*>(p + (int64_t)c * 2 * kKeysWg * D + 4);
+    for (int c0 = 0; c0 < chunks; c0 += 8) {
+        v4f u[8], v[8];
 #pragma unroll
-        for (int e = 0; e < 4; e++) y[e] += u[e], y[4 + e] += v[e];
+        for (int n = 0; n < 8; n++) {
+            const float* at_c = p + (int64_t)min(c0 + n, chunks - 1) * 2 * kKeysWg * D;
+            u[n] = *reinterpret_cast<const v4f*>(at_c);
+            v[n] = *reinterpret_cast<const v4f*>(at_c + 4);
+        }
+#pragma unroll
+        for (int n = 0; n < 8; n++) {
+            if (c0 + n >= chunks) break;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] += u[n][e], y[4 + e] += v[n][e];
+        }
     }
     const int j = block * kKeysWg + key, b = bh / a.w.Hk, kvh = bh % a.w.Hk;
     if (j >= a.w.Skv) return;
@@ -594,7 +606,7 @@ __global__ __launch_bounds__(256) void window_bwd_join_kernel(WindowBwdArgs a) {
 template <int T, int D> hipError_t launch_td(const WindowBwdArgs& a, hipStream_t st) {
     const int64_t heads = (int64_t)a.w.B * a.w.Hk, rows = (int64_t)a.w.Sq * a.w.g, blocks = (a.w.Skv + kKeysWg - 1) / kKeysWg;
     const int64_t prep = (heads * a.w.g * a.sq_pad * (D / 8) + 255) / 256;
-    const int64_t grid = heads * ((rows + kRowsWg - 1) / kRowsWg + a.sink_blocks * a.sink_chunks + (blocks - a.sink_blocks) * a.chunks);
+    const int64_t grid = heads * ((rows + kRowsWg - 1) / kRowsWg + (int64_t)a.sink_blocks * a.sink_chunks + (blocks - a.sink_blocks) * a.chunks);
     const int64_t shared = (a.sink_chunks > 1 ? a.sink_blocks : 0) + (a.chunks > 1 ? blocks - a.sink_blocks : 0);
     const int64_t join = (heads * shared * 2 * kKeysWg * (D / 8) + 255) / 256;
     if (prep > 0x7FFFFFFF || grid > 0x7FFFFFFF || join > 0x7FFFFFFF) return hipErrorInvalidValue;
@@ -607,22 +619,32 @@ template <int T, int D> hipError_t launch_td(const WindowBwdArgs& a, hipStream_t
 }  // namespace
 
 // A key block's pairs without sinks: as many as its window spans.  They are dealt to several workgroups where whole blocks would leave the chip
-// partly empty (four to a compute unit are wanted), down to 16 pairs; a block with sinks to as many as give each about that share too.
+// partly empty (four to a compute unit are wanted), down to 16 pairs.  A block with sinks is reached by every later query: its pairs go to as many workgroups as
+// give each a window block's share, but to no more than two to a compute unit over all heads and blocks (the parts, 64 KiB each at 128 channels, stay within 32 MiB),
+// and no more than twice the root of the pairs, since the join's time grows with the parts as the walks shrink.  (Gradients, us, with a window block's share whatever
+// the length, one to a unit, two: [1,16896,8,128] window 16 + 4 187, 140, 140; [1,16896,30,128] 16 + 77 762, 617, 557; [1,65536,4 on 2,128] 63 + 4
+// 381, 291, 287; [1,16896,2,128] 256 + 256 87, 100, 89.)
 void window_bwd_plan(WindowBwdArgs* a) {
+    constexpr int64_t kUnits = 256;
     const WindowArgs& w = a->w;
     const int64_t keys = kWindowBwdKeys;
     const int64_t all = (w.Sq + 31) / 32, blocks = (w.Skv + keys - 1) / keys, heads = (int64_t)w.B * w.Hk;
     const int64_t tiles = std::min<int64_t>(all, ((int64_t)w.left + w.right + keys + 30) / 32 + 1), pairs = tiles * w.g;
-    const int64_t want = std::max<int64_t>(1, 1024 / (blocks * heads)), most = std::max<int64_t>(1, pairs / 16);
+    const int64_t want = std::max<int64_t>(1, 4 * kUnits / (blocks * heads)), most = std::max<int64_t>(1, pairs / 16);
     const int64_t chunks = std::min(want, most), per = (pairs + chunks - 1) / chunks;
     a->chunks = (int)((pairs + per - 1) / per);
     a->chunk_tiles = (int)per;
     a->sink_blocks = tiles < all ? (int)((w.sinks + keys - 1) / keys) : 0;
-    a->sink_chunks = (int)((all * w.g + per - 1) / per);
+    const int64_t sink_pairs = all * w.g, room = std::max<int64_t>(1, 2 * kUnits / std::max<int64_t>(1, a->sink_blocks * heads));
+    int64_t n = std::min((sink_pairs + per - 1) / per, room);
+    while (n * n > 4 * sink_pairs) n--;
+    const int64_t sink_per = (sink_pairs + n - 1) / n;
+    a->sink_tiles = (int)sink_per;
+    a->sink_chunks = (int)((sink_pairs + sink_per - 1) / sink_per);
 }
 int64_t window_bwd_parts(const WindowBwdArgs& a) {
     const int64_t keys = kWindowBwdKeys, blocks = (a.w.Skv + keys - 1) / keys;
-    return (int64_t)a.w.B * a.w.Hk * ((a.sink_chunks > 1 ? a.sink_blocks * a.sink_chunks : 0) + (a.chunks > 1 ? (blocks - a.sink_blocks) * a.chunks : 0));
+    return (int64_t)a.w.B * a.w.Hk * ((a.sink_chunks > 1 ? (int64_t)a.sink_blocks * a.sink_chunks : 0) + (a.chunks > 1 ? (blocks - a.sink_blocks) * a.chunks : 0));
 }
 
 hipError_t launch_window_bwd(const WindowBwdArgs& a, hipStream_t st) {

@@ -53,3 +53,46 @@ def test_a_query_that_is_not_finite(B, Sq, Skv, Hq, Hk, D, dtype, left, sinks):
                 x[at] = y[at]
                 assert torch.equal(x, y), bad
             assert torch.isfinite(want[0]).all()
+
+
+def test_workspace_of_the_gradients():
+    """Two fp32 statistics a query row (three at the most), and parts: those of the blocks with sinks no more than two for each of 256 compute units, those of the others
+    no more than four.  (Sizes only: nothing runs.)"""
+    from mojodiffusion_amd import _lib
+    size = _lib.lib().mi355_sage_window_bwd_workspace_bytes
+    for B, Hq, Hk, S, D, left, sinks in ((1, 8, 8, 16896, 128, 16, 4), (1, 30, 30, 16896, 128, 16, 77), (1, 40, 40, 16896, 128, 16, 1024), (1, 32, 32, 16384, 128, 128, 16384),
+                                         (1, 8, 8, 131072, 128, 63, 4), (1, 8, 8, 131072, 128, 63, 77), (1, 8, 8, 16896, 128, 63, 16896), (2, 24, 8, 8192, 64, 1023, 4),
+                                         (1, 1, 1, 1 << 22, 64, 0, 1 << 22), (1, 2, 1, 1 << 27, 64, 0, 1 << 27), (1, 64, 1, 1 << 20, 64, 1, 1 << 27), (1, 1, 1, 300, 64, 2, 300),
+                                         (4, 4, 2, 1000, 128, 999, 3), (1, 1, 1, 131072, 64, 16, 1), (64, 32, 8, 4096, 128, 64, 64)):
+        stats = 3 * 4 * B * Hq * (S + 63)
+        got = size(B, Hq, Hk, S, S, D, left, 0, sinks)
+        assert 0 < got <= stats + 4 * 256 + (512 + 1024) * 2 * 64 * D * 4, (S, left, sinks, got)
+        plain = size(B, Hq, Hk, S, S, D, left, 0, 0)
+        assert got <= plain + 256 + 512 * 2 * 64 * D * 4, (S, left, sinks, got)
+
+
+# Many sinks on short windows: whole blocks of them, ends inside a block, all keys, and one block whose pairs many workgroups share.
+SINKS = [
+    # B, S, Hq, Hk, D, type, left, sinks, lens
+    (1, 1500, 2, 2, 64, BF, 16, 1024, None),
+    (1, 1500, 3, 1, 128, FP, 16, 1500, [1490]),
+    (2, 900, 2, 1, 64, FP, 0, 130, [900, 100]),
+    (1, 5000, 2, 2, 64, BF, 16, 4, None),
+    (1, 3500, 1, 1, 128, BF, 8, 70, [3400]),
+    (1, 700, 40, 20, 64, BF, 30, 700, None),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S,Hq,Hk,D,dtype,left,sinks,lens", SINKS)
+def test_gradients_with_many_sinks(B, S, Hq, Hk, D, dtype, left, sinks, lens):
+    q, k, v = tensors(B, S, S, Hq, Hk, D, dtype, S)
+    d = torch.randn(q.shape, generator=torch.Generator().manual_seed(4)).to(dtype)
+    n = [S] * B if lens is None else lens
+    want = backward(q, k, v, d, D ** -0.5, forward(q, k, v, D ** -0.5, left, 0, sinks, n, [0] * B), Hq // Hk)
+    lens = None if lens is None else torch.tensor(lens, dtype=torch.int32).cuda()
+    args = (q.cuda(), k.cuda(), v.cuda(), d.cuda(), D ** -0.5, left, 0, sinks)
+    got = grads(*args, lens=lens)[1]
+    check_backward(got, want)
+    for x, y in zip(got, grads(*args, lens=lens)[1]):
+        assert torch.equal(x, y)
