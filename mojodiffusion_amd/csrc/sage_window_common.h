@@ -74,8 +74,8 @@ template <int KT> __device__ __forceinline__ Span key_span(const WindowArgs& a, 
 // The key whose row is copied for row j of the tile that starts at j0: j itself where some row of the workgroup sees it, else a neighbour that one sees.
 template <int KT> __device__ __forceinline__ int copied_key(const Span& s, int j0, int j) {
     const int gap = s.lo <= min(j0 + KT - 1, s.hi) ? s.lo : s.s_end - 1;
-    if (j >= s.s_end && j < s.lo) j = gap;
-    return min(j, s.hi);
+    j = min(j, s.hi);                    // (first: a window that begins behind the last key leaves that key in the gap)
+    return j >= s.s_end && j < s.lo ? gap : j;
 }
 
 // The keys a row sees: lo .. hi, and those below `sinks` up to hi.  (Relative to a key, so that a tile's comparisons are with constants.)

@@ -96,3 +96,18 @@ def test_gradients_with_many_sinks(B, S, Hq, Hk, D, dtype, left, sinks, lens):
     check_backward(got, want)
     for x, y in zip(got, grads(*args, lens=lens)[1]):
         assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H", [(1, 2), (64, 8)])
+def test_a_key_between_the_sinks_and_a_window_behind_the_last(B, H):
+    """Queries so far behind a sequence's end that their window holds no key: they see the sinks alone, and the last key may hold anything."""
+    q, k, v = (t.cuda() for t in tensors(B, 3, 64, H, H, 64, BF, 1))
+    lens = torch.full((B,), 20, dtype=torch.int32).cuda()
+    call = lambda k, v: W.sdpa_window(q, k, v, 0.125, 8, 0, 4, kv_lens=lens, q_start=30)
+    want = call(k, v)
+    for bad in (NAN, INF, -3e38):
+        k2, v2 = k.clone(), v.clone()
+        k2[:, 4:], v2[:, 4:] = bad, bad
+        assert torch.equal(call(k2, v2), want), bad
+    assert torch.isfinite(want).all()
