@@ -527,7 +527,9 @@ int mi355_sage_sdpa_window_decode(
 /* Gradient of mi355_sage_sdpa_window: O, O_rest and Stats as the forward wrote them (O_rest may be NULL: rows that see few keys, whose O is large, then
  * carry its rounding into dK: relative error 0.0032 for 0.0026 at a padded batch with sinks), dO upstream -> dQ [B,Hq,N_q,D], dK, dV [B,Hk,N_kv,D] (of a
  * shared key head: summed over its query heads), every row written, those of keys that no query sees and of queries that see none
- * as zeros.  D 64 or 128.  The same bits on every call (no atomics).  No output may overlap another tensor of the call. */
+ * as zeros.  Rows of Q, O, O_rest and dO of queries that see no key may hold anything; those of queries that see one must be finite (one that is
+ * not reaches the gradients of keys next to those it sees, too).  D 64 or 128.  The same bits on every call (no atomics).  No output may overlap another
+ * tensor of the call. */
 size_t mi355_sage_window_bwd_workspace_bytes(int B, int Hq, int Hk, int N_q, int N_kv, int D, int left, int right, int sinks);
 int mi355_sage_sdpa_window_bwd(
     const void* Q, const void* K, const void* V, const void* O, const void* O_rest, const void* dO, const void* Stats, void* dQ, void* dK, void* dV,

@@ -169,7 +169,8 @@ def sdpa_window_train_fwd(q, k, v, scale, left, right=0, sinks=0, kv_lens=None, 
 
 def sdpa_window_backward(fwd, d_out):
     """d_q [B,Sq,Hq,Dh], d_k, d_v [B,Skv,Hk,Dh] from a sdpa_window_train_fwd and the upstream gradient (Dh 64 or 128; the gradients of a
-    shared key head are summed over its query heads; rows of padding and of keys that nothing sees are zeros)."""
+    shared key head are summed over its query heads; rows of padding, of keys that nothing sees and of queries that see nothing are zeros, whatever
+    those rows of q, d_out, k and v hold)."""
     name = "sdpa_window_backward"
     r = _lib.host().window_bwd(fwd.q, fwd.k, fwd.v, fwd.o, fwd.o_rest, d_out, fwd.stats, fwd.scale, fwd.left, fwd.right, fwd.sinks, fwd.kv_lens, fwd.q_start)
     if r is not None:

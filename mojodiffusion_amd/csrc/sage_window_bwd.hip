@@ -37,7 +37,8 @@ __global__ __launch_bounds__(256) void window_bwd_prep_kernel(WindowBwdArgs a) {
     const int64_t row = (int64_t)blockIdx.x * RPP + threadIdx.x / CPR;                // over [B, H, sq_pad]
     if (row >= (int64_t)a.w.B * H * a.sq_pad) return;
     const int i = (int)(row % a.sq_pad), bh = (int)(row / a.sq_pad), b = bh / H, h = bh % H, col = (int)(threadIdx.x % CPR) * 8;
-    const bool real = i < a.w.Sq;
+    const int len = sequence_len(a.w, b);
+    const bool real = seeing(a.w, first_position(a.w, b, len), len).has(i);           // (rows that see nothing are not read: they may hold anything)
     float sum = 0.0f;
     if (real) {
         const int64_t at = b * a.w.o_sb + h * a.w.o_sh + i * a.w.o_sn + col;
@@ -210,6 +211,14 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
                 for (int e = 0; e < 4; e++) acc[d][q * 4 + e] = fmaf(-rs, c4[e], acc[d][q * 4 + e]);
             }
     }
+    // Rows that see nothing: zeros, also where they or their upstream gradients are no numbers.
+    const bool blind = !mask.sees_any();
+    if (__any(blind)) {
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[d][e] = blind ? 0.0f : acc[d][e];
+    }
 #pragma unroll
     for (int d = 0; d < DB; d++) row_put<T, D>(os, acc[d], d, w.scale, end_lane);
     if (x0 < rows) query_rows_out<D>(w, os, a.dq + b * a.dq_sb + (int64_t)kvh * w.g * a.dq_sh, a.dq_sn, a.dq_sh, x0, end_lane);
@@ -312,10 +321,14 @@ template <int D> struct QueryRows {
     int64_t tile, turn;                  // from a tile to the next, from a head's last to the next head's first
     uint32_t sn, off[Pieces::N];
     int qt, nt, t0;
-    __device__ QueryRows(const Pieces& p, const uint16_t* head, int64_t sh, int64_t sn_, const QuerySpan& q, int first, int lane) {
+    Seeing rows;                         // (others are not read: one of these stands in, with a statistic that makes its weights vanish)
+    Range whole;                         // the tiles, from t0 on, that hold only such
+    __device__ QueryRows(const Pieces& p, const uint16_t* head, int64_t sh, int64_t sn_, const QuerySpan& q, const Seeing& rows_, int first, int lane) {
         const int hg = q.nt > 0 ? first / q.nt : 0;
         nt = q.nt;
         t0 = q.t0;
+        rows = rows_;
+        whole = Range{(rows.lo + 31) / 32 - t0, (unsigned)max((rows.hi + 1) / 32 - (rows.lo + 31) / 32, 0)};
         qt = first - hg * nt;
         at = head + hg * sh + (int64_t)(t0 + qt) * 32 * sn_;
         tile = 32 * sn_;
@@ -324,12 +337,14 @@ template <int D> struct QueryRows {
 #pragma unroll
         for (int n = 0; n < Pieces::N; n++) off[n] = p.row(n) * sn + p.col(n, lane);
     }
-    __device__ void copy(const Pieces& p, int Sq, uint32_t to, int wave, int lane) {
-        const int left = Sq - (t0 + qt) * 32;            // (rows behind the last query repeat it)
+    __device__ void copy(const Pieces& p, uint32_t to, int wave, int lane) {
 #pragma unroll
         for (int n = 0; n < Pieces::N; n++) {
             uint32_t o = off[n];
-            if (left < 32) o = (uint32_t)min(p.row(n), left - 1) * sn + p.col(n, lane);
+            if (!whole.has(qt)) {        // (every tile that is copied holds one of them)
+                const int i0 = (t0 + qt) * 32;
+                o = (uint32_t)min(max(p.row(n), rows.lo - i0), rows.hi - i0) * sn + p.col(n, lane);
+            }
             dma16(at, o, __builtin_amdgcn_readfirstlane(to + (n * kWaves + wave) * 1024));
         }
         const bool last = qt == nt - 1;
@@ -418,11 +433,12 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
     const int len = sequence_len(w, b), p0 = first_position(w, b, len), p_last = p0 + w.Sq - 1;
     const QuerySpan qs = query_span(w, work.k0, kKeysWg, p0, len);
     const int n_tiles = max(0, min(qs.nt * w.g - work.first, work.count));
+    const Seeing real = seeing(w, p0, len);
     const KeyMask mask = key_mask(w, j, len, p0);
     const uint32_t lds = lds_addr(smem);
     const typename QueryRows<D>::Pieces pieces(wave, lane);
-    QueryRows<D> q(pieces, w.q + b * w.q_sb + (int64_t)kvh * w.g * w.q_sh, w.q_sh, w.q_sn, qs, work.first, lane);
-    QueryRows<D> d(pieces, a.dout + b * a.do_sb + (int64_t)kvh * w.g * a.do_sh, a.do_sh, a.do_sn, qs, work.first, lane);
+    QueryRows<D> q(pieces, w.q + b * w.q_sb + (int64_t)kvh * w.g * w.q_sh, w.q_sh, w.q_sn, qs, real, work.first, lane);
+    QueryRows<D> d(pieces, a.dout + b * a.do_sb + (int64_t)kvh * w.g * a.do_sh, a.do_sh, a.do_sn, qs, real, work.first, lane);
     QueryStats st(a, (int64_t)b * w.Hk * w.g + kvh * w.g, qs, work.first, lane);
     QueryWalk walk(qs, work.first, p0);
 
@@ -433,8 +449,8 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
     key_rows_in<D>(keys_seen, ROLE == 0 ? w.k + b * w.k_sb + kvh * w.k_sh : w.v + b * w.v_sb + kvh * w.v_sh, ROLE == 0 ? w.k_sn : w.v_sn, work.k0, x0, lds + own, lane);
     auto copy = [&](int slot) {
         if (wave == 0) st.copy(lds + slot * 256);
-        q.copy(pieces, w.Sq, lds + L::q(slot), wave, lane);
-        d.copy(pieces, w.Sq, lds + L::d(slot), wave, lane);
+        q.copy(pieces, lds + L::q(slot), wave, lane);
+        d.copy(pieces, lds + L::d(slot), wave, lane);
     };
     if (n_tiles > 0) copy(0);
     dma_wait<0>();

@@ -83,6 +83,7 @@ struct RowMask {
     int lo, hi, sinks;
     __device__ RowMask from(int j) const { return RowMask{lo - j, hi - j, sinks - j}; }
     __device__ bool sees(int j) const { return j <= hi && (j >= lo || j < sinks); }
+    __device__ bool sees_any() const { return hi >= 0 && (hi >= lo || sinks > 0); }
 };
 
 // The lane's number, formed where it is used: not kept in a register through a loop for what follows it.

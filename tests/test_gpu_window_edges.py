@@ -111,3 +111,35 @@ def test_a_key_between_the_sinks_and_a_window_behind_the_last(B, H):
         k2[:, 4:], v2[:, 4:] = bad, bad
         assert torch.equal(call(k2, v2), want), bad
     assert torch.isfinite(want).all()
+
+
+# Queries before the first key (right edge), behind the last (left edge, no sinks), both; of one sequence and of some.
+BLIND = [
+    # B, Sq, Skv, Hq, Hk, D, type, left, right, lens, first
+    (1, 70, 64, 2, 1, 64, BF, 8, 0, [20], 0),
+    (2, 200, 200, 3, 3, 128, FP, 30, 2, [200, 77], -11),
+    (1, 300, 130, 4, 2, 64, FP, 9, 0, [130], -40),
+    (2, 45, 45, 2, 2, 128, BF, 3, 1, [0, 5], 0),
+    (1, 500, 100, 5, 1, 128, BF, 50, 60, [90], -150),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Sq,Skv,Hq,Hk,D,dtype,left,right,lens,first", BLIND)
+def test_gradients_past_queries_that_see_nothing(B, Sq, Skv, Hq, Hk, D, dtype, left, right, lens, first):
+    """Whatever such rows and their upstream gradients hold: zeros for their dQ, the same bits for the rest."""
+    q, k, v = (t.cuda() for t in tensors(B, Sq, Skv, Hq, Hk, D, dtype, 3))
+    d = torch.randn(q.shape, generator=torch.Generator().manual_seed(4)).to(dtype).cuda()
+    n = torch.tensor(lens, dtype=torch.int32).cuda()
+    p = first + torch.arange(Sq)
+    blind = torch.stack([(p + right < 0) | (p - left > x - 1) | (x == 0) for x in lens])
+    assert blind.any() and not blind.all()
+    run = lambda q, d: grads(q, k, v, d, D ** -0.5, left, right, 0, lens=n, first=first)[1]
+    want = run(q, d)
+    for bad in (NAN, INF, -6e4):
+        q2, d2 = q.clone(), d.clone()
+        q2[blind.cuda()], d2[blind.cuda()] = bad, bad
+        got = run(q2, d2)
+        for name, x, y in zip(("dQ", "dK", "dV"), got, want):
+            assert torch.equal(x, y), (name, bad)
+    assert (want[0].cpu()[blind] == 0).all() and all(torch.isfinite(x).all() for x in want)
