@@ -25,6 +25,11 @@ typedef __fp16 v2fp __attribute__((ext_vector_type(2)));
 constexpr int kWaves = 4, kRowsWg = kWaves * 32;
 constexpr int kKeysWg = kWindowBwdKeys;                          // (pairs of waves share 32 keys)
 
+// bf16: weights are carried times 2^14 (by their statistic, at no cost), so that those down to 2^-28 keep all bits of the fp16 in which they are handed on
+// (PairLds), whose normal range ends at 2^-14; what is made of them is multiplied by kWeightInv at the end.
+template <int T> constexpr float kWeightBits = T == kBF16 ? 14.0f : 0.0f;
+template <int T> constexpr float kWeightInv = T == kBF16 ? 0x1p-14f : 1.0f;
+
 template <int T> __device__ __forceinline__ float widen(uint32_t w, int i) {
     if constexpr (T == kBF16) return __uint_as_float(i ? w & 0xFFFF0000u : w << 16);
     else return (float)__builtin_bit_cast(v2hf, w)[i];
@@ -56,7 +61,7 @@ __global__ __launch_bounds__(256) void window_bwd_prep_kernel(WindowBwdArgs a) {
     if (col == 0) {
         const float l = real ? a.w.stats[(int64_t)bh * a.w.Sq + i] : -INFINITY;
         a.ndelta[row] = real ? -sum : 0.0f;
-        a.lse2[row] = l == -INFINITY ? INFINITY : l * kLog2e;           // (nothing seen: every probability vanishes)
+        a.lse2[row] = l == -INFINITY ? INFINITY : fmaf(l, kLog2e, -kWeightBits<T>);           // (nothing seen: every probability vanishes)
     }
 }
 
@@ -220,7 +225,7 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
             for (int e = 0; e < 16; e++) acc[d][e] = blind ? 0.0f : acc[d][e];
     }
 #pragma unroll
-    for (int d = 0; d < DB; d++) row_put<T, D>(os, acc[d], d, w.scale, end_lane);
+    for (int d = 0; d < DB; d++) row_put<T, D>(os, acc[d], d, w.scale * kWeightInv<T>, end_lane);
     if (x0 < rows) query_rows_out<D>(w, os, a.dq + b * a.dq_sb + (int64_t)kvh * w.g * a.dq_sh, a.dq_sn, a.dq_sh, x0, end_lane);
 }
 
@@ -397,7 +402,8 @@ __device__ __forceinline__ void start_scores(v16f& s, const KeyMask& mask, int p
 }
 
 // A pair of waves shares 32 keys, the P wave with K rows and dV, the S wave, one tile behind, with V rows and dK; P crosses
-// over through LDS with some bits more than dS is rounded to: as fp16 pairs where that is bf16 (see sage_bwd.hip), as the upper three bytes of fp32
+// over through LDS with some bits more than dS is rounded to: as fp16 pairs, times 2^14, where that is bf16 (11 bits for weights down to 2^-28, fewer
+// below, none below 2^-39), as the upper three bytes of fp32
 // where it is fp16 (with fp16 there dK's relative error was 3.5e-4, with these 2.9e-4).  Three slots of Q, dO and their statistics: the tile on its way
 // in, the P wave's and the S wave's.
 template <int T, int D> struct PairLds {
@@ -499,8 +505,8 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
                 pk[n * 2] = pack2<T>(y[0], y[1]);
                 pk[n * 2 + 1] = pack2<T>(y[2], y[3]);
                 if constexpr (T == kBF16) {
-                    hp[n * 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[0], y[1]));
-                    hp[n * 2 + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[2], y[3]));
+                    hp[n * 2] = pack2<kF16>(y[0], y[1]);
+                    hp[n * 2 + 1] = pack2<kF16>(y[2], y[3]);
                 } else {
                     pack24(y, &hp[n * 3]);
                 }
@@ -556,8 +562,8 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
     }
     __syncthreads();                     // (every copy has landed, every tile has been read: the ring takes the output rows)
     uint8_t* os = smem + L::RING + wave * 64 * D;
-    if constexpr (ROLE == 0) key_rows_out<T, D>(a, acc, 1.0f, os, work.part, 1, a.dv + b * a.dv_sb + kvh * a.dv_sh, a.dv_sn, x0, work.k0, lane);
-    else key_rows_out<T, D>(a, acc, w.scale, os, work.part, 0, a.dk + b * a.dk_sb + kvh * a.dk_sh, a.dk_sn, x0, work.k0, lane);
+    if constexpr (ROLE == 0) key_rows_out<T, D>(a, acc, kWeightInv<T>, os, work.part, 1, a.dv + b * a.dv_sb + kvh * a.dv_sh, a.dv_sn, x0, work.k0, lane);
+    else key_rows_out<T, D>(a, acc, w.scale * kWeightInv<T>, os, work.part, 0, a.dk + b * a.dk_sb + kvh * a.dk_sh, a.dk_sn, x0, work.k0, lane);
 }
 
 template <int T, int D>

@@ -143,3 +143,29 @@ def test_gradients_past_queries_that_see_nothing(B, Sq, Skv, Hq, Hk, D, dtype, l
         for name, x, y in zip(("dQ", "dK", "dV"), got, want):
             assert torch.equal(x, y), (name, bad)
     assert (want[0].cpu()[blind] == 0).all() and all(torch.isfinite(x).all() for x in want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,Hq,Hk", [(64, 2, 2), (128, 4, 2)])
+def test_gradients_of_keys_with_small_weights(D, Hq, Hk):
+    """Half of the keys lie 12 lower than the others: weights about 2^-25.  The bounds are relative to every weight."""
+    S = 300
+    q, k, v = tensors(1, S, S, Hq, Hk, D, BF, 11)
+    q, k = q * 0.25, k * 0.25
+    q[..., 0], k[..., 0] = 4.0, 0.0
+    k[:, S // 3:, :, 0] = -3.0
+    q, k = q.to(BF), k.to(BF)
+    d = torch.randn(q.shape, generator=torch.Generator().manual_seed(4)).to(BF)
+    ref = forward(q, k, v, 1.0, -1, -1, 0, [S], [0])
+    assert 2.0 ** -30 < float(ref[2].min()) < 2.0 ** -23
+    want = list(backward(q, k, v, d, 1.0, ref, Hq // Hk))
+    # (the bounds grant a weight that is handed on 2^-10 of it: half a step of fp16 and as much again.  Carried times 2^14, a weight below 2^-28 is below fp16's
+    # normal range there: half a step is 2^-25 / 2^14 whatever the weight.  That much of |dP - Delta| |q| comes on top of dK's bound.)
+    extra = torch.zeros_like(want[1][1])
+    for h in range(Hq):
+        dp = d[0, :, h].double() @ v[0, :, h // (Hq // Hk)].double().T
+        away = (dp - (ref[2][0, h] * dp).sum(1, keepdim=True)).abs() * (ref[2][0, h] < 2.0 ** -28)
+        extra[0, :, h // (Hq // Hk)] += 2.0 ** -39 * away.T @ q[0, :, h].double().abs()
+    want[1] = (want[1][0], want[1][1] + extra)
+    assert float(extra.max()) < 0.02 * float(want[1][0][:, S // 3:].abs().max())
+    check_backward(grads(q.cuda(), k.cuda(), v.cuda(), d.cuda(), 1.0, -1, -1, 0)[1], want)
