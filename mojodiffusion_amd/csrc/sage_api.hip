@@ -1337,14 +1337,15 @@ int mi355_sage_sdpa_window_decode(const void* Q, const void* K, const void* V, v
                           a, stream, workspace, workspace_bytes);
 }
 
-struct WindowBwdCarve { size_t lse2, delta, part, total; };
+struct WindowBwdCarve { size_t lse2, delta, size, part, total; };
 static WindowBwdCarve window_bwd_carve(WindowBwdArgs* a) {
     window_bwd_plan(a);
     a->sq_pad = (int)pad_to(a->w.Sq, 64);
     const size_t rows = (size_t)a->w.B * a->w.Hk * a->w.g * a->sq_pad * sizeof(float);
     WindowBwdCarve c{};
     c.delta = align_up(rows);
-    c.part = c.delta + align_up(rows);
+    c.size = c.delta + align_up(rows);
+    c.part = c.size + align_up(rows);                    // (the query of the bytes knows no type: fp16's third statistic has its place in every call's)
     c.total = c.part + align_up((size_t)window_bwd_parts(*a) * 2 * kWindowBwdKeys * a->w.D * sizeof(float));
     return c;
 }
@@ -1384,6 +1385,7 @@ int mi355_sage_sdpa_window_bwd(const void* Q, const void* K, const void* V, cons
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     a.lse2 = reinterpret_cast<float*>(ws);
     a.ndelta = reinterpret_cast<float*>(ws + c.delta);
+    a.dsize = reinterpret_cast<float*>(ws + c.size);
     a.part = reinterpret_cast<float*>(ws + c.part);
     const View q = make_view(Q, q_strides, q_off), k = make_view(K, k_strides, k_off), v = make_view(V, v_strides, v_off), d = make_view(dO, do_strides, do_off);
     a.w.q = q.p; a.w.q_sb = q.sb; a.w.q_sh = q.sh; a.w.q_sn = q.sn;

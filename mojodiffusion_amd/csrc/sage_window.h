@@ -71,6 +71,7 @@ struct WindowBwdArgs {
     int64_t do_sb, do_sh, do_sn, dq_sb, dq_sh, dq_sn, dk_sb, dk_sh, dk_sn, dv_sb, dv_sh, dv_sn;
     // workspace
     float *lse2, *ndelta;                        // [B, Hk * g, sq_pad]: Stats * log2(e) less kWeightBits (+inf: no such row, or nothing seen), -rowsum(dO * O)
+    float* dsize;                                // [B, Hk * g, sq_pad]: rowsum |dO| (fp16 only)
     int sq_pad;                                  // Sq rounded up to a multiple of 64
     // How a key block's (head, query tile) pairs are dealt: `sink_blocks` blocks of kWindowBwdKeys keys with sinks in them go to sink_chunks workgroups
     // each, of sink_tiles pairs, the others to chunks, of chunk_tiles pairs.

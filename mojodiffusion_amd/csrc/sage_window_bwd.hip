@@ -25,10 +25,13 @@ typedef __fp16 v2fp __attribute__((ext_vector_type(2)));
 constexpr int kWaves = 4, kRowsWg = kWaves * 32;
 constexpr int kKeysWg = kWindowBwdKeys;                          // (pairs of waves share 32 keys)
 
-// bf16: weights are carried times 2^14 (by their statistic, at no cost), so that those down to 2^-28 keep all bits of the fp16 in which they are handed on
-// (PairLds), whose normal range ends at 2^-14; what is made of them is multiplied by kWeightInv at the end.
-template <int T> constexpr float kWeightBits = T == kBF16 ? 14.0f : 0.0f;
-template <int T> constexpr float kWeightInv = T == kBF16 ? 0x1p-14f : 1.0f;
+// Weights are carried times 2^14 (by their statistic, at no cost): as fp16, which is how dV takes them where that is the type, and how they are handed on
+// where it is bf16 (PairLds), those down to 2^-28 keep all bits.  What is made of them is multiplied by kWeightInv at the end.
+constexpr float kWeightBits = 14.0f, kWeightInv = 0x1p-14f;
+// fp16: the power of two that dS = P (dP - Delta) is rounded with, from the sum of its row's |dO|, or the largest such sum of the rows that meet in a dK.
+// |dS| <= sum |dO| max |v| / 2, so that it stays within fp16's range for |v| < 511, and the largest keep all bits for weights down to 2^-18 or so,
+// whatever the size of dO.  (Without it the relative error of dQ and dK was 3 times that of one rounding at dO of 1e-3 and 4 times at 1e-4.)
+__device__ __forceinline__ int ds_power(float sum) { return 8 - __builtin_amdgcn_frexp_expf(sum); }
 
 template <int T> __device__ __forceinline__ float widen(uint32_t w, int i) {
     if constexpr (T == kBF16) return __uint_as_float(i ? w & 0xFFFF0000u : w << 16);
@@ -44,7 +47,7 @@ __global__ __launch_bounds__(256) void window_bwd_prep_kernel(WindowBwdArgs a) {
     const int i = (int)(row % a.sq_pad), bh = (int)(row / a.sq_pad), b = bh / H, h = bh % H, col = (int)(threadIdx.x % CPR) * 8;
     const int len = sequence_len(a.w, b);
     const bool real = seeing(a.w, first_position(a.w, b, len), len).has(i);           // (rows that see nothing are not read: they may hold anything)
-    float sum = 0.0f;
+    float sum = 0.0f, size = 0.0f;
     if (real) {
         const int64_t at = b * a.w.o_sb + h * a.w.o_sh + i * a.w.o_sn + col;
         const u32x4 o = *reinterpret_cast<const u32x4*>(a.w.o + at);
@@ -54,14 +57,19 @@ __global__ __launch_bounds__(256) void window_bwd_prep_kernel(WindowBwdArgs a) {
         for (int e = 0; e < 8; e++) {
             const uint32_t ow = o[e >> 1], rw = rest[e >> 1], gw = g[e >> 1];
             sum = fmaf(widen<T>(ow, e & 1) + widen<T>(rw, e & 1), widen<T>(gw, e & 1), sum);
+            if constexpr (T == kF16) size += fabsf(widen<T>(gw, e & 1));
         }
     }
 #pragma unroll
-    for (int m = 1; m < CPR; m <<= 1) sum += __shfl_xor(sum, m);
+    for (int m = 1; m < CPR; m <<= 1) {
+        sum += __shfl_xor(sum, m);
+        if constexpr (T == kF16) size += __shfl_xor(size, m);
+    }
     if (col == 0) {
         const float l = real ? a.w.stats[(int64_t)bh * a.w.Sq + i] : -INFINITY;
         a.ndelta[row] = real ? -sum : 0.0f;
-        a.lse2[row] = l == -INFINITY ? INFINITY : fmaf(l, kLog2e, -kWeightBits<T>);           // (nothing seen: every probability vanishes)
+        if constexpr (T == kF16) a.dsize[row] = size;
+        a.lse2[row] = l == -INFINITY ? INFINITY : fmaf(l, kLog2e, -kWeightBits);           // (nothing seen: every probability vanishes)
     }
 }
 
@@ -110,12 +118,19 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
     query_rows_in<D>(w, a.dout + b * a.do_sb + (int64_t)kvh * w.g * a.do_sh + (int64_t)i_lo * a.do_sn, a.do_sn, a.do_sh, i_lo, x0, lds + own + 64 * D, lane);
     if (span.n > 0) tiles.copy(k, 0, L::keys(0)), tiles.copy(v, 0, L::values(0));
     const int64_t at = ((int64_t)b * H + kvh * w.g + hg) * a.sq_pad + i;
-    float lse = a.lse2[at], ndelta = a.ndelta[at];
+    float lse = a.lse2[at], ndelta = a.ndelta[at], mul = w.scale * kWeightInv;
+    if constexpr (T == kF16) mul = a.dsize[at];
     dma_wait<0>();
 #pragma unroll
     for (int s = 0; s < KS; s++) b1[s] = fr.along(smem + own, s), b2[s] = fr.along(smem + own + 64 * D, s);
 #pragma unroll
     for (int s = 0; s < KS; s++) asm volatile("" : "+v"(b1[s]), "+v"(b2[s]));
+    if constexpr (T == kF16) {           // (a power of the row's own, for the weights' one)
+        const int power = ds_power(mul);
+        lse += kWeightBits - (float)power;
+        mul = w.scale * __builtin_amdgcn_ldexpf(1.0f, -power);
+        asm volatile("" : "+v"(mul));
+    }
     asm volatile("" : "+v"(lse), "+v"(ndelta));
 
     v16f acc[DB];
@@ -225,7 +240,7 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
             for (int e = 0; e < 16; e++) acc[d][e] = blind ? 0.0f : acc[d][e];
     }
 #pragma unroll
-    for (int d = 0; d < DB; d++) row_put<T, D>(os, acc[d], d, w.scale * kWeightInv<T>, end_lane);
+    for (int d = 0; d < DB; d++) row_put<T, D>(os, acc[d], d, mul, end_lane);
     if (x0 < rows) query_rows_out<D>(w, os, a.dq + b * a.dq_sb + (int64_t)kvh * w.g * a.dq_sh, a.dq_sn, a.dq_sh, x0, end_lane);
 }
 
@@ -378,6 +393,20 @@ struct QueryStats {
         qt = last ? 0 : qt + 1;
     }
 };
+// The largest sum of |dO| of the rows of those tiles.
+__device__ __forceinline__ float largest_size(const WindowBwdArgs& a, int64_t head, const QuerySpan& q, int first, int n, int lane) {
+    float top = 0.0f;
+    for (int hg = q.nt > 0 ? first / q.nt : 0, qt = first - hg * q.nt; n > 0; hg++, qt = 0) {
+        const int here = min(n, q.nt - qt);
+        const v4f* at = reinterpret_cast<const v4f*>(a.dsize + (head + hg) * a.sq_pad + (q.t0 + qt) * 32);
+#pragma unroll 4
+        for (int e = lane; e < here * 8; e += 64) top = fmaxf(top, fmaxf(fmaxf(at[e][0], at[e][1]), fmaxf(at[e][2], at[e][3])));
+        n -= here;
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(top)));
+}
 // Positions of the tiles' first queries.
 struct QueryWalk {
     int p, qt, nt, p_first;
@@ -459,6 +488,12 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
         d.copy(pieces, lds + L::d(slot), wave, lane);
     };
     if (n_tiles > 0) copy(0);
+    float ds_mul = 1.0f, out_mul = ROLE == 0 ? kWeightInv : w.scale * kWeightInv;
+    if constexpr (T == kF16 && ROLE == 1) {
+        const int power = ds_power(largest_size(a, (int64_t)b * w.Hk * w.g + kvh * w.g, qs, work.first, n_tiles, lane));
+        ds_mul = __builtin_amdgcn_ldexpf(kWeightInv, power);
+        out_mul = w.scale * __builtin_amdgcn_ldexpf(1.0f, -power);
+    }
     dma_wait<0>();
 #pragma unroll
     for (int s = 0; s < KS; s++) bx[s] = fr.along(smem + own, s);
@@ -527,7 +562,7 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
                 for (int e = 0; e < 2; e++) {
                     // (as a multiply-add: one instruction with the fp16 operand's conversion in it)
                     if constexpr (T == kBF16) y[e] = fmaf((float)__builtin_bit_cast(v2fp, hp[n >> 1])[e], s[n + e], 0.0f);
-                    else y[e] = unpack24(&hp[(n >> 2) * 3], (n & 3) + e) * s[n + e];
+                    else y[e] = unpack24(&hp[(n >> 2) * 3], (n & 3) + e) * s[n + e] * ds_mul;
                 }
                 pk[n >> 1] = pack2<T>(y[0], y[1]);
             }
@@ -562,8 +597,8 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
     }
     __syncthreads();                     // (every copy has landed, every tile has been read: the ring takes the output rows)
     uint8_t* os = smem + L::RING + wave * 64 * D;
-    if constexpr (ROLE == 0) key_rows_out<T, D>(a, acc, kWeightInv<T>, os, work.part, 1, a.dv + b * a.dv_sb + kvh * a.dv_sh, a.dv_sn, x0, work.k0, lane);
-    else key_rows_out<T, D>(a, acc, w.scale * kWeightInv<T>, os, work.part, 0, a.dk + b * a.dk_sb + kvh * a.dk_sh, a.dk_sn, x0, work.k0, lane);
+    if constexpr (ROLE == 0) key_rows_out<T, D>(a, acc, out_mul, os, work.part, 1, a.dv + b * a.dv_sb + kvh * a.dv_sh, a.dv_sn, x0, work.k0, lane);
+    else key_rows_out<T, D>(a, acc, out_mul, os, work.part, 0, a.dk + b * a.dk_sb + kvh * a.dk_sh, a.dk_sn, x0, work.k0, lane);
 }
 
 template <int T, int D>

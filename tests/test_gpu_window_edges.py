@@ -169,3 +169,51 @@ def test_gradients_of_keys_with_small_weights(D, Hq, Hk):
     want[1] = (want[1][0], want[1][1] + extra)
     assert float(extra.max()) < 0.02 * float(want[1][0][:, S // 3:].abs().max())
     check_backward(grads(q.cuda(), k.cuda(), v.cuda(), d.cuda(), 1.0, -1, -1, 0)[1], want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("power", [-16, -12, -6])
+@pytest.mark.parametrize("S,Hq,Hk,D,left,sinks", [(1500, 2, 1, 64, -1, 0), (333, 3, 3, 128, 40, 3), (900, 1, 1, 128, -1, 0)])
+def test_fp16_gradients_of_small_upstream_gradients(power, S, Hq, Hk, D, left, sinks):
+    """Gradients are linear in the upstream gradient.  Of size 2^power, which fp16 holds exactly here, it gives those of size 1 times 2^power but for one rounding
+    of either result: half a step, 2^-11 of the value, 2^-25 below fp16's normal range.
+
+    And but for single dS that are rounded another way: a row's power is added to its statistic in fp32, a sum of less than 64 in size (off by 2^-19 at most, either
+    time: weights by 2^-18 relatively), so a dS within 2^-18 of a tie may fall on its other side.  Ties are a step of 2^-11 to 2^-10 apart: that is 2^-6 of the
+    dS at most, by a step, 2^-10 of each, of either sign.  Elementwise that is more than the bounds of results near zero (a restatement of dQ's roundings on the CPU, in which the
+    statistics' sums are all that differs, has two rows of 1500 beyond them, by 1.69), so norms are compared: 2^-10 sqrt(2^-6) of the root sum
+    of the squared terms comes on top."""
+    q, k, v = (t.cuda() for t in tensors(1, S, S, Hq, Hk, D, FP, 5))
+    d = (torch.randint(-64, 65, q.shape, generator=torch.Generator().manual_seed(4)) / 64.0).to(FP)
+    small = (d.double() * 2.0 ** power).to(FP)
+    assert torch.equal(small.double(), d.double() * 2.0 ** power)
+    got, one = (grads(q, k, v, x.cuda(), D ** -0.5, left, 0, sinks)[1] for x in (small, d))
+    w, g = forward(q, k, v, D ** -0.5, left, 0, sinks, [S], [0])[2], Hq // Hk
+    terms = [torch.zeros(x.shape, dtype=torch.float64) for x in one]
+    for h in range(Hq):
+        qh, dh, kh, vh = (x[0, :, y].double().cpu() for x, y in ((q, h), (d, h), (k, h // g), (v, h // g)))
+        dp = dh @ vh.T
+        ds = w[0, h] * (dp - (w[0, h] * dp).sum(1, keepdim=True)) * D ** -0.5
+        terms[0][0, :, h] = ds.square() @ kh.square()
+        terms[1][0, :, h // g] += ds.T.square() @ qh.square()
+        terms[2][0, :, h // g] += w[0, h].T.square() @ dh.square()
+    for name, x, y, t in zip(("dQ", "dK", "dV"), got, one, terms):
+        x, y = x.double(), y.double() * 2.0 ** power
+        bound = 2.0 ** -10 * 1.001 * y.abs() + 2.0 ** -25 + 2.0 ** (power - 25)
+        other = 2.0 ** (power - 13) * float(t.sum().sqrt())
+        assert float((x - y).norm()) <= float(bound.norm()) + other, (name, float((x - y).norm()), float(bound.norm()), other)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_fp16_gradients_of_large_upstream_gradients(D):
+    """dS beyond fp16's range where dQ, dK and dV are not: the bounds of an upstream gradient of size 1, times 2^13."""
+    S, scale, size = 16, 2.0 ** -10, 2.0 ** 13
+    q, k, v = tensors(1, S, S, 2, 2, D, FP, 5)
+    v = v * 8.0
+    d = (torch.randint(-64, 65, q.shape, generator=torch.Generator().manual_seed(4)) / 64.0).to(FP)
+    ref = forward(q, k, v, scale, -1, 0, 0, [S], [0])
+    want = [(x * size, y * size) for x, y in backward(q, k, v, d, scale, ref, 1)]
+    ds = ref[2][0, 0] * (d[0, :, 0].double() @ v[0, :, 0].double().T)
+    assert float(ds.abs().max()) * size > 65504 and all(float(x.abs().max()) < 6e4 for x, _ in want)
+    check_backward(grads(q.cuda(), k.cuda(), v.cuda(), (d * size).cuda(), scale, -1, 0, 0)[1], want)
