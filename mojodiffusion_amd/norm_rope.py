@@ -129,6 +129,11 @@ def _out(name, out, like):
     return out
 
 
+def _written(*outs):
+    """Counts a write into tensors that the caller gave, as torch's own calls do: a node that has saved one of them then refuses its backward."""
+    torch.autograd.graph.increment_version([t for t in outs if t is not None and not t.is_inference()])
+
+
 def qk_norm_rope(q, k, q_norm, k_norm, eps, cos, sin, halfsplit=False, positions=None, q_out=None, k_out=None):
     """(q_rot, k_rot) for q [B,S,Hq,Dh] and k [B,S,Hk,Dh] of one type (BF16, F16 or F32): every head's row
     divided by its root mean square (eps inside the root), times its gain [Dh], then its first rot channels rotated by the
@@ -148,6 +153,7 @@ def qk_norm_rope(q, k, q_norm, k_norm, eps, cos, sin, halfsplit=False, positions
     B, S, Hq, Dh = q.shape
     qi, ki = _rows(q), _rows(k)
     qo, ko = _out(name, q_out, q), _out(name, k_out, k)
+    _written(q_out, k_out)
     with torch.cuda.device(q.device):
         rc = _lib.lib().mi355_sage_qk_norm_rope(
             qi.data_ptr(), ki.data_ptr(), qo.data_ptr(), ko.data_ptr(), B, S, Hq, k.shape[2], Dh, _TYPES[q.dtype],
