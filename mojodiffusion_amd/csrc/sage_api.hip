@@ -1193,6 +1193,20 @@ static int norm_rope_args(const NormRopeView (&q)[3], const NormRopeView (&k)[3]
     return 0;
 }
 
+// An output in the place of the other side's input, whose rows another workgroup has still to read, of the other output, or of its own input in another
+// order.  (Places that overlap in another way cannot be told from the parts of a joint tensor; the header rules them out.)
+static int norm_rope_places(const NormRopeArgs& a) {
+    auto other_order = [&](int64_t b, int64_t h, int64_t n, const NormRopeSide& x, int H) { return (a.B > 1 && b != x.osb) || (H > 1 && h != x.osh) || (a.S > 1 && n != x.osn); };
+    auto moved = [&](const NormRopeSide& x, int H) {
+        return (x.out == x.p && other_order(x.sb, x.sh, x.sn, x, H)) || (x.out == x.d && other_order(x.dsb, x.dsh, x.dsn, x, H));
+    };
+    if (a.q.out == a.k.out || a.q.out == a.k.p || a.q.out == a.k.d || a.k.out == a.q.p || a.k.out == a.q.d || moved(a.q, a.Hq) || moved(a.k, a.Hk)) {
+        SAGE_LOG("norm_rope: an output lies over the other input, the other output, or its own input in another order");
+        return MI355_SAGE_EINVAL;
+    }
+    return 0;
+}
+
 int mi355_sage_qk_norm_rope(const void* Q, const void* K, void* Q_out, void* K_out, int B, int S, int Hq, int Hk, int D, int type,
                             const int64_t* q_strides, const int64_t* k_strides, const int64_t* qo_strides, const int64_t* ko_strides,
                             int64_t q_off, int64_t k_off, int64_t qo_off, int64_t ko_off,
@@ -1205,6 +1219,7 @@ int mi355_sage_qk_norm_rope(const void* Q, const void* K, void* Q_out, void* K_o
     if (int rc = norm_rope_args(q, k, 2, B, S, Hq, Hk, D, type, q_gain, k_gain, gain_type, eps, rope_cos, rope_sin, table_type, rot, table_rows,
                                 table_stride, halfsplit, positions, pos_stride, pos_bytes, &a))
         return rc;
+    if (int rc = norm_rope_places(a)) return rc;
     SAGE_HIP(launch_norm_rope(a, static_cast<hipStream_t>(stream)));
     return MI355_SAGE_OK;
 }
@@ -1235,6 +1250,7 @@ int mi355_sage_qk_norm_rope_bwd(const void* dQ_out, const void* dK_out, const vo
     hipStream_t st = static_cast<hipStream_t>(stream);
     std::lock_guard<std::mutex> together(launch_mutex(st));
     if ((rc = call_workspace("norm_rope backward", need, st, &workspace, workspace_bytes))) return rc;
+    if ((rc = norm_rope_places(a))) return rc;
     a.partial = static_cast<float*>(workspace);
     a.d_gain_q = static_cast<float*>(d_q_gain);
     a.d_gain_k = static_cast<float*>(d_k_gain);

@@ -143,7 +143,8 @@ def qk_norm_rope(q, k, q_norm, k_norm, eps, cos, sin, halfsplit=False, positions
     sampling/klein_sampler.mojo:305-307, repeat every row H times: pass cos[::H]); None for the norm alone.  rot may be less than
     Dh: the other channels pass.  halfsplit: pairs (i, i + rot/2) instead of (2i, 2i+1).  positions: int32 or int64
     [B,S] or [S], rows of the tables by token (a token whose position is not in the tables comes out as NaN);
-    without it token s takes row s.  q_out/k_out: where to write, e.g. rows of a cache; q and k themselves are allowed."""
+    without it token s takes row s.  q_out/k_out: where to write, e.g. rows of a cache; q_out may be q itself and k_out k; otherwise
+    they must overlap neither q, k nor each other."""
     if q_out is None and k_out is None:
         r = _lib.host().rope(q, k, q_norm, k_norm, eps, cos, sin, halfsplit, positions)
         if r is not None:
@@ -153,7 +154,6 @@ def qk_norm_rope(q, k, q_norm, k_norm, eps, cos, sin, halfsplit=False, positions
     B, S, Hq, Dh = q.shape
     qi, ki = _rows(q), _rows(k)
     qo, ko = _out(name, q_out, q), _out(name, k_out, k)
-    _written(q_out, k_out)
     with torch.cuda.device(q.device):
         rc = _lib.lib().mi355_sage_qk_norm_rope(
             qi.data_ptr(), ki.data_ptr(), qo.data_ptr(), ko.data_ptr(), B, S, Hq, k.shape[2], Dh, _TYPES[q.dtype],
@@ -162,6 +162,7 @@ def qk_norm_rope(q, k, q_norm, k_norm, eps, cos, sin, halfsplit=False, positions
             torch.cuda.current_stream(q.device).cuda_stream)
     if rc != 0:
         raise Error("%s: shim rc=%d (B=%d S=%d Hq=%d Hk=%d Dh=%d)" % (name, rc, B, S, Hq, k.shape[2], Dh))
+    _written(q_out, k_out)
     return qo, ko
 
 
