@@ -80,7 +80,17 @@ def _lens(name, what, t, B):
 
 
 def _int32(t):
-    return None if t is None else t.to(torch.int32).contiguous()
+    """t as dense int32, what lies beyond as the nearer end."""
+    if t is not None and t.dtype == torch.int64:
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
+    return None if t is None else t.contiguous()
+
+
+def _start(name, q_start):
+    start = int(q_start)
+    if not -2 ** 29 <= start <= 2 ** 29:
+        raise Error("%s: q_start=%d is not supported (at most 2^29 either way)" % (name, start))
+    return start
 
 
 def _ptr(t):
@@ -101,7 +111,7 @@ def _forward(name, q, k, v, scale, left, right, sinks, kv_lens, q_start, trainin
     Skv, Hk = k.shape[1], k.shape[2]
     kv_lens = _lens(name, "kv_lens", kv_lens, B)
     starts = _lens(name, "q_start", q_start, B) if isinstance(q_start, torch.Tensor) else None
-    start = 0 if starts is not None else int(q_start)
+    start = 0 if starts is not None else _start(name, q_start)
     _check_device(name, q, k, v, kv_lens, starts)
     L = _lib.lib()
     with torch.cuda.device(q.device):
@@ -123,7 +133,7 @@ def sdpa_window(q, k, v, scale, left, right=0, sinks=0, kv_lens=None, q_start=0)
 
     kv_lens: int32 or int64 [B] on the device, the sequences' lengths (keys from there on are padding: hidden, never read); None: all
     Skv.  q_start: the position of every sequence's first query, an int or int32 / int64 [B] on the device (a
-    chunk of a prompt whose first part is already in the cache).  A query that sees no key gives zeros; one that sees some and holds a NaN or an
+    chunk of a prompt whose first part is already in the cache), within 2^29 either way (an int beyond is refused, an element taken as the nearer end).  A query that sees no key gives zeros; one that sees some and holds a NaN or an
     infinity gives NaN in its own row."""
     return _forward("sdpa_window", q, k, v, scale, left, right, sinks, kv_lens, q_start, False)[0]
 
@@ -187,7 +197,7 @@ def sdpa_window_backward(fwd, d_out):
     Skv, Hk = k.shape[1], k.shape[2]
     if stats.dtype != torch.float32 or stats.numel() != B * Hq * Sq or not stats.is_contiguous():
         raise Error("%s: stats must be F32 [B,H,S,1]" % name)
-    lens = _lens(name, "kv_lens", fwd.kv_lens, B)
+    lens, start = _lens(name, "kv_lens", fwd.kv_lens, B), _start(name, fwd.q_start)
     _check_device(name, q, k, v, o, rest, d_out, stats, lens)
     L = _lib.lib()
     with torch.cuda.device(q.device):
@@ -200,7 +210,7 @@ def sdpa_window_backward(fwd, d_out):
         rc = L.mi355_sage_sdpa_window_bwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), rest.data_ptr(), d.data_ptr(), stats.data_ptr(), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(),
             B, Hq, Hk, Sq, Skv, Dh, _TYPES[q.dtype], fwd.scale, _strides(q), _strides(k), _strides(v), _strides(o), _strides(d), _strides(d_q),
-            _strides(d_k), _strides(d_v), 0, 0, 0, 0, 0, 0, 0, 0, 0, _bound(fwd.left), _bound(fwd.right), _bound(fwd.sinks), _ptr(lens), fwd.q_start,
+            _strides(d_k), _strides(d_v), 0, 0, 0, 0, 0, 0, 0, 0, 0, _bound(fwd.left), _bound(fwd.right), _bound(fwd.sinks), _ptr(lens), start,
             torch.cuda.current_stream(q.device).cuda_stream, ws.data_ptr(), ws.numel())
     if rc != 0:
         raise Error("%s: shim rc=%d (B=%d Sq=%d Skv=%d Hq=%d Hk=%d Dh=%d)" % (name, rc, B, Sq, Skv, Hq, Hk, Dh))

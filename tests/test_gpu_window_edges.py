@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from mojodiffusion_amd import attention_window as W
+from mojodiffusion_amd.attention_sage import Error
 from test_gpu_window import BF, FP, grads, tensors
 from window_reference import backward, check_backward, forward
 
@@ -217,3 +218,27 @@ def test_fp16_gradients_of_large_upstream_gradients(D):
     ds = ref[2][0, 0] * (d[0, :, 0].double() @ v[0, :, 0].double().T)
     assert float(ds.abs().max()) * size > 65504 and all(float(x.abs().max()) < 6e4 for x, _ in want)
     check_backward(grads(q.cuda(), k.cuda(), v.cuda(), (d * size).cuda(), scale, -1, 0, 0)[1], want)
+
+
+@pytest.mark.gpu
+def test_lengths_and_positions_past_32_bits():
+    q, k, v = (t.cuda() for t in tensors(2, 3, 90, 2, 2, 64, BF, 2))
+    call = lambda lens: W.sdpa_window_decode(q, k, v, torch.tensor(lens).cuda(), 0.125, 30)
+    assert torch.equal(call([2 ** 32 + 5, 90]), call([90, 90])) and torch.equal(call([-2 ** 32 + 60, 90]), call([0, 90]))
+    call = lambda starts: W.sdpa_window(q, k, v, 0.125, 30, q_start=torch.tensor(starts).cuda())
+    assert torch.equal(call([2 ** 32 + 40, -2 ** 33 + 40]), call([2 ** 29, -2 ** 29]))
+    assert (call([2 ** 32 + 40, -2 ** 33 + 40]) == 0).all()
+
+
+def test_positions_past_32_bits_are_refused():
+    q, k = torch.zeros((2, 4, 4, 64), dtype=BF), torch.zeros((2, 6, 2, 64), dtype=BF)
+    for start in (2 ** 29 + 1, -2 ** 29 - 1, 2 ** 32, 2 ** 32 + 5, -2 ** 64):
+        for call in (W.sdpa_window, W.sdpa_window_train_fwd):
+            with pytest.raises(Error, match="q_start"):
+                call(q, k, k, 0.1, 3, q_start=start)
+        with pytest.raises(Error, match="q_start"):
+            W.sdpa_window_backward(W.SdpaWindowFwd(q, q, torch.zeros((2, 4, 4, 1)), q, k, k, 0.1, 3, 0, 0, None, start), q)
+    for start in (2 ** 29, -2 ** 29):
+        with pytest.raises(Error, match="must live on the GPU"):
+            W.sdpa_window(q, k, k, 0.1, 3, q_start=start)
+    assert W._int32(torch.tensor([2 ** 32 + 5, -2 ** 33, 7])).tolist() == [2 ** 31 - 1, -2 ** 31, 7]
