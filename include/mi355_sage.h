@@ -528,7 +528,7 @@ int mi355_sage_sdpa_window_decode(
  * carry its rounding into dK: relative error 0.0032 for 0.0026 at a padded batch with sinks), dO upstream -> dQ [B,Hq,N_q,D], dK, dV [B,Hk,N_kv,D] (of a
  * shared key head: summed over its query heads), every row written, those of keys that no query sees and of queries that see none
  * as zeros.  Rows of Q, O, O_rest and dO of queries that see no key may hold anything; those of queries that see one must be finite (one that is
- * not reaches the gradients of keys next to those it sees, too).  D 64 or 128.  The same bits on every call (no atomics).  No output may overlap another
+ * not reaches the gradients of keys next to those it sees, too); fp16: finite results for |V| < 511 where they are in the type's range.  D 64 or 128.  The same bits on every call (no atomics).  No output may overlap another
  * tensor of the call. */
 size_t mi355_sage_window_bwd_workspace_bytes(int B, int Hq, int Hk, int N_q, int N_kv, int D, int left, int right, int sinks);
 int mi355_sage_sdpa_window_bwd(

@@ -242,3 +242,44 @@ def test_positions_past_32_bits_are_refused():
         with pytest.raises(Error, match="must live on the GPU"):
             W.sdpa_window(q, k, k, 0.1, 3, q_start=start)
     assert W._int32(torch.tensor([2 ** 32 + 5, -2 ** 33, 7])).tolist() == [2 ** 31 - 1, -2 ** 31, 7]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,Hq,Hk,dtype", [(64, 2, 1, FP), (128, 3, 3, BF)])
+def test_gradients_past_queries_before_the_sinks(D, Hq, Hk, dtype):
+    """With sinks every later query sees something: those before the first key alone do not, and an empty sequence's."""
+    B, Sq, Skv, left, right, sinks, first = 2, 300, 130, 9, 1, 5, -40
+    q, k, v = tensors(B, Sq, Skv, Hq, Hk, D, dtype, 3)
+    d = torch.randn(q.shape, generator=torch.Generator().manual_seed(4)).to(dtype)
+    lens = [120, 0]
+    blind = torch.stack([(first + torch.arange(Sq) + right < 0) | (n == 0) for n in lens])
+    want = backward(q, k, v, d, D ** -0.5, forward(q, k, v, D ** -0.5, left, right, sinks, lens, [first] * B), Hq // Hk)
+    q[blind], d[blind] = NAN, INF
+    n = torch.tensor(lens, dtype=torch.int32).cuda()
+    fwd, got = grads(q.cuda(), k.cuda(), v.cuda(), d.cuda(), D ** -0.5, left, right, sinks, lens=n, first=first)
+    check_backward(got, want)
+    assert (fwd.o.cpu()[blind] == 0).all() and (got[0].cpu()[blind] == 0).all()
+
+
+@pytest.mark.gpu
+def test_fp16_gradients_captured():
+    """A graph whose upstream gradient changes its size between replays, with the program's own calls in between."""
+    B, S, H, D = 2, 300, 2, 64
+    q, k, v = (t.cuda() for t in tensors(B, S, S, H, H, D, FP, 8))
+    first = torch.randn(q.shape, generator=torch.Generator().manual_seed(1)).cuda()
+    d = first.half()
+    step = lambda: grads(q, k, v, d, 0.125, 80, 0, 3)[1]
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for power in (0, -14, 10, -8, 3):
+        d.copy_(first * 2.0 ** power)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in out]
+        want = step()
+        torch.cuda.synchronize()
+        for x, y in zip(got, want):
+            assert torch.equal(x, y) and torch.isfinite(x).all() and x.abs().max() > 0, power
