@@ -540,6 +540,50 @@ int mi355_sage_sdpa_window_bwd(
     int64_t stats_offset_elems, int64_t dq_offset_elems, int64_t dk_offset_elems, int64_t dv_offset_elems,
     int left, int right, int sinks, const void* kv_lens, int q_start, void* stream, void* workspace, size_t workspace_bytes);
 
+/* ------------------------------------------------------------------------
+ * A paged cache of keys and values in 8 bits (no counterpart in the reference, which keeps no cache), for bf16 or fp16 activations.
+ *
+ * A page holds `page` tokens (32 times a power of two), in blocks of 32.  Of a block and key head: 32 x D e4m3 codes of K, a token after the
+ * other, D x 32 of V, a channel after the other (the operand order of the second matrix product), and one scale each.
+ *     k_pages [pages, page / 32, Hk, 32, D],  v_pages [pages, page / 32, Hk, D, 32],  k_scale, v_scale F32 [pages, page / 32, Hk]
+ * dense, 16-byte aligned.  A value is its code times its scale.  Scales are powers of two, the least with which a block's largest
+ * value stays within e4m3's 448, and at least 2^-100 (what lies below 2^-110 becomes zero).  While a block fills, its scale only rises; codes that are there are then rounded
+ * again, which changes those that leave e4m3's normal range and no others.  A value that is not finite becomes NaN and does not count for the scale.
+ * page_table: int32 [B, table_width], rows table_stride apart: the pages of a sequence's tokens in order; only the entries that its tokens need are looked at.
+ * kv_lens: int32 [B], tokens of a sequence with the new ones among them.  Both on the device.  A length beyond the table counts as the
+ * table's table_width * page tokens, one below zero as zero.
+ *
+ * Appends the last tokens of every sequence: token i of the n new ones of sequence b stands at kv_lens[b] - n + i.  K, V [B,Hk,N,D] (n = N for
+ * every sequence), or, with cu_seqlens (int32 [B+1] on the device, not falling; the first counts as 0), sequences that lie one behind the other in [1,Hk,N,D], rows cu_seqlens[b] .. cu_seqlens[b+1] - 1.
+ * Four element strides each, D stride 1, rows 16-byte aligned (slices of a joint projection are taken as they are).  K's rows are divided by their
+ * root mean square (eps inside the root) times k_gain [D] if that is not NULL, then rotated by the row of rope_cos / rope_sin that
+ * their position names, as in mi355_sage_qk_norm_rope (rot 0: not at all; a position outside the tables: NaN); V's go as they are.  Q (may be NULL) [B,Hq,N,D] or [1,Hq,N,D] likewise, with q_gain, to Q_out,
+ * which may be Q itself and must otherwise overlap nothing that is read; rows of Q that belong to no sequence come out as zeros.
+ * Tokens at positions below zero or beyond the table, or whose page is not in [0, pages), are not stored.  Rows of a block behind the last token keep
+ * what they hold.  Blocks that a call appends to must belong to one sequence each (pages that sequences share must be full).  The same
+ * call again leaves the same cache.  One launch; no workspace. */
+int mi355_sage_kv_append(
+    const void* K, const void* V, const void* Q, void* Q_out,
+    void* k_pages, void* v_pages, void* k_scale, void* v_scale, int64_t pages, int page,
+    const void* page_table, int64_t table_stride, int table_width, const void* kv_lens, const void* cu_seqlens,
+    int B, int N, int Hq, int Hk, int D, int type,
+    const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides, const int64_t* qo_strides,
+    int64_t k_offset_elems, int64_t v_offset_elems, int64_t q_offset_elems, int64_t qo_offset_elems,
+    const void* q_gain, const void* k_gain, int gain_type, float eps,
+    const void* rope_cos, const void* rope_sin, int table_type, int rot, int64_t rope_rows, int64_t rope_stride, int halfsplit, void* stream);
+
+/* Attention of the last N_q tokens of every sequence over the cache: query i of sequence b stands at kv_lens[b] - N_q + i and sees the keys up to
+ * itself; one before a sequence's first token gives zeros.  Q, O [B,Hq,N_q,D] of `type`, Hq a multiple of Hk: query heads h Hq/Hk .. share key head
+ * h.  Any N_q; meant for few.  Keys behind a sequence's length are never part of a result, whatever their codes are.  A NaN in a key that a query sees gives NaN in
+ * its row, one in a value that some query of the call sees may reach the rows of queries before it; a page outside [0, pages) gives NaN in the rows of its sequence.  Workspace: mi355_sage_paged_workspace_bytes(...) bytes,
+ * 256-byte aligned, or NULL for the library's per-stream buffer (the rules of mi355_sage_sdpa_bf16).  The same bits on every call. */
+size_t mi355_sage_paged_workspace_bytes(int B, int Hq, int Hk, int N_q, int D, int table_width, int page);
+int mi355_sage_sdpa_paged(
+    const void* Q, void* O, const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale, int64_t pages, int page,
+    const void* page_table, int64_t table_stride, int table_width, const void* kv_lens,
+    int B, int Hq, int Hk, int N_q, int D, int type, float scale, const int64_t* q_strides, const int64_t* o_strides,
+    int64_t q_offset_elems, int64_t o_offset_elems, void* stream, void* workspace, size_t workspace_bytes);
+
 /* Library identification: "mi355_sage <version> gfx950". */
 const char* mi355_sage_version(void);
 

@@ -3,6 +3,7 @@
 #include "../../include/mi355_sage.h"
 #include "../../include/mi355_sage_test.h"
 #include "sage_internal.h"
+#include "sage_kv.h"
 #include "sage_window.h"
 
 #include <atomic>
@@ -1416,6 +1417,111 @@ int mi355_sage_sdpa_window_bwd(const void* Q, const void* K, const void* V, cons
     a.dk = static_cast<uint16_t*>(dK) + dk_off; a.dk_sb = dk_strides[0]; a.dk_sh = dk_strides[1]; a.dk_sn = dk_strides[2];
     a.dv = static_cast<uint16_t*>(dV) + dv_off; a.dv_sb = dv_strides[0]; a.dv_sh = dv_strides[1]; a.dv_sn = dv_strides[2];
     SAGE_HIP(launch_window_bwd(a, st));
+    return MI355_SAGE_OK;
+}
+
+// ---- paged cache of e4m3 codes ----------------------------------------------------------------------
+static int kv_pool(const char* name, void* k_pages, void* v_pages, void* k_scale, void* v_scale, int64_t pages, int page, const void* table, int64_t table_stride,
+                   int table_width, const void* kv_lens, int B, int Hk, int D, KvPool* out) {
+    if (!k_pages || !v_pages || !k_scale || !v_scale || !table || !kv_lens || pages <= 0 || page <= 0 || table_width <= 0 || B <= 0 || Hk <= 0 || D <= 0) return MI355_SAGE_EINVAL;
+    if (!dims_ok(D)) { SAGE_LOG("%s: head dim %d not supported (64, 128 or 256)", name, D); return MI355_SAGE_EUNSUPPORTED; }
+    if (page % kKvBlock || (page & (page - 1)) || page > 1 << 16) { SAGE_LOG("%s: a page holds 32, 64, 128, .. tokens", name); return MI355_SAGE_EUNSUPPORTED; }
+    if (pages > 0x7FFFFFFF / (page / kKvBlock) || (int64_t)table_width * page > 1 << 29) { SAGE_LOG("%s: too many pages", name); return MI355_SAGE_EUNSUPPORTED; }
+    if ((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15) { SAGE_LOG("%s: pages must be 16-byte aligned", name); return MI355_SAGE_EUNSUPPORTED; }
+    KvPool c{};
+    c.k = static_cast<uint8_t*>(k_pages); c.v = static_cast<uint8_t*>(v_pages);
+    c.ks = static_cast<float*>(k_scale); c.vs = static_cast<float*>(v_scale);
+    c.pages = pages;
+    for (int n = page / kKvBlock; n > 1; n >>= 1) c.sub++;
+    c.table = static_cast<const int32_t*>(table); c.table_stride = table_stride; c.width = table_width;
+    c.lens = static_cast<const int32_t*>(kv_lens);
+    c.Hk = Hk;
+    *out = c;
+    return 0;
+}
+
+int mi355_sage_kv_append(const void* K, const void* V, const void* Q, void* Q_out, void* k_pages, void* v_pages, void* k_scale, void* v_scale, int64_t pages, int page,
+                         const void* page_table, int64_t table_stride, int table_width, const void* kv_lens, const void* cu_seqlens, int B, int N, int Hq, int Hk, int D,
+                         int type, const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides, const int64_t* qo_strides, int64_t k_off, int64_t v_off,
+                         int64_t q_off, int64_t qo_off, const void* q_gain, const void* k_gain, int gain_type, float eps, const void* rope_cos, const void* rope_sin,
+                         int table_type, int rot, int64_t rope_rows, int64_t rope_stride, int halfsplit, void* stream) {
+    if (!K || !V || !k_strides || !v_strides || (Q == nullptr) != (Q_out == nullptr) || (Q && (!q_strides || !qo_strides || Hq <= 0)) || N <= 0) return MI355_SAGE_EINVAL;
+    KvAppendArgs a{};
+    int rc = kv_pool("kv_append", k_pages, v_pages, k_scale, v_scale, pages, page, page_table, table_stride, table_width, kv_lens, B, Hk, D, &a.pool);
+    if (rc) return rc;
+    if (type != MI355_SAGE_BF16 && type != MI355_SAGE_FP16) { SAGE_LOG("kv_append: bf16 or fp16"); return MI355_SAGE_EUNSUPPORTED; }
+    if (rot < 0 || rot > D || !(eps >= 0.0f) || (rot > 0 && (!rope_cos || !rope_sin || rope_rows <= 0 || table_type < 0 || table_type > 2))) return MI355_SAGE_EINVAL;
+    if ((q_gain || k_gain) && (gain_type < 0 || gain_type > 2)) return MI355_SAGE_EINVAL;
+    if (rot % 16) { SAGE_LOG("kv_append: %d rotated channels (a multiple of 16)", rot); return MI355_SAGE_EUNSUPPORTED; }
+    uintptr_t bits = reinterpret_cast<uintptr_t>(q_gain) | reinterpret_cast<uintptr_t>(k_gain);
+    if (rot > 0) bits |= reinterpret_cast<uintptr_t>(rope_cos) | reinterpret_cast<uintptr_t>(rope_sin) | (uintptr_t)(rope_stride * (table_type == MI355_SAGE_F32 ? 4 : 2));
+    if (bits & 15) { SAGE_LOG("kv_append: gains and table rows must be 16-byte aligned"); return MI355_SAGE_EUNSUPPORTED; }
+    if ((rc = check_view("K", K, k_strides, k_off)) || (rc = check_view("V", V, v_strides, v_off))) return rc;
+    if (Q && ((rc = check_view("Q", Q, q_strides, q_off)) || (rc = check_view("Q_out", Q_out, qo_strides, qo_off)))) return rc;
+    a.B = B; a.S = cu_seqlens ? 0 : N; a.Hq = Q ? Hq : 0; a.D = D; a.type = type;
+    const int64_t rows = cu_seqlens ? N : (int64_t)B * N;
+    if (rows > 1 << 29 || B > 1 << 20 || N > 1 << 29) { SAGE_LOG("kv_append: too many rows"); return MI355_SAGE_EUNSUPPORTED; }
+    a.rows = (int)rows;
+    auto side = [](const void* p, const int64_t* s, int64_t off) { return KvSide{static_cast<const uint16_t*>(p) + off, s[0], s[1], s[2]}; };
+    a.k = side(K, k_strides, k_off);
+    a.v = side(V, v_strides, v_off);
+    if (Q) {
+        if ((rc = distinct_rows("Q_out", qo_strides, cu_seqlens ? 1 : B, Hq, N))) return rc;
+        a.q = side(Q, q_strides, q_off);
+        a.qo = static_cast<uint16_t*>(Q_out) + qo_off;
+        a.qo_sb = qo_strides[0]; a.qo_sh = qo_strides[1]; a.qo_sn = qo_strides[2];
+        const bool moved = a.qo == a.q.p && (((cu_seqlens ? 1 : B) > 1 && a.qo_sb != a.q.sb) || (Hq > 1 && a.qo_sh != a.q.sh) || (N > 1 && a.qo_sn != a.q.sn));
+        if (moved || a.qo == a.k.p || a.qo == a.v.p) { SAGE_LOG("kv_append: Q_out lies over K, V, or Q in another order"); return MI355_SAGE_EINVAL; }
+    }
+    a.cu = static_cast<const int32_t*>(cu_seqlens);
+    a.q_gain = q_gain; a.k_gain = k_gain; a.gain_type = gain_type; a.eps = eps; a.inv_d = 1.0f / D;
+    a.cos = rope_cos; a.sin = rope_sin; a.table_type = table_type; a.rot = rot; a.halfsplit = halfsplit != 0;
+    a.table_rows = rope_rows; a.table_stride = rope_stride;
+    if (!kv_append_grid_ok(a)) { SAGE_LOG("kv_append: too many workgroups"); return MI355_SAGE_EUNSUPPORTED; }
+    SAGE_HIP(launch_kv_append(a, static_cast<hipStream_t>(stream)));
+    return MI355_SAGE_OK;
+}
+
+static int paged_dims(int B, int Hq, int Hk, int N_q, int D, int table_width, int page, PagedArgs* a) {
+    if (B <= 0 || Hq <= 0 || Hk <= 0 || N_q <= 0 || D <= 0 || table_width <= 0 || page <= 0 || Hq % Hk) return MI355_SAGE_EINVAL;
+    if (!dims_ok(D) || page % kKvBlock || (page & (page - 1)) || page > 1 << 16 || (int64_t)table_width * page > 1 << 29) return MI355_SAGE_EUNSUPPORTED;
+    *a = PagedArgs{};
+    a->B = B; a->g = Hq / Hk; a->Sq = N_q; a->D = D;
+    a->pool.Hk = Hk; a->pool.width = table_width;
+    for (int n = page / kKvBlock; n > 1; n >>= 1) a->pool.sub++;
+    if ((int64_t)B * Hq > (1 << 29) / N_q || B > 1 << 20 || paged_tiles(*a) > 1 << 30) { SAGE_LOG("paged attention: too many blocks or rows"); return MI355_SAGE_EUNSUPPORTED; }
+    a->wgs = paged_wgs(*a);
+    return 0;
+}
+
+size_t mi355_sage_paged_workspace_bytes(int B, int Hq, int Hk, int N_q, int D, int table_width, int page) {
+    PagedArgs a;
+    return paged_dims(B, Hq, Hk, N_q, D, table_width, page, &a) ? 0 : align_up(paged_part_bytes(a));
+}
+
+int mi355_sage_sdpa_paged(const void* Q, void* O, const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale, int64_t pages, int page,
+                          const void* page_table, int64_t table_stride, int table_width, const void* kv_lens, int B, int Hq, int Hk, int N_q, int D, int type, float scale,
+                          const int64_t* q_strides, const int64_t* o_strides, int64_t q_off, int64_t o_off, void* stream, void* workspace, size_t workspace_bytes) {
+    if (!Q || !O || !q_strides || !o_strides || !(scale > 0.0f) || !(scale < INFINITY)) return MI355_SAGE_EINVAL;
+    PagedArgs a;
+    KvPool pool;
+    int rc = kv_pool("paged attention", const_cast<void*>(k_pages), const_cast<void*>(v_pages), const_cast<void*>(k_scale), const_cast<void*>(v_scale), pages, page, page_table,
+                     table_stride, table_width, kv_lens, B, Hk, D, &pool);
+    if (rc || (rc = paged_dims(B, Hq, Hk, N_q, D, table_width, page, &a))) return rc;
+    if (type != MI355_SAGE_BF16 && type != MI355_SAGE_FP16) { SAGE_LOG("paged attention: bf16 or fp16"); return MI355_SAGE_EUNSUPPORTED; }
+    if ((rc = check_view("Q", Q, q_strides, q_off)) || (rc = check_view("O", O, o_strides, o_off)) || (rc = distinct_rows("O", o_strides, B, Hq, N_q))) return rc;
+    a.pool = pool;
+    a.type = type;
+    a.scale = scale;
+    a.q = static_cast<const uint16_t*>(Q) + q_off; a.q_sb = q_strides[0]; a.q_sh = q_strides[1]; a.q_sn = q_strides[2];
+    a.o = static_cast<uint16_t*>(O) + o_off; a.o_sb = o_strides[0]; a.o_sh = o_strides[1]; a.o_sn = o_strides[2];
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    std::lock_guard<std::mutex> together(launch_mutex(st));
+    const size_t need = paged_part_bytes(a);
+    if ((rc = call_workspace("paged attention", need, st, &workspace, workspace_bytes))) return rc;
+    a.part = static_cast<float*>(workspace);
+    a.part_ml = a.part + need / sizeof(float) / (a.D + 2) * a.D;
+    SAGE_HIP(launch_paged(a, st));
     return MI355_SAGE_OK;
 }
 

@@ -42,6 +42,9 @@ struct Api {
     decltype(&mi355_sage_sdpa_window_decode) window_decode;
     decltype(&mi355_sage_window_bwd_workspace_bytes) window_bwd_workspace_bytes;
     decltype(&mi355_sage_sdpa_window_bwd) window_bwd;
+    decltype(&mi355_sage_kv_append) kv_append;
+    decltype(&mi355_sage_paged_workspace_bytes) paged_workspace_bytes;
+    decltype(&mi355_sage_sdpa_paged) paged;
 } api;
 constexpr int kApiEntries = sizeof(Api) / sizeof(void*);
 static_assert(sizeof(Api) == kApiEntries * sizeof(void*), "one pointer per entry");
@@ -625,6 +628,121 @@ PyObject* py_window_bwd(PyObject* const* a, Py_ssize_t n) {
     return t;
 }
 
+// ---- paged cache (kv_cache.py) ------------------------------------------------------------------------
+struct CacheCall {
+    const at::Tensor *k, *v, *ks, *vs, *table, *lens;
+    int B, Hk, D, page;
+};
+// a: k pages, v pages, their scales, page table, lengths
+bool cache_args(PyObject* const* pages, PyObject* table, PyObject* lens, CacheCall& c) {
+    if (!tensor_arg(pages[0], c.k) || !tensor_arg(pages[1], c.v) || !tensor_arg(pages[2], c.ks) || !tensor_arg(pages[3], c.vs) || !tensor_arg(table, c.table) ||
+        !tensor_arg(lens, c.lens))
+        return false;
+    const at::Tensor &k = *c.k, &v = *c.v;
+    if (k.dim() != 5 || v.dim() != 5 || k.scalar_type() != at::kFloat8_e4m3fn || v.scalar_type() != at::kFloat8_e4m3fn || !k.is_cuda()) return false;
+    const int64_t P = k.size(0), n = k.size(1), H = k.size(2), D = k.size(4);
+    if (k.size(3) != 32 || v.size(0) != P || v.size(1) != n || v.size(2) != H || v.size(3) != D || v.size(4) != 32 || k.numel() == 0 || (n & (n - 1)) != 0 || n > 2048) return false;
+    for (const at::Tensor* t : {c.ks, c.vs})
+        if (t->dim() != 3 || t->size(0) != P || t->size(1) != n || t->size(2) != H || t->scalar_type() != at::kFloat) return false;
+    for (const at::Tensor* t : {c.k, c.v, c.ks, c.vs})
+        if (!t->is_contiguous() || !aligned16(*t) || t->device() != k.device()) return false;
+    const at::Tensor& pt = *c.table;
+    if (pt.dim() != 2 || pt.scalar_type() != at::kInt || pt.device() != k.device() || pt.numel() == 0 || (pt.size(1) > 1 && pt.stride(1) != 1) || !fits(pt.size(0)) || !fits(pt.size(1))) return false;
+    if (c.lens->dim() != 1 || c.lens->size(0) != pt.size(0) || c.lens->scalar_type() != at::kInt || !c.lens->is_contiguous() || c.lens->device() != k.device()) return false;
+    if (!fits(H) || !fits(D)) return false;
+    c.B = pt.size(0); c.Hk = H; c.D = D; c.page = n * 32;
+    return true;
+}
+// [B,S,H,D], or rows of all sequences one behind the other [T,H,D], as logical [B,H,S,D]
+bool dense_tokens(const at::Tensor& t, int dims) {
+    if (t.dim() != dims || !t.is_cuda() || t.stride(-1) != 1 || !aligned16(t)) return false;
+    for (int i = 0; i + 1 < dims; i++)
+        if (t.stride(i) % 8 != 0) return false;
+    return true;
+}
+Strides token_strides(const at::Tensor& t) { return t.dim() == 4 ? bhsd(t) : Strides{{0, t.stride(1), t.stride(0), 1}}; }
+// What the call has written, told to torch as its own calls do.
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// kv_append(k_pages, v_pages, k_scale, v_scale, k, v, page_table, kv_lens, cu_seqlens, k_norm, eps, cos, sin, halfsplit, q, q_norm) -> q rotated (True without q) or None
+PyObject* py_kv_append(PyObject* const* a, Py_ssize_t n) {
+    CacheCall c;
+    const at::Tensor *k, *v, *cu = nullptr, *gk = nullptr, *cs = nullptr, *sn = nullptr, *q = nullptr, *gq = nullptr;
+    double eps;
+    if (intercepted() || n != 16 || !cache_args(a, a[6], a[7], c) || !tensor_arg(a[4], k) || !tensor_arg(a[5], v) || !double_arg(a[10], eps) || !(eps >= 0.0) ||
+        (a[13] != Py_True && a[13] != Py_False))
+        Py_RETURN_NONE;
+    if ((a[8] != Py_None && !tensor_arg(a[8], cu)) || (a[9] != Py_None && !tensor_arg(a[9], gk)) || (a[11] == Py_None) != (a[12] == Py_None) ||
+        (a[11] != Py_None && (!tensor_arg(a[11], cs) || !tensor_arg(a[12], sn))) || (a[14] != Py_None && !tensor_arg(a[14], q)) || (a[15] != Py_None && !tensor_arg(a[15], gq)))
+        Py_RETURN_NONE;
+    const at::Device dev = c.k->device();
+    const int dims = cu ? 3 : 4;
+    const int type = element_type(k->scalar_type());
+    if (type != MI355_SAGE_BF16 && type != MI355_SAGE_FP16) Py_RETURN_NONE;
+    if (cu && (cu->dim() != 1 || cu->size(0) != (int64_t)c.B + 1 || cu->scalar_type() != at::kInt || !cu->is_contiguous() || cu->device() != dev)) Py_RETURN_NONE;
+    if (!dense_tokens(*k, dims) || !dense_tokens(*v, dims) || k->sizes() != v->sizes() || v->scalar_type() != k->scalar_type() || k->device() != dev || v->device() != dev) Py_RETURN_NONE;
+    if (k->size(-2) != c.Hk || k->size(-1) != c.D || k->numel() == 0 || (!cu && k->size(0) != c.B) || !fits(k->size(dims - 3))) Py_RETURN_NONE;
+    if (!q && gq) Py_RETURN_NONE;
+    if (q && (!dense_tokens(*q, dims) || q->scalar_type() != k->scalar_type() || q->device() != dev || q->size(-1) != c.D || q->numel() == 0 || q->size(0) != k->size(0) ||
+              (!cu && q->size(1) != k->size(1)) || !fits(q->size(-2))))
+        Py_RETURN_NONE;
+    int gain_type = 0, table_type = 0, rot = 0;
+    for (const at::Tensor* g : {gk, gq}) {
+        if (!g) continue;
+        if ((gain_type = element_type(g->scalar_type())) < 0 || (gk && g->scalar_type() != gk->scalar_type())) Py_RETURN_NONE;
+        if (g->dim() != 1 || g->numel() != c.D || !g->is_contiguous() || !aligned16(*g) || g->device() != dev) Py_RETURN_NONE;
+    }
+    if (cs) {
+        if (cs->dim() != 2 || cs->sizes() != sn->sizes() || cs->strides() != sn->strides() || (table_type = element_type(cs->scalar_type())) < 0 || sn->scalar_type() != cs->scalar_type())
+            Py_RETURN_NONE;
+        if (cs->size(0) < 1 || cs->size(1) < 1 || cs->size(1) * 2 > c.D || cs->stride(1) != 1 || (cs->stride(0) * (int64_t)cs->element_size()) % 16 || !aligned16(*cs) || !aligned16(*sn) ||
+            cs->device() != dev || sn->device() != dev)
+            Py_RETURN_NONE;
+        rot = (int)cs->size(1) * 2;
+    }
+    at::Tensor out;
+    const int rc = without_gil([&] {
+        const c10::DeviceGuard guard(dev);
+        if (q) out = fresh(q->sizes(), *q, q->scalar_type());
+        const Strides ks = token_strides(*k), vs = token_strides(*v), qs = q ? token_strides(*q) : Strides{}, os = q ? token_strides(out) : Strides{};
+        return api.kv_append(k->data_ptr(), v->data_ptr(), data_or_null(q), q ? out.data_ptr() : nullptr, c.k->data_ptr(), c.v->data_ptr(), c.ks->data_ptr(), c.vs->data_ptr(),
+                             c.k->size(0), c.page, c.table->data_ptr(), c.table->stride(0), c.table->size(1), c.lens->data_ptr(), data_or_null(cu), c.B, k->size(dims - 3),
+                             q ? (int)q->size(-2) : 0, c.Hk, c.D, type, ks.s, vs.s, q ? qs.s : nullptr, q ? os.s : nullptr, 0, 0, 0, 0, data_or_null(gq), data_or_null(gk), gain_type,
+                             (float)eps, data_or_null(cs), data_or_null(sn), table_type, rot, cs ? cs->size(0) : 0, cs ? cs->stride(0) : 0, a[13] == Py_True, stream_of(*k));
+    });
+    if (rc != 0) Py_RETURN_NONE;
+    for (const at::Tensor* t : {c.k, c.v, c.ks, c.vs}) written(*t);
+    if (!q) Py_RETURN_TRUE;
+    return THPVariable_Wrap(std::move(out));
+}
+
+// paged(q, k_pages, v_pages, k_scale, v_scale, page_table, kv_lens, scale) -> o or None
+PyObject* py_paged(PyObject* const* a, Py_ssize_t n) {
+    CacheCall c;
+    const at::Tensor* q;
+    double scale;
+    if (intercepted() || n != 8 || !tensor_arg(a[0], q) || !cache_args(a + 1, a[5], a[6], c) || !double_arg(a[7], scale)) Py_RETURN_NONE;
+    const int type = element_type(q->scalar_type());
+    if (!dense_tokens(*q, 4) || (type != MI355_SAGE_BF16 && type != MI355_SAGE_FP16) || q->device() != c.k->device() || q->numel() == 0) Py_RETURN_NONE;
+    if (q->size(0) != c.B || q->size(3) != c.D || q->size(2) % c.Hk || !fits(q->size(1)) || !fits(q->size(2))) Py_RETURN_NONE;
+    at::Tensor o;
+    const int rc = without_gil([&] {
+        const int Sq = q->size(1), Hq = q->size(2);
+        const size_t need = api.paged_workspace_bytes(c.B, Hq, c.Hk, Sq, c.D, c.table->size(1), c.page);
+        if (need == 0) return MI355_SAGE_EUNSUPPORTED;
+        const c10::DeviceGuard guard(q->device());
+        o = fresh(q->sizes(), *q, q->scalar_type());
+        const at::Tensor ws = fresh({(int64_t)need}, *q, at::kByte);        // (a call's own: see norm_rope.py)
+        const Strides qs = bhsd(*q), os = bhsd(o);
+        return api.paged(q->data_ptr(), o.data_ptr(), c.k->data_ptr(), c.v->data_ptr(), c.ks->data_ptr(), c.vs->data_ptr(), c.k->size(0), c.page, c.table->data_ptr(),
+                         c.table->stride(0), c.table->size(1), c.lens->data_ptr(), c.B, Hq, c.Hk, Sq, c.D, type, (float)scale, qs.s, os.s, 0, 0, stream_of(*q), ws.data_ptr(), need);
+    });
+    if (rc != 0) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(o));
+}
+
 // workspace(nbytes, tensor) -> this (device, stream)'s buffer
 PyObject* py_workspace(PyObject* const* a, Py_ssize_t n) {
     if (n != 2 || !PyLong_Check(a[0]) || !THPVariable_Check(a[1])) {
@@ -657,7 +775,8 @@ PyObject* py_bind(PyObject* const* a, Py_ssize_t n) {
 
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(entry<py_##name>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(fwd), METHOD(bias), METHOD(norm_rope), METHOD(bwd), METHOD(record), METHOD(workspace), METHOD(bind),
-                         METHOD(rope), METHOD(rope_bwd), METHOD(window), METHOD(window_decode), METHOD(window_bwd), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(rope), METHOD(rope_bwd), METHOD(window), METHOD(window_decode), METHOD(window_bwd), METHOD(kv_append), METHOD(paged),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_sage_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
