@@ -541,6 +541,34 @@ int mi355_sage_sdpa_window_bwd(
     int left, int right, int sinks, const void* kv_lens, int q_start, void* stream, void* workspace, size_t workspace_bytes);
 
 /* ------------------------------------------------------------------------
+ * Attention over whole sequences of different lengths that lie one behind the other, without padding; bf16 or fp16 matrix products, no quantization (the
+ * reference's batches are padded to one length).
+ *
+ * Sequence b's queries are rows cu_q[b] .. cu_q[b+1] - 1 of Q, its keys rows cu_k[b] .. cu_k[b+1] - 1 of K and V (int32 [B+1] on the device, not falling; the
+ * first counts as 0; entries beyond T_q, T_k as those; cu_q and cu_k may be one array).  Its n_q queries stand at the last positions of its n_k keys: query i at n_k - n_q + i.  With causal != 0 a
+ * query sees keys up to its own position, else all keys of its sequence.  A query that sees no key gets O = 0 and a statistic of -inf; so do rows behind the last sequence.
+ * Q, O [Hq,T_q,D], K, V [Hk,T_k,D] through four element strides each, of which the first is not used, Hq a multiple of Hk: query heads
+ * h Hq/Hk .. share key head h.  Types, D, scale, O_rest and what may not be finite as for mi355_sage_sdpa_window; Stats (may be NULL): F32 [Hq,T_q].  One launch; no
+ * workspace; the same bits on every call. */
+int mi355_sage_sdpa_packed(
+    const void* Q, const void* K, const void* V, void* O, void* O_rest, void* Stats, const void* cu_q, const void* cu_k,
+    int B, int Hq, int Hk, int T_q, int T_k, int D, int type, float scale,
+    const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+    int64_t q_offset_elems, int64_t k_offset_elems, int64_t v_offset_elems, int64_t o_offset_elems, int64_t stats_offset_elems, int causal, void* stream);
+
+/* Its gradient: O, O_rest (may be NULL) and Stats as the forward wrote them, dO upstream -> dQ [Hq,T_q,D], dK, dV [Hk,T_k,D], every row written, those of
+ * queries that see no key, of keys that no query sees and behind the last sequence as zeros.  D 64 or 128; the rest, workspace included, as for mi355_sage_sdpa_window_bwd. */
+size_t mi355_sage_packed_bwd_workspace_bytes(int B, int Hq, int Hk, int T_q, int T_k, int D);
+int mi355_sage_sdpa_packed_bwd(
+    const void* Q, const void* K, const void* V, const void* O, const void* O_rest, const void* dO, const void* Stats, void* dQ, void* dK, void* dV,
+    const void* cu_q, const void* cu_k, int B, int Hq, int Hk, int T_q, int T_k, int D, int type, float scale,
+    const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides, const int64_t* do_strides,
+    const int64_t* dq_strides, const int64_t* dk_strides, const int64_t* dv_strides,
+    int64_t q_offset_elems, int64_t k_offset_elems, int64_t v_offset_elems, int64_t o_offset_elems, int64_t do_offset_elems,
+    int64_t stats_offset_elems, int64_t dq_offset_elems, int64_t dk_offset_elems, int64_t dv_offset_elems,
+    int causal, void* stream, void* workspace, size_t workspace_bytes);
+
+/* ------------------------------------------------------------------------
  * A paged cache of keys and values in 8 bits (no counterpart in the reference, which keeps no cache), for bf16 or fp16 activations.
  *
  * A page holds `page` tokens (32 times a power of two), in blocks of 32.  Of a block and key head: 32 x D e4m3 codes of K, a token after the

@@ -86,6 +86,9 @@ SIGNATURES = {
     "mi355_sage_window_bwd_workspace_bytes": (ctypes.c_size_t, [_int] * 9),
     "mi355_sage_sdpa_window_bwd": (_int, [_vp] * 10 + [_int] * 7 + [ctypes.c_float] + [_i64p] * 8 + [_i64] * 9 + [_int] * 3
                                    + [_vp, _int] + [_vp, _vp, ctypes.c_size_t]),
+    "mi355_sage_sdpa_packed": (_int, [_vp] * 8 + [_int] * 7 + [ctypes.c_float] + [_i64p] * 4 + [_i64] * 5 + [_int, _vp]),
+    "mi355_sage_packed_bwd_workspace_bytes": (ctypes.c_size_t, [_int] * 6),
+    "mi355_sage_sdpa_packed_bwd": (_int, [_vp] * 12 + [_int] * 7 + [ctypes.c_float] + [_i64p] * 8 + [_i64] * 9 + [_int, _vp, _vp, ctypes.c_size_t]),
     "mi355_sage_kv_append": (_int, [_vp] * 8 + [_i64, _int, _vp, _i64, _int, _vp, _vp] + [_int] * 6 + [_i64p] * 4 + [_i64] * 4
                              + [_vp, _vp, _int, ctypes.c_float, _vp, _vp, _int, _int, _i64, _i64, _int, _vp]),
     "mi355_sage_paged_workspace_bytes": (ctypes.c_size_t, [_int] * 7),
@@ -106,7 +109,8 @@ BF16, FP16, F32 = 0, 1, 2
 _HOST_ENTRIES = ("workspace_bytes", "bwd_workspace_bytes", "sdpa_bf16", "sdpa_bf16_train_fwd", "sdpa_bf16_keymask", "sdpa_bf16_mask_any",
                  "sdpa_bf16_norm_rope", "sdpa_bf16_norm_rope_train_fwd", "sdpa_bwd_bf16", "sdpa_bwd_f32_grads", "cast", "qk_norm_rope",
                  "qk_norm_rope_bwd_workspace_bytes", "qk_norm_rope_bwd", "window_workspace_bytes", "sdpa_window", "sdpa_window_decode",
-                 "window_bwd_workspace_bytes", "sdpa_window_bwd", "kv_append", "paged_workspace_bytes", "sdpa_paged")
+                 "window_bwd_workspace_bytes", "sdpa_window_bwd", "kv_append", "paged_workspace_bytes", "sdpa_paged",
+                 "sdpa_packed", "packed_bwd_workspace_bytes", "sdpa_packed_bwd")
 
 _lib = None
 _host = None

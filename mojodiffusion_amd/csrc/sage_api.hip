@@ -1278,6 +1278,7 @@ static int window_dims(const char* name, int B, int Hq, int Hk, int N_q, int N_k
     a->right = right < 0 || right > kWindowFar ? kWindowFar : right;
     a->sinks = sinks > N_kv ? N_kv : sinks;
     a->start = q_start;
+    a->stats_n = N_q;
     return 0;
 }
 // The kernels address the rows of a block, and of a key tile, by 32-bit byte offsets from its first.
@@ -1417,6 +1418,112 @@ int mi355_sage_sdpa_window_bwd(const void* Q, const void* K, const void* V, cons
     a.dk = static_cast<uint16_t*>(dK) + dk_off; a.dk_sb = dk_strides[0]; a.dk_sh = dk_strides[1]; a.dk_sn = dk_strides[2];
     a.dv = static_cast<uint16_t*>(dV) + dv_off; a.dv_sb = dv_strides[0]; a.dv_sh = dv_strides[1]; a.dv_sn = dv_strides[2];
     SAGE_HIP(launch_window_bwd(a, st));
+    return MI355_SAGE_OK;
+}
+
+// ---- attention over whole sequences that lie one behind the other ----------------------------------------
+static int packed_dims(const char* name, int B, int Hq, int Hk, int T_q, int T_k, int D, int type, float scale, int causal, PackedArgs* a) {
+    *a = PackedArgs{};
+    if (B <= 0) return MI355_SAGE_EINVAL;
+    if (int rc = window_dims(name, 1, Hq, Hk, T_q, T_k, D, type, scale, -1, causal ? 0 : -1, 0, 0, &a->w)) return rc;
+    a->B = B; a->rows_q = T_q; a->rows_k = T_k;
+    if (B > 1 << 20 || (int64_t)Hq * packed_stats_rows(*a) > 1 << 30) { SAGE_LOG("%s: too many sequences", name); return MI355_SAGE_EUNSUPPORTED; }
+    a->few = packed_few(*a);
+    return 0;
+}
+
+int mi355_sage_sdpa_packed(const void* Q, const void* K, const void* V, void* O, void* O_rest, void* Stats, const void* cu_q, const void* cu_k, int B, int Hq, int Hk, int T_q,
+                           int T_k, int D, int type, float scale, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+                           int64_t q_off, int64_t k_off, int64_t v_off, int64_t o_off, int64_t stats_off, int causal, void* stream) {
+    if (!Q || !K || !V || !O || !cu_q || !cu_k || !q_strides || !k_strides || !v_strides || !o_strides) return MI355_SAGE_EINVAL;
+    PackedArgs a;
+    int rc = packed_dims("packed attention", B, Hq, Hk, T_q, T_k, D, type, scale, causal, &a);
+    if (rc) return rc;
+    WindowArgs& w = a.w;
+    if ((rc = check_view("Q", Q, q_strides, q_off)) || (rc = check_view("K", K, k_strides, k_off)) || (rc = check_view("V", V, v_strides, v_off)) ||
+        (rc = check_view("O", O, o_strides, o_off)) || (O_rest && (rc = check_view("O_rest", O_rest, o_strides, o_off))) || (rc = distinct_rows("O", o_strides, 1, Hq, T_q)) ||
+        (rc = window_span("Q", q_strides, 256 / w.g + 2, w.g, D)) || (rc = window_span("K", k_strides, 64, 1, D)) || (rc = window_span("V", v_strides, 64, 1, D)))
+        return rc;
+    if (!packed_grid_ok(a)) { SAGE_LOG("packed attention: too many workgroups"); return MI355_SAGE_EUNSUPPORTED; }
+    const View q = make_view(Q, q_strides, q_off), k = make_view(K, k_strides, k_off), v = make_view(V, v_strides, v_off);
+    w.q = q.p; w.q_sh = q.sh; w.q_sn = q.sn;
+    w.k = k.p; w.k_sh = k.sh; w.k_sn = k.sn;
+    w.v = v.p; w.v_sh = v.sh; w.v_sn = v.sn;
+    w.o = static_cast<uint16_t*>(O) + o_off; w.o_sh = o_strides[1]; w.o_sn = o_strides[2];
+    w.rest = O_rest ? static_cast<uint16_t*>(O_rest) + o_off : nullptr;
+    w.stats = Stats ? static_cast<float*>(Stats) + stats_off : nullptr;
+    a.cu_q = static_cast<const int32_t*>(cu_q);
+    a.cu_k = static_cast<const int32_t*>(cu_k);
+    SAGE_HIP(launch_packed(a, static_cast<hipStream_t>(stream)));
+    return MI355_SAGE_OK;
+}
+
+static WindowBwdCarve packed_bwd_carve(PackedBwdArgs* a) {
+    packed_bwd_plan(a);
+    a->w.sq_pad = packed_stats_rows(a->p);
+    const size_t rows = (size_t)a->w.w.Hk * a->w.w.g * a->w.sq_pad * sizeof(float);
+    WindowBwdCarve c{};
+    c.delta = align_up(rows);
+    c.size = c.delta + align_up(rows);
+    c.part = c.size + align_up(rows);
+    c.total = c.part + align_up((size_t)packed_bwd_parts(*a) * 2 * kWindowBwdKeys * a->w.w.D * sizeof(float));
+    return c;
+}
+
+size_t mi355_sage_packed_bwd_workspace_bytes(int B, int Hq, int Hk, int T_q, int T_k, int D) {
+    PackedBwdArgs a{};
+    if (packed_dims("packed backward", B, Hq, Hk, T_q, T_k, D, MI355_SAGE_BF16, 1.0f, 1, &a.p) || !bwd_dims_ok(D)) return 0;
+    a.w.w = a.p.w;
+    return packed_bwd_carve(&a).total;
+}
+
+int mi355_sage_sdpa_packed_bwd(const void* Q, const void* K, const void* V, const void* O, const void* O_rest, const void* dO, const void* Stats, void* dQ, void* dK, void* dV,
+                               const void* cu_q, const void* cu_k, int B, int Hq, int Hk, int T_q, int T_k, int D, int type, float scale, const int64_t* q_strides,
+                               const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides, const int64_t* do_strides, const int64_t* dq_strides,
+                               const int64_t* dk_strides, const int64_t* dv_strides, int64_t q_off, int64_t k_off, int64_t v_off, int64_t o_off, int64_t do_off,
+                               int64_t stats_off, int64_t dq_off, int64_t dk_off, int64_t dv_off, int causal, void* stream, void* workspace, size_t workspace_bytes) {
+    if (!Q || !K || !V || !O || !dO || !Stats || !dQ || !dK || !dV || !cu_q || !cu_k) return MI355_SAGE_EINVAL;
+    if (!q_strides || !k_strides || !v_strides || !o_strides || !do_strides || !dq_strides || !dk_strides || !dv_strides) return MI355_SAGE_EINVAL;
+    PackedBwdArgs a{};
+    int rc = packed_dims("packed backward", B, Hq, Hk, T_q, T_k, D, type, scale, causal, &a.p);
+    if (rc) return rc;
+    if (!bwd_dims_ok(D)) { SAGE_LOG("packed backward: head dim %d is not supported (64 or 128)", D); return MI355_SAGE_EUNSUPPORTED; }
+    if ((rc = check_view("Q", Q, q_strides, q_off)) || (rc = check_view("K", K, k_strides, k_off)) || (rc = check_view("V", V, v_strides, v_off)) ||
+        (rc = check_view("O", O, o_strides, o_off)) || (rc = check_view("dO", dO, do_strides, do_off)) || (rc = check_view("dQ", dQ, dq_strides, dq_off)) ||
+        (rc = check_view("dK", dK, dk_strides, dk_off)) || (rc = check_view("dV", dV, dv_strides, dv_off)) ||
+        (O_rest && (rc = check_view("O_rest", O_rest, o_strides, o_off))) || (rc = distinct_rows("dQ", dq_strides, 1, Hq, T_q)) ||
+        (rc = distinct_rows("dK", dk_strides, 1, Hk, T_k)) || (rc = distinct_rows("dV", dv_strides, 1, Hk, T_k)))
+        return rc;
+    WindowArgs& w = a.w.w;
+    w = a.p.w;
+    const int64_t rows = 256 / w.g + 66;
+    if ((rc = window_span("Q", q_strides, rows, w.g, D)) || (rc = window_span("dO", do_strides, rows, w.g, D)) || (rc = window_span("K", k_strides, 128, 1, D)) ||
+        (rc = window_span("V", v_strides, 128, 1, D)))
+        return rc;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    std::lock_guard<std::mutex> together(launch_mutex(st));
+    const WindowBwdCarve c = packed_bwd_carve(&a);
+    if (!packed_bwd_grid_ok(a)) { SAGE_LOG("packed backward: too many workgroups"); return MI355_SAGE_EUNSUPPORTED; }
+    if ((rc = call_workspace("packed backward", c.total, st, &workspace, workspace_bytes))) return rc;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    a.w.lse2 = reinterpret_cast<float*>(ws);
+    a.w.ndelta = reinterpret_cast<float*>(ws + c.delta);
+    a.w.dsize = reinterpret_cast<float*>(ws + c.size);
+    a.w.part = reinterpret_cast<float*>(ws + c.part);
+    const View q = make_view(Q, q_strides, q_off), k = make_view(K, k_strides, k_off), v = make_view(V, v_strides, v_off), d = make_view(dO, do_strides, do_off);
+    w.q = q.p; w.q_sh = q.sh; w.q_sn = q.sn;
+    w.k = k.p; w.k_sh = k.sh; w.k_sn = k.sn;
+    w.v = v.p; w.v_sh = v.sh; w.v_sn = v.sn;
+    w.o = const_cast<uint16_t*>(static_cast<const uint16_t*>(O)) + o_off; w.o_sh = o_strides[1]; w.o_sn = o_strides[2];
+    w.rest = O_rest ? const_cast<uint16_t*>(static_cast<const uint16_t*>(O_rest)) + o_off : nullptr;
+    w.stats = const_cast<float*>(static_cast<const float*>(Stats)) + stats_off;
+    a.w.dout = d.p; a.w.do_sh = d.sh; a.w.do_sn = d.sn;
+    a.w.dq = static_cast<uint16_t*>(dQ) + dq_off; a.w.dq_sh = dq_strides[1]; a.w.dq_sn = dq_strides[2];
+    a.w.dk = static_cast<uint16_t*>(dK) + dk_off; a.w.dk_sh = dk_strides[1]; a.w.dk_sn = dk_strides[2];
+    a.w.dv = static_cast<uint16_t*>(dV) + dv_off; a.w.dv_sh = dv_strides[1]; a.w.dv_sn = dv_strides[2];
+    a.p.cu_q = static_cast<const int32_t*>(cu_q);
+    a.p.cu_k = static_cast<const int32_t*>(cu_k);
+    SAGE_HIP(launch_packed_bwd(a, st));
     return MI355_SAGE_OK;
 }
 

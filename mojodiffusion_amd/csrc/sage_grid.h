@@ -49,4 +49,17 @@ __host__ __device__ inline long long set_grid(long long sets, int members) {
     return (sets + kSetGroup - 1) / kSetGroup * kSetGroup * members;
 }
 
+// `slots` pieces of work of each of `heads` heads, of falling size, in even shares for the XCDs: where the heads do not divide among the 8, those that are shared are dealt out
+// slot by slot (every second, fourth or eighth to one XCD), not in halves of which the first is the heavier.  A slot beyond the last: no work.
+__host__ __device__ inline int spread_ways(int heads) { return (heads & 7) == 0 ? 1 : (heads & 3) == 0 ? 2 : (heads & 1) == 0 ? 4 : 8; }
+__host__ __device__ inline long long spread_grid(long long heads, long long slots) {
+    const int m = spread_ways((int)(heads & 7));
+    return heads * m * ((slots + m - 1) / m);
+}
+struct HeadSlot { int head, slot; };
+__host__ __device__ inline HeadSlot spread_item(int id, int heads, int slots) {
+    const int m = spread_ways(heads), per = (slots + m - 1) / m, item = xcd_item(id, heads * m * per), p = item % (m * per);
+    return HeadSlot{item / (m * per), p % per * m + p / per};
+}
+
 }  // namespace sage

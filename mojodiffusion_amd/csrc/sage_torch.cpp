@@ -45,6 +45,9 @@ struct Api {
     decltype(&mi355_sage_kv_append) kv_append;
     decltype(&mi355_sage_paged_workspace_bytes) paged_workspace_bytes;
     decltype(&mi355_sage_sdpa_paged) paged;
+    decltype(&mi355_sage_sdpa_packed) packed;
+    decltype(&mi355_sage_packed_bwd_workspace_bytes) packed_bwd_workspace_bytes;
+    decltype(&mi355_sage_sdpa_packed_bwd) packed_bwd;
 } api;
 constexpr int kApiEntries = sizeof(Api) / sizeof(void*);
 static_assert(sizeof(Api) == kApiEntries * sizeof(void*), "one pointer per entry");
@@ -743,6 +746,93 @@ PyObject* py_paged(PyObject* const* a, Py_ssize_t n) {
     return THPVariable_Wrap(std::move(o));
 }
 
+// ---- sequences one behind the other (attention_packed.py) -----------------------------------------------
+struct PackedCall {
+    const at::Tensor *q, *k, *v, *cu, *cu_k;
+    double scale;
+    int causal, type, B;
+};
+// a: q, k, v, cu_seqlens, cu_seqlens_k (None: the same), scale, causal
+bool packed_args(PyObject* const* a, PyObject* cu, PyObject* cu_k, PyObject* scale, PyObject* causal, PackedCall& c) {
+    if (!tensor_arg(a[0], c.q) || !tensor_arg(a[1], c.k) || !tensor_arg(a[2], c.v) || !tensor_arg(cu, c.cu) || !double_arg(scale, c.scale) || (causal != Py_True && causal != Py_False))
+        return false;
+    c.cu_k = c.cu;
+    if (cu_k != Py_None && !tensor_arg(cu_k, c.cu_k)) return false;
+    c.causal = causal == Py_True;
+    const at::Tensor &q = *c.q, &k = *c.k, &v = *c.v;
+    if (!dense_tokens(q, 3) || !dense_tokens(k, 3) || !dense_tokens(v, 3) || k.sizes() != v.sizes() || q.device() != k.device() || q.device() != v.device()) return false;
+    c.type = element_type(q.scalar_type());
+    if ((c.type != MI355_SAGE_BF16 && c.type != MI355_SAGE_FP16) || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) return false;
+    if (q.numel() == 0 || k.numel() == 0 || q.size(2) != k.size(2) || q.size(1) % k.size(1) || (cu_k == Py_None && q.size(0) != k.size(0))) return false;
+    if (!fits(q.size(0)) || !fits(k.size(0)) || !fits(q.size(1)) || q.size(2) > 256) return false;
+    for (const at::Tensor* t : {c.cu, c.cu_k})
+        if (t->dim() != 1 || t->size(0) < 2 || t->size(0) != c.cu->size(0) || t->scalar_type() != at::kInt || !t->is_contiguous() || t->device() != q.device()) return false;
+    c.B = c.cu->size(0) - 1;
+    return true;
+}
+
+// packed(q, k, v, cu_seqlens, cu_seqlens_k, scale, causal, training) -> o, (o, rest, stats) with training, or None
+PyObject* py_packed(PyObject* const* a, Py_ssize_t n) {
+    PackedCall c;
+    int training;
+    if (intercepted() || n != 8 || !packed_args(a, a[3], a[4], a[5], a[6], c) || !int_arg(a[7], training)) Py_RETURN_NONE;
+    at::Tensor o, rest, stats;
+    const int rc = without_gil([&] {
+        const at::Tensor &q = *c.q, &k = *c.k, &v = *c.v;
+        const c10::DeviceGuard guard(q.device());
+        o = fresh(q.sizes(), q, q.scalar_type());
+        if (training) {
+            rest = fresh(q.sizes(), q, q.scalar_type());
+            stats = fresh({q.size(1), q.size(0)}, q, at::kFloat);
+        }
+        const Strides qs = token_strides(q), ks = token_strides(k), vs = token_strides(v), os = token_strides(o);
+        return api.packed(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), training ? rest.data_ptr() : nullptr, training ? stats.data_ptr() : nullptr, c.cu->data_ptr(),
+                          c.cu_k->data_ptr(), c.B, q.size(1), k.size(1), q.size(0), k.size(0), q.size(2), c.type, (float)c.scale, qs.s, ks.s, vs.s, os.s, 0, 0, 0, 0, 0, c.causal,
+                          stream_of(q));
+    });
+    if (rc != 0) Py_RETURN_NONE;
+    if (!training) return THPVariable_Wrap(std::move(o));
+    PyObject* t = PyTuple_New(3);
+    PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(std::move(o)));
+    PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(std::move(rest)));
+    PyTuple_SET_ITEM(t, 2, THPVariable_Wrap(std::move(stats)));
+    return t;
+}
+
+// packed_bwd(q, k, v, o, rest, d_out, stats, cu_seqlens, cu_seqlens_k, scale, causal) -> (d_q, d_k, d_v) or None
+PyObject* py_packed_bwd(PyObject* const* a, Py_ssize_t n) {
+    PackedCall c;
+    const at::Tensor *o, *rest, *d, *stats;
+    if (intercepted() || n != 11 || !packed_args(a, a[7], a[8], a[9], a[10], c) || !tensor_arg(a[3], o) || !tensor_arg(a[4], rest) || !tensor_arg(a[5], d) || !tensor_arg(a[6], stats))
+        Py_RETURN_NONE;
+    const at::Tensor& q = *c.q;
+    for (const at::Tensor* t : {o, rest, d})
+        if (!dense_tokens(*t, 3) || t->sizes() != q.sizes() || t->scalar_type() != q.scalar_type() || t->device() != q.device()) Py_RETURN_NONE;
+    if (o->strides() != rest->strides() || stats->scalar_type() != at::kFloat || stats->device() != q.device() || !stats->is_contiguous() ||
+        stats->numel() != q.size(0) * q.size(1))
+        Py_RETURN_NONE;
+    at::Tensor g[3];
+    const int rc = without_gil([&] {
+        const at::Tensor &k = *c.k, &v = *c.v;
+        const size_t need = api.packed_bwd_workspace_bytes(c.B, q.size(1), k.size(1), q.size(0), k.size(0), q.size(2));
+        if (need == 0) return MI355_SAGE_EUNSUPPORTED;
+        const c10::DeviceGuard guard(q.device());
+        g[0] = fresh(q.sizes(), q, q.scalar_type());
+        g[1] = fresh(k.sizes(), q, q.scalar_type());
+        g[2] = fresh(v.sizes(), q, q.scalar_type());
+        const at::Tensor ws = fresh({(int64_t)need}, q, at::kByte);
+        const Strides qs = token_strides(q), ks = token_strides(k), vs = token_strides(v), os = token_strides(*o), ds = token_strides(*d), dqs = token_strides(g[0]),
+                      dks = token_strides(g[1]), dvs = token_strides(g[2]);
+        return api.packed_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o->data_ptr(), rest->data_ptr(), d->data_ptr(), stats->data_ptr(), g[0].data_ptr(), g[1].data_ptr(),
+                              g[2].data_ptr(), c.cu->data_ptr(), c.cu_k->data_ptr(), c.B, q.size(1), k.size(1), q.size(0), k.size(0), q.size(2), c.type, (float)c.scale, qs.s, ks.s,
+                              vs.s, os.s, ds.s, dqs.s, dks.s, dvs.s, 0, 0, 0, 0, 0, 0, 0, 0, 0, c.causal, stream_of(q), ws.data_ptr(), need);
+    });
+    if (rc != 0) Py_RETURN_NONE;
+    PyObject* t = PyTuple_New(3);
+    for (int i = 0; i < 3; i++) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(std::move(g[i])));
+    return t;
+}
+
 // workspace(nbytes, tensor) -> this (device, stream)'s buffer
 PyObject* py_workspace(PyObject* const* a, Py_ssize_t n) {
     if (n != 2 || !PyLong_Check(a[0]) || !THPVariable_Check(a[1])) {
@@ -775,7 +865,7 @@ PyObject* py_bind(PyObject* const* a, Py_ssize_t n) {
 
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(entry<py_##name>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(fwd), METHOD(bias), METHOD(norm_rope), METHOD(bwd), METHOD(record), METHOD(workspace), METHOD(bind),
-                         METHOD(rope), METHOD(rope_bwd), METHOD(window), METHOD(window_decode), METHOD(window_bwd), METHOD(kv_append), METHOD(paged),
+                         METHOD(rope), METHOD(rope_bwd), METHOD(window), METHOD(window_decode), METHOD(window_bwd), METHOD(kv_append), METHOD(paged), METHOD(packed), METHOD(packed_bwd),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_sage_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -50,7 +50,8 @@ struct WindowArgs {
     const int32_t *lens, *starts;                // [B] on the device, or null
     int start, at_end;
     float scale;                                 // > 0
-    float* stats;                                // [B, Hk * g, Sq] natural log-sum-exp, or null
+    float* stats;                                // [B, Hk * g, stats_n] natural log-sum-exp of the Sq rows, or null
+    int stats_n;
     // keys split over workgroups: unnormalised partial rows, their references and sums
     int splits;
     float *part, *part_ml;                       // [row block, split, 32, D], [row block, split, 32, 2]
@@ -82,5 +83,28 @@ void window_bwd_plan(WindowBwdArgs* a);          // fills in the five above from
 constexpr int kWindowBwdKeys = 64;               // keys of a workgroup
 int64_t window_bwd_parts(const WindowBwdArgs& a);        // workgroups that leave parts
 hipError_t launch_window_bwd(const WindowBwdArgs& a, hipStream_t st);
+
+// ---- attention over whole sequences that lie one behind the other -------------------------------------
+// Sequence b: rows cu_q[b] .. cu_q[b + 1] - 1 of Q and O, rows cu_k[b] .. cu_k[b + 1] - 1 of K and V; its queries are the last of its positions.  Rows behind the last
+// sequence: zeros.  w: of all rows, as one sequence (B 1, lens and starts null, left, right, sinks as they are to be).
+struct PackedArgs {
+    WindowArgs w;
+    const int32_t *cu_q, *cu_k;                  // [B + 1]
+    int B, rows_q, rows_k;
+    int few;                                     // rows of a workgroup: 0: 128, their key tiles shared by its waves; 1: 32, its waves taking key tiles in turn
+};
+bool packed_few(const PackedArgs& a);
+bool packed_grid_ok(const PackedArgs& a);
+hipError_t launch_packed(const PackedArgs& a, hipStream_t st);
+struct PackedBwdArgs {
+    PackedArgs p;                                // p.w: not used; the rest as the forward's
+    WindowBwdArgs w;                             // lse2, ndelta, dsize [Hk * g, sq_pad]: sequence b's rows from (cu_q[b] / 32 + b) * 32 on
+    int chunks;                                  // workgroups that the (head, query tile) pairs of a key block are dealt to; several: parts
+};
+int packed_stats_rows(const PackedArgs& a);      // sq_pad
+void packed_bwd_plan(PackedBwdArgs* a);
+int64_t packed_bwd_parts(const PackedBwdArgs& a);
+bool packed_bwd_grid_ok(const PackedBwdArgs& a);
+hipError_t launch_packed_bwd(const PackedBwdArgs& a, hipStream_t st);
 
 }  // namespace sage

@@ -114,7 +114,7 @@ __device__ __forceinline__ void finish_rows(const WindowArgs& a, const RowState<
     for (int d = 0; d < D / 32; d++) row_put<T, D>(os, st.acc[d], d, inv, lane);
     if (a.stats != nullptr && lane < 32 && x < rows) {
         const int i = x / a.g;
-        a.stats[((int64_t)b * a.Hk * a.g + kvh * a.g + (x - i * a.g)) * a.Sq + i] = sum == 0.0f ? -INFINITY : (st.ref + __builtin_amdgcn_logf(sum)) * kLn2;
+        a.stats[((int64_t)b * a.Hk * a.g + kvh * a.g + (x - i * a.g)) * a.stats_n + i] = sum == 0.0f ? -INFINITY : (st.ref + __builtin_amdgcn_logf(sum)) * kLn2;
     }
     const int64_t at = b * a.o_sb + (int64_t)kvh * a.g * a.o_sh;
     query_rows_out<D>(a, os, a.o + at, a.o_sn, a.o_sh, x0, lane);
@@ -136,15 +136,10 @@ template <int D> struct WindowLds {
 // workgroups on the same SIMD, which meet no common barrier with it: five at 64 channels, three at 128, two at 256 (by registers: O, Q and one
 // tile's scores are 64, 112, 208 of them).  The next tile's scores taken beside this one's weights, with a wave less, was slower: [1,16896,48 on 12,128]
 // window 4096 + 4 1615 us, this form 1553; a training step of [2,1248,30,128] +-256 180, 175.  Two waves of this form at 128 channels: 1950.
-template <int T, int D>
-__global__ __launch_bounds__(256, D == 64 ? 5 : D == 128 ? 3 : 2) void window_kernel(WindowArgs a) {
+template <int T, int D> __device__ __forceinline__ void window_body(const WindowArgs& a, uint8_t* smem, int b, int kvh, int row0) {
     using L = WindowLds<D>;
     constexpr int NW = L::NW, KT = L::KT, KS = D / 16;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
-    const int rows = a.Sq * a.g, blocks = (rows + NW * 32 - 1) / (NW * 32);
-    const int item = xcd_item((int)blockIdx.x, a.B * a.Hk * blocks);
-    const int bh = item / blocks, row0 = (blocks - 1 - item % blocks) * NW * 32;       // (the last rows first: without a left edge they see most keys)
-    const int b = bh / a.Hk, kvh = bh % a.Hk;
+    const int rows = a.Sq * a.g;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int x0 = row0 + wave * 32;
@@ -199,6 +194,15 @@ __global__ __launch_bounds__(256, D == 64 ? 5 : D == 128 ? 3 : 2) void window_ke
     __syncthreads();                     // (no copy is in flight: the last step's wait was for all of them)
     if (x0 < rows) finish_rows<T, D>(a, st, smem + wave * 64 * D, b, kvh, x0, lane);
 }
+constexpr int kWindowWaves(int D) { return D == 64 ? 5 : D == 128 ? 3 : 2; }
+template <int T, int D> __global__ __launch_bounds__(256, kWindowWaves(D)) void window_kernel(WindowArgs a) {
+    using L = WindowLds<D>;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
+    const int rows = a.Sq * a.g, blocks = (rows + L::NW * 32 - 1) / (L::NW * 32);
+    const int item = xcd_item((int)blockIdx.x, a.B * a.Hk * blocks);
+    const int bh = item / blocks;
+    window_body<T, D>(a, smem, bh / a.Hk, bh % a.Hk, (blocks - 1 - item % blocks) * L::NW * 32);       // (the last rows first: without a left edge they see most keys)
+}
 
 // N neighbouring channels of a finished row, and what rounding left of them.
 template <int T, int N> __device__ __forceinline__ void store_row(const WindowArgs& a, int64_t at, const float (&y)[N]) {
@@ -230,15 +234,10 @@ template <int D> struct SplitLds {
 };
 
 template <int T, int D>
-__global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
+__device__ __forceinline__ void split_body(const WindowArgs& a, uint8_t* smem, float (&meet_ml)[SplitLds<D>::NW][32][2], int b, int kvh, int x0, int item, int split) {
     using L = SplitLds<D>;
     constexpr int NW = L::NW, KT = L::KT, CPR = D / 8, RUNS = L::TILE / 1024, KS = D / 16, DB = D / 32;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
-    __shared__ float meet_ml[NW][32][2];
-    const int rows = a.Sq * a.g, blocks = (rows + 31) / 32;
-    const int split = (int)blockIdx.x % a.splits, item = (int)blockIdx.x / a.splits;
-    const int bh = item / blocks, x0 = item % blocks * 32;
-    const int b = bh / a.Hk, kvh = bh % a.Hk;
+    const int rows = a.Sq * a.g;
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l32 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
@@ -368,9 +367,19 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
             float* ml = a.part_ml + (((int64_t)item * a.splits + split) * 32 + r) * 2;
             ml[0] = ref, ml[1] = sum;
         } else if (a.stats != nullptr) {
-            a.stats[((int64_t)b * a.Hk * a.g + kvh * a.g + hg) * a.Sq + i] = sum == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(sum)) * kLn2;
+            a.stats[((int64_t)b * a.Hk * a.g + kvh * a.g + hg) * a.stats_n + i] = sum == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(sum)) * kLn2;
         }
     }
+}
+
+template <int T, int D> __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
+    using L = SplitLds<D>;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
+    __shared__ float meet_ml[L::NW][32][2];
+    const int blocks = (a.Sq * a.g + 31) / 32;
+    const int split = (int)blockIdx.x % a.splits, item = (int)blockIdx.x / a.splits;
+    const int bh = item / blocks;
+    split_body<T, D>(a, smem, meet_ml, bh / a.Hk, bh % a.Hk, item % blocks * 32, item, split);
 }
 
 // 64 lanes of D / 64 channels each to a row; WAVES of them share a row's parts and meet in LDS: four where there are more than eight parts, one else.
@@ -451,7 +460,50 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
     for (int e = 0; e < N; e++) y[e] *= inv;
     store_row<T, N>(a, b * a.o_sb + ((int64_t)kvh * a.g + hg) * a.o_sh + i * a.o_sn + lane * N, y);
     if (a.stats != nullptr && lane == 0)
-        a.stats[((int64_t)b * a.Hk * a.g + kvh * a.g + hg) * a.Sq + i] = sum == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(sum)) * kLn2;
+        a.stats[((int64_t)b * a.Hk * a.g + kvh * a.g + hg) * a.stats_n + i] = sum == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// ---- sequences one behind the other ----------------------------------------------------------------------
+// The same workgroups, each on the rows of one sequence: a slot of the grid names its sequence and its rows in it.  The last rows first, as above.
+template <int T, int D> __global__ __launch_bounds__(256, kWindowWaves(D)) void packed_kernel(PackedArgs a, int slots) {
+    using L = WindowLds<D>;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
+    const HeadSlot at = spread_item((int)blockIdx.x, a.w.Hk, slots);
+    if (at.slot >= slots) return;
+    const int slot = slots - 1 - at.slot;
+    const Slots rows = {a.cu_q, a.rows_q, a.w.g, L::NW * 32};
+    const int b = rows.owner(slot, a.B), row0 = (slot - rows.first(b)) * L::NW * 32;
+    const Sequence s = sequence(a, b);
+    if (row0 >= s.nq * a.w.g) return;
+    window_body<T, D>(view(a.w, s, s.nq, b < a.B ? s.nk : 0), smem, 0, at.head, row0);
+}
+template <int T, int D> __global__ __launch_bounds__(256) void packed_few_kernel(PackedArgs a, int slots) {
+    using L = SplitLds<D>;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
+    __shared__ float meet_ml[L::NW][32][2];
+    const HeadSlot at = spread_item((int)blockIdx.x, a.w.Hk, slots);
+    if (at.slot >= slots) return;
+    const int slot = slots - 1 - at.slot;
+    const Slots rows = {a.cu_q, a.rows_q, a.w.g, 32};
+    const int b = rows.owner(slot, a.B), x0 = (slot - rows.first(b)) * 32;
+    const Sequence s = sequence(a, b);
+    if (x0 >= s.nq * a.w.g) return;
+    WindowArgs w = view(a.w, s, s.nq, b < a.B ? s.nk : 0);
+    w.splits = 1;
+    split_body<T, D>(w, smem, meet_ml, 0, at.head, x0, 0, 0);
+}
+int64_t packed_slots(const PackedArgs& a, int rows) { return slots_total(a.rows_q, a.w.g, rows, a.B); }
+template <int T, int D> hipError_t launch_packed_td(const PackedArgs& a, hipStream_t st) {
+    const int64_t slots = packed_slots(a, a.few ? 32 : 128);
+    const dim3 grid((unsigned)spread_grid(a.w.Hk, slots));
+    if (a.few) hipLaunchKernelGGL((packed_few_kernel<T, D>), grid, dim3(256), 0, st, a, (int)slots);
+    else hipLaunchKernelGGL((packed_kernel<T, D>), grid, dim3(256), 0, st, a, (int)slots);
+    return hipGetLastError();
+}
+template <int T> hipError_t launch_packed_t(const PackedArgs& a, hipStream_t st) {
+    if (a.w.D == 64) return launch_packed_td<T, 64>(a, st);
+    if (a.w.D == 128) return launch_packed_td<T, 128>(a, st);
+    return launch_packed_td<T, 256>(a, st);
 }
 
 int64_t row_blocks(const WindowArgs& a, int rows) { return (int64_t)a.B * a.Hk * (((int64_t)a.Sq * a.g + rows - 1) / rows); }
@@ -511,5 +563,10 @@ size_t window_part_bytes(const WindowArgs& a, const WindowPlan& p) {
 hipError_t launch_window(const WindowArgs& a, const WindowPlan& p, hipStream_t st) {
     return a.type == kBF16 ? launch_t<kBF16>(a, p, st) : launch_t<kF16>(a, p, st);
 }
+
+// (as window_plan: workgroups of 128 rows for half the chip)
+bool packed_few(const PackedArgs& a) { return (int64_t)a.rows_q * a.w.g / 128 * a.w.Hk < 128; }
+bool packed_grid_ok(const PackedArgs& a) { return spread_grid(a.w.Hk, packed_slots(a, a.few ? 32 : 128)) <= 0x7FFFFFFF; }
+hipError_t launch_packed(const PackedArgs& a, hipStream_t st) { return a.w.type == kBF16 ? launch_packed_t<kBF16>(a, st) : launch_packed_t<kF16>(a, st); }
 
 }  // namespace sage

@@ -38,13 +38,10 @@ template <int T> __device__ __forceinline__ float widen(uint32_t w, int i) {
     else return (float)__builtin_bit_cast(v2hf, w)[i];
 }
 
-template <int T, int D>
-__global__ __launch_bounds__(256) void window_bwd_prep_kernel(WindowBwdArgs a) {
-    constexpr int CPR = D / 8, RPP = 256 / CPR;      // threads per row, rows per workgroup
-    const int H = a.w.Hk * a.w.g;
-    const int64_t row = (int64_t)blockIdx.x * RPP + threadIdx.x / CPR;                // over [B, H, sq_pad]
-    if (row >= (int64_t)a.w.B * H * a.sq_pad) return;
-    const int i = (int)(row % a.sq_pad), bh = (int)(row / a.sq_pad), b = bh / H, h = bh % H, col = (int)(threadIdx.x % CPR) * 8;
+// Row i of head bh, CPR threads to it; `at`: its place in the workspace.
+template <int T, int D> __device__ __forceinline__ void prep_row(const WindowBwdArgs& a, int bh, int i, int64_t at_row) {
+    constexpr int CPR = D / 8;
+    const int H = a.w.Hk * a.w.g, b = bh / H, h = bh % H, col = (int)(threadIdx.x % CPR) * 8;
     const int len = sequence_len(a.w, b);
     const bool real = seeing(a.w, first_position(a.w, b, len), len).has(i);           // (rows that see nothing are not read: they may hold anything)
     float sum = 0.0f, size = 0.0f;
@@ -66,11 +63,19 @@ __global__ __launch_bounds__(256) void window_bwd_prep_kernel(WindowBwdArgs a) {
         if constexpr (T == kF16) size += __shfl_xor(size, m);
     }
     if (col == 0) {
-        const float l = real ? a.w.stats[(int64_t)bh * a.w.Sq + i] : -INFINITY;
-        a.ndelta[row] = real ? -sum : 0.0f;
-        if constexpr (T == kF16) a.dsize[row] = size;
-        a.lse2[row] = l == -INFINITY ? INFINITY : fmaf(l, kLog2e, -kWeightBits);           // (nothing seen: every probability vanishes)
+        const float l = real ? a.w.stats[(int64_t)bh * a.w.stats_n + i] : -INFINITY;
+        a.ndelta[at_row] = real ? -sum : 0.0f;
+        if constexpr (T == kF16) a.dsize[at_row] = size;
+        a.lse2[at_row] = l == -INFINITY ? INFINITY : fmaf(l, kLog2e, -kWeightBits);           // (nothing seen: every probability vanishes)
     }
+}
+
+template <int T, int D>
+__global__ __launch_bounds__(256) void window_bwd_prep_kernel(WindowBwdArgs a) {
+    constexpr int CPR = D / 8, RPP = 256 / CPR;      // threads per row, rows per workgroup
+    const int64_t row = (int64_t)blockIdx.x * RPP + threadIdx.x / CPR;                // over [B, H, sq_pad]
+    if (row >= (int64_t)a.w.B * a.w.Hk * a.w.g * a.sq_pad) return;
+    prep_row<T, D>(a, (int)(row / a.sq_pad), (int)(row % a.sq_pad), row);
 }
 
 // Both passes walk tiles of 32 rows, one after the other, and scores of pairs that do not see each other start, and stay, at -inf.  What hides the
@@ -660,6 +665,115 @@ __global__ __launch_bounds__(256) void window_bwd_join_kernel(WindowBwdArgs a) {
     *reinterpret_cast<u32x4*>(out + col) = u32x4{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7])};
 }
 
+// ---- sequences one behind the other ----------------------------------------------------------------------
+__device__ __forceinline__ WindowBwdArgs view(const PackedBwdArgs& all, const Sequence& s, int nq, int nk, int b) {
+    WindowBwdArgs a = all.w;
+    a.w = view(all.w.w, s, nq, nk);
+    a.dout += s.q0 * a.do_sn;
+    a.dq += s.q0 * a.dq_sn;
+    a.dk += s.k0 * a.dk_sn;
+    a.dv += s.k0 * a.dv_sn;
+    const int row = (s.q0 / 32 + b) * 32;
+    a.lse2 += row;
+    a.ndelta += row;
+    a.dsize += row;
+    return a;
+}
+template <int T, int D> __global__ __launch_bounds__(256) void packed_bwd_prep_kernel(PackedBwdArgs a) {
+    constexpr int CPR = D / 8, RPP = 256 / CPR;
+    const int64_t row = (int64_t)blockIdx.x * RPP + threadIdx.x / CPR;                // over [H, sq_pad]
+    if (row >= (int64_t)a.w.w.Hk * a.w.w.g * a.w.sq_pad) return;
+    const int h = (int)(row / a.w.sq_pad), y = (int)(row % a.w.sq_pad);
+    const Slots tiles = {a.p.cu_q, a.p.rows_q, 1, 32};
+    const int b = tiles.owner(y / 32, a.p.B), i = y - tiles.first(b) * 32;
+    const Sequence s = sequence(a.p, b);
+    prep_row<T, D>(view(a, s, s.nq, b < a.p.B ? s.nk : 0, b), h, i, (int64_t)h * a.w.sq_pad + i);
+}
+template <int T, int D>
+__global__ __launch_bounds__(kWaves * 64, D > 64 ? 2 : 4) void packed_bwd_kernel(PackedBwdArgs a, int q_slots, int k_slots) {
+    constexpr int KV = PairLds<T, D>::BYTES;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[KV > DqLds<D>::BYTES ? KV : DqLds<D>::BYTES];
+    const int nq = (int)spread_grid(a.w.w.Hk, q_slots), id = (int)blockIdx.x;
+    if (id < nq) {
+        const HeadSlot at = spread_item(id, a.w.w.Hk, q_slots);
+        if (at.slot >= q_slots) return;
+        const int slot = q_slots - 1 - at.slot;          // (the last rows first: they see most keys)
+        const Slots rows = {a.p.cu_q, a.p.rows_q, a.w.w.g, kRowsWg};
+        const int b = rows.owner(slot, a.p.B), row0 = (slot - rows.first(b)) * kRowsWg;
+        const Sequence s = sequence(a.p, b);
+        if (row0 >= s.nq * a.w.w.g) return;
+        dq_body<T, D>(view(a, s, s.nq, b < a.p.B ? s.nk : 0, b), smem, at.head, row0);
+        return;
+    }
+    const HeadSlot at = spread_item(id - nq, a.w.w.Hk, k_slots * a.chunks);
+    if (at.slot >= k_slots * a.chunks) return;
+    const int slot = at.slot / a.chunks, chunk = at.slot - slot * a.chunks;
+    const Slots blocks = {a.p.cu_k, a.p.rows_k, 1, kKeysWg};
+    const int b = blocks.owner(slot, a.p.B), k0 = (slot - blocks.first(b)) * kKeysWg;
+    const Sequence s = sequence(a.p, b);
+    if (k0 >= s.nk) return;
+    const WindowBwdArgs v = view(a, s, b < a.p.B ? s.nq : 0, s.nk, b);
+    const QuerySpan qs = query_span(v.w, k0, kKeysWg, v.w.start, s.nk);
+    KeyWork work;
+    work.k0 = k0;
+    work.count = (qs.nt * v.w.g + a.chunks - 1) / a.chunks;
+    work.first = chunk * work.count;
+    work.part = a.chunks > 1 ? ((int64_t)at.head * k_slots + slot) * a.chunks + chunk : -1;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    if (wave < 2) dkdv_role<T, D, 0>(v, smem, at.head, work, wave, lane);
+    else dkdv_role<T, D, 1>(v, smem, at.head, work, wave, lane);
+}
+// Their parts added up, in order, as above.
+template <int T, int D> __global__ __launch_bounds__(256) void packed_bwd_join_kernel(PackedBwdArgs a, int k_slots) {
+    constexpr int CPR = D / 8;
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= (int64_t)a.w.w.Hk * k_slots * 2 * kKeysWg * CPR) return;
+    const int col = (int)(at % CPR) * 8, key = (int)(at / CPR % kKeysWg), which = (int)(at / (CPR * kKeysWg) & 1);
+    const int item = (int)(at / (2 * CPR * kKeysWg)), kvh = item / k_slots, slot = item - kvh * k_slots;
+    const Slots blocks = {a.p.cu_k, a.p.rows_k, 1, kKeysWg};
+    const int b = blocks.owner(slot, a.p.B), j = (slot - blocks.first(b)) * kKeysWg + key;
+    const Sequence s = sequence(a.p, b);
+    if (j >= s.nk) return;
+    const float* p = a.w.part + (((int64_t)item * a.chunks * 2 + which) * kKeysWg + key) * D + col;
+    float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int c0 = 0; c0 < a.chunks; c0 += 8) {
+        v4f u[8], v[8];
+#pragma unroll
+        for (int n = 0; n < 8; n++) {
+            const float* at_c = p + (int64_t)min(c0 + n, a.chunks - 1) * 2 * kKeysWg * D;
+            u[n] = *reinterpret_cast<const v4f*>(at_c);
+            v[n] = *reinterpret_cast<const v4f*>(at_c + 4);
+        }
+#pragma unroll
+        for (int n = 0; n < 8; n++) {
+            if (c0 + n >= a.chunks) break;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] += u[n][e], y[4 + e] += v[n][e];
+        }
+    }
+    const int64_t row = s.k0 + j;
+    uint16_t* out = which ? a.w.dv + kvh * a.w.dv_sh + row * a.w.dv_sn : a.w.dk + kvh * a.w.dk_sh + row * a.w.dk_sn;
+    *reinterpret_cast<u32x4*>(out + col) = u32x4{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7])};
+}
+struct PackedGrid { int64_t q_slots, k_slots, prep, grid, join; };
+PackedGrid packed_grid(const PackedBwdArgs& a) {
+    const int64_t Hk = a.w.w.Hk, D = a.w.w.D;
+    PackedGrid g;
+    g.q_slots = slots_total(a.p.rows_q, a.w.w.g, kRowsWg, a.p.B);
+    g.k_slots = slots_total(a.p.rows_k, 1, kKeysWg, a.p.B);
+    g.prep = (Hk * a.w.w.g * packed_stats_rows(a.p) * (D / 8) + 255) / 256;
+    g.grid = spread_grid(Hk, g.q_slots) + spread_grid(Hk, g.k_slots * a.chunks);
+    g.join = a.chunks > 1 ? (Hk * g.k_slots * 2 * kKeysWg * (D / 8) + 255) / 256 : 0;
+    return g;
+}
+template <int T, int D> hipError_t launch_packed_td(const PackedBwdArgs& a, hipStream_t st) {
+    const PackedGrid g = packed_grid(a);
+    hipLaunchKernelGGL((packed_bwd_prep_kernel<T, D>), dim3((unsigned)g.prep), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((packed_bwd_kernel<T, D>), dim3((unsigned)g.grid), dim3(kWaves * 64), 0, st, a, (int)g.q_slots, (int)g.k_slots);
+    if (g.join > 0) hipLaunchKernelGGL((packed_bwd_join_kernel<T, D>), dim3((unsigned)g.join), dim3(256), 0, st, a, (int)g.k_slots);
+    return hipGetLastError();
+}
+
 template <int T, int D> hipError_t launch_td(const WindowBwdArgs& a, hipStream_t st) {
     const int64_t heads = (int64_t)a.w.B * a.w.Hk, rows = (int64_t)a.w.Sq * a.w.g, blocks = (a.w.Skv + kKeysWg - 1) / kKeysWg;
     const int64_t prep = (heads * a.w.g * a.sq_pad * (D / 8) + 255) / 256;
@@ -707,6 +821,23 @@ int64_t window_bwd_parts(const WindowBwdArgs& a) {
 hipError_t launch_window_bwd(const WindowBwdArgs& a, hipStream_t st) {
     if (a.w.D == 64) return a.w.type == kBF16 ? launch_td<kBF16, 64>(a, st) : launch_td<kF16, 64>(a, st);
     return a.w.type == kBF16 ? launch_td<kBF16, 128>(a, st) : launch_td<kF16, 128>(a, st);
+}
+
+int packed_stats_rows(const PackedArgs& a) { return (int)slots_total(a.rows_q, 1, 32, a.B) * 32; }
+// Few key blocks: their pairs dealt to several workgroups until there are four to a compute unit, down to 16 pairs of the average.
+void packed_bwd_plan(PackedBwdArgs* a) {
+    const int64_t blocks = (a->p.rows_k + kWindowBwdKeys - 1) / kWindowBwdKeys, heads = a->w.w.Hk;
+    const int64_t pairs = (a->p.rows_q / std::max(a->p.B, 1) + 31) / 32 * a->w.w.g;
+    a->chunks = (int)std::max<int64_t>(1, std::min(1024 / (blocks * heads), pairs / 16));
+}
+int64_t packed_bwd_parts(const PackedBwdArgs& a) { return a.chunks > 1 ? (int64_t)a.w.w.Hk * slots_total(a.p.rows_k, 1, kWindowBwdKeys, a.p.B) * a.chunks : 0; }
+bool packed_bwd_grid_ok(const PackedBwdArgs& a) {
+    const PackedGrid g = packed_grid(a);
+    return g.prep <= 0x7FFFFFFF && g.grid <= 0x7FFFFFFF && g.join <= 0x7FFFFFFF;
+}
+hipError_t launch_packed_bwd(const PackedBwdArgs& a, hipStream_t st) {
+    if (a.w.w.D == 64) return a.w.w.type == kBF16 ? launch_packed_td<kBF16, 64>(a, st) : launch_packed_td<kF16, 64>(a, st);
+    return a.w.w.type == kBF16 ? launch_packed_td<kBF16, 128>(a, st) : launch_packed_td<kF16, 128>(a, st);
 }
 
 }  // namespace sage

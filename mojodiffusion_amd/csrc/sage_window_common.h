@@ -229,6 +229,53 @@ template <int T, int D, bool REST = false> __device__ __forceinline__ void row_p
     }
 }
 
+// ---- sequences one behind the other ----------------------------------------------------------------------
+// Sequence b's rows, b = B: those behind the last sequence (queries without keys, keys without queries).
+struct Sequence { int q0, nq, k0, nk; };
+__device__ __forceinline__ int sequence_start(const int32_t* cu, int b, int rows) { return b == 0 ? 0 : max(0, min(cu[b], rows)); }
+__device__ __forceinline__ Sequence sequence(const PackedArgs& a, int b) {
+    Sequence s;
+    s.q0 = sequence_start(a.cu_q, b, a.rows_q);
+    s.k0 = sequence_start(a.cu_k, b, a.rows_k);
+    s.nq = b < a.B ? max(0, min(a.cu_q[b + 1], a.rows_q) - s.q0) : a.rows_q - s.q0;
+    s.nk = b < a.B ? max(0, min(a.cu_k[b + 1], a.rows_k) - s.k0) : a.rows_k - s.k0;
+    return s;
+}
+// Its rows as a batch of one; where sides are asked for behind the last sequence, the other one is empty.
+__device__ __forceinline__ WindowArgs view(const WindowArgs& all, const Sequence& s, int nq, int nk) {
+    WindowArgs w = all;
+    w.B = 1;
+    w.q += s.q0 * w.q_sn;
+    w.k += s.k0 * w.k_sn;
+    w.v += s.k0 * w.v_sn;
+    w.o += s.q0 * w.o_sn;
+    if (w.rest != nullptr) w.rest += s.q0 * w.o_sn;
+    if (w.stats != nullptr) w.stats += s.q0;
+    w.Sq = nq;
+    w.Skv = nk;
+    w.lens = w.starts = nullptr;
+    w.at_end = 0;
+    w.start = nk - nq;
+    return w;
+}
+// Slots of `rows` rows for a sequence's n: from cu[b] * per / rows + b on, which leaves n * per / rows + 1 at the least, so that a slot names its sequence without a
+// sum over those before it.  With slots for the rows behind the last there are total(..).
+struct Slots {
+    const int32_t* cu;
+    int rows_all, per, rows;
+    __device__ int first(int b) const { return (int)((uint32_t)sequence_start(cu, b, rows_all) * (uint32_t)per / (uint32_t)rows) + b; }
+    __device__ int owner(int slot, int B) const {
+        int lo = 0, hi = B + 1;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first(mid) <= slot) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    }
+};
+__host__ __device__ inline int64_t slots_total(int64_t rows_all, int64_t per, int64_t rows, int64_t B) { return rows_all * per / rows + B + 1; }
+
 }  // namespace
 
 }  // namespace sage
