@@ -64,57 +64,68 @@ __device__ __forceinline__ int cached(const PagedArgs& a, int b) { return max(0,
 // Blocks of a sequence; one at the least, so that rows which see nothing have an owner too.
 __device__ __forceinline__ int blocks_of(int len) { return max(1, (len + kKvBlock - 1) / kKvBlock); }
 
+// Sums over a wave's lanes by moves between neighbours, rows and halves (lane shuffles go through LDS; six of them are a fifth of a microsecond, of
+// which a call of one token has few).
+template <int CTRL, int ROWS = 0xF> __device__ __forceinline__ int moved(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, true); }
+template <class F> __device__ __forceinline__ int wave_all(int x, F f) {
+    x = f(x, moved<0xB1>(x));            // lanes ^ 1, ^ 2, then the other half of 8, of 16
+    x = f(x, moved<0x4E>(x));
+    x = f(x, moved<0x141>(x));
+    x = f(x, moved<0x140>(x));
+    const v2u a = __builtin_amdgcn_permlane16_swap((unsigned)x, (unsigned)x, false, false);
+    x = f((int)a.x, (int)a.y);
+    const v2u b = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)x, false, false);
+    return __builtin_amdgcn_readfirstlane(f((int)b.x, (int)b.y));
+}
+__device__ __forceinline__ int wave_sum(int x) { return wave_all(x, [](int p, int q) { return p + q; }); }
+__device__ __forceinline__ int wave_max(int x) { return wave_all(x, [](int p, int q) { return max(p, q); }); }
+// Sums of the lanes up to and with each.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += moved<0x111>(x);                // from 1, 2, 4, 8 lanes before in the row of 16
+    x += moved<0x112>(x);
+    x += moved<0x114>(x);
+    x += moved<0x118>(x);
+    x += moved<0x142, 0xA>(x);           // the row before, the half before
+    x += moved<0x143, 0xC>(x);
+    return x;
+}
+
 // The list of blocks: sequence after sequence, in each head after head, row block after row block, block after block.
 // The share of a workgroup: all of them evenly, eight at the least (two to a wave), and at the least half the root of the longest sequence's
 // blocks, since the second launch's time grows with the parts as the shares shrink.
-struct Deal { int total, per; };
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m);
-    return x;
-}
-__device__ __forceinline__ int wave_max(int x) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) x = max(x, __shfl_xor(x, m));
-    return x;
-}
+struct Deal {
+    int total, per;
+    int len;                             // of the lane's sequence, of the first 64
+};
 __device__ __forceinline__ Deal deal(const PagedArgs& a, int mult, int lane) {
-    int sum = 0, most = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
+    Deal d;
+    d.len = lane < a.B ? cached(a, lane) : 0;
+    int sum = lane < a.B ? blocks_of(d.len) : 0, most = sum;
+    for (int b0 = 64; b0 < a.B; b0 += 64) {
         const int n = b0 + lane < a.B ? blocks_of(cached(a, b0 + lane)) : 0;
         sum += n;
         most = max(most, n);
     }
-    Deal d;
-    d.total = __builtin_amdgcn_readfirstlane(wave_sum(sum)) * mult;
-    most = __builtin_amdgcn_readfirstlane(wave_max(most));
+    d.total = wave_sum(sum) * mult;
+    most = wave_max(most);
     d.per = max(max((d.total + a.wgs - 1) / a.wgs, 8), (int)(0.5f * sqrtf((float)most)));
     return d;
 }
-// The sequence that block t of the list belongs to, its first place in the list and its own blocks.
-struct Place { int b, begin, n; };
-__device__ __forceinline__ Place place(const PagedArgs& a, int mult, int t, int lane) {
-    Place p = {0, 0, 1};
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const int n = b0 + lane < a.B ? blocks_of(cached(a, b0 + lane)) : 0;
-        int before = n * mult;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const int x = __shfl_up(before, m);
-            before += lane >= m ? x : 0;
-        }
-        // (before: up to and with this one)
-        const unsigned long long past = __ballot(p.begin + before > t);
+// The sequence that block t of the list belongs to, its first place in the list, its own blocks and its length.
+struct Place { int b, begin, n, len; };
+__device__ __forceinline__ Place place(const PagedArgs& a, const Deal& d, int mult, int t, int lane) {
+    int begin = 0;
+    for (int b0 = 0;; b0 += 64) {
+        const int len = b0 == 0 ? d.len : b0 + lane < a.B ? cached(a, b0 + lane) : 0, n = b0 + lane < a.B ? blocks_of(len) : 0;
+        const int end = begin + wave_scan(n) * mult;
+        const unsigned long long past = __ballot(end > t);
         if (past != 0) {
-            const int l = __builtin_ctzll(past);
-            p.b = b0 + l;
-            p.n = __shfl(n, l);
-            p.begin += __shfl(before, l) - p.n * mult;
-            break;
+            const int l = (int)__builtin_ctzll(past), n_l = __builtin_amdgcn_readlane(n, l);
+            return Place{b0 + l, __builtin_amdgcn_readlane(end, l) - n_l * mult, n_l, __builtin_amdgcn_readlane(len, l)};
         }
-        p.begin += __shfl(before, 63);
+        begin = __builtin_amdgcn_readlane(end, 63);
+        if (b0 + 64 >= a.B) return Place{0, t, 1, 0};    // (t lies in the list: not reached)
     }
-    return Place{__builtin_amdgcn_readfirstlane(p.b), __builtin_amdgcn_readfirstlane(p.begin), __builtin_amdgcn_readfirstlane(p.n)};
 }
 
 // A block's codes as a wave holds them.
@@ -223,12 +234,12 @@ template <int T, int D, int COLS> __global__ __launch_bounds__(256, D == 256 ? 1
     const uint32_t k_off = (uint32_t)(((l16 >> 2) * 8 + (l16 & 3)) * D + quad * 16), v_off = (uint32_t)(l16 * kKvBlock + quad * 8);
     const KvPool& c = a.pool;
 
-    Place at = {0, 0, 0};
+    Place at = {0, 0, 0, 0};
     for (int t = t_begin; t < t_end;) {
-        if (t >= at.begin + at.n * mult) at = place(a, mult, t, lane);
+        if (t >= at.begin + at.n * mult) at = place(a, deal_, mult, t, lane);
         const int unit = (t - at.begin) / at.n, first = t - at.begin - unit * at.n, n = min(at.n - first, t_end - t);
         const int b = at.b, h = unit / rblocks, x0 = (unit - h * rblocks) * ROWS;
-        const int len = cached(a, b), p0 = len - a.Sq;
+        const int len = at.len, p0 = len - a.Sq;
         const int p_lo = p0 + x0 / a.g, p_hi = p0 + (min(x0 + ROWS, rows) - 1) / a.g;
 
         v4i q[COLS][D / 32];
@@ -331,29 +342,30 @@ template <int T, int D, int COLS> __global__ __launch_bounds__(256, D == 256 ? 1
     }
 }
 
-// Rows whose blocks fell to several workgroups: their parts added up, in order.  A workgroup to a row, whose waves take eight parts at a time.
-constexpr int kJoinParts = 8;
-template <int T, int D> __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int part_rows, int all_rows) {
-    constexpr int N = D / 64;
+// Rows whose blocks fell to several workgroups: their parts added up, in order, eight at a time.  What it takes are latencies.  SHARED: a workgroup to a
+// row, whose waves share the parts, for up to 512 rows (48 rows of 32 parts 5 us); else a wave to a row.
+constexpr int kJoinParts = 8, kJoinShared = 512;
+template <int T, int D, bool SHARED> __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int part_rows, int all_rows) {
+    constexpr int N = D / 64, WAVES = SHARED ? kWaves : 1;
     typedef float vnf __attribute__((ext_vector_type(N)));
-    __shared__ float meet[kWaves][N + 2][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int rows = a.Sq * a.g, rblocks = (rows + part_rows - 1) / part_rows, mult = a.pool.Hk * rblocks;
     const Deal d = deal(a, mult, lane);
-    for (int item = (int)blockIdx.x; item < all_rows; item += (int)gridDim.x) {
+    const int first = SHARED ? (int)blockIdx.x : (int)blockIdx.x * kWaves + wave, step = (int)gridDim.x * (SHARED ? 1 : kWaves), share = SHARED ? wave : 0;
+    for (int item = first; item < all_rows; item += step) {
         const int bh = item / rows, x = item - bh * rows, b = bh / a.pool.Hk, h = bh - b * a.pool.Hk;
         // where this row's blocks begin in the list, and how many they are
-        int before = 0;
-        for (int b0 = 0; b0 < b; b0 += 64) before += b0 + lane < b ? blocks_of(cached(a, b0 + lane)) : 0;
-        const int len = cached(a, b), n = blocks_of(len);
-        const int u0 = __builtin_amdgcn_readfirstlane(wave_sum(before)) * mult + (h * rblocks + x / part_rows) * n;
+        int before = lane < b ? blocks_of(d.len) : 0;
+        for (int b0 = 64; b0 < b; b0 += 64) before += b0 + lane < b ? blocks_of(cached(a, b0 + lane)) : 0;
+        const int len = b < 64 ? __builtin_amdgcn_readlane(d.len, b) : cached(a, b), n = blocks_of(len);
+        const int u0 = wave_sum(before) * mult + (h * rblocks + x / part_rows) * n;
         const int w0 = u0 / d.per, w1 = (u0 + n - 1) / d.per;
         if (w0 == w1) continue;                          // (one workgroup had them all)
         const bool aligned = u0 == w0 * d.per;
         float ref = -INFINITY, sum = 0.0f, y[N];
 #pragma unroll
         for (int e = 0; e < N; e++) y[e] = 0.0f;
-        for (int s0 = w0 + wave * kJoinParts; s0 <= w1; s0 += kWaves * kJoinParts) {
+        for (int s0 = w0 + share * kJoinParts; s0 <= w1; s0 += WAVES * kJoinParts) {
             vnf v[kJoinParts];
             float m[kJoinParts], l[kJoinParts], top = ref;
 #pragma unroll
@@ -374,18 +386,22 @@ template <int T, int D> __global__ __launch_bounds__(256) void paged_join_kernel
             for (int e = 0; e < N; e++) y[e] *= f0;
 #pragma unroll
             for (int u = 0; u < kJoinParts; u++) {
-                if (s0 + u > w1) break;
+                // (no branch: the loads of all eight are to be on their way at once)
+                const bool real = s0 + u <= w1;
                 const float f = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[u] - ref);
-                sum = fmaf(l[u], f, sum);
+                sum = real ? fmaf(l[u], f, sum) : sum;
 #pragma unroll
-                for (int e = 0; e < N; e++) y[e] = fmaf(v[u][e], f, y[e]);
+                for (int e = 0; e < N; e++) y[e] = real ? fmaf(v[u][e], f, y[e]) : y[e];
             }
         }
-        meet[wave][N][lane] = ref, meet[wave][N + 1][lane] = sum;
+        if constexpr (SHARED) {
+            __shared__ float meet[kWaves][N + 2][64];
+            __syncthreads();             // (the row before has been read)
+            meet[wave][N][lane] = ref, meet[wave][N + 1][lane] = sum;
 #pragma unroll
-        for (int e = 0; e < N; e++) meet[wave][e][lane] = y[e];
-        __syncthreads();
-        if (wave == 0) {
+            for (int e = 0; e < N; e++) meet[wave][e][lane] = y[e];
+            __syncthreads();
+            if (wave > 0) continue;
 #pragma unroll
             for (int m = 1; m < kWaves; m++) ref = fmaxf(ref, meet[m][N][lane]);
             sum = 0.0f;
@@ -398,18 +414,17 @@ template <int T, int D> __global__ __launch_bounds__(256) void paged_join_kernel
 #pragma unroll
                 for (int e = 0; e < N; e++) y[e] = fmaf(meet[m][e][lane], f, y[e]);
             }
-            const int i = x / a.g, hg = x - i * a.g;
-            const bool blind = len - a.Sq + i < 0;
-            const float inv = weight_of(sum, blind) / kVHalf<T>;
-            uint16_t* o = a.o + b * a.o_sb + ((int64_t)h * a.g + hg) * a.o_sh + i * a.o_sn + lane * N;
-#pragma unroll
-            for (int e = 0; e < N; e++) y[e] = blind ? 0.0f : y[e] * inv;
-            if constexpr (N == 1) o[0] = (uint16_t)pack2<T>(y[0], 0.0f);
-            else
-#pragma unroll
-                for (int e = 0; e < N; e += 2) *reinterpret_cast<uint32_t*>(o + e) = pack2<T>(y[e], y[e + 1]);
         }
-        __syncthreads();
+        const int i = x / a.g, hg = x - i * a.g;
+        const bool blind = len - a.Sq + i < 0;
+        const float inv = weight_of(sum, blind) / kVHalf<T>;
+        uint16_t* o = a.o + b * a.o_sb + ((int64_t)h * a.g + hg) * a.o_sh + i * a.o_sn + lane * N;
+#pragma unroll
+        for (int e = 0; e < N; e++) y[e] = blind ? 0.0f : y[e] * inv;
+        if constexpr (N == 1) o[0] = (uint16_t)pack2<T>(y[0], 0.0f);
+        else
+#pragma unroll
+            for (int e = 0; e < N; e += 2) *reinterpret_cast<uint32_t*>(o + e) = pack2<T>(y[e], y[e + 1]);
     }
 }
 
@@ -418,7 +433,9 @@ int64_t all_rows(const PagedArgs& a) { return (int64_t)a.B * a.pool.Hk * a.Sq * 
 template <int T, int D> hipError_t launch_td(const PagedArgs& a, hipStream_t st) {
     if (paged_rows(a) == 16) hipLaunchKernelGGL((paged_kernel<T, D, 1>), dim3((unsigned)a.wgs), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((paged_kernel<T, D, 2>), dim3((unsigned)a.wgs), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)std::min<int64_t>(all_rows(a), 4096)), dim3(256), 0, st, a, paged_rows(a), (int)all_rows(a));
+    const int64_t rows = all_rows(a);
+    if (rows <= kJoinShared) hipLaunchKernelGGL((paged_join_kernel<T, D, true>), dim3((unsigned)rows), dim3(256), 0, st, a, paged_rows(a), (int)rows);
+    else hipLaunchKernelGGL((paged_join_kernel<T, D, false>), dim3((unsigned)std::min<int64_t>((rows + 3) / 4, 4096)), dim3(256), 0, st, a, paged_rows(a), (int)rows);
     return hipGetLastError();
 }
 template <int T> hipError_t launch_t(const PagedArgs& a, hipStream_t st) {

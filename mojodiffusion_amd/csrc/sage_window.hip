@@ -124,20 +124,22 @@ __device__ __forceinline__ void finish_rows(const WindowArgs& a, const RowState<
     query_rows_out<D>(a, os, a.rest + at, a.o_sn, a.o_sh, x0, lane);
 }
 
-// Tiles of 32 keys, two slots.  The waves' own rows lie over all of them but K's first at the start, and over the front again at the end.
-template <int D> struct WindowLds {
+// Tiles of 32 keys, two slots or three.  The waves' own rows lie over all of them but K's first (and V's third) at the start, and over the front again at the end.
+template <int D, int SLOTS = 2> struct WindowLds {
     static constexpr int NW = 4, KT = 32, TILE = KT * D * 2, OWN = NW * 64 * D;
-    static constexpr int K0 = 3 * TILE > OWN ? 3 * TILE : OWN, BYTES = K0 + TILE;
-    static __device__ int keys(int t) { return t & 1 ? 2 * TILE : K0; }
-    static __device__ int values(int t) { return (t & 1) * TILE; }
+    static constexpr int K0 = 3 * TILE > OWN ? 3 * TILE : OWN, BYTES = K0 + (SLOTS - 1) * TILE;
+    static_assert(SLOTS == 2 || (SLOTS == 3 && OWN == 4 * TILE), "the slots but these two lie under the rows");
+    static __device__ int keys(int slot) { return slot == 0 ? K0 : SLOTS == 2 ? 2 * TILE : (slot * 2 - 1) * TILE; }
+    static __device__ int values(int slot) { return slot == 2 ? K0 + TILE : SLOTS == 2 ? slot * TILE : slot * 2 * TILE; }
 };
 
 // Workgroups of four waves, 128 rows.  A wave's step from scores to exponentials to products is one chain; what fills the gaps is the waves of other
 // workgroups on the same SIMD, which meet no common barrier with it: five at 64 channels, three at 128, two at 256 (by registers: O, Q and one
 // tile's scores are 64, 112, 208 of them).  The next tile's scores taken beside this one's weights, with a wave less, was slower: [1,16896,48 on 12,128]
 // window 4096 + 4 1615 us, this form 1553; a training step of [2,1248,30,128] +-256 180, 175.  Two waves of this form at 128 channels: 1950.
-template <int T, int D> __device__ __forceinline__ void window_body(const WindowArgs& a, uint8_t* smem, int b, int kvh, int row0) {
-    using L = WindowLds<D>;
+// SLOTS: two: the next tile is on its way while one is computed; three: the next two.
+template <int T, int D, int SLOTS = 2> __device__ __forceinline__ void window_body(const WindowArgs& a, uint8_t* smem, int b, int kvh, int row0) {
+    using L = WindowLds<D, SLOTS>;
     constexpr int NW = L::NW, KT = L::KT, KS = D / 16;
     const int rows = a.Sq * a.g;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -167,20 +169,30 @@ template <int T, int D> __device__ __forceinline__ void window_body(const Window
     for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));
     __syncthreads();                     // the rows' LDS becomes the rings' slots
     if (span.n > 0) tiles.copy(v, 0, L::values(0));
+    if (SLOTS == 3 && span.n > 1) tiles.copy(k, 1, L::keys(1)), tiles.copy(v, 1, L::values(1));
 
     RowState<D> st;
     st.clear();
     const float c = a.scale * kLog2e;
     auto walk = [&](auto fine) {
         auto tile = [&](int t, int slot) {
-            dma_wait<0>();
+            constexpr int AHEAD = SLOTS - 1, PIECES = KeyTiles<D, NW>::Pieces::N;
+            if (SLOTS == 3 && t + 1 < span.n) dma_wait<2 * PIECES>();          // (the tile after it may be on its way)
+            else dma_wait<0>();
             __syncthreads();             // tile t is visible; every wave is done with tile t - 1
-            if (t + 1 < span.n) tiles.copy(k, t + 1, L::keys(slot + 1)), tiles.copy(v, t + 1, L::values(slot + 1));
+            const int to = slot + AHEAD >= SLOTS ? slot - 1 : slot + AHEAD;
+            if (t + AHEAD < span.n) tiles.copy(k, t + AHEAD, L::keys(to)), tiles.copy(v, t + AHEAD, L::values(to));
             const int j0 = span.tile(t) * KT;
             const Seen what = all.has(t) ? Seen::kAll : x0 < rows ? seen<KT>(a, wp_lo, wp_hi, len, j0) : Seen::kNone;
             if (what != Seen::kNone) attend_tile<T, D, decltype(fine)::value>(st, q, lds + L::keys(slot), lds + L::values(slot), fr, what, j0, mask, c);
         };
-        if constexpr (D == 64 && !decltype(fine)::value) {     // (slots known ahead: 147 -> 138 us at [2,8192,24 on 8] window 1024 + 4)
+        if constexpr (SLOTS == 3) {
+            for (int t = 0; t < span.n; t += 3) {
+                tile(t, 0);
+                if (t + 1 < span.n) tile(t + 1, 1);
+                if (t + 2 < span.n) tile(t + 2, 2);
+            }
+        } else if constexpr (D == 64 && !decltype(fine)::value) {     // (slots known ahead: 147 -> 138 us at [2,8192,24 on 8] window 1024 + 4)
             for (int t = 0; t < span.n; t += 2) {
                 tile(t, 0);
                 if (t + 1 < span.n) tile(t + 1, 1);
@@ -465,17 +477,16 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
 
 // ---- sequences one behind the other ----------------------------------------------------------------------
 // The same workgroups, each on the rows of one sequence: a slot of the grid names its sequence and its rows in it.  The last rows first, as above.
+constexpr int kPackedSlots(int D) { return D == 256 ? 2 : 3; }
 template <int T, int D> __global__ __launch_bounds__(256, kWindowWaves(D)) void packed_kernel(PackedArgs a, int slots) {
-    using L = WindowLds<D>;
+    using L = WindowLds<D, kPackedSlots(D)>;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
     const HeadSlot at = spread_item((int)blockIdx.x, a.w.Hk, slots);
     if (at.slot >= slots) return;
-    const int slot = slots - 1 - at.slot;
-    const Slots rows = {a.cu_q, a.rows_q, a.w.g, L::NW * 32};
-    const int b = rows.owner(slot, a.B), row0 = (slot - rows.first(b)) * L::NW * 32;
-    const Sequence s = sequence(a, b);
-    if (row0 >= s.nq * a.w.g) return;
-    window_body<T, D>(view(a.w, s, s.nq, b < a.B ? s.nk : 0), smem, 0, at.head, row0);
+    const Found f = find_slot<false>(a, a.w.g, L::NW * 32, at.slot);
+    if (f.index >= f.n) return;
+    const Sequence& s = f.s;
+    window_body<T, D, kPackedSlots(D)>(view(a.w, s, s.nq, f.b < a.B ? s.nk : 0), smem, 0, at.head, (f.n - 1 - f.index) * L::NW * 32);
 }
 template <int T, int D> __global__ __launch_bounds__(256) void packed_few_kernel(PackedArgs a, int slots) {
     using L = SplitLds<D>;
@@ -483,14 +494,12 @@ template <int T, int D> __global__ __launch_bounds__(256) void packed_few_kernel
     __shared__ float meet_ml[L::NW][32][2];
     const HeadSlot at = spread_item((int)blockIdx.x, a.w.Hk, slots);
     if (at.slot >= slots) return;
-    const int slot = slots - 1 - at.slot;
-    const Slots rows = {a.cu_q, a.rows_q, a.w.g, 32};
-    const int b = rows.owner(slot, a.B), x0 = (slot - rows.first(b)) * 32;
-    const Sequence s = sequence(a, b);
-    if (x0 >= s.nq * a.w.g) return;
-    WindowArgs w = view(a.w, s, s.nq, b < a.B ? s.nk : 0);
+    const Found f = find_slot<false>(a, a.w.g, 32, at.slot);
+    if (f.index >= f.n) return;
+    const Sequence& s = f.s;
+    WindowArgs w = view(a.w, s, s.nq, f.b < a.B ? s.nk : 0);
     w.splits = 1;
-    split_body<T, D>(w, smem, meet_ml, 0, at.head, x0, 0, 0);
+    split_body<T, D>(w, smem, meet_ml, 0, at.head, (f.n - 1 - f.index) * 32, 0, 0);
 }
 int64_t packed_slots(const PackedArgs& a, int rows) { return slots_total(a.rows_q, a.w.g, rows, a.B); }
 template <int T, int D> hipError_t launch_packed_td(const PackedArgs& a, hipStream_t st) {

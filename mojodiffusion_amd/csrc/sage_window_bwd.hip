@@ -697,22 +697,20 @@ __global__ __launch_bounds__(kWaves * 64, D > 64 ? 2 : 4) void packed_bwd_kernel
     if (id < nq) {
         const HeadSlot at = spread_item(id, a.w.w.Hk, q_slots);
         if (at.slot >= q_slots) return;
-        const int slot = q_slots - 1 - at.slot;          // (the last rows first: they see most keys)
-        const Slots rows = {a.p.cu_q, a.p.rows_q, a.w.w.g, kRowsWg};
-        const int b = rows.owner(slot, a.p.B), row0 = (slot - rows.first(b)) * kRowsWg;
-        const Sequence s = sequence(a.p, b);
-        if (row0 >= s.nq * a.w.w.g) return;
-        dq_body<T, D>(view(a, s, s.nq, b < a.p.B ? s.nk : 0, b), smem, at.head, row0);
+        const Found f = find_slot<false>(a.p, a.w.w.g, kRowsWg, at.slot);
+        if (f.index >= f.n) return;
+        const Sequence& s = f.s;
+        dq_body<T, D>(view(a, s, s.nq, f.b < a.p.B ? s.nk : 0, f.b), smem, at.head, (f.n - 1 - f.index) * kRowsWg);      // (the last rows first: they see most keys)
         return;
     }
     const HeadSlot at = spread_item(id - nq, a.w.w.Hk, k_slots * a.chunks);
     if (at.slot >= k_slots * a.chunks) return;
     const int slot = at.slot / a.chunks, chunk = at.slot - slot * a.chunks;
-    const Slots blocks = {a.p.cu_k, a.p.rows_k, 1, kKeysWg};
-    const int b = blocks.owner(slot, a.p.B), k0 = (slot - blocks.first(b)) * kKeysWg;
-    const Sequence s = sequence(a.p, b);
-    if (k0 >= s.nk) return;
-    const WindowBwdArgs v = view(a, s, b < a.p.B ? s.nq : 0, s.nk, b);
+    const Found f = find_slot<true>(a.p, 1, kKeysWg, slot);
+    if (f.index >= f.n) return;
+    const Sequence& s = f.s;
+    const int k0 = f.index * kKeysWg;                    // (the first keys first: most queries see them)
+    const WindowBwdArgs v = view(a, s, f.b < a.p.B ? s.nq : 0, s.nk, f.b);
     const QuerySpan qs = query_span(v.w, k0, kKeysWg, v.w.start, s.nk);
     KeyWork work;
     work.k0 = k0;
@@ -730,9 +728,9 @@ template <int T, int D> __global__ __launch_bounds__(256) void packed_bwd_join_k
     if (at >= (int64_t)a.w.w.Hk * k_slots * 2 * kKeysWg * CPR) return;
     const int col = (int)(at % CPR) * 8, key = (int)(at / CPR % kKeysWg), which = (int)(at / (CPR * kKeysWg) & 1);
     const int item = (int)(at / (2 * CPR * kKeysWg)), kvh = item / k_slots, slot = item - kvh * k_slots;
-    const Slots blocks = {a.p.cu_k, a.p.rows_k, 1, kKeysWg};
-    const int b = blocks.owner(slot, a.p.B), j = (slot - blocks.first(b)) * kKeysWg + key;
-    const Sequence s = sequence(a.p, b);
+    const Found f = find_slot<true>(a.p, 1, kKeysWg, slot);
+    const Sequence& s = f.s;
+    const int j = f.index * kKeysWg + key;
     if (j >= s.nk) return;
     const float* p = a.w.part + (((int64_t)item * a.chunks * 2 + which) * kKeysWg + key) * D + col;
     float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};

@@ -276,6 +276,39 @@ struct Slots {
 };
 __host__ __device__ inline int64_t slots_total(int64_t rows_all, int64_t per, int64_t rows, int64_t B) { return rows_all * per / rows + B + 1; }
 
+// The sequence that a slot names and which of its blocks of rows (KEYS: of keys), the heaviest first: sequences in the order of how much a block of theirs
+// has to walk (up to 64 of them, a lane each; more are taken as they come, their slots as above).  The blocks of a sequence: `n`; an index of n or beyond: no work.
+struct Found { int b, index, n; Sequence s; };
+template <bool KEYS> __device__ __forceinline__ Found find_slot(const PackedArgs& a, int per, int rows, int slot) {
+    if (a.B > 64) {
+        const Slots slots = {KEYS ? a.cu_k : a.cu_q, KEYS ? a.rows_k : a.rows_q, per, rows};
+        const int b = slots.owner(slot, a.B);
+        const Sequence s = sequence(a, b);
+        return Found{b, slot - slots.first(b), (int)(((uint32_t)(KEYS ? s.nk : s.nq) * (uint32_t)per + (uint32_t)rows - 1) / (uint32_t)rows), s};
+    }
+    const int lane = (int)threadIdx.x & 63;
+    int count = 0, size = -1, start = 0, total = 0;
+    Sequence s = {0, 0, 0, 0};
+    if (lane < a.B) {
+        s = sequence(a, lane);
+        count = (int)(((uint32_t)(KEYS ? s.nk : s.nq) * (uint32_t)per + (uint32_t)rows - 1) / (uint32_t)rows);
+        size = KEYS ? s.nq : s.nk;
+    }
+    for (int j = 0; j < a.B; j++) {
+        const int size_j = __builtin_amdgcn_readlane(size, j), count_j = __builtin_amdgcn_readlane(count, j);
+        start += size_j > size || (size_j == size && j < lane) ? count_j : 0;
+        total += count_j;
+    }
+    const unsigned long long here = __ballot(lane < a.B && slot >= start && slot < start + count);
+    if (here == 0) {                     // (rows behind the last sequence, or nothing)
+        s = sequence(a, a.B);
+        return Found{a.B, slot - total, (int)(((uint32_t)(KEYS ? s.nk : s.nq) * (uint32_t)per + (uint32_t)rows - 1) / (uint32_t)rows), s};
+    }
+    const int b = (int)__builtin_ctzll(here);
+    return Found{b, slot - __builtin_amdgcn_readlane(start, b), __builtin_amdgcn_readlane(count, b),
+                 Sequence{__builtin_amdgcn_readlane(s.q0, b), __builtin_amdgcn_readlane(s.nq, b), __builtin_amdgcn_readlane(s.k0, b), __builtin_amdgcn_readlane(s.nk, b)}};
+}
+
 }  // namespace
 
 }  // namespace sage
