@@ -52,8 +52,8 @@ __device__ __forceinline__ Rows sequence_rows(const KvAppendArgs& a, int b) {
 __device__ __forceinline__ int64_t row_at(const KvAppendArgs& a, const Rows& r, int64_t sb, int64_t sn, int b, int i) {
     return a.cu == nullptr ? b * sb + i * sn : (int64_t)(r.first + i) * sn;
 }
-// Position of a sequence's first new token.  (A length below zero counts as zero; the new tokens are the last of the length.)
-__device__ __forceinline__ int first_new(const KvAppendArgs& a, int b, int n) { return max(a.pool.lens[b], 0) - n; }
+// Position of a sequence's first new token.  (A length below zero counts as zero, one beyond any table, 2^30, as that: positions of blocks stay within 32 bits.)
+__device__ __forceinline__ int first_new(const KvAppendArgs& a, int b, int n) { return max(0, min(a.pool.lens[b], 1 << 30)) - n; }
 
 // Workgroup slots of sequences that lie one behind the other: sequence b's begin at cu[b] / 32 + 2 b, which leaves n / 32 + 2 at the least, and n rows
 // touch no more blocks than that.

@@ -187,7 +187,7 @@ def sdpa_paged(q, cache, page_table, kv_lens, scale):
     """The last Sq tokens of every sequence (one, or a few) against the cache: q [B,Sq,Hq,Dh], BF16 or F16 -> [B,Sq,Hq,Dh].
 
     Query i of sequence b stands at kv_lens[b] - Sq + i and sees keys up to itself; kv_lens counts the keys in the cache, the new tokens' among them.  Queries
-    before a sequence's first token (kv_lens[b] < Sq) give zeros.  q's heads h*Hq/Hk .. share key head h.  page_table and kv_lens as in kv_append; a
+    before a sequence's first token (kv_lens[b] < Sq) give zeros; a length beyond its row of the page table counts as what that holds.  q's heads h*Hq/Hk .. share key head h.  page_table and kv_lens as in kv_append; a
     sequence one of whose pages is not one of cache's gives NaN."""
     o = _lib.host().paged(q, cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, kv_lens, scale)
     if o is not None:

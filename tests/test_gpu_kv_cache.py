@@ -165,6 +165,28 @@ def test_tokens_that_have_no_place():
         want.check(cache)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 3, 40])
+@pytest.mark.parametrize("packed", [False, True])
+def test_lengths_at_the_end_of_32_bits(n, packed):
+    """Positions beyond every table: nothing is stored, queries find no row of the tables; a sequence beside them is stored as ever."""
+    cache = pool(4, 1, 64, 32)
+    want = Cache(cache)
+    g = torch.Generator().manual_seed(n)
+    q, k, v = (torch.randn((4, n, 1, 64), generator=g).to(BF) for _ in range(3))
+    ids = torch.tensor([[0, 1], [2, 3], [2, 3], [2, 3]], dtype=torch.int32)
+    lens = torch.tensor([n + 5, 2 ** 31 - 1, 2 ** 40, 2 ** 30 + 7])
+    cos, sin = tables(64, 64, F32)
+    z, err = rows(k[0], None, 0.0, cos, sin, torch.arange(5, 5 + n), True)
+    want.append(z, v[0].double(), err, [0, 1], 5)
+    shape = lambda t: (t.reshape(4 * n, 1, 64) if packed else t).cuda()
+    cu = torch.arange(5).cuda() * n if packed else None
+    got = C.kv_append(cache, shape(k), shape(v), ids.cuda(), lens.cuda(), cu_seqlens=cu, cos=cos.cuda(), sin=sin.cuda(), halfsplit=True, q=shape(q))
+    want.check(cache)
+    got = got.view(4, n, 1, 64)
+    assert torch.isfinite(got[0]).all() and torch.isnan(got[1:]).all()
+
+
 def filled(lens, Hk, D, page, seed, spare=2):
     """A cache of normal values with pages in no order, its page table, and its values [B, longest, Hk, D] (zeros behind the lengths) in float64."""
     g = torch.Generator().manual_seed(seed)
@@ -262,6 +284,17 @@ def test_queries_and_keys_that_are_not_finite():
     ids[1, 1] = 99
     got = call(q)
     assert torch.isnan(got[1, 1]).all() and torch.equal(got[0, 0], want[0, 0])
+
+
+@pytest.mark.gpu
+def test_lengths_beyond_the_table():
+    """A length past the pages of its row counts as what they hold."""
+    cache, ids, k, v = filled([64, 64], 2, 64, 32, 7)
+    q = torch.randn((2, 3, 4, 64), generator=torch.Generator().manual_seed(1)).to(BF)
+    want = C.sdpa_paged(q.cuda(), cache, ids, torch.tensor([64, 64]).cuda(), 0.125)
+    check_forward(want, None, forward(q, k, v, 0.125, -1, 0, 0, [64, 64], [61, 61]), BF)
+    for lens in ([65, 2 ** 31 - 1], [2 ** 40, 2 ** 30]):
+        assert torch.equal(C.sdpa_paged(q.cuda(), cache, ids, torch.tensor(lens).cuda(), 0.125), want)
 
 
 @pytest.mark.gpu

@@ -95,6 +95,29 @@ def test_packed(nq, nk, Hq, Hk, D, dtype, causal, tail):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B", [64, 65, 90])
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_sequences(B, causal):
+    """As many as one lane each takes, and more, in workgroups of 128 rows: every sequence as it is alone among few."""
+    lens = [(b * 37) % 61 for b in range(B - 1)] + [200]
+    T = sum(lens)
+    q, k, v, d = (t.cuda() for t in tensors(lens, lens, 12, 12, 64, BF, 6, B))
+    f = P.sdpa_packed_train_fwd(q, k, v, offsets(lens).cuda(), 0.125, causal)
+    g = P.sdpa_packed_backward(f, d)
+    for t in (f.o, g.d_q, g.d_k, g.d_v):
+        assert (t[T:] == 0).all()
+    assert torch.isneginf(f.stats[:, T:]).all()
+    at = 0
+    for b, n in enumerate(lens):
+        r, at = slice(at, at + n), at + n
+        if not n or (b % 7 and n != 200):
+            continue
+        ref = forward(q[None, r], k[None, r], v[None, r], 0.125, -1, 0 if causal else -1, 0, [n], [0])
+        check_forward(f.o[None, r], f.stats[None, :, r], ref, BF)
+        check_backward([t[None, r] for t in (g.d_q, g.d_k, g.d_v)], backward(*(t[None, r] for t in (q, k, v, d)), 0.125, ref, 1))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("D,dtype,causal", [(64, BF, True), (128, FP, True), (128, BF, False)])
 def test_gradients_against_differences(D, dtype, causal):
     """The slope of sum(O d) along a direction, from differences of the float64 forward, and the recorded node's gradients: no further apart than the bounds of
