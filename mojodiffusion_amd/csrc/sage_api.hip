@@ -1597,7 +1597,7 @@ static int paged_dims(int B, int Hq, int Hk, int N_q, int D, int table_width, in
     a->pool.Hk = Hk; a->pool.width = table_width;
     for (int n = page / kKvBlock; n > 1; n >>= 1) a->pool.sub++;
     if ((int64_t)B * Hq > (1 << 29) / N_q || B > 1 << 20 || paged_tiles(*a) > 1 << 30) { SAGE_LOG("paged attention: too many blocks or rows"); return MI355_SAGE_EUNSUPPORTED; }
-    a->wgs = paged_wgs(*a);
+    paged_plan(a);
     return 0;
 }
 

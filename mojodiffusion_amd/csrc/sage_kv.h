@@ -53,12 +53,12 @@ struct PagedArgs {
     int64_t q_sb, q_sh, q_sn, o_sb, o_sh, o_sn;
     int B, g, Sq, D, type;                       // g query heads share a key head
     float scale;
-    int wgs;                                     // workgroups that the blocks are dealt to
+    int wgs, more;                               // workgroups that the blocks are dealt to (paged_plan)
     float *part, *part_ml;                       // [workgroup, 2, rows, D], [workgroup, 2, rows, 2]: parts of rows that several workgroups share
 };
 int paged_rows(const PagedArgs& a);              // rows of a part: 16 or 32
 int64_t paged_tiles(const PagedArgs& a);         // blocks times row blocks times heads, of the longest sequences that the table holds
-int paged_wgs(const PagedArgs& a);
+void paged_plan(PagedArgs* a);
 size_t paged_part_bytes(const PagedArgs& a);
 hipError_t launch_paged(const PagedArgs& a, hipStream_t st);
 

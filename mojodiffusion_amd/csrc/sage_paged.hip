@@ -92,10 +92,15 @@ __device__ __forceinline__ int wave_scan(int x) {
 
 // The list of blocks: sequence after sequence, in each head after head, row block after row block, block after block.
 // The share of a workgroup: all of them evenly, eight at the least (two to a wave), and at the least half the root of the longest sequence's
-// blocks, since the second launch's time grows with the parts as the shares shrink.
+// blocks, since the second launch's time grows with the parts as the shares shrink.  Where shares are small (up to 16) a workgroup that had the
+// end of one row's blocks and the beginning of another's would go through the chain of latencies twice, and all would wait for it: there every row's blocks are
+// divided into shares of their own, of 8 or 16.
 struct Deal {
     int total, per;
     int len;                             // of the lane's sequence, of the first 64
+    int shift;                           // log2 of the rows' own shares, or 0
+    // places of a row with n blocks in the list: blocks, or shares
+    __device__ int places(int n) const { return (n + (1 << shift) - 1) >> shift; }
 };
 __device__ __forceinline__ Deal deal(const PagedArgs& a, int mult, int lane) {
     Deal d;
@@ -109,22 +114,24 @@ __device__ __forceinline__ Deal deal(const PagedArgs& a, int mult, int lane) {
     d.total = wave_sum(sum) * mult;
     most = wave_max(most);
     d.per = max(max((d.total + a.wgs - 1) / a.wgs, 8), (int)(0.5f * sqrtf((float)most)));
+    d.shift = a.more == 0 || d.per > 16 ? 0 : d.per > 8 ? 4 : 3;
+    if (d.shift > 0) d.per = 1;          // (places of the list)
     return d;
 }
-// The sequence that block t of the list belongs to, its first place in the list, its own blocks and its length.
+// The sequence that place t of the list belongs to, its first place in the list, its own blocks and its length.  n 0: behind the list's end.
 struct Place { int b, begin, n, len; };
 __device__ __forceinline__ Place place(const PagedArgs& a, const Deal& d, int mult, int t, int lane) {
     int begin = 0;
     for (int b0 = 0;; b0 += 64) {
         const int len = b0 == 0 ? d.len : b0 + lane < a.B ? cached(a, b0 + lane) : 0, n = b0 + lane < a.B ? blocks_of(len) : 0;
-        const int end = begin + wave_scan(n) * mult;
+        const int here = d.places(n) * mult, end = begin + wave_scan(here);
         const unsigned long long past = __ballot(end > t);
         if (past != 0) {
-            const int l = (int)__builtin_ctzll(past), n_l = __builtin_amdgcn_readlane(n, l);
-            return Place{b0 + l, __builtin_amdgcn_readlane(end, l) - n_l * mult, n_l, __builtin_amdgcn_readlane(len, l)};
+            const int l = (int)__builtin_ctzll(past);
+            return Place{b0 + l, __builtin_amdgcn_readlane(end - here, l), __builtin_amdgcn_readlane(n, l), __builtin_amdgcn_readlane(len, l)};
         }
         begin = __builtin_amdgcn_readlane(end, 63);
-        if (b0 + 64 >= a.B) return Place{0, t, 1, 0};    // (t lies in the list: not reached)
+        if (b0 + 64 >= a.B) return Place{0, t, 0, 0};
     }
 }
 
@@ -236,8 +243,10 @@ template <int T, int D, int COLS> __global__ __launch_bounds__(256, D == 256 ? 1
 
     Place at = {0, 0, 0, 0};
     for (int t = t_begin; t < t_end;) {
-        if (t >= at.begin + at.n * mult) at = place(a, deal_, mult, t, lane);
-        const int unit = (t - at.begin) / at.n, first = t - at.begin - unit * at.n, n = min(at.n - first, t_end - t);
+        if (t >= at.begin + deal_.places(at.n) * mult) at = place(a, deal_, mult, t, lane);
+        if (at.n == 0) return;
+        const int places = deal_.places(at.n), unit = (t - at.begin) / places, step = t - at.begin - unit * places;
+        const int first = step << deal_.shift, n = min(at.n - first, (t_end - t) << deal_.shift);
         const int b = at.b, h = unit / rblocks, x0 = (unit - h * rblocks) * ROWS;
         const int len = at.len, p0 = len - a.Sq;
         const int p_lo = p0 + x0 / a.g, p_hi = p0 + (min(x0 + ROWS, rows) - 1) / a.g;
@@ -338,13 +347,13 @@ template <int T, int D, int COLS> __global__ __launch_bounds__(256, D == 256 ? 1
             if (!whole && tid % TPR == 0) a.part_ml[(part + r) * 2] = ref, a.part_ml[(part + r) * 2 + 1] = sum;
         }
         __syncthreads();
-        t += n;
+        t += deal_.places(n);
     }
 }
 
 // Rows whose blocks fell to several workgroups: their parts added up, in order, eight at a time.  What it takes are latencies.  SHARED: a workgroup to a
-// row, whose waves share the parts, for up to 512 rows (48 rows of 32 parts 5 us); else a wave to a row.
-constexpr int kJoinParts = 8, kJoinShared = 512;
+// row, whose waves share the parts: where a row of the table's length has more than eight (paged_shared); else a wave to a row.
+constexpr int kJoinParts = 8;
 template <int T, int D, bool SHARED> __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int part_rows, int all_rows) {
     constexpr int N = D / 64, WAVES = SHARED ? kWaves : 1;
     typedef float vnf __attribute__((ext_vector_type(N)));
@@ -355,9 +364,9 @@ template <int T, int D, bool SHARED> __global__ __launch_bounds__(256) void page
     for (int item = first; item < all_rows; item += step) {
         const int bh = item / rows, x = item - bh * rows, b = bh / a.pool.Hk, h = bh - b * a.pool.Hk;
         // where this row's blocks begin in the list, and how many they are
-        int before = lane < b ? blocks_of(d.len) : 0;
-        for (int b0 = 64; b0 < b; b0 += 64) before += b0 + lane < b ? blocks_of(cached(a, b0 + lane)) : 0;
-        const int len = b < 64 ? __builtin_amdgcn_readlane(d.len, b) : cached(a, b), n = blocks_of(len);
+        int before = lane < b ? d.places(blocks_of(d.len)) : 0;
+        for (int b0 = 64; b0 < b; b0 += 64) before += b0 + lane < b ? d.places(blocks_of(cached(a, b0 + lane))) : 0;
+        const int len = b < 64 ? __builtin_amdgcn_readlane(d.len, b) : cached(a, b), n = d.places(blocks_of(len));
         const int u0 = wave_sum(before) * mult + (h * rblocks + x / part_rows) * n;
         const int w0 = u0 / d.per, w1 = (u0 + n - 1) / d.per;
         if (w0 == w1) continue;                          // (one workgroup had them all)
@@ -428,13 +437,19 @@ template <int T, int D, bool SHARED> __global__ __launch_bounds__(256) void page
     }
 }
 
+// (fewer than 128 row blocks then: else the shares are larger.)  [8 x 4 tokens, 4429 keys, 40 on 10 heads x 64] 16.4 us with a wave to a row, 15.7; [32 x 16384 keys,
+// 48 on 12 x 128], up to five parts, 173 and 174.
+bool paged_shared(const PagedArgs& a) {
+    const int64_t most = (int64_t)a.pool.width << a.pool.sub, per = std::max<int64_t>(8, (paged_tiles(a) + a.wgs - 1) / a.wgs);
+    return most > kJoinParts * per;
+}
 int64_t all_rows(const PagedArgs& a) { return (int64_t)a.B * a.pool.Hk * a.Sq * a.g; }
 
 template <int T, int D> hipError_t launch_td(const PagedArgs& a, hipStream_t st) {
-    if (paged_rows(a) == 16) hipLaunchKernelGGL((paged_kernel<T, D, 1>), dim3((unsigned)a.wgs), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((paged_kernel<T, D, 2>), dim3((unsigned)a.wgs), dim3(256), 0, st, a);
+    if (paged_rows(a) == 16) hipLaunchKernelGGL((paged_kernel<T, D, 1>), dim3((unsigned)(a.wgs + a.more)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((paged_kernel<T, D, 2>), dim3((unsigned)(a.wgs + a.more)), dim3(256), 0, st, a);
     const int64_t rows = all_rows(a);
-    if (rows <= kJoinShared) hipLaunchKernelGGL((paged_join_kernel<T, D, true>), dim3((unsigned)rows), dim3(256), 0, st, a, paged_rows(a), (int)rows);
+    if (paged_shared(a)) hipLaunchKernelGGL((paged_join_kernel<T, D, true>), dim3((unsigned)rows), dim3(256), 0, st, a, paged_rows(a), (int)rows);
     else hipLaunchKernelGGL((paged_join_kernel<T, D, false>), dim3((unsigned)std::min<int64_t>((rows + 3) / 4, 4096)), dim3(256), 0, st, a, paged_rows(a), (int)rows);
     return hipGetLastError();
 }
@@ -451,8 +466,13 @@ int64_t paged_tiles(const PagedArgs& a) {
     const int64_t rblocks = ((int64_t)a.Sq * a.g + paged_rows(a) - 1) / paged_rows(a);
     return (int64_t)a.B * a.pool.Hk * rblocks * std::max<int64_t>(1, (int64_t)a.pool.width << a.pool.sub);
 }
-int paged_wgs(const PagedArgs& a) { return (int)std::min<int64_t>(1024, std::max<int64_t>(1, (paged_tiles(a) + 7) / 8)); }
-size_t paged_part_bytes(const PagedArgs& a) { return (size_t)paged_wgs(a) * 2 * paged_rows(a) * (a.D + 2) * sizeof(float); }
+// Workgroups for even shares, and how many more shares there may be where every row has its own (one for each row block of a head; with more than 2048 of them: even shares).
+void paged_plan(PagedArgs* a) {
+    a->wgs = (int)std::min<int64_t>(1024, std::max<int64_t>(1, (paged_tiles(*a) + 7) / 8));
+    const int64_t units = (int64_t)a->B * a->pool.Hk * (((int64_t)a->Sq * a->g + paged_rows(*a) - 1) / paged_rows(*a));
+    a->more = units <= 2048 ? (int)units : 0;
+}
+size_t paged_part_bytes(const PagedArgs& a) { return (size_t)(a.wgs + a.more) * 2 * paged_rows(a) * (a.D + 2) * sizeof(float); }
 
 hipError_t launch_paged(const PagedArgs& a, hipStream_t st) { return a.type == kBF16 ? launch_t<kBF16>(a, st) : launch_t<kF16>(a, st); }
 
