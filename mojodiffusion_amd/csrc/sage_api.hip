@@ -1428,7 +1428,7 @@ static int packed_dims(const char* name, int B, int Hq, int Hk, int T_q, int T_k
     if (int rc = window_dims(name, 1, Hq, Hk, T_q, T_k, D, type, scale, -1, causal ? 0 : -1, 0, 0, &a->w)) return rc;
     a->B = B; a->rows_q = T_q; a->rows_k = T_k;
     if (B > 1 << 20 || (int64_t)Hq * packed_stats_rows(*a) > 1 << 29) { SAGE_LOG("%s: too many sequences", name); return MI355_SAGE_EUNSUPPORTED; }
-    a->few = packed_few(*a);
+    a->form = packed_form(*a);
     return 0;
 }
 

@@ -87,13 +87,16 @@ hipError_t launch_window_bwd(const WindowBwdArgs& a, hipStream_t st);
 // ---- attention over whole sequences that lie one behind the other -------------------------------------
 // Sequence b: rows cu_q[b] .. cu_q[b + 1] - 1 of Q and O, rows cu_k[b] .. cu_k[b + 1] - 1 of K and V; its queries are the last of its positions.  Rows behind the last
 // sequence: zeros.  w: of all rows, as one sequence (B 1, lens and starts null, left, right, sinks as they are to be).
+// kFull: workgroups of 128 rows, a wave to 32, their key tiles shared; kPaired: two waves to 32 rows, even key tiles and odd; kFew: workgroups of 32 rows whose
+// waves take key tiles in turn.
+enum class PackedForm { kFull, kPaired, kFew };
 struct PackedArgs {
     WindowArgs w;
     const int32_t *cu_q, *cu_k;                  // [B + 1]
     int B, rows_q, rows_k;
-    int few;                                     // rows of a workgroup: 0: 128, their key tiles shared by its waves; 1: 32, its waves taking key tiles in turn
+    PackedForm form;
 };
-bool packed_few(const PackedArgs& a);
+PackedForm packed_form(const PackedArgs& a);
 bool packed_grid_ok(const PackedArgs& a);
 hipError_t launch_packed(const PackedArgs& a, hipStream_t st);
 struct PackedBwdArgs {

@@ -488,6 +488,106 @@ template <int T, int D> __global__ __launch_bounds__(256, kWindowWaves(D)) void 
     const Sequence& s = f.s;
     window_body<T, D, kPackedSlots(D)>(view(a.w, s, s.nq, f.b < a.B ? s.nk : 0), smem, 0, at.head, (f.n - 1 - f.index) * L::NW * 32);
 }
+// The same with two waves to every 32 rows: one takes the even key tiles, one the odd ones, and where the walk ends their parts meet in LDS, register by register.  For
+// grids that leave a SIMD one wave of the form above, on a chain that nothing fills the gaps of (packed_form has the figures).  Two pairs of tiles further ahead: no
+// gain, the copies are in time; one wave for two tiles at a time: as slow as a wave for one.
+template <int D> struct PairedLds {
+    static constexpr int NW = 4, KT = 32, TILE = KT * D * 2, OWN = NW * 64 * D, MEET = NW * (D / 2) * 256;
+    static constexpr int STATS = 8 * TILE, BYTES = STATS + NW * 64 * 8;
+    // slot, even or odd: K, then V.  The rows lie over the second slot at the start.
+    static __device__ int keys(int slot, int odd) { return (slot * 4 + odd * 2) * TILE; }
+    static __device__ int values(int slot, int odd) { return keys(slot, odd) + TILE; }
+    static_assert(OWN <= 4 * TILE && MEET <= STATS, "rows and parts lie over the slots");
+};
+// (no sinks: the tiles of a walk lie one behind the other)
+template <int T, int D> __device__ __forceinline__ void paired_body(const WindowArgs& a, uint8_t* smem, int kvh, int row0) {
+    using L = PairedLds<D>;
+    constexpr int NW = L::NW, KT = L::KT, KS = D / 16;
+    const int rows = a.Sq * a.g;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & (NW - 1), odd = __builtin_amdgcn_readfirstlane(tid >> 8);
+    const int x0 = row0 + wave * 32;
+
+    const int len = a.Skv, p0 = a.start;
+    const int i_lo = row0 / a.g;
+    const Span span = key_span<KT>(a, p0 + i_lo, p0 + (min(row0 + NW * 32, rows) - 1) / a.g, len);
+    const int wp_lo = p0 + min(x0, rows - 1) / a.g, wp_hi = p0 + min(x0 + 31, rows - 1) / a.g;
+    const int p = p0 + min(x0 + (lane & 31), rows - 1) / a.g;
+    const RowMask mask = {p - a.left, min(p + a.right, len - 1), a.sinks};
+
+    const uint32_t lds = lds_addr(smem);
+    const KeyTiles<D, NW> tiles(span, lds, wave, lane);
+    const Range all = tiles.within(wp_hi - a.left, x0 < rows ? min(wp_lo + a.right, len - 1) : -1);
+    auto k = tiles.rows(a.k + kvh * a.k_sh, a.k_sn), v = tiles.rows(a.v + kvh * a.v_sh, a.v_sn);
+    k.at += odd * k.tile;
+    v.at += odd * v.tile;
+    auto copy = [&](int t, int slot) {
+        if (t >= span.n) return;
+        tiles.copy(k, t, L::keys(slot, odd));
+        tiles.copy(v, t, L::values(slot, odd));
+        k.at += k.tile;                  // (past the other wave's)
+        v.at += v.tile;
+    };
+
+    v4i q[KS];
+    const Fragments<D> fr(lane);
+    const int own = L::keys(1, 0) + wave * 64 * D;
+    if (odd == 0) query_rows_in<D>(a, a.q + (int64_t)kvh * a.g * a.q_sh + (int64_t)i_lo * a.q_sn, a.q_sn, a.q_sh, i_lo, x0, lds + own, lane);
+    copy(odd, 0);
+    dma_wait<0>();
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < KS; s++) q[s] = fr.along(smem + own, s);
+#pragma unroll
+    for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));
+
+    RowState<D> st;
+    st.clear();
+    const float c = a.scale * kLog2e;
+    auto walk = [&](auto fine) {
+        for (int t = odd, slot = 0; t - odd < span.n; t += 2, slot ^= 1) {
+            dma_wait<0>();
+            __syncthreads();             // both tiles are visible; every wave is done with the two before (and has its rows)
+            copy(t + 2, slot ^ 1);
+            const int j0 = t * KT;
+            const Seen what = t >= span.n ? Seen::kNone : all.has(t) ? Seen::kAll : x0 < rows ? seen<KT>(a, wp_lo, wp_hi, len, j0) : Seen::kNone;
+            if (what != Seen::kNone) attend_tile<T, D, decltype(fine)::value>(st, q, lds + L::keys(slot, odd), lds + L::values(slot, odd), fr, what, j0, mask, c);
+        }
+    };
+    if (D <= 128 && span.n * KT <= kFineKeys) walk(std::bool_constant<D <= 128>{});
+    else walk(std::false_type{});
+    __syncthreads();                     // (no copy is in flight: a step's wait is for all of them, and the last step copies nothing)
+    float* meet = reinterpret_cast<float*>(smem) + wave * (D / 2) * 64 + lane;
+    float* stats = reinterpret_cast<float*>(smem + L::STATS) + wave * 128 + lane;
+    if (odd != 0) {
+        stats[0] = st.ref, stats[64] = st.sum;
+#pragma unroll
+        for (int d = 0; d < D / 32; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) meet[(d * 16 + i) * 64] = st.acc[d][i];
+    }
+    __syncthreads();
+    if (odd != 0 || x0 >= rows) return;
+    const float other = stats[0];
+    st.raise(other);
+    const float f = st.ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(other - st.ref);
+    st.sum = fmaf(stats[64], f, st.sum);
+#pragma unroll
+    for (int d = 0; d < D / 32; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) st.acc[d][i] = fmaf(meet[(d * 16 + i) * 64], f, st.acc[d][i]);
+    finish_rows<T, D>(a, st, smem + wave * 128 * D, 0, kvh, x0, lane);
+}
+template <int T, int D> __global__ __launch_bounds__(512, D == 64 ? 4 : 2) void packed_paired_kernel(PackedArgs a, int slots) {
+    using L = PairedLds<D>;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
+    const HeadSlot at = spread_item((int)blockIdx.x, a.w.Hk, slots);
+    if (at.slot >= slots) return;
+    const Found f = find_slot<false>(a, a.w.g, L::NW * 32, at.slot);
+    if (f.index >= f.n) return;
+    const Sequence& s = f.s;
+    paired_body<T, D>(view(a.w, s, s.nq, f.b < a.B ? s.nk : 0), smem, at.head, (f.n - 1 - f.index) * L::NW * 32);
+}
 template <int T, int D> __global__ __launch_bounds__(256) void packed_few_kernel(PackedArgs a, int slots) {
     using L = SplitLds<D>;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
@@ -501,11 +601,13 @@ template <int T, int D> __global__ __launch_bounds__(256) void packed_few_kernel
     w.splits = 1;
     split_body<T, D>(w, smem, meet_ml, 0, at.head, (f.n - 1 - f.index) * 32, 0, 0);
 }
+int packed_rows(const PackedArgs& a) { return a.form == PackedForm::kFew ? 32 : 128; }
 int64_t packed_slots(const PackedArgs& a, int rows) { return slots_total(a.rows_q, a.w.g, rows, a.B); }
 template <int T, int D> hipError_t launch_packed_td(const PackedArgs& a, hipStream_t st) {
-    const int64_t slots = packed_slots(a, a.few ? 32 : 128);
+    const int64_t slots = packed_slots(a, packed_rows(a));
     const dim3 grid((unsigned)spread_grid(a.w.Hk, slots));
-    if (a.few) hipLaunchKernelGGL((packed_few_kernel<T, D>), grid, dim3(256), 0, st, a, (int)slots);
+    if (a.form == PackedForm::kPaired) hipLaunchKernelGGL((packed_paired_kernel<T, D>), grid, dim3(512), 0, st, a, (int)slots);
+    else if (a.form == PackedForm::kFew) hipLaunchKernelGGL((packed_few_kernel<T, D>), grid, dim3(256), 0, st, a, (int)slots);
     else hipLaunchKernelGGL((packed_kernel<T, D>), grid, dim3(256), 0, st, a, (int)slots);
     return hipGetLastError();
 }
@@ -573,9 +675,19 @@ hipError_t launch_window(const WindowArgs& a, const WindowPlan& p, hipStream_t s
     return a.type == kBF16 ? launch_t<kBF16>(a, p, st) : launch_t<kF16>(a, p, st);
 }
 
-// (as window_plan: workgroups of 128 rows for half the chip)
-bool packed_few(const PackedArgs& a) { return (int64_t)a.rows_q * a.w.g / 128 * a.w.Hk < 128; }
-bool packed_grid_ok(const PackedArgs& a) { return spread_grid(a.w.Hk, packed_slots(a, a.few ? 32 : 128)) <= 0x7FFFFFFF; }
+// By the workgroups of 128 rows (`wgs`, one to a compute unit up to 256) and the keys of a sequence on the average.  Measured over sequences of one length, bf16, few / paired /
+// full in us:
+//   64 channels, full attention of 1024 keys, 128 wgs 15 / 19 / 23, 192: 22 / 19 / 23, 256: 26 / 27 / 27; of 4096 keys, causal, 192: 41 / 58 / 76, 384: 70 / 84 / 89;
+//   128 channels, full, 4096 keys, 64 wgs 47 / 76 / 105, 128: 92 / 77 / 106, 256: 183 / 81 / 107, 384: 272 / 153 / 129; causal, 128: 54 / 77 / 107; of 333 keys, 129: 23 / 18 / 19, 192: 25 / 15 / 16,
+//   255: 32 / 27 / 20;
+//   256 channels, full, 4096 keys, 128 wgs 143 / 132 / 207, 256: 285 / 141 / 210.
+PackedForm packed_form(const PackedArgs& a) {
+    const int64_t wgs = (int64_t)a.rows_q * a.w.g * a.w.Hk / 128, keys = a.rows_k / a.B;
+    const bool causal = a.w.right < kWindowFar;
+    const int few = a.w.D == 64 ? (causal && keys >= 2048 ? 320 : 176) : causal && keys >= 768 ? 144 : 104, paired = keys >= 1024 ? 256 : 208;
+    return wgs < few ? PackedForm::kFew : wgs <= paired ? PackedForm::kPaired : PackedForm::kFull;
+}
+bool packed_grid_ok(const PackedArgs& a) { return spread_grid(a.w.Hk, packed_slots(a, packed_rows(a))) <= 0x7FFFFFFF; }
 hipError_t launch_packed(const PackedArgs& a, hipStream_t st) { return a.w.type == kBF16 ? launch_packed_t<kBF16>(a, st) : launch_packed_t<kF16>(a, st); }
 
 }  // namespace sage

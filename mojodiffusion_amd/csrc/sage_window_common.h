@@ -287,18 +287,20 @@ template <bool KEYS> __device__ __forceinline__ Found find_slot(const PackedArgs
         return Found{b, slot - slots.first(b), (int)(((uint32_t)(KEYS ? s.nk : s.nq) * (uint32_t)per + (uint32_t)rows - 1) / (uint32_t)rows), s};
     }
     const int lane = (int)threadIdx.x & 63;
-    int count = 0, size = -1, start = 0, total = 0;
+    int count = 0, order = -1, start = 0, total = 0;
     Sequence s = {0, 0, 0, 0};
     if (lane < a.B) {
         s = sequence(a, lane);
         count = (int)(((uint32_t)(KEYS ? s.nk : s.nq) * (uint32_t)per + (uint32_t)rows - 1) / (uint32_t)rows);
-        size = KEYS ? s.nq : s.nk;
+        order = min(KEYS ? s.nq : s.nk, (1 << 25) - 1) << 6 | (63 - lane);
     }
-    for (int j = 0; j < a.B; j++) {
-        const int size_j = __builtin_amdgcn_readlane(size, j), count_j = __builtin_amdgcn_readlane(count, j);
-        start += size_j > size || (size_j == size && j < lane) ? count_j : 0;
-        total += count_j;
-    }
+    for (int j0 = 0; j0 < a.B; j0 += 4)
+#pragma unroll
+        for (int j = j0; j < j0 + 4; j++) {              // (lanes from B on: no blocks)
+            const int order_j = __builtin_amdgcn_readlane(order, j), count_j = __builtin_amdgcn_readlane(count, j);
+            start += order_j > order ? count_j : 0;
+            total += count_j;
+        }
     const unsigned long long here = __ballot(lane < a.B && slot >= start && slot < start + count);
     if (here == 0) {                     // (rows behind the last sequence, or nothing)
         s = sequence(a, a.B);

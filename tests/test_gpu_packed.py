@@ -94,6 +94,42 @@ def test_packed(nq, nk, Hq, Hk, D, dtype, causal, tail):
         assert torch.equal(x, y)
 
 
+FORMS = [
+    # workgroups of 128 rows with a wave or two to 32 rows, all head dims, rows that see nothing among them
+    ([300, 1, 513, 129, 90], None, 24, 8, 128, BF, True, 70),
+    ([300, 1, 513, 129, 90], None, 60, 12, 128, FP, True, 5),
+    ([333, 70, 500], [333, 31, 900], 24, 24, 128, FP, False, 0),
+    ([200, 333, 128], [100, 400, 129], 32, 32, 128, BF, True, 1),
+    ([600, 1, 401], None, 18, 6, 256, BF, True, 3),
+    ([600, 1, 401], [40, 33, 500], 36, 36, 256, FP, True, 3),
+    ([100, 333, 64, 31, 600], None, 22, 11, 64, BF, False, 1),
+    ([1100], [1200], 20, 4, 64, FP, True, 0),
+    ([1111], None, 24, 24, 64, BF, True, 9),
+    ([95, 1030], [1500, 2100], 10, 10, 128, BF, True, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nk,Hq,Hk,D,dtype,causal,tail", FORMS)
+def test_packed_in_larger_grids(nq, nk, Hq, Hk, D, dtype, causal, tail):
+    test_packed(nq, nk, Hq, Hk, D, dtype, causal, tail)
+
+
+@pytest.mark.gpu
+def test_more_sequences_than_lanes_in_a_large_grid():
+    lens = [(b * 37) % 61 for b in range(70)] + [300, 0, 5]
+    T = sum(lens)
+    q, k, v, _ = (t.cuda() for t in tensors(lens, lens, 16, 16, 64, FP, 11, 7))
+    assert T * 16 // 128 > 256
+    o = P.sdpa_packed(q, k, v, offsets(lens).cuda(), 0.125)
+    assert (o[T:] == 0).all()
+    at = 0
+    for n in lens:
+        r, at = slice(at, at + n), at + n
+        if n:
+            check_forward(o[None, r], None, forward(q[None, r], k[None, r], v[None, r], 0.125, -1, 0, 0, [n], [0]), FP)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("B", [64, 65, 90])
 @pytest.mark.parametrize("causal", [True, False])
