@@ -51,9 +51,9 @@ template <int D> struct RowState {
 // taken from O, on a padded batch with sinks: 0.0027 without, 0.0024 with it; the products are a small part of what such a workgroup does).  By the keys of a workgroup, not of
 // a row: rows of short windows in longer spans gain nothing from it (window 16 + 1 on [1,1024,heads,64], dQ: 0.00236 without it, one head to a group, 0.00234 with it, four).
 constexpr int kFineKeys = 128;
-template <int T, int D, bool FINE>
+template <int T, int D, bool FINE, class Mask>
 __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 16], uint32_t kt, uint32_t vt, const Fragments<D>& kept,
-                                            Seen what, int j0, const RowMask& m, float c) {
+                                            Seen what, int j0, const Mask& m, float c) {
     constexpr int KS = D / 16, DB = D / 32;
     const Fragments<D> f = D > 64 || FINE ? kept.fresh() : kept;         // (at 64 channels there is room for the addresses)
     auto key = [&](int ks) { return lds_read(kt + (f.nat ^ ((ks & 7) << 5)) + (ks >> 3) * 256); };
@@ -61,7 +61,7 @@ __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 
 #pragma unroll
     for (int ks = 1; ks < KS; ks++) s = product<T>(key(ks), q[ks], s);
     if (what != Seen::kAll) {
-        const RowMask rel = m.from(j0 + (lane_here() >> 5) * 4);
+        const Mask rel = m.from(j0 + (lane_here() >> 5) * 4);
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = rel.sees((i >> 2) * 8 + (i & 3)) ? s[i] : -INFINITY;
     }
@@ -124,24 +124,28 @@ __device__ __forceinline__ void finish_rows(const WindowArgs& a, const RowState<
     query_rows_out<D>(a, os, a.rest + at, a.o_sn, a.o_sh, x0, lane);
 }
 
-// Tiles of 32 keys, two slots or three.  The waves' own rows lie over all of them but K's first (and V's third) at the start, and over the front again at the end.
-template <int D, int SLOTS = 2> struct WindowLds {
+// Tiles of 32 keys, two slots.  The waves' own rows lie over all of them but K's first at the start, and over the front again at the end.
+template <int D> struct WindowLds {
     static constexpr int NW = 4, KT = 32, TILE = KT * D * 2, OWN = NW * 64 * D;
-    static constexpr int K0 = 3 * TILE > OWN ? 3 * TILE : OWN, BYTES = K0 + (SLOTS - 1) * TILE;
-    static_assert(SLOTS == 2 || (SLOTS == 3 && OWN == 4 * TILE), "the slots but these two lie under the rows");
-    static __device__ int keys(int slot) { return slot == 0 ? K0 : SLOTS == 2 ? 2 * TILE : (slot * 2 - 1) * TILE; }
-    static __device__ int values(int slot) { return slot == 2 ? K0 + TILE : SLOTS == 2 ? slot * TILE : slot * 2 * TILE; }
+    static constexpr int K0 = 3 * TILE > OWN ? 3 * TILE : OWN, BYTES = K0 + TILE;
+    static __device__ int keys(int t) { return t & 1 ? 2 * TILE : K0; }
+    static __device__ int values(int t) { return (t & 1) * TILE; }
 };
 
 // Workgroups of four waves, 128 rows.  A wave's step from scores to exponentials to products is one chain; what fills the gaps is the waves of other
 // workgroups on the same SIMD, which meet no common barrier with it: five at 64 channels, three at 128, two at 256 (by registers: O, Q and one
 // tile's scores are 64, 112, 208 of them).  The next tile's scores taken beside this one's weights, with a wave less, was slower: [1,16896,48 on 12,128]
 // window 4096 + 4 1615 us, this form 1553; a training step of [2,1248,30,128] +-256 180, 175.  Two waves of this form at 128 channels: 1950.
-// SLOTS: two: the next tile is on its way while one is computed; three: the next two.
-template <int T, int D, int SLOTS = 2> __device__ __forceinline__ void window_body(const WindowArgs& a, uint8_t* smem, int b, int kvh, int row0) {
-    using L = WindowLds<D, SLOTS>;
+constexpr int kWindowWaves(int D) { return D == 64 ? 5 : D == 128 ? 3 : 2; }
+template <int T, int D>
+__global__ __launch_bounds__(256, kWindowWaves(D)) void window_kernel(WindowArgs a) {
+    using L = WindowLds<D>;
     constexpr int NW = L::NW, KT = L::KT, KS = D / 16;
-    const int rows = a.Sq * a.g;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
+    const int rows = a.Sq * a.g, blocks = (rows + NW * 32 - 1) / (NW * 32);
+    const int item = xcd_item((int)blockIdx.x, a.B * a.Hk * blocks);
+    const int bh = item / blocks, row0 = (blocks - 1 - item % blocks) * NW * 32;       // (the last rows first: without a left edge they see most keys)
+    const int b = bh / a.Hk, kvh = bh % a.Hk;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int x0 = row0 + wave * 32;
@@ -169,30 +173,20 @@ template <int T, int D, int SLOTS = 2> __device__ __forceinline__ void window_bo
     for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));
     __syncthreads();                     // the rows' LDS becomes the rings' slots
     if (span.n > 0) tiles.copy(v, 0, L::values(0));
-    if (SLOTS == 3 && span.n > 1) tiles.copy(k, 1, L::keys(1)), tiles.copy(v, 1, L::values(1));
 
     RowState<D> st;
     st.clear();
     const float c = a.scale * kLog2e;
     auto walk = [&](auto fine) {
         auto tile = [&](int t, int slot) {
-            constexpr int AHEAD = SLOTS - 1, PIECES = KeyTiles<D, NW>::Pieces::N;
-            if (SLOTS == 3 && t + 1 < span.n) dma_wait<2 * PIECES>();          // (the tile after it may be on its way)
-            else dma_wait<0>();
+            dma_wait<0>();
             __syncthreads();             // tile t is visible; every wave is done with tile t - 1
-            const int to = slot + AHEAD >= SLOTS ? slot - 1 : slot + AHEAD;
-            if (t + AHEAD < span.n) tiles.copy(k, t + AHEAD, L::keys(to)), tiles.copy(v, t + AHEAD, L::values(to));
+            if (t + 1 < span.n) tiles.copy(k, t + 1, L::keys(slot + 1)), tiles.copy(v, t + 1, L::values(slot + 1));
             const int j0 = span.tile(t) * KT;
             const Seen what = all.has(t) ? Seen::kAll : x0 < rows ? seen<KT>(a, wp_lo, wp_hi, len, j0) : Seen::kNone;
             if (what != Seen::kNone) attend_tile<T, D, decltype(fine)::value>(st, q, lds + L::keys(slot), lds + L::values(slot), fr, what, j0, mask, c);
         };
-        if constexpr (SLOTS == 3) {
-            for (int t = 0; t < span.n; t += 3) {
-                tile(t, 0);
-                if (t + 1 < span.n) tile(t + 1, 1);
-                if (t + 2 < span.n) tile(t + 2, 2);
-            }
-        } else if constexpr (D == 64 && !decltype(fine)::value) {     // (slots known ahead: 147 -> 138 us at [2,8192,24 on 8] window 1024 + 4)
+        if constexpr (D == 64 && !decltype(fine)::value) {     // (slots known ahead: 147 -> 138 us at [2,8192,24 on 8] window 1024 + 4)
             for (int t = 0; t < span.n; t += 2) {
                 tile(t, 0);
                 if (t + 1 < span.n) tile(t + 1, 1);
@@ -205,15 +199,6 @@ template <int T, int D, int SLOTS = 2> __device__ __forceinline__ void window_bo
     else walk(std::false_type{});
     __syncthreads();                     // (no copy is in flight: the last step's wait was for all of them)
     if (x0 < rows) finish_rows<T, D>(a, st, smem + wave * 64 * D, b, kvh, x0, lane);
-}
-constexpr int kWindowWaves(int D) { return D == 64 ? 5 : D == 128 ? 3 : 2; }
-template <int T, int D> __global__ __launch_bounds__(256, kWindowWaves(D)) void window_kernel(WindowArgs a) {
-    using L = WindowLds<D>;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
-    const int rows = a.Sq * a.g, blocks = (rows + L::NW * 32 - 1) / (L::NW * 32);
-    const int item = xcd_item((int)blockIdx.x, a.B * a.Hk * blocks);
-    const int bh = item / blocks;
-    window_body<T, D>(a, smem, bh / a.Hk, bh % a.Hk, (blocks - 1 - item % blocks) * L::NW * 32);       // (the last rows first: without a left edge they see most keys)
 }
 
 // N neighbouring channels of a finished row, and what rounding left of them.
@@ -476,117 +461,151 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
 }
 
 // ---- sequences one behind the other ----------------------------------------------------------------------
-// The same workgroups, each on the rows of one sequence: a slot of the grid names its sequence and its rows in it.  The last rows first, as above.
-constexpr int kPackedSlots(int D) { return D == 256 ? 2 : 3; }
-template <int T, int D> __global__ __launch_bounds__(256, kWindowWaves(D)) void packed_kernel(PackedArgs a, int slots) {
-    using L = WindowLds<D, kPackedSlots(D)>;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
-    const HeadSlot at = spread_item((int)blockIdx.x, a.w.Hk, slots);
-    if (at.slot >= slots) return;
-    const Found f = find_slot<false>(a, a.w.g, L::NW * 32, at.slot);
-    if (f.index >= f.n) return;
-    const Sequence& s = f.s;
-    window_body<T, D, kPackedSlots(D)>(view(a.w, s, s.nq, f.b < a.B ? s.nk : 0), smem, 0, at.head, (f.n - 1 - f.index) * L::NW * 32);
-}
-// The same with two waves to every 32 rows: one takes the even key tiles, one the odd ones, and where the walk ends their parts meet in LDS, register by register.  For
-// grids that leave a SIMD one wave of the form above, on a chain that nothing fills the gaps of (packed_form has the figures).  Two pairs of tiles further ahead: no
-// gain, the copies are in time; one wave for two tiles at a time: as slow as a wave for one.
-template <int D> struct PairedLds {
-    static constexpr int NW = 4, KT = 32, TILE = KT * D * 2, OWN = NW * 64 * D, MEET = NW * (D / 2) * 256;
-    static constexpr int STATS = 8 * TILE, BYTES = STATS + NW * 64 * 8;
-    // slot, even or odd: K, then V.  The rows lie over the second slot at the start.
-    static __device__ int keys(int slot, int odd) { return (slot * 4 + odd * 2) * TILE; }
-    static __device__ int values(int slot, int odd) { return keys(slot, odd) + TILE; }
-    static_assert(OWN <= 4 * TILE && MEET <= STATS, "rows and parts lie over the slots");
+// A slot of the grid names a sequence and its rows in it (find_slot).  Workgroups of 128 rows, four waves to them (WAYS 1), as window_kernel, or eight (WAYS 2): there one of
+// two waves with the same rows takes the even key tiles, one the odd ones, and their parts meet in LDS at the end, register by register.  That is for grids that leave a SIMD
+// one wave of the first kind, on a chain that nothing fills the gaps of (packed_form has the figures).  Two pairs of tiles further ahead: no gain, the copies
+// are in time; one wave for two tiles at a time: as slow as a wave for one.
+//
+// The tiles that a wave sees all of come first, in a loop of their own without a question but for the ring's ends: a wave that is alone on its SIMD waits for its own
+// scalar instructions ([16 sequences of up to 333, 12 x 64] 14.4 -> 12.6 us, [31234 rows in 6, 48 on 12 x 128] 2215 -> 2160).  A training step does without: there the
+// chip is at its power limit, and the gradients' kernel pays for a denser forward in clocks ([20576 rows in 8, 24 on 8 x 64] forward 230 -> 225 us, the step after it
+// 1065 -> 1100; without the loop 1073).
+template <int D, int WAYS> struct PackedLds {
+    static constexpr int NW = 4, KT = 32, TILE = KT * D * 2, OWN = NW * 64 * D, SLOTS = WAYS == 1 && D == 128 ? 3 : 2, RING = SLOTS * WAYS * 2 * TILE;
+    // The waves' rows lie behind the first slot at the start (with two slots of WAYS 1 behind its keys), and over the front again at the end.
+    static constexpr int ROWS = RING >= WAYS * 2 * TILE + OWN ? RING - OWN : TILE;
+    static constexpr bool VALUES_FIRST = ROWS >= WAYS * 2 * TILE;
+    static constexpr int STATS = RING > ROWS + OWN ? RING : ROWS + OWN, BYTES = STATS + (WAYS == 2 ? NW * 64 * 8 : 0);
+    static __device__ int keys(int slot, int way) { return (slot * WAYS + way) * 2 * TILE; }
+    static __device__ int values(int slot, int way) { return keys(slot, way) + TILE; }
+    static_assert(WAYS == 1 || NW * (D / 2) * 256 <= RING, "parts lie over the slots");
 };
-// (no sinks: the tiles of a walk lie one behind the other)
-template <int T, int D> __device__ __forceinline__ void paired_body(const WindowArgs& a, uint8_t* smem, int kvh, int row0) {
-    using L = PairedLds<D>;
-    constexpr int NW = L::NW, KT = L::KT, KS = D / 16;
+struct EndMask {                         // keys up to hi
+    int hi;
+    __device__ EndMask from(int j) const { return EndMask{hi - j}; }
+    __device__ bool sees(int j) const { return j <= hi; }
+};
+template <int T, int D, int WAYS> __device__ __forceinline__ void packed_body(const WindowArgs& a, uint8_t* smem, int kvh, int row0) {
+    using L = PackedLds<D, WAYS>;
+    using Tiles = KeyTiles<D, L::NW>;
+    constexpr int NW = L::NW, KT = L::KT, KS = D / 16, AHEAD = L::SLOTS - 1, PIECES = Tiles::Pieces::N;
     const int rows = a.Sq * a.g;
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & (NW - 1), odd = __builtin_amdgcn_readfirstlane(tid >> 8);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & (NW - 1), way = WAYS == 2 ? __builtin_amdgcn_readfirstlane(tid >> 8) : 0;
     const int x0 = row0 + wave * 32;
 
     const int len = a.Skv, p0 = a.start;
     const int i_lo = row0 / a.g;
-    const Span span = key_span<KT>(a, p0 + i_lo, p0 + (min(row0 + NW * 32, rows) - 1) / a.g, len);
+    const Span span = key_span<KT>(a, p0 + i_lo, p0 + (min(row0 + NW * 32, rows) - 1) / a.g, len);       // (from the first key on)
     const int wp_lo = p0 + min(x0, rows - 1) / a.g, wp_hi = p0 + min(x0 + 31, rows - 1) / a.g;
     const int p = p0 + min(x0 + (lane & 31), rows - 1) / a.g;
-    const RowMask mask = {p - a.left, min(p + a.right, len - 1), a.sinks};
+    const EndMask mask = {min(p + a.right, len - 1)};
+    // Tiles that this wave sees all of, that it sees some of, and that are copied as they are.
+    const int all = x0 < rows ? max(min(wp_lo + a.right, len - 1) + 1, 0) / KT : 0, some = x0 < rows ? (max(min(wp_hi + a.right, len - 1) + 1, 0) + KT - 1) / KT : 0;
+    const int whole = max(span.hi + 1, 0) / KT;
 
     const uint32_t lds = lds_addr(smem);
-    const KeyTiles<D, NW> tiles(span, lds, wave, lane);
-    const Range all = tiles.within(wp_hi - a.left, x0 < rows ? min(wp_lo + a.right, len - 1) : -1);
+    const Tiles tiles(span, lds, wave, lane);
     auto k = tiles.rows(a.k + kvh * a.k_sh, a.k_sn), v = tiles.rows(a.v + kvh * a.v_sh, a.v_sn);
-    k.at += odd * k.tile;
-    v.at += odd * v.tile;
-    auto copy = [&](int t, int slot) {
-        if (t >= span.n) return;
-        tiles.copy(k, t, L::keys(slot, odd));
-        tiles.copy(v, t, L::values(slot, odd));
-        k.at += k.tile;                  // (past the other wave's)
-        v.at += v.tile;
+    k.at += way * k.tile;
+    v.at += way * v.tile;
+    auto copy = [&](typename Tiles::Rows& r, int t, int to) {
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) {
+            const int row = tiles.pieces.row(i);
+            const uint32_t off = t < whole ? r.off[i] : (uint32_t)(min(t * KT + row, span.hi) - t * KT) * r.sn + tiles.pieces.col(i, lane);
+            dma16(r.at, off, __builtin_amdgcn_readfirstlane(lds + to + (i * NW + wave) * 1024));
+        }
+        r.at += WAYS * r.tile;
     };
 
     v4i q[KS];
     const Fragments<D> fr(lane);
-    const int own = L::keys(1, 0) + wave * 64 * D;
-    if (odd == 0) query_rows_in<D>(a, a.q + (int64_t)kvh * a.g * a.q_sh + (int64_t)i_lo * a.q_sn, a.q_sn, a.q_sh, i_lo, x0, lds + own, lane);
-    copy(odd, 0);
+    const int own = L::ROWS + wave * 64 * D;
+    if (way == 0) query_rows_in<D>(a, a.q + (int64_t)kvh * a.g * a.q_sh + (int64_t)i_lo * a.q_sn, a.q_sn, a.q_sh, i_lo, x0, lds + own, lane);
+    if (way < span.n) {
+        copy(k, way, L::keys(0, way));
+        if (L::VALUES_FIRST) copy(v, way, L::values(0, way));
+    }
     dma_wait<0>();
-    __syncthreads();
+    if (WAYS == 2) __syncthreads();
 #pragma unroll
     for (int s = 0; s < KS; s++) q[s] = fr.along(smem + own, s);
 #pragma unroll
     for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));
+    if (!L::VALUES_FIRST || AHEAD == 2) __syncthreads();               // (else the first tile's barrier comes before what lands over the rows)
+    if (!L::VALUES_FIRST && way < span.n) copy(v, way, L::values(0, way));
+    if (AHEAD == 2 && way + WAYS < span.n) copy(k, way + WAYS, L::keys(1, way)), copy(v, way + WAYS, L::values(1, way));
 
     RowState<D> st;
     st.clear();
     const float c = a.scale * kLog2e;
-    auto walk = [&](auto fine) {
-        for (int t = odd, slot = 0; t - odd < span.n; t += 2, slot ^= 1) {
-            dma_wait<0>();
-            __syncthreads();             // both tiles are visible; every wave is done with the two before (and has its rows)
-            copy(t + 2, slot ^ 1);
-            const int j0 = t * KT;
-            const Seen what = t >= span.n ? Seen::kNone : all.has(t) ? Seen::kAll : x0 < rows ? seen<KT>(a, wp_lo, wp_hi, len, j0) : Seen::kNone;
-            if (what != Seen::kNone) attend_tile<T, D, decltype(fine)::value>(st, q, lds + L::keys(slot, odd), lds + L::values(slot, odd), fr, what, j0, mask, c);
+    // Tile t, of `slot`, is visible once every wave has come here, and every wave is done with the one before; the one AHEAD steps further is requested.
+    auto turn = [&](int t, int slot) {
+        if (AHEAD == 2 && t + WAYS < span.n) dma_wait<2 * PIECES>();
+        else dma_wait<0>();
+        __syncthreads();
+        const int ahead = t + AHEAD * WAYS, to = slot == 0 ? AHEAD : slot - 1;
+        if (ahead < span.n) copy(k, ahead, L::keys(to, way)), copy(v, ahead, L::values(to, way));
+    };
+    auto walk = [&](auto fine, int t, int slot) {
+        for (; t - way < span.n; t += WAYS, slot = slot == AHEAD ? 0 : slot + 1) {
+            turn(t, slot);
+            const Seen what = t < all ? Seen::kAll : t < some ? Seen::kSome : Seen::kNone;
+            if (what != Seen::kNone) attend_tile<T, D, decltype(fine)::value>(st, q, lds + L::keys(slot, way), lds + L::values(slot, way), fr, what, t * KT, mask, c);
         }
     };
-    if (D <= 128 && span.n * KT <= kFineKeys) walk(std::bool_constant<D <= 128>{});
-    else walk(std::false_type{});
-    __syncthreads();                     // (no copy is in flight: a step's wait is for all of them, and the last step copies nothing)
-    float* meet = reinterpret_cast<float*>(smem) + wave * (D / 2) * 64 + lane;
-    float* stats = reinterpret_cast<float*>(smem + L::STATS) + wave * 128 + lane;
-    if (odd != 0) {
-        stats[0] = st.ref, stats[64] = st.sum;
+    if (D <= 128 && span.n * KT <= kFineKeys) {
+        walk(std::bool_constant<D <= 128>{}, way, 0);
+    } else {
+        const int direct = a.stats == nullptr ? all : 0;
+        int t = way, slot = 0;
+        while (t < direct) {
+#pragma unroll
+            for (int u = 0; u < L::SLOTS; u++) {                       // (slots known ahead)
+                turn(t, u);
+                attend_tile<T, D, false>(st, q, lds + L::keys(u, way), lds + L::values(u, way), fr, Seen::kAll, t * KT, mask, c);
+                t += WAYS;
+                slot = u == AHEAD ? 0 : u + 1;
+                if (t >= direct) break;
+            }
+        }
+        walk(std::false_type{}, t, slot);
+    }
+    __syncthreads();                     // (no copy is in flight: the last step's wait was for all of them)
+    if constexpr (WAYS == 2) {
+        float* meet = reinterpret_cast<float*>(smem) + wave * (D / 2) * 64 + lane;
+        float* stats = reinterpret_cast<float*>(smem + L::STATS) + wave * 128 + lane;
+        if (way != 0) {
+            stats[0] = st.ref, stats[64] = st.sum;
+#pragma unroll
+            for (int d = 0; d < D / 32; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) meet[(d * 16 + i) * 64] = st.acc[d][i];
+        }
+        __syncthreads();
+        if (way != 0 || x0 >= rows) return;
+        const float other = stats[0];
+        st.raise(other);
+        const float f = st.ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(other - st.ref);
+        st.sum = fmaf(stats[64], f, st.sum);
 #pragma unroll
         for (int d = 0; d < D / 32; d++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) meet[(d * 16 + i) * 64] = st.acc[d][i];
+            for (int i = 0; i < 16; i++) st.acc[d][i] = fmaf(meet[(d * 16 + i) * 64], f, st.acc[d][i]);
     }
-    __syncthreads();
-    if (odd != 0 || x0 >= rows) return;
-    const float other = stats[0];
-    st.raise(other);
-    const float f = st.ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(other - st.ref);
-    st.sum = fmaf(stats[64], f, st.sum);
-#pragma unroll
-    for (int d = 0; d < D / 32; d++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) st.acc[d][i] = fmaf(meet[(d * 16 + i) * 64], f, st.acc[d][i]);
-    finish_rows<T, D>(a, st, smem + wave * 128 * D, 0, kvh, x0, lane);
+    if (x0 < rows) finish_rows<T, D>(a, st, smem + wave * WAYS * 64 * D, 0, kvh, x0, lane);
 }
-template <int T, int D> __global__ __launch_bounds__(512, D == 64 ? 4 : 2) void packed_paired_kernel(PackedArgs a, int slots) {
-    using L = PairedLds<D>;
+constexpr int kPackedWaves(int D, int ways) { return ways == 1 ? kWindowWaves(D) : D == 64 ? 4 : 2; }
+template <int T, int D, int WAYS> __global__ __launch_bounds__(256 * WAYS, kPackedWaves(D, WAYS)) void packed_kernel(PackedArgs a, int slots) {
+    using L = PackedLds<D, WAYS>;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[L::BYTES];
     const HeadSlot at = spread_item((int)blockIdx.x, a.w.Hk, slots);
     if (at.slot >= slots) return;
     const Found f = find_slot<false>(a, a.w.g, L::NW * 32, at.slot);
     if (f.index >= f.n) return;
     const Sequence& s = f.s;
-    paired_body<T, D>(view(a.w, s, s.nq, f.b < a.B ? s.nk : 0), smem, at.head, (f.n - 1 - f.index) * L::NW * 32);
+    packed_body<T, D, WAYS>(view(a.w, s, s.nq, f.b < a.B ? s.nk : 0), smem, at.head, (f.n - 1 - f.index) * L::NW * 32);      // (the last rows first, as above)
 }
 template <int T, int D> __global__ __launch_bounds__(256) void packed_few_kernel(PackedArgs a, int slots) {
     using L = SplitLds<D>;
@@ -606,9 +625,9 @@ int64_t packed_slots(const PackedArgs& a, int rows) { return slots_total(a.rows_
 template <int T, int D> hipError_t launch_packed_td(const PackedArgs& a, hipStream_t st) {
     const int64_t slots = packed_slots(a, packed_rows(a));
     const dim3 grid((unsigned)spread_grid(a.w.Hk, slots));
-    if (a.form == PackedForm::kPaired) hipLaunchKernelGGL((packed_paired_kernel<T, D>), grid, dim3(512), 0, st, a, (int)slots);
+    if (a.form == PackedForm::kPaired) hipLaunchKernelGGL((packed_kernel<T, D, 2>), grid, dim3(512), 0, st, a, (int)slots);
     else if (a.form == PackedForm::kFew) hipLaunchKernelGGL((packed_few_kernel<T, D>), grid, dim3(256), 0, st, a, (int)slots);
-    else hipLaunchKernelGGL((packed_kernel<T, D>), grid, dim3(256), 0, st, a, (int)slots);
+    else hipLaunchKernelGGL((packed_kernel<T, D, 1>), grid, dim3(256), 0, st, a, (int)slots);
     return hipGetLastError();
 }
 template <int T> hipError_t launch_packed_t(const PackedArgs& a, hipStream_t st) {
