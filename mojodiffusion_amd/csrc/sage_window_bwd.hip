@@ -266,6 +266,11 @@ __device__ __forceinline__ Seen seen_by(const WindowArgs& w, int x0, int len, in
     if (x0 >= len || x0 > pb + w.right || (x1 < pa - w.left && x0 >= w.sinks)) return Seen::kNone;
     return x1 < len && x1 <= pa + w.right && (x0 >= pb - w.left || x1 < w.sinks) ? Seen::kAll : Seen::kSome;
 }
+// The tiles of 32 queries, by the first one's position, that all see all of a wave's keys, as far as one comparison can tell: what every tile of a walk would ask, answered once.
+__device__ __forceinline__ Range all_seeing(const WindowArgs& w, int x0, int len) {
+    const int x1 = x0 + 31, lo = x1 - w.right, hi = x1 < w.sinks ? kWindowFar : x0 + w.left - 31;
+    return Range{lo, x1 < len && hi >= lo ? (unsigned)(hi - lo) + 1u : 0u};
+}
 // Positions of queries p that see the lane's key: lo <= p <= hi.  (Up to the last query: the padding of its tile stands at further ones.)
 struct KeyMask {
     int lo, hi;
@@ -475,6 +480,7 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
     const int n_tiles = max(0, min(qs.nt * w.g - work.first, work.count));
     const Seeing real = seeing(w, p0, len);
     const KeyMask mask = key_mask(w, j, len, p0);
+    const Range all = all_seeing(w, x0, len);
     const uint32_t lds = lds_addr(smem);
     const typename QueryRows<D>::Pieces pieces(wave, lane);
     QueryRows<D> q(pieces, w.q + b * w.q_sb + (int64_t)kvh * w.g * w.q_sh, w.q_sh, w.q_sn, qs, real, work.first, lane);
@@ -585,7 +591,7 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
         if (t + 1 < n_tiles) copy(slot == 2 ? 0 : slot + 1);
         if (ROLE == 0 ? t >= n_tiles : t == 0) return;
         const int pa = walk.p;
-        const Seen what = seen_by(w, x0, len, pa, min(pa + 31, p_last));
+        const Seen what = all.has(pa) ? Seen::kAll : seen_by(w, x0, len, pa, min(pa + 31, p_last));
         walk.next();
         if (what != Seen::kNone) step(what, pa, ROLE == 0 ? slot : slot == 0 ? 2 : slot - 1, (t - ROLE) & 1);
     };
