@@ -828,11 +828,15 @@ hipError_t launch_window_bwd(const WindowBwdArgs& a, hipStream_t st) {
 }
 
 int packed_stats_rows(const PackedArgs& a) { return (int)slots_total(a.rows_q, 1, 32, a.B) * 32; }
-// Few key blocks: their pairs dealt to several workgroups until there are four to a compute unit, down to 16 pairs of the average.
+// Few key blocks: their pairs dealt to several workgroups until there are four to a compute unit, down to 8 pairs of the average and to no more than the root of
+// the pairs, since the join's time grows with the parts.  (A step of [5 x 75 rows, 16 on 2 x 64] down to 16 pairs 40 us, 8: 31; of [1000 rows, 8 on 1 x 64] with
+// 16 workgroups to a block 53, with 32 60.)
 void packed_bwd_plan(PackedBwdArgs* a) {
     const int64_t blocks = (a->p.rows_k + kWindowBwdKeys - 1) / kWindowBwdKeys, heads = a->w.w.Hk;
     const int64_t pairs = (a->p.rows_q / std::max(a->p.B, 1) + 31) / 32 * a->w.w.g;
-    a->chunks = (int)std::max<int64_t>(1, std::min(1024 / (blocks * heads), pairs / 16));
+    int64_t n = std::max<int64_t>(1, std::min(1024 / (blocks * heads), pairs / 8));
+    while (n > 1 && n * n > pairs) n--;
+    a->chunks = (int)n;
 }
 int64_t packed_bwd_parts(const PackedBwdArgs& a) { return a.chunks > 1 ? (int64_t)a.w.w.Hk * slots_total(a.p.rows_k, 1, kWindowBwdKeys, a.p.B) * a.chunks : 0; }
 bool packed_bwd_grid_ok(const PackedBwdArgs& a) {
