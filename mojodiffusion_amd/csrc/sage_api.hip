@@ -1355,7 +1355,7 @@ int mi355_sage_sdpa_window_decode(const void* Q, const void* K, const void* V, v
                           a, stream, workspace, workspace_bytes);
 }
 
-struct WindowBwdCarve { size_t lse2, delta, size, part, total; };
+struct WindowBwdCarve { size_t lse2, delta, size, part, q_part, total; };
 static WindowBwdCarve window_bwd_carve(WindowBwdArgs* a) {
     window_bwd_plan(a);
     a->sq_pad = (int)pad_to(a->w.Sq, 64);
@@ -1466,7 +1466,8 @@ static WindowBwdCarve packed_bwd_carve(PackedBwdArgs* a) {
     c.delta = align_up(rows);
     c.size = c.delta + align_up(rows);
     c.part = c.size + align_up(rows);
-    c.total = c.part + align_up((size_t)packed_bwd_parts(*a) * 2 * kWindowBwdKeys * a->w.w.D * sizeof(float));
+    c.q_part = c.part + align_up((size_t)packed_bwd_parts(*a) * 2 * kWindowBwdKeys * a->w.w.D * sizeof(float));
+    c.total = c.q_part + align_up((size_t)packed_bwd_q_part_rows(*a) * a->w.w.D * sizeof(float));
     return c;
 }
 
@@ -1510,6 +1511,7 @@ int mi355_sage_sdpa_packed_bwd(const void* Q, const void* K, const void* V, cons
     a.w.ndelta = reinterpret_cast<float*>(ws + c.delta);
     a.w.dsize = reinterpret_cast<float*>(ws + c.size);
     a.w.part = reinterpret_cast<float*>(ws + c.part);
+    a.q_part = reinterpret_cast<float*>(ws + c.q_part);
     const View q = make_view(Q, q_strides, q_off), k = make_view(K, k_strides, k_off), v = make_view(V, v_strides, v_off), d = make_view(dO, do_strides, do_off);
     w.q = q.p; w.q_sh = q.sh; w.q_sn = q.sn;
     w.k = k.p; w.k_sh = k.sh; w.k_sn = k.sn;

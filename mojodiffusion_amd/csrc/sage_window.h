@@ -103,10 +103,13 @@ struct PackedBwdArgs {
     PackedArgs p;                                // p.w: not used; the rest as the forward's
     WindowBwdArgs w;                             // lse2, ndelta, dsize [Hk * g, sq_pad]: sequence b's rows from (cu_q[b] / 32 + b) * 32 on
     int chunks;                                  // workgroups that the (head, query tile) pairs of a key block are dealt to; several: parts
+    int q_chunks;                                // workgroups that the key tiles of 128 rows are dealt to
+    float* q_part;                               // [head, slot, chunk, 128, D]
 };
 int packed_stats_rows(const PackedArgs& a);      // sq_pad
 void packed_bwd_plan(PackedBwdArgs* a);
 int64_t packed_bwd_parts(const PackedBwdArgs& a);
+int64_t packed_bwd_q_part_rows(const PackedBwdArgs& a);
 bool packed_bwd_grid_ok(const PackedBwdArgs& a);
 hipError_t launch_packed_bwd(const PackedBwdArgs& a, hipStream_t st);
 

@@ -96,8 +96,9 @@ template <int D> struct DqLds {
     static_assert(CENTRE + GROUPS * D * 4 <= OWN && kWaves * 64 * D <= CENTRE, "the centre lies behind the second slot and behind the rows on their way out");
 };
 
+// share, shares: which of the workgroups that the key tiles of these rows are dealt to; with several of them `part` takes the rows in fp32.
 template <int T, int D>
-__device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, int bh, int row0) {
+__device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, int bh, int row0, int share = 0, int shares = 1, float* part = nullptr) {
     using L = DqLds<D>;
     constexpr int NW = kWaves, CPR = D / 8, KS = D / 16, DB = D / 32;
     const WindowArgs& w = a.w;
@@ -115,13 +116,14 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
     const uint32_t lds = lds_addr(smem);
     const KeyTiles<D, NW> tiles(span, lds, wave, lane);
     const Range all = tiles.within(wp_hi - w.left, x0 < rows ? min(wp_lo + w.right, len - 1) : -1);
-    auto k = tiles.rows(w.k + b * w.k_sb + kvh * w.k_sh, w.k_sn), v = tiles.rows(w.v + b * w.v_sb + kvh * w.v_sh, w.v_sn);
+    const int each = (span.n + shares - 1) / shares, t_begin = min(share * each, span.n), t_end = min(t_begin + each, span.n);
+    auto k = tiles.rows(w.k + b * w.k_sb + kvh * w.k_sh, w.k_sn, t_begin), v = tiles.rows(w.v + b * w.v_sb + kvh * w.v_sh, w.v_sn, t_begin);
     const Fragments<D> fr(lane);
     v4i b1[KS], b2[KS];
     const uint32_t own = wave * 2 * 64 * D;
     query_rows_in<D>(w, w.q + b * w.q_sb + (int64_t)kvh * w.g * w.q_sh + (int64_t)i_lo * w.q_sn, w.q_sn, w.q_sh, i_lo, x0, lds + own, lane);
     query_rows_in<D>(w, a.dout + b * a.do_sb + (int64_t)kvh * w.g * a.do_sh + (int64_t)i_lo * a.do_sn, a.do_sn, a.do_sh, i_lo, x0, lds + own + 64 * D, lane);
-    if (span.n > 0) tiles.copy(k, 0, L::keys(0)), tiles.copy(v, 0, L::values(0));
+    if (t_end > t_begin) tiles.copy(k, t_begin, L::keys(0)), tiles.copy(v, t_begin, L::values(0));
     const int64_t at = ((int64_t)b * H + kvh * w.g + hg) * a.sq_pad + i;
     float lse = a.lse2[at], ndelta = a.ndelta[at], mul = w.scale * kWeightInv;
     if constexpr (T == kF16) mul = a.dsize[at];
@@ -160,10 +162,30 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
         const int t = span.first + (span.n - span.first - n) / 2;
         if (t >= 0 && t < span.n && keys_of(t) > keys_of(centre)) centre = t;
     }
+    auto take_centre = [&](int t, int slot) {
+        const int me = wave * 64 + lane_here(), ch = me % D, first = me / D * (32 / L::GROUPS), j0 = span.tile(t) * 32;
+        const uint8_t* kt = smem + L::keys(slot);
+        float sum = 0.0f;
+#pragma unroll 1
+        for (int r = first; r < first + 32 / L::GROUPS; r++) {
+            const float key = widen<T>(*reinterpret_cast<const uint16_t*>(kt + nat_off<CPR>(r, ch >> 3) + (ch & 7) * 2), 0);
+            sum += copied_key<32>(span, j0, j0 + r) == j0 + r ? key : 0.0f;
+        }
+        reinterpret_cast<float*>(smem + L::CENTRE)[me] = sum / (float)keys_of(t);
+    };
+    // Several workgroups: a row's dS sum to zero over all of them, so all take the same c; its tile is fetched ahead of the walk.
+    if (shares > 1 && t_end > t_begin) {
+        __syncthreads();                 // (every wave has its rows)
+        auto kc = tiles.rows(w.k + b * w.k_sb + kvh * w.k_sh, w.k_sn, centre);
+        tiles.copy(kc, centre, L::keys(1));
+        dma_wait<0>();
+        __syncthreads();
+        take_centre(centre, 1);
+    }
     auto tile = [&](int t, int slot) {
         dma_wait<0>();
         __syncthreads();                 // tile t is visible; every wave is done with tile t - 1
-        if (t + 1 < span.n) tiles.copy(k, t + 1, L::keys(slot + 1)), tiles.copy(v, t + 1, L::values(slot + 1));
+        if (t + 1 < t_end) tiles.copy(k, t + 1, L::keys(slot + 1)), tiles.copy(v, t + 1, L::values(slot + 1));
         const uint32_t keys = lds + L::keys(slot), values = lds + L::values(slot);
         const int j0 = span.tile(t) * 32;
         const Seen what = all.has(t) ? Seen::kAll : x0 < rows ? seen<32>(w, wp_lo, wp_hi, len, j0) : Seen::kNone;
@@ -199,30 +221,20 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
                                     v4i{(int)ds[j2 * 4], (int)ds[j2 * 4 + 1], (int)ds[j2 * 4 + 2], (int)ds[j2 * 4 + 3]}, acc[d]);
             }
         }
-        if (t == centre) {
-            const int me = wave * 64 + lane_here(), ch = me % D, first = me / D * (32 / L::GROUPS);
-            const uint8_t* kt = smem + L::keys(slot);
-            float sum = 0.0f;
-#pragma unroll 1
-            for (int r = first; r < first + 32 / L::GROUPS; r++) {
-                const float key = widen<T>(*reinterpret_cast<const uint16_t*>(kt + nat_off<CPR>(r, ch >> 3) + (ch & 7) * 2), 0);
-                sum += copied_key<32>(span, j0, j0 + r) == j0 + r ? key : 0.0f;
-            }
-            reinterpret_cast<float*>(smem + L::CENTRE)[me] = sum / (float)keys_of(t);
-        }
+        if (shares == 1 && t == centre) take_centre(t, slot);
     };
     if constexpr (D > 64) {
-        for (int t = 0; t < span.n; t++) tile(t, t & 1);
+        for (int t = t_begin; t < t_end; t++) tile(t, (t - t_begin) & 1);
     } else {                             // (slots known ahead: addresses stay in registers, the slots in the reads' offsets)
-        for (int t = 0; t < span.n; t += 2) {
+        for (int t = t_begin; t < t_end; t += 2) {
             tile(t, 0);
-            if (t + 1 < span.n) tile(t + 1, 1);
+            if (t + 1 < t_end) tile(t + 1, 1);
         }
     }
     __syncthreads();
     uint8_t* os = smem + wave * 64 * D;
     const int end_lane = lane_here(), end_half = end_lane >> 5;
-    if (span.n > 0) {
+    if (t_end > t_begin) {
         const float rs = sum_halves(ds_sum);
         const float* centre = reinterpret_cast<const float*>(smem + L::CENTRE);
 #pragma unroll
@@ -243,6 +255,14 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
         for (int d = 0; d < DB; d++)
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[d][e] = blind ? 0.0f : acc[d][e];
+    }
+    if (shares > 1) {
+        float* p = part + (wave * 32 + (end_lane & 31)) * D + end_half * 4;
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) *reinterpret_cast<v4f*>(p + d * 32 + g * 8) = v4f{acc[d][g * 4] * mul, acc[d][g * 4 + 1] * mul, acc[d][g * 4 + 2] * mul, acc[d][g * 4 + 3] * mul};
+        return;
     }
 #pragma unroll
     for (int d = 0; d < DB; d++) row_put<T, D>(os, acc[d], d, mul, end_lane);
@@ -695,18 +715,23 @@ template <int T, int D> __global__ __launch_bounds__(256) void packed_bwd_prep_k
     const Sequence s = sequence(a.p, b);
     prep_row<T, D>(view(a, s, s.nq, b < a.p.B ? s.nk : 0, b), h, i, (int64_t)h * a.w.sq_pad + i);
 }
-template <int T, int D>
+// SPLIT: the rows' key tiles are dealt to several workgroups.
+template <int T, int D, bool SPLIT>
 __global__ __launch_bounds__(kWaves * 64, D > 64 ? 2 : 4) void packed_bwd_kernel(PackedBwdArgs a, int q_slots, int k_slots) {
     constexpr int KV = PairLds<T, D>::BYTES;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[KV > DqLds<D>::BYTES ? KV : DqLds<D>::BYTES];
-    const int nq = (int)spread_grid(a.w.w.Hk, q_slots), id = (int)blockIdx.x;
+    const int shares = SPLIT ? a.q_chunks : 1, nq = (int)spread_grid(a.w.w.Hk, q_slots * shares), id = (int)blockIdx.x;
     if (id < nq) {
-        const HeadSlot at = spread_item(id, a.w.w.Hk, q_slots);
-        if (at.slot >= q_slots) return;
-        const Found f = find_slot<false>(a.p, a.w.w.g, kRowsWg, at.slot);
+        const HeadSlot at = spread_item(id, a.w.w.Hk, q_slots * shares);
+        if (at.slot >= q_slots * shares) return;
+        const int slot = SPLIT ? at.slot / shares : at.slot;
+        const Found f = find_slot<false>(a.p, a.w.w.g, kRowsWg, slot);
         if (f.index >= f.n) return;
         const Sequence& s = f.s;
-        dq_body<T, D>(view(a, s, s.nq, f.b < a.p.B ? s.nk : 0, f.b), smem, at.head, (f.n - 1 - f.index) * kRowsWg);      // (the last rows first: they see most keys)
+        const WindowBwdArgs v = view(a, s, s.nq, f.b < a.p.B ? s.nk : 0, f.b);
+        const int row0 = (f.n - 1 - f.index) * kRowsWg;                // (the last rows first: they see most keys)
+        if constexpr (SPLIT) dq_body<T, D>(v, smem, at.head, row0, at.slot - slot * shares, shares, a.q_part + ((int64_t)at.head * q_slots * shares + at.slot) * kRowsWg * D);
+        else dq_body<T, D>(v, smem, at.head, row0);
         return;
     }
     const HeadSlot at = spread_item(id - nq, a.w.w.Hk, k_slots * a.chunks);
@@ -727,37 +752,52 @@ __global__ __launch_bounds__(kWaves * 64, D > 64 ? 2 : 4) void packed_bwd_kernel
     if (wave < 2) dkdv_role<T, D, 0>(v, smem, at.head, work, wave, lane);
     else dkdv_role<T, D, 1>(v, smem, at.head, work, wave, lane);
 }
-// Their parts added up, in order, as above.
-template <int T, int D> __global__ __launch_bounds__(256) void packed_bwd_join_kernel(PackedBwdArgs a, int k_slots) {
-    constexpr int CPR = D / 8;
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= (int64_t)a.w.w.Hk * k_slots * 2 * kKeysWg * CPR) return;
-    const int col = (int)(at % CPR) * 8, key = (int)(at / CPR % kKeysWg), which = (int)(at / (CPR * kKeysWg) & 1);
-    const int item = (int)(at / (2 * CPR * kKeysWg)), kvh = item / k_slots, slot = item - kvh * k_slots;
-    const Found f = find_slot<true>(a.p, 1, kKeysWg, slot);
-    const Sequence& s = f.s;
-    const int j = f.index * kKeysWg + key;
-    if (j >= s.nk) return;
-    const float* p = a.w.part + (((int64_t)item * a.chunks * 2 + which) * kKeysWg + key) * D + col;
+// Eight channels of parts that lie `pitch` apart, added up in order, as above.
+template <int T> __device__ __forceinline__ void join_parts(const float* p, int n, int64_t pitch, uint16_t* out) {
     float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int c0 = 0; c0 < a.chunks; c0 += 8) {
+    for (int c0 = 0; c0 < n; c0 += 8) {
         v4f u[8], v[8];
 #pragma unroll
-        for (int n = 0; n < 8; n++) {
-            const float* at_c = p + (int64_t)min(c0 + n, a.chunks - 1) * 2 * kKeysWg * D;
-            u[n] = *reinterpret_cast<const v4f*>(at_c);
-            v[n] = *reinterpret_cast<const v4f*>(at_c + 4);
+        for (int m = 0; m < 8; m++) {
+            const float* at_c = p + min(c0 + m, n - 1) * pitch;
+            u[m] = *reinterpret_cast<const v4f*>(at_c);
+            v[m] = *reinterpret_cast<const v4f*>(at_c + 4);
         }
 #pragma unroll
-        for (int n = 0; n < 8; n++) {
-            if (c0 + n >= a.chunks) break;
+        for (int m = 0; m < 8; m++) {
+            if (c0 + m >= n) break;
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] += u[n][e], y[4 + e] += v[n][e];
+            for (int e = 0; e < 4; e++) y[e] += u[m][e], y[4 + e] += v[m][e];
         }
     }
-    const int64_t row = s.k0 + j;
-    uint16_t* out = which ? a.w.dv + kvh * a.w.dv_sh + row * a.w.dv_sn : a.w.dk + kvh * a.w.dk_sh + row * a.w.dk_sn;
-    *reinterpret_cast<u32x4*>(out + col) = u32x4{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7])};
+    *reinterpret_cast<u32x4*>(out) = u32x4{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7])};
+}
+// (A workgroup's threads are of one slot: 256 divides a slot's pieces.)
+template <int T, int D> __global__ __launch_bounds__(256) void packed_bwd_join_kernel(PackedBwdArgs a, int q_slots, int k_slots) {
+    constexpr int CPR = D / 8;
+    const int Hk = a.w.w.Hk, g = a.w.w.g;
+    const int64_t k_pieces = a.chunks > 1 ? (int64_t)Hk * k_slots * 2 * kKeysWg * CPR : 0;
+    int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at < k_pieces) {
+        const int col = (int)(at % CPR) * 8, key = (int)(at / CPR % kKeysWg), which = (int)(at / (CPR * kKeysWg) & 1);
+        const int item = (int)(at / (2 * CPR * kKeysWg)), kvh = item / k_slots, slot = item - kvh * k_slots;
+        const Found f = find_slot<true>(a.p, 1, kKeysWg, slot);
+        const int j = f.index * kKeysWg + key;
+        if (j >= f.s.nk) return;
+        const int64_t row = f.s.k0 + j;
+        join_parts<T>(a.w.part + (((int64_t)item * a.chunks * 2 + which) * kKeysWg + key) * D + col, a.chunks, 2 * kKeysWg * D,
+                      (which ? a.w.dv + kvh * a.w.dv_sh + row * a.w.dv_sn : a.w.dk + kvh * a.w.dk_sh + row * a.w.dk_sn) + col);
+        return;
+    }
+    at -= k_pieces;
+    if (a.q_chunks == 1 || at >= (int64_t)Hk * q_slots * kRowsWg * CPR) return;
+    const int col = (int)(at % CPR) * 8, r = (int)(at / CPR % kRowsWg), item = (int)(at / (CPR * kRowsWg)), kvh = item / q_slots, slot = item - kvh * q_slots;
+    const Found f = find_slot<false>(a.p, g, kRowsWg, slot);
+    const int x = (f.n - 1 - f.index) * kRowsWg + r;
+    if (f.index >= f.n || x >= f.s.nq * g) return;
+    const int i = x / g;
+    join_parts<T>(a.q_part + ((int64_t)item * a.q_chunks * kRowsWg + r) * D + col, a.q_chunks, kRowsWg * D,
+                  a.w.dq + (f.s.q0 + i) * a.w.dq_sn + (kvh * g + x - i * g) * a.w.dq_sh + col);
 }
 struct PackedGrid { int64_t q_slots, k_slots, prep, grid, join; };
 PackedGrid packed_grid(const PackedBwdArgs& a) {
@@ -766,15 +806,16 @@ PackedGrid packed_grid(const PackedBwdArgs& a) {
     g.q_slots = slots_total(a.p.rows_q, a.w.w.g, kRowsWg, a.p.B);
     g.k_slots = slots_total(a.p.rows_k, 1, kKeysWg, a.p.B);
     g.prep = (Hk * a.w.w.g * packed_stats_rows(a.p) * (D / 8) + 255) / 256;
-    g.grid = spread_grid(Hk, g.q_slots) + spread_grid(Hk, g.k_slots * a.chunks);
-    g.join = a.chunks > 1 ? (Hk * g.k_slots * 2 * kKeysWg * (D / 8) + 255) / 256 : 0;
+    g.grid = spread_grid(Hk, g.q_slots * a.q_chunks) + spread_grid(Hk, g.k_slots * a.chunks);
+    g.join = ((a.chunks > 1 ? Hk * g.k_slots * 2 * kKeysWg : 0) + (a.q_chunks > 1 ? Hk * g.q_slots * kRowsWg : 0)) * (D / 8) / 256;
     return g;
 }
 template <int T, int D> hipError_t launch_packed_td(const PackedBwdArgs& a, hipStream_t st) {
     const PackedGrid g = packed_grid(a);
     hipLaunchKernelGGL((packed_bwd_prep_kernel<T, D>), dim3((unsigned)g.prep), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((packed_bwd_kernel<T, D>), dim3((unsigned)g.grid), dim3(kWaves * 64), 0, st, a, (int)g.q_slots, (int)g.k_slots);
-    if (g.join > 0) hipLaunchKernelGGL((packed_bwd_join_kernel<T, D>), dim3((unsigned)g.join), dim3(256), 0, st, a, (int)g.k_slots);
+    if (a.q_chunks > 1) hipLaunchKernelGGL((packed_bwd_kernel<T, D, true>), dim3((unsigned)g.grid), dim3(kWaves * 64), 0, st, a, (int)g.q_slots, (int)g.k_slots);
+    else hipLaunchKernelGGL((packed_bwd_kernel<T, D, false>), dim3((unsigned)g.grid), dim3(kWaves * 64), 0, st, a, (int)g.q_slots, (int)g.k_slots);
+    if (g.join > 0) hipLaunchKernelGGL((packed_bwd_join_kernel<T, D>), dim3((unsigned)g.join), dim3(256), 0, st, a, (int)g.q_slots, (int)g.k_slots);
     return hipGetLastError();
 }
 
@@ -837,7 +878,14 @@ void packed_bwd_plan(PackedBwdArgs* a) {
     int64_t n = std::max<int64_t>(1, std::min(1024 / (blocks * heads), pairs / 8));
     while (n > 1 && n * n > pairs) n--;
     a->chunks = (int)n;
+    // Rows whose walk over the keys would take longer than the chip's average (four or two workgroups to a compute unit): their key tiles dealt out likewise, to no more
+    // than half the places, since two rounds gain nothing ([1292 rows, 30 x 64] in two parts 88 -> 103 us).  A step of [8000 rows, 1 x 64] 244 -> 120, [4000, 4 on 1 x 128] 221 -> 162,
+    // [2048, 8 x 128] 134 -> 112.
+    const int64_t tiles = (a->p.rows_k / std::max(a->p.B, 1) + 31) / 32, row_blocks = (a->p.rows_q * a->w.w.g + kRowsWg - 1) / kRowsWg * heads, places = a->w.w.D == 64 ? 1024 : 512;
+    const int64_t load = (row_blocks * tiles + blocks * heads * pairs) / (a->w.w.right < kWindowFar ? 2 : 1) / places;
+    a->q_chunks = (int)std::max<int64_t>(1, std::min({tiles / std::max<int64_t>(load, 8), tiles / 8, places / 2 / row_blocks, (int64_t)8}));
 }
+int64_t packed_bwd_q_part_rows(const PackedBwdArgs& a) { return a.q_chunks > 1 ? a.w.w.Hk * slots_total(a.p.rows_q, a.w.w.g, kRowsWg, a.p.B) * a.q_chunks * kRowsWg : 0; }
 int64_t packed_bwd_parts(const PackedBwdArgs& a) { return a.chunks > 1 ? (int64_t)a.w.w.Hk * slots_total(a.p.rows_k, 1, kWindowBwdKeys, a.p.B) * a.chunks : 0; }
 bool packed_bwd_grid_ok(const PackedBwdArgs& a) {
     const PackedGrid g = packed_grid(a);

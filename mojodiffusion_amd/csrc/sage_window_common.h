@@ -160,9 +160,9 @@ template <int D, int NW> struct KeyTiles {
         int64_t tile;
         uint32_t sn, off[Pieces::N];
     };
-    __device__ Rows rows(const uint16_t* head, int64_t sn) const {
+    __device__ Rows rows(const uint16_t* head, int64_t sn, int t = 0) const {      // (from tile t on)
         Rows r;
-        r.at = head + (int64_t)span.tile(0) * KT * sn;
+        r.at = head + (int64_t)span.tile(t) * KT * sn;
         r.tile = KT * sn;
         r.sn = (uint32_t)sn * 2u;
 #pragma unroll

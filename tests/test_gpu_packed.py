@@ -107,11 +107,25 @@ FORMS = [
     ([1111], None, 24, 24, 64, BF, True, 9),
     ([95, 1030], [1500, 2100], 10, 10, 128, BF, True, 0),
 ]
+LONG_WALKS = [
+    # few rows that walk many keys: gradients in parts; queries before the first key among them
+    ([900], [700], 6, 2, 64, BF, True, 3),
+    ([900], [700], 4, 4, 128, FP, True, 0),
+    ([600], [2000], 8, 2, 128, BF, False, 2),
+    ([1, 1], [1800, 600], 4, 4, 64, FP, True, 0),
+    ([700, 0, 300], [900, 1400, 40], 3, 1, 128, BF, True, 1),
+]
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("nq,nk,Hq,Hk,D,dtype,causal,tail", FORMS)
 def test_packed_in_larger_grids(nq, nk, Hq, Hk, D, dtype, causal, tail):
+    test_packed(nq, nk, Hq, Hk, D, dtype, causal, tail)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nk,Hq,Hk,D,dtype,causal,tail", LONG_WALKS)
+def test_packed_long_walks(nq, nk, Hq, Hk, D, dtype, causal, tail):
     test_packed(nq, nk, Hq, Hk, D, dtype, causal, tail)
 
 
