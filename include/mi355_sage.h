@@ -578,8 +578,7 @@ int mi355_sage_sdpa_packed_bwd(
  * value stays within e4m3's 448, and at least 2^-100 (what lies below 2^-110 becomes zero).  While a block fills, its scale only rises; codes that are there are then rounded
  * again, which changes those that leave e4m3's normal range and no others.  A value that is not finite becomes NaN and does not count for the scale.
  * page_table: int32 [B, table_width], rows table_stride apart: the pages of a sequence's tokens in order; only the entries that its tokens need are looked at.
- * kv_lens: int32 [B], tokens of a sequence with the new ones among them.  Both on the device.  A length beyond the table counts as the
- * table's table_width * page tokens, one below zero as zero.
+ * kv_lens: int32 [B], tokens of a sequence with the new ones among them; below zero counts as zero.  Both on the device.
  *
  * Appends the last tokens of every sequence: token i of the n new ones of sequence b stands at kv_lens[b] - n + i.  K, V [B,Hk,N,D] (n = N for
  * every sequence), or, with cu_seqlens (int32 [B+1] on the device, not falling; the first counts as 0), sequences that lie one behind the other in [1,Hk,N,D], rows cu_seqlens[b] .. cu_seqlens[b+1] - 1.
@@ -602,7 +601,7 @@ int mi355_sage_kv_append(
 
 /* Attention of the last N_q tokens of every sequence over the cache: query i of sequence b stands at kv_lens[b] - N_q + i and sees the keys up to
  * itself; one before a sequence's first token gives zeros.  Q, O [B,Hq,N_q,D] of `type`, Hq a multiple of Hk: query heads h Hq/Hk .. share key head
- * h.  Any N_q; meant for few.  Keys behind a sequence's length are never part of a result, whatever their codes are.  A NaN in a key that a query sees gives NaN in
+ * h.  Any N_q; meant for few.  A length beyond the table counts as its table_width * page tokens.  Keys behind a sequence's length are never part of a result, whatever their codes are.  A NaN in a key that a query sees gives NaN in
  * its row, one in a value that some query of the call sees may reach the rows of queries before it; a page outside [0, pages) gives NaN in the rows of its sequence.  Workspace: mi355_sage_paged_workspace_bytes(...) bytes,
  * 256-byte aligned, or NULL for the library's per-stream buffer (the rules of mi355_sage_sdpa_bf16).  The same bits on every call. */
 size_t mi355_sage_paged_workspace_bytes(int B, int Hq, int Hk, int N_q, int D, int table_width, int page);
