@@ -207,6 +207,7 @@ def filled(lens, Hk, D, page, seed, spare=2):
 
 def spoil(cache, ids, lens, page):
     """NaN in every code behind the sequences' lengths, and in every page that no sequence has."""
+    ids = ids.cpu()
     used = torch.zeros((*cache.k.shape[:2], 32), dtype=torch.bool)
     for b, n in enumerate(lens):
         for j in range(0, n):
@@ -257,6 +258,21 @@ def test_attention_over_the_cache(lens, Sq, Hq, Hk, D, dtype, page):
     # a longer table, whose further entries are no pages, may deal the blocks otherwise; the values stay within the bounds
     longer = torch.cat((ids, torch.full((len(lens), 40), -7, dtype=torch.int32).cuda()), 1)
     check_forward(C.sdpa_paged(q.cuda(), cache, longer, lens_t, D ** -0.5), None, want, dtype)
+
+
+DEALT = [
+    # larger lists: rows' own shares of 16 blocks; even shares that straddle rows, by blocks and by more rows than are given their own
+    ([9000, 33], 1, 30, 30, 64, FP, 128),
+    ([20000, 700], 1, 30, 30, 64, BF, 256),
+    ([n * 13 % 97 for n in range(520)], 1, 8, 4, 64, BF, 32),
+    ([n * 29 % 300 for n in range(90)], 9, 24, 12, 128, FP, 64),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,Sq,Hq,Hk,D,dtype,page", DEALT)
+def test_attention_over_larger_lists(lens, Sq, Hq, Hk, D, dtype, page):
+    test_attention_over_the_cache(lens, Sq, Hq, Hk, D, dtype, page)
 
 
 @pytest.mark.gpu
