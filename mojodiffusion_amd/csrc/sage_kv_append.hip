@@ -198,7 +198,8 @@ __device__ __forceinline__ void append_block(const KvAppendArgs& a, uint8_t* tur
     if (tid == 0) c.ks[unit] = power_of_two(ek), c.vs[unit] = power_of_two(ev);
 }
 
-// HB heads of a token to a group of lanes, as in sage_norm_rope.hip.
+// HB heads of a token to a group of lanes, as in sage_norm_rope.hip.  (Two: four take registers from the other workgroups too; [3 x 1153 tokens, 18 + 6 heads x 256] 22.0
+// and 20.7 us, one head 21.9; [31234 tokens, 48 + 12 x 128] 224, 224 and 272.)
 template <int T, int D, int HB> __device__ __forceinline__ void rotate_queries(const KvAppendArgs& a, int wg) {
     constexpr int LPR = D / 16, GROUPS = 2 * D / LPR;
     const int nblk = (a.Hq + HB - 1) / HB, item = wg * GROUPS + (int)threadIdx.x / LPR, token = item / nblk, blk = item % nblk;
@@ -236,7 +237,7 @@ template <int T, int D, int HB> __device__ __forceinline__ void rotate_queries(c
     }
 }
 
-constexpr int kHeads = 4;
+constexpr int kHeads = 2;
 template <int T, int D> __global__ __launch_bounds__(2 * D) void kv_append_kernel(KvAppendArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t turned[D * (kKvBlock + 4)];
     __shared__ float tops[2 * D / 64][2];
