@@ -53,7 +53,7 @@ struct PagedArgs {
     int64_t q_sb, q_sh, q_sn, o_sb, o_sh, o_sn;
     int B, g, Sq, D, type;                       // g query heads share a key head
     float scale;
-    int wgs, more;                               // workgroups that the blocks are dealt to (paged_plan)
+    int wgs, more, least;                        // workgroups that the blocks are dealt to, blocks of a share at the least (paged_plan)
     float *part, *part_ml;                       // [workgroup, 2, rows, D], [workgroup, 2, rows, 2]: parts of rows that several workgroups share
 };
 int paged_rows(const PagedArgs& a);              // rows of a part: 16 or 32

@@ -92,10 +92,10 @@ __device__ __forceinline__ int wave_scan(int x) {
 }
 
 // The list of blocks: sequence after sequence, in each head after head, row block after row block, block after block.
-// The share of a workgroup: all of them evenly, eight at the least (two to a wave), and at the least half the root of the longest sequence's
-// blocks, since the second launch's time grows with the parts as the shares shrink.  Where shares are small (up to 16) a workgroup that had the
+// The share of a workgroup: all of them evenly, eight at the least (two to a wave; 16 from 96 rows on, 32 from 192: fewer parts where the chip is full without them), and at the least half the root of the longest sequence's
+// blocks, since the second launch's time grows with the parts as the shares shrink.  Where shares are small (up to 32) a workgroup that had the
 // end of one row's blocks and the beginning of another's would go through the chain of latencies twice, and all would wait for it: there every row's blocks are
-// divided into shares of their own, of 8 or 16.
+// divided into shares of their own, of 8, 16 or 32.
 struct Deal {
     int total, per;
     int len;                             // of the lane's sequence, of the first 64
@@ -114,8 +114,8 @@ __device__ __forceinline__ Deal deal(const PagedArgs& a, int mult, int lane) {
     }
     d.total = wave_sum(sum) * mult;
     most = wave_max(most);
-    d.per = max(max((d.total + a.wgs - 1) / a.wgs, 8), (int)(0.5f * sqrtf((float)most)));
-    d.shift = a.more == 0 || d.per > 16 ? 0 : d.per > 8 ? 4 : 3;
+    d.per = max(max((d.total + a.wgs - 1) / a.wgs, a.least), (int)(0.5f * sqrtf((float)most)));
+    d.shift = a.more == 0 || d.per > 32 ? 0 : d.per > 16 ? 5 : d.per > 8 ? 4 : 3;
     if (d.shift > 0) d.per = 1;          // (places of the list)
     return d;
 }
@@ -444,12 +444,18 @@ bool paged_shared(const PagedArgs& a) {
     const int64_t most = (int64_t)a.pool.width << a.pool.sub, per = std::max<int64_t>(8, (paged_tiles(a) + a.wgs - 1) / a.wgs);
     return most > kJoinParts * per;
 }
+// No row of the table's length has more blocks than a share of its own: nothing to add up.  (Shares are the rows' own up to 32 blocks: see deal.)
+bool paged_whole(const PagedArgs& a) {
+    const int64_t most = std::max<int64_t>(1, (int64_t)a.pool.width << a.pool.sub);
+    return a.more > 0 && most <= a.least && paged_tiles(a) <= 32 * (int64_t)a.wgs;
+}
 int64_t all_rows(const PagedArgs& a) { return (int64_t)a.B * a.pool.Hk * a.Sq * a.g; }
 
 template <int T, int D> hipError_t launch_td(const PagedArgs& a, hipStream_t st) {
     if (paged_rows(a) == 16) hipLaunchKernelGGL((paged_kernel<T, D, 1>), dim3((unsigned)(a.wgs + a.more)), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((paged_kernel<T, D, 2>), dim3((unsigned)(a.wgs + a.more)), dim3(256), 0, st, a);
     const int64_t rows = all_rows(a);
+    if (paged_whole(a)) return hipGetLastError();
     if (paged_shared(a)) hipLaunchKernelGGL((paged_join_kernel<T, D, true>), dim3((unsigned)rows), dim3(256), 0, st, a, paged_rows(a), (int)rows);
     else hipLaunchKernelGGL((paged_join_kernel<T, D, false>), dim3((unsigned)std::min<int64_t>((rows + 3) / 4, 4096)), dim3(256), 0, st, a, paged_rows(a), (int)rows);
     return hipGetLastError();
@@ -472,6 +478,7 @@ void paged_plan(PagedArgs* a) {
     a->wgs = (int)std::min<int64_t>(1024, std::max<int64_t>(1, (paged_tiles(*a) + 7) / 8));
     const int64_t units = (int64_t)a->B * a->pool.Hk * (((int64_t)a->Sq * a->g + paged_rows(*a) - 1) / paged_rows(*a));
     a->more = units <= 2048 ? (int)units : 0;
+    a->least = units < 96 ? 8 : units < 192 ? 16 : 32;
 }
 size_t paged_part_bytes(const PagedArgs& a) { return (size_t)(a.wgs + a.more) * 2 * paged_rows(a) * (a.D + 2) * sizeof(float); }
 
