@@ -54,7 +54,9 @@ template <int D> struct RowState {
 // taken from O, on a padded batch with sinks: 0.0027 without, 0.0024 with it; the products are a small part of what such a workgroup does).  By the keys of a workgroup, not of
 // a row: rows of short windows in longer spans gain nothing from it (window 16 + 1 on [1,1024,heads,64], dQ: 0.00236 without it, one head to a group, 0.00234 with it, four).
 constexpr int kFineKeys = 128;
-template <int T, int D, bool FINE, class Mask>
+// LATE: whether the reference is high enough is seen from the tile's sum, after the weights, instead of from its largest score; where it is not, they are formed again.  A fifth
+// of the vector instructions besides the exponentials go ([31234 rows in 6, 48 on 12 x 128] 2223 -> 2148 us, full [11696 rows in 4, 30 x 128] 629 -> 607).
+template <int T, int D, bool FINE, bool LATE = false, class Mask>
 __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 16], uint32_t kt, uint32_t vt, const Fragments<D>& kept,
                                             Seen what, int j0, const Mask& m, float c) {
     constexpr int KS = D / 16, DB = D / 32;
@@ -68,23 +70,38 @@ __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = rel.sees((i >> 2) * 8 + (i & 3)) ? s[i] : -INFINITY;
     }
-    float top = s[0];
+    auto highest = [&] {
+        float top = s[0];
 #pragma unroll
-    for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
-    top = max_halves(top) * c;
-    // A new reference only where the old one lies more than 8 below: the weights stay under 2^8, and the sums have
-    // room for that; O is multiplied on few tiles instead of on most.
-    if (__any(top > st.ref + 8.0f)) st.raise(top);
-    const float ref = st.ref == -INFINITY ? 0.0f : st.ref;       // (no key so far: every weight is exp2(-inf))
+        for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
+        return max_halves(top) * c;
+    };
     uint32_t p[8], fine[FINE ? 8 : 1];
-    float part[2] = {0.0f, 0.0f};
+    float part[2];
+    auto weights = [&](float ref) {
+        part[0] = part[1] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ref)), y = __builtin_amdgcn_exp2f(fmaf(s[i + 1], c, -ref));
-        part[0] += x;
-        part[1] += y;
-        p[i >> 1] = pack2<T>(x, y);
-        if constexpr (FINE) fine[i >> 1] = pack2<T>(rounded_off<T>(x), rounded_off<T>(y));
+        for (int i = 0; i < 16; i += 2) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ref)), y = __builtin_amdgcn_exp2f(fmaf(s[i + 1], c, -ref));
+            part[0] += x;
+            part[1] += y;
+            p[i >> 1] = pack2<T>(x, y);
+            if constexpr (LATE) asm volatile("" : "+v"(p[i >> 1]));
+            if constexpr (FINE) fine[i >> 1] = pack2<T>(rounded_off<T>(x), rounded_off<T>(y));
+        }
+    };
+    // A new reference only where the old one lies more than 8 below: the weights stay under 2^8, and the sums have
+    // room for that; O is multiplied on few tiles instead of on most.  (No key so far: every weight is exp2(-inf).)
+    if constexpr (LATE) {
+        weights(st.ref);
+        if (__any(part[0] + part[1] > 256.0f || st.ref == -INFINITY)) {
+            st.raise(highest());
+            weights(st.ref == -INFINITY ? 0.0f : st.ref);
+        }
+    } else {
+        const float top = highest();
+        if (__any(top > st.ref + 8.0f)) st.raise(top);
+        weights(st.ref == -INFINITY ? 0.0f : st.ref);
     }
     st.sum += part[0] + part[1];
 #pragma unroll
@@ -493,6 +510,7 @@ template <int T, int D, int WAYS> __device__ __forceinline__ void packed_body(co
     using L = PackedLds<D, WAYS>;
     using Tiles = KeyTiles<D, L::NW>;
     constexpr int NW = L::NW, KT = L::KT, KS = D / 16, AHEAD = L::SLOTS - 1, PIECES = Tiles::Pieces::N;
+    constexpr bool LATE = WAYS == 1;     // (the first tile's weights twice: too much of a short walk that two waves share)
     const int rows = a.Sq * a.g;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & (NW - 1), way = WAYS == 2 ? __builtin_amdgcn_readfirstlane(tid >> 8) : 0;
@@ -556,7 +574,7 @@ template <int T, int D, int WAYS> __device__ __forceinline__ void packed_body(co
         for (; t - way < span.n; t += WAYS, slot = slot == AHEAD ? 0 : slot + 1) {
             turn(t, slot);
             const Seen what = t < all ? Seen::kAll : t < some ? Seen::kSome : Seen::kNone;
-            if (what != Seen::kNone) attend_tile<T, D, decltype(fine)::value>(st, q, lds + L::keys(slot, way), lds + L::values(slot, way), fr, what, t * KT, mask, c);
+            if (what != Seen::kNone) attend_tile<T, D, decltype(fine)::value, LATE && !decltype(fine)::value>(st, q, lds + L::keys(slot, way), lds + L::values(slot, way), fr, what, t * KT, mask, c);
         }
     };
     if (D <= 128 && span.n * KT <= kFineKeys) {
@@ -568,7 +586,7 @@ template <int T, int D, int WAYS> __device__ __forceinline__ void packed_body(co
 #pragma unroll
             for (int u = 0; u < L::SLOTS; u++) {                       // (slots known ahead)
                 turn(t, u);
-                attend_tile<T, D, false>(st, q, lds + L::keys(u, way), lds + L::values(u, way), fr, Seen::kAll, t * KT, mask, c);
+                attend_tile<T, D, false, LATE>(st, q, lds + L::keys(u, way), lds + L::values(u, way), fr, Seen::kAll, t * KT, mask, c);
                 t += WAYS;
                 slot = u == AHEAD ? 0 : u + 1;
                 if (t >= direct) break;
