@@ -79,12 +79,11 @@ __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 
     uint32_t p[8], fine[FINE ? 8 : 1];
     float part[2];
     auto weights = [&](float ref) {
-        part[0] = part[1] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
             const float x = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ref)), y = __builtin_amdgcn_exp2f(fmaf(s[i + 1], c, -ref));
-            part[0] += x;
-            part[1] += y;
+            part[0] = i == 0 ? x : part[0] + x;
+            part[1] = i == 0 ? y : part[1] + y;
             p[i >> 1] = pack2<T>(x, y);
             if constexpr (LATE) asm volatile("" : "+v"(p[i >> 1]));
             if constexpr (FINE) fine[i >> 1] = pack2<T>(rounded_off<T>(x), rounded_off<T>(y));
@@ -532,11 +531,16 @@ template <int T, int D, int WAYS> __device__ __forceinline__ void packed_body(co
     k.at += way * k.tile;
     v.at += way * v.tile;
     auto copy = [&](typename Tiles::Rows& r, int t, int to) {
+        auto place = [&](int i) { return __builtin_amdgcn_readfirstlane(lds + to + (i * NW + wave) * 1024); };
+        if (PIECES > 1 && t < whole) {
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) {
-            const int row = tiles.pieces.row(i);
-            const uint32_t off = t < whole ? r.off[i] : (uint32_t)(min(t * KT + row, span.hi) - t * KT) * r.sn + tiles.pieces.col(i, lane);
-            dma16(r.at, off, __builtin_amdgcn_readfirstlane(lds + to + (i * NW + wave) * 1024));
+            for (int i = 0; i < PIECES; i++) dma16(r.at, r.off[i], place(i));
+        } else {
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) {
+                const uint32_t last = (uint32_t)(min(t * KT + tiles.pieces.row(i), span.hi) - t * KT) * r.sn + tiles.pieces.col(i, lane);
+                dma16(r.at, t < whole ? r.off[i] : last, place(i));
+            }
         }
         r.at += WAYS * r.tile;
     };
