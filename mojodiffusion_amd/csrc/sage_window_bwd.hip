@@ -390,14 +390,20 @@ template <int D> struct QueryRows {
         for (int n = 0; n < Pieces::N; n++) off[n] = p.row(n) * sn + p.col(n, lane);
     }
     __device__ void copy(const Pieces& p, uint32_t to, int wave, int lane) {
+        auto place = [&](int n) { return __builtin_amdgcn_readfirstlane(to + (n * kWaves + wave) * 1024); };
+        if (Pieces::N > 1 && whole.has(qt)) {
 #pragma unroll
-        for (int n = 0; n < Pieces::N; n++) {
-            uint32_t o = off[n];
-            if (!whole.has(qt)) {        // (every tile that is copied holds one of them)
-                const int i0 = (t0 + qt) * 32;
-                o = (uint32_t)min(max(p.row(n), rows.lo - i0), rows.hi - i0) * sn + p.col(n, lane);
+            for (int n = 0; n < Pieces::N; n++) dma16(at, off[n], place(n));
+        } else {
+#pragma unroll
+            for (int n = 0; n < Pieces::N; n++) {
+                uint32_t o = off[n];
+                if (!whole.has(qt)) {    // (every tile that is copied holds one of them)
+                    const int i0 = (t0 + qt) * 32;
+                    o = (uint32_t)min(max(p.row(n), rows.lo - i0), rows.hi - i0) * sn + p.col(n, lane);
+                }
+                dma16(at, o, place(n));
             }
-            dma16(at, o, __builtin_amdgcn_readfirstlane(to + (n * kWaves + wave) * 1024));
         }
         const bool last = qt == nt - 1;
         at += last ? turn : tile;

@@ -170,14 +170,20 @@ template <int D, int NW> struct KeyTiles {
         return r;
     }
     __device__ void copy(Rows& r, int t, int to) const {
+        auto place = [&](int i) { return __builtin_amdgcn_readfirstlane(lds + to + (i * NW + wave) * 1024); };
+        if (Pieces::N > 1 && whole.has(t)) {
 #pragma unroll
-        for (int i = 0; i < Pieces::N; i++) {
-            uint32_t off = r.off[i];
-            if (!whole.has(t)) {
-                const int j0 = span.tile(t) * KT;
-                off = (uint32_t)(copied_key<KT>(span, j0, j0 + pieces.row(i)) - j0) * r.sn + pieces.col(i, lane);
+            for (int i = 0; i < Pieces::N; i++) dma16(r.at, r.off[i], place(i));
+        } else {
+#pragma unroll
+            for (int i = 0; i < Pieces::N; i++) {
+                uint32_t off = r.off[i];
+                if (!whole.has(t)) {
+                    const int j0 = span.tile(t) * KT;
+                    off = (uint32_t)(copied_key<KT>(span, j0, j0 + pieces.row(i)) - j0) * r.sn + pieces.col(i, lane);
+                }
+                dma16(r.at, off, place(i));
             }
-            dma16(r.at, off, __builtin_amdgcn_readfirstlane(lds + to + (i * NW + wave) * 1024));
         }
         r.at += (t + 1 == span.first ? span.next - t : 1) * r.tile;        // (from the tiles with sinks to the window's)
     }
