@@ -192,7 +192,7 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
         const int j0 = span.tile(t) * 32;
         const Seen what = all.has(t) ? Seen::kAll : x0 < rows ? seen<32>(w, wp_lo, wp_hi, len, j0) : Seen::kNone;
         if (what != Seen::kNone) {
-            const Fragments<D> f = D > 64 ? fr.fresh() : fr;
+            const Fragments<D>& f = fr;
             v16f s, g;
             if (what == Seen::kAll) {
                 s = product<T>(lds_read(keys + f.nat), b1[0], v16f{});
@@ -549,7 +549,7 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
 
     // One tile of this wave's: scores (P wave: Q K^T, S wave: dO V^T - Delta), then the product with the rows (dO, Q) of the same tile.
     auto step = [&](Seen what, int pa, int slot, int parity) {
-        const Fragments<D> f = D > 64 ? fr.fresh() : fr;
+        const Fragments<D>& f = fr;
         const uint32_t score = lds + (ROLE == 0 ? L::q(slot) : L::d(slot)), rows = lds + (ROLE == 0 ? L::d(slot) : L::q(slot));
         const uint8_t* stats = smem + slot * 256 + ROLE * 128 + half * 16;
         v16f s;
