@@ -103,6 +103,7 @@ template <int T, int D>
 __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, int bh, int row0, int share = 0, int shares = 1, float* part = nullptr) {
     using L = DqLds<D>;
     constexpr int NW = kWaves, CPR = D / 8, KS = D / 16, DB = D / 32;
+    constexpr bool EARLY = D > 64;
     const WindowArgs& w = a.w;
     const int rows = w.Sq * w.g, H = w.Hk * w.g;
     const int b = bh / w.Hk, kvh = bh % w.Hk;
@@ -193,20 +194,36 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
         const Seen what = all.has(t) ? Seen::kAll : x0 < rows ? seen<32>(w, wp_lo, wp_hi, len, j0) : Seen::kNone;
         if (what != Seen::kNone) {
             const Fragments<D>& f = fr;
+            // (128 channels leave room to request all fragments ahead of the first product, and those of the last product ahead of the exponentials)
+            v4i kf[EARLY ? KS : 1], vf[EARLY ? KS : 1];
+            auto key = [&](int ks) { return EARLY ? kf[EARLY ? ks : 0] : lds_read(keys + (f.nat ^ (ks << 5))); };
+            auto value = [&](int ks) { return EARLY ? vf[EARLY ? ks : 0] : lds_read(values + (f.nat ^ (ks << 5))); };
+            if constexpr (EARLY) {
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) kf[ks] = lds_read(keys + (f.nat ^ (ks << 5))), vf[ks] = lds_read(values + (f.nat ^ (ks << 5)));
+                __builtin_amdgcn_sched_barrier(0);
+            }
             v16f s, g;
             if (what == Seen::kAll) {
-                s = product<T>(lds_read(keys + f.nat), b1[0], v16f{});
+                s = product<T>(key(0), b1[0], v16f{});
             } else {
                 const RowMask rel = mask.from(j0 + (lane_here() >> 5) * 4);
 #pragma unroll
                 for (int e = 0; e < 16; e++) s[e] = rel.sees((e >> 2) * 8 + (e & 3)) ? 0.0f : -INFINITY;
-                s = product<T>(lds_read(keys + f.nat), b1[0], s);
+                s = product<T>(key(0), b1[0], s);
             }
-            g = product<T>(lds_read(values + f.nat), b2[0], v16f{});
+            g = product<T>(value(0), b2[0], v16f{});
 #pragma unroll
             for (int ks = 1; ks < KS; ks++) {
-                s = product<T>(lds_read(keys + (f.nat ^ (ks << 5))), b1[ks], s);
-                g = product<T>(lds_read(values + (f.nat ^ (ks << 5))), b2[ks], g);
+                s = product<T>(key(ks), b1[ks], s);
+                g = product<T>(value(ks), b2[ks], g);
+            }
+            v4i rf[EARLY ? 2 * DB : 1];
+            auto row = [&](int m) { return lds_read_across(keys + (f.tr[0] ^ (m % DB << 6)) + m / DB * 32 * D, keys + (f.tr[1] ^ (m % DB << 6)) + m / DB * 32 * D); };
+            if constexpr (EARLY) {
+#pragma unroll
+                for (int m = 0; m < 2 * DB; m++) rf[m] = row(m);
+                __builtin_amdgcn_sched_barrier(0);
             }
             uint32_t ds[8];
 #pragma unroll
@@ -219,8 +236,7 @@ __device__ __forceinline__ void dq_body(const WindowBwdArgs& a, uint8_t* smem, i
 #pragma unroll
             for (int m = 0; m < 2 * DB; m++) {
                 const int j2 = m / DB, d = m % DB;
-                acc[d] = product<T>(lds_read_across(keys + (f.tr[0] ^ (d << 6)) + j2 * 32 * D, keys + (f.tr[1] ^ (d << 6)) + j2 * 32 * D),
-                                    v4i{(int)ds[j2 * 4], (int)ds[j2 * 4 + 1], (int)ds[j2 * 4 + 2], (int)ds[j2 * 4 + 3]}, acc[d]);
+                acc[d] = product<T>(EARLY ? rf[EARLY ? m : 0] : row(m), v4i{(int)ds[j2 * 4], (int)ds[j2 * 4 + 1], (int)ds[j2 * 4 + 2], (int)ds[j2 * 4 + 3]}, acc[d]);
             }
         }
         if (shares == 1 && t == centre) take_centre(t, slot);
@@ -552,10 +568,26 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
         const Fragments<D>& f = fr;
         const uint32_t score = lds + (ROLE == 0 ? L::q(slot) : L::d(slot)), rows = lds + (ROLE == 0 ? L::d(slot) : L::q(slot));
         const uint8_t* stats = smem + slot * 256 + ROLE * 128 + half * 16;
+        // (128 channels leave room to request all fragments ahead of the first product: two waves to a SIMD do not cover the reads' latencies.  [2652 rows in 3, 30 x 128] a step
+        // 279 -> 260 us with what dq_body does likewise; at 64 channels, where that takes a wave of four, no gain)
+        constexpr bool EARLY = D > 64;
+        v4i sf[EARLY ? KS : 1], rf[EARLY ? 2 * DB : 1];
+        auto scores = [&](int ks) { return EARLY ? sf[EARLY ? ks : 0] : lds_read(score + (f.nat ^ (ks << 5))); };
+        auto row = [&](int m) {
+            const uint32_t lo = (f.tr[0] ^ (m % DB << 6)) + m / DB * 32 * D, hi = (f.tr[1] ^ (m % DB << 6)) + m / DB * 32 * D;
+            return lds_read_across(rows + lo, rows + hi);
+        };
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) sf[ks] = lds_read(score + (f.nat ^ (ks << 5)));
+#pragma unroll
+            for (int m = 0; m < 2 * DB; m++) rf[m] = row(m);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         v16f s;
         if constexpr (ROLE == 0) {
             if (what != Seen::kAll) start_scores(s, mask, pa, half);
-            s = what == Seen::kAll ? product<T>(lds_read(score + f.nat), bx[0], v16f{}) : product<T>(lds_read(score + f.nat), bx[0], s);
+            s = what == Seen::kAll ? product<T>(scores(0), bx[0], v16f{}) : product<T>(scores(0), bx[0], s);
         } else {
 #pragma unroll
             for (int n = 0; n < 4; n++) {
@@ -563,10 +595,10 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
 #pragma unroll
                 for (int e = 0; e < 4; e++) s[n * 4 + e] = nd[e];
             }
-            s = product<T>(lds_read(score + f.nat), bx[0], s);
+            s = product<T>(scores(0), bx[0], s);
         }
 #pragma unroll
-        for (int ks = 1; ks < KS; ks++) s = product<T>(lds_read(score + (f.nat ^ (ks << 5))), bx[ks], s);
+        for (int ks = 1; ks < KS; ks++) s = product<T>(scores(ks), bx[ks], s);
         uint32_t pk[8], hp[4 * L::WORDS];
         u32x4* mine = hand + parity * (L::HAND / 16);
         if constexpr (ROLE == 0) {
@@ -609,8 +641,7 @@ __device__ __forceinline__ void dkdv_role(const WindowBwdArgs& a, uint8_t* smem,
 #pragma unroll
         for (int m = 0; m < 2 * DB; m++) {
             const int j2 = m / DB, d = m % DB;
-            const uint32_t lo = (f.tr[0] ^ (d << 6)) + j2 * 32 * D, hi = (f.tr[1] ^ (d << 6)) + j2 * 32 * D;
-            acc[d] = product<T>(lds_read_across(rows + lo, rows + hi), v4i{(int)pk[j2 * 4], (int)pk[j2 * 4 + 1], (int)pk[j2 * 4 + 2], (int)pk[j2 * 4 + 3]}, acc[d]);
+            acc[d] = product<T>(EARLY ? rf[EARLY ? m : 0] : row(m), v4i{(int)pk[j2 * 4], (int)pk[j2 * 4 + 1], (int)pk[j2 * 4 + 2], (int)pk[j2 * 4 + 3]}, acc[d]);
         }
     };
     auto tile = [&](int t, int slot) {   // slot: t % 3
