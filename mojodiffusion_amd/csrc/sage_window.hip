@@ -56,15 +56,29 @@ template <int D> struct RowState {
 constexpr int kFineKeys = 128;
 // LATE: whether the reference is high enough is seen from the tile's sum, after the weights, instead of from its largest score; where it is not, they are formed again.  A fifth
 // of the vector instructions besides the exponentials go ([31234 rows in 6, 48 on 12 x 128] 2223 -> 2148 us, full [11696 rows in 4, 30 x 128] 629 -> 607).
-template <int T, int D, bool FINE, bool LATE = false, class Mask>
+// EARLY: all fragments are requested ahead of the first product, where there are registers for it and one wave to a SIMD ([64 blocks of 128 rows, 4096 keys, 256 channels] 73 -> 70 us, 128
+// channels 47.7 -> 46.3; two waves, 128 channels: 66 -> 67).
+template <int T, int D, bool FINE, bool LATE = false, bool EARLY = false, class Mask>
 __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 16], uint32_t kt, uint32_t vt, const Fragments<D>& kept,
                                             Seen what, int j0, const Mask& m, float c) {
     constexpr int KS = D / 16, DB = D / 32;
     const Fragments<D> f = D > 64 || FINE ? kept.fresh() : kept;         // (at 64 channels there is room for the addresses)
     auto key = [&](int ks) { return lds_read(kt + (f.nat ^ ((ks & 7) << 5)) + (ks >> 3) * 256); };
-    v16f s = product<T>(key(0), q[0], v16f{});
+    auto value = [&](int j2, int d) {
+        const uint32_t at = vt + j2 * 32 * D + (d >> 2) * 256;
+        return lds_read_across(at + (f.tr[0] ^ ((d & 3) << 6)), at + (f.tr[1] ^ ((d & 3) << 6)));
+    };
+    v4i kf[EARLY ? KS : 1], vf[EARLY ? 2 * DB : 1];
+    if constexpr (EARLY) {
 #pragma unroll
-    for (int ks = 1; ks < KS; ks++) s = product<T>(key(ks), q[ks], s);
+        for (int ks = 0; ks < KS; ks++) kf[ks] = key(ks);
+#pragma unroll
+        for (int m = 0; m < 2 * DB; m++) vf[m] = value(m / DB, m % DB);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    v16f s = product<T>(EARLY ? kf[0] : key(0), q[0], v16f{});
+#pragma unroll
+    for (int ks = 1; ks < KS; ks++) s = product<T>(EARLY ? kf[EARLY ? ks : 0] : key(ks), q[ks], s);
     if (what != Seen::kAll) {
         const Mask rel = m.from(j0 + (lane_here() >> 5) * 4);
 #pragma unroll
@@ -107,11 +121,10 @@ __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 
     for (int j2 = 0; j2 < 2; j2++)
 #pragma unroll
         for (int d = 0; d < DB; d++) {
-            const uint32_t at = vt + j2 * 32 * D + (d >> 2) * 256;
-            const v4i vf = lds_read_across(at + (f.tr[0] ^ ((d & 3) << 6)), at + (f.tr[1] ^ ((d & 3) << 6)));
-            st.acc[d] = product<T>(vf, v4i{(int)p[j2 * 4], (int)p[j2 * 4 + 1], (int)p[j2 * 4 + 2], (int)p[j2 * 4 + 3]}, st.acc[d]);
+            const v4i x = EARLY ? vf[EARLY ? j2 * DB + d : 0] : value(j2, d);
+            st.acc[d] = product<T>(x, v4i{(int)p[j2 * 4], (int)p[j2 * 4 + 1], (int)p[j2 * 4 + 2], (int)p[j2 * 4 + 3]}, st.acc[d]);
             if constexpr (FINE)
-                st.acc[d] = product<T>(vf, v4i{(int)fine[j2 * 4], (int)fine[j2 * 4 + 1], (int)fine[j2 * 4 + 2], (int)fine[j2 * 4 + 3]}, st.acc[d]);
+                st.acc[d] = product<T>(x, v4i{(int)fine[j2 * 4], (int)fine[j2 * 4 + 1], (int)fine[j2 * 4 + 2], (int)fine[j2 * 4 + 3]}, st.acc[d]);
         }
 }
 
@@ -249,7 +262,7 @@ template <int D> struct SplitLds {
     static_assert(64 * D <= RING, "a wave's rows pass through its ring");
 };
 
-template <int T, int D>
+template <int T, int D, bool EARLY = false>
 __device__ __forceinline__ void split_body(const WindowArgs& a, uint8_t* smem, float (&meet_ml)[SplitLds<D>::NW][32][2], int b, int kvh, int x0, int item, int split) {
     using L = SplitLds<D>;
     constexpr int NW = L::NW, KT = L::KT, CPR = D / 8, RUNS = L::TILE / 1024, KS = D / 16, DB = D / 32;
@@ -317,8 +330,8 @@ __device__ __forceinline__ void split_body(const WindowArgs& a, uint8_t* smem, f
         const int j0 = span.tile(t) * KT;
         const uint32_t kt = ring + slot * L::SLOT;
         const Seen what = seen<KT>(a, p_lo, p_hi, len, j0);
-        if (D <= 128 && span.n * KT <= kFineKeys) attend_tile<T, D, D <= 128>(st, q, kt, kt + L::TILE, fr, what, j0, mask, c);
-        else attend_tile<T, D, false>(st, q, kt, kt + L::TILE, fr, what, j0, mask, c);
+        if (D <= 128 && span.n * KT <= kFineKeys) attend_tile<T, D, D <= 128, false, EARLY>(st, q, kt, kt + L::TILE, fr, what, j0, mask, c);
+        else attend_tile<T, D, false, false, EARLY>(st, q, kt, kt + L::TILE, fr, what, j0, mask, c);
         if (L::SLOTS == 2) slot ^= 1;
         else if (t + NW < t1) {
             reads_done();
@@ -644,7 +657,7 @@ template <int T, int D> __global__ __launch_bounds__(256) void packed_few_kernel
     const Sequence& s = f.s;
     WindowArgs w = view(a.w, s, s.nq, f.b < a.B ? s.nk : 0);
     w.splits = 1;
-    split_body<T, D>(w, smem, meet_ml, 0, at.head, (f.n - 1 - f.index) * 32, 0, 0);
+    split_body<T, D, true>(w, smem, meet_ml, 0, at.head, (f.n - 1 - f.index) * 32, 0, 0);
 }
 int packed_rows(const PackedArgs& a) { return a.form == PackedForm::kFew ? 32 : 128; }
 int64_t packed_slots(const PackedArgs& a, int rows) { return slots_total(a.rows_q, a.w.g, rows, a.B); }
