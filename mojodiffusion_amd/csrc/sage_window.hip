@@ -499,9 +499,7 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
 // are in time; one wave for two tiles at a time: as slow as a wave for one.
 //
 // The tiles that a wave sees all of come first, in a loop of their own without a question but for the ring's ends: a wave that is alone on its SIMD waits for its own
-// scalar instructions ([16 sequences of up to 333, 12 x 64] 14.4 -> 12.6 us, [31234 rows in 6, 48 on 12 x 128] 2215 -> 2160).  A training step that fills the chip more than once does
-// without: there it is at its power limit, and the gradients' kernel pays for a denser forward in clocks ([20576 rows in 8, 24 on 8 x 64] forward 230 -> 225 us, the step
-// 1065 -> 1100; without the loop 1073; but [1292 rows, 30 x 64] with it 98 -> 86).
+// scalar instructions ([16 sequences of up to 333, 12 x 64] 14.4 -> 12.6 us, [31234 rows in 6, 48 on 12 x 128] 2215 -> 2160).
 template <int D, int WAYS> struct PackedLds {
     static constexpr int NW = 4, KT = 32, TILE = KT * D * 2, OWN = NW * 64 * D, SLOTS = WAYS == 1 && D == 128 ? 3 : 2, RING = SLOTS * WAYS * 2 * TILE;
     // The waves' rows lie behind the first slot at the start (with two slots of WAYS 1 behind its keys), and over the front again at the end.
@@ -517,7 +515,6 @@ struct EndMask {                         // keys up to hi
     __device__ EndMask from(int j) const { return EndMask{hi - j}; }
     __device__ bool sees(int j) const { return j <= hi; }
 };
-constexpr unsigned kCoolGrid = 768;
 template <int T, int D, int WAYS> __device__ __forceinline__ void packed_body(const WindowArgs& a, uint8_t* smem, int kvh, int row0) {
     using L = PackedLds<D, WAYS>;
     using Tiles = KeyTiles<D, L::NW>;
@@ -597,16 +594,15 @@ template <int T, int D, int WAYS> __device__ __forceinline__ void packed_body(co
     if (D <= 128 && span.n * KT <= kFineKeys) {
         walk(std::bool_constant<D <= 128>{}, way, 0);
     } else {
-        const int direct = a.stats == nullptr || gridDim.x <= kCoolGrid ? all : 0;
         int t = way, slot = 0;
-        while (t < direct) {
+        while (t < all) {
 #pragma unroll
             for (int u = 0; u < L::SLOTS; u++) {                       // (slots known ahead)
                 turn(t, u);
                 attend_tile<T, D, false, LATE>(st, q, lds + L::keys(u, way), lds + L::values(u, way), fr, Seen::kAll, t * KT, mask, c);
                 t += WAYS;
                 slot = u == AHEAD ? 0 : u + 1;
-                if (t >= direct) break;
+                if (t >= all) break;
             }
         }
         walk(std::false_type{}, t, slot);
