@@ -744,13 +744,14 @@ __device__ __forceinline__ WindowBwdArgs view(const PackedBwdArgs& all, const Se
     a.dsize += row;
     return a;
 }
+// (A workgroup's rows are of one tile of 32, so that head and sequence are found once for all of them.)
 template <int T, int D> __global__ __launch_bounds__(256) void packed_bwd_prep_kernel(PackedBwdArgs a) {
     constexpr int CPR = D / 8, RPP = 256 / CPR;
-    const int64_t row = (int64_t)blockIdx.x * RPP + threadIdx.x / CPR;                // over [H, sq_pad]
-    if (row >= (int64_t)a.w.w.Hk * a.w.w.g * a.w.sq_pad) return;
-    const int h = (int)(row / a.w.sq_pad), y = (int)(row % a.w.sq_pad);
+    static_assert(32 % RPP == 0, "part of a tile");
+    const uint32_t row0 = blockIdx.x * (uint32_t)RPP, tiles_head = (uint32_t)a.w.sq_pad / 32u, tile = row0 / 32u;
+    const int h = (int)(tile / tiles_head), t = (int)(tile - (uint32_t)h * tiles_head);          // over [H, sq_pad]
     const Slots tiles = {a.p.cu_q, a.p.rows_q, 1, 32};
-    const int b = tiles.owner(y / 32, a.p.B), i = y - tiles.first(b) * 32;
+    const int b = tiles.owner(t, a.p.B), i = (t - tiles.first(b)) * 32 + (int)(row0 % 32u) + (int)threadIdx.x / CPR;
     const Sequence s = sequence(a.p, b);
     prep_row<T, D>(view(a, s, s.nq, b < a.p.B ? s.nk : 0, b), h, i, (int64_t)h * a.w.sq_pad + i);
 }
@@ -844,7 +845,7 @@ PackedGrid packed_grid(const PackedBwdArgs& a) {
     PackedGrid g;
     g.q_slots = slots_total(a.p.rows_q, a.w.w.g, kRowsWg, a.p.B);
     g.k_slots = slots_total(a.p.rows_k, 1, kKeysWg, a.p.B);
-    g.prep = (Hk * a.w.w.g * packed_stats_rows(a.p) * (D / 8) + 255) / 256;
+    g.prep = Hk * a.w.w.g * packed_stats_rows(a.p) * (D / 8) / 256;
     g.grid = spread_grid(Hk, g.q_slots * a.q_chunks) + spread_grid(Hk, g.k_slots * a.chunks);
     g.join = ((a.chunks > 1 ? Hk * g.k_slots * 2 * kKeysWg : 0) + (a.q_chunks > 1 ? Hk * g.q_slots * kRowsWg : 0)) * (D / 8) / 256;
     return g;
