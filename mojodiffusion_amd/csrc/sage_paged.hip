@@ -10,7 +10,7 @@
 //
 // Blocks of all sequences and heads are one list, dealt to the workgroups in equal shares, so sequences of any lengths fill the chip; rows whose
 // blocks fall to several workgroups are left as parts in fp32 that a second launch adds up, in order: the same bits on every call.
-// Measured, bf16, 48 on 12 heads of 128: one token of 32 sequences of 2 to 16 thousand keys 172 us, 5.4 TB/s; of one with 8192 keys 13 us, in launches of 8.5 and 3.1.
+// Measured, bf16, 48 on 12 heads of 128: one token of 32 sequences of 2 to 16 thousand keys 171 us, 5.4 TB/s; of one with 8192 keys 13 us, in launches of 8.4 and 3.2.
 #include "sage_kv.h"
 #include "sage_tile.h"
 #include "sage_window.h"

@@ -14,8 +14,8 @@
 // none of its rows sees.  Rows of a tile that no row of the workgroup sees are not read at all (another key's row stands
 // in), so whatever lies there, or behind a sequence's end, cannot reach a result.
 //
-// The same for whole sequences that lie one behind the other (packed_body).  Measured, bf16: [31234 rows in 6 sequences, 48 on 12 heads x 128] causal 2160 to 2340 us by
-// card, 1.03 PFLOP/s; full [11696 rows in 4, 30 x 128] 644 us, 0.93.
+// The same for whole sequences that lie one behind the other (packed_body).  Measured, bf16: [31234 rows in 6 sequences, 48 on 12 heads x 128] causal 2069 us, 1.11 PFLOP/s;
+// full [11696 rows in 4, 30 x 128] 584 us, 1.02.
 #include "sage_grid.h"
 #include "sage_window_common.h"
 
