@@ -11,7 +11,7 @@
 // pairs are dealt to several workgroups (window_bwd_plan), which leave fp32 parts for launch 3
 // to add up in order.  The same where there are too few key blocks to fill the chip.
 //
-// The same for whole sequences that lie one behind the other: bf16, [20576 rows in 8, 24 on 8 heads x 64] causal 745 us, Delta 35; [2652 rows in 3, 30 x 128] full 195, 13.
+// The same for whole sequences that lie one behind the other: bf16, [20576 rows in 8, 24 on 8 heads x 64] causal 745 to 780 us, Delta 30; [2652 rows in 3, 30 x 128] full 200, 12.
 #include "sage_grid.h"
 #include "sage_window_common.h"
 
