@@ -1471,6 +1471,7 @@ static WindowBwdCarve packed_bwd_carve(PackedBwdArgs* a) {
     return c;
 }
 
+// (Causal calls take the most: the query knows no mask.)
 size_t mi355_sage_packed_bwd_workspace_bytes(int B, int Hq, int Hk, int T_q, int T_k, int D) {
     PackedBwdArgs a{};
     if (packed_dims("packed backward", B, Hq, Hk, T_q, T_k, D, MI355_SAGE_BF16, 1.0f, 1, &a.p) || !bwd_dims_ok(D)) return 0;
