@@ -11,6 +11,7 @@
 // in flight at once, one exchange for the two largest values, V turned through LDS.  Where a block's earlier codes stay, their 16-byte pieces that
 // new rows share are read ahead and written back with them.  Queries are other workgroups of the same launch.
 // Measured, bf16, 48 + 12 heads of 128: 31234 tokens of 6 prompts 224 us, 4.7 TB/s of 5.2 that a large copy reaches; one token of 32 sequences 6.7 us.
+#include "sage_grid.h"
 #include "sage_kv.h"
 #include "sage_rows.h"
 
@@ -242,7 +243,10 @@ template <int T, int D> __global__ __launch_bounds__(2 * D) void kv_append_kerne
     __shared__ __attribute__((aligned(16))) uint8_t turned[D * (kKvBlock + 4)];
     __shared__ float tops[2 * D / 64][2];
     const int id = (int)blockIdx.x;
-    if (id < a.kv_wgs) append_block<T, D>(a, turned, tops, id / a.pool.Hk, id % a.pool.Hk);
+    if (id < a.kv_wgs) {
+        const int item = xcd_item(id, a.kv_wgs);         // (the heads of a block, which share rows of the tables, go to one XCD)
+        append_block<T, D>(a, turned, tops, item / a.pool.Hk, item % a.pool.Hk);
+    }
     else rotate_queries<T, D, kHeads>(a, id - a.kv_wgs);
 }
 
