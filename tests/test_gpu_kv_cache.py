@@ -416,6 +416,42 @@ def test_two_threads_on_streams_of_their_own():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D,dtype", [(64, FP), (128, BF), (256, BF)])
+def test_other_orders_in_memory(D, dtype):
+    """Heads first, rows far apart, rows that are not aligned (copied), tables whose rows are parts of wider ones: the bits of dense tensors."""
+    g = torch.Generator().manual_seed(D)
+    B, S, Hq, Hk = 2, 37, 4, 2
+    q, k, v = (torch.randn((B, S, h, D), generator=g).to(dtype).cuda() for h in (Hq, Hk, Hk))
+    ids, lens = torch.tensor([[3, 0, 9], [1, 2, 9]], dtype=torch.int32).cuda()[:, :2], torch.tensor([50, 37], dtype=torch.int32).cuda()
+    cos, sin = cuda(*tables(32, 64, F32))
+    wide = [torch.cat((t, t), 1)[:, 16:] for t in (cos, sin)]
+    gain = (1 + 0.1 * torch.randn(D, generator=g)).cuda()
+
+    def step(q, k, v, cos, sin):
+        cache = pool(4, Hk, D, 32, 4)
+        z = C.kv_append(cache, k, v, ids, lens, k_norm=gain, cos=cos, sin=sin, halfsplit=True, q=q, q_norm=gain)
+        return z, cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale, C.sdpa_paged(q[:, -3:], cache, ids, lens, 0.1)
+
+    want = step(q, k, v, cos, sin)
+    heads_first = lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)
+
+    def apart(t):
+        w = torch.full((B, 2 * S, t.shape[2] + 2, 2 * D), NAN, dtype=dtype, device="cuda")
+        w[:, 1::2, 1:-1, D:] = t
+        return w[:, 1::2, 1:-1, D:]
+
+    def unaligned(t):
+        w = torch.zeros(t.numel() + 1, dtype=dtype, device="cuda")[1:].view(t.shape)
+        w.copy_(t)
+        return w
+
+    for order in (heads_first, apart, unaligned):
+        for table in ((cos, sin), wide):
+            for x, y in zip(step(order(q), order(k), order(v), *table), want):
+                assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
 def test_q_in_place_and_refusals_on_the_device():
     g = torch.Generator().manual_seed(2)
     cache = pool(4, 2, 64, 32)

@@ -269,6 +269,79 @@ def test_a_captured_training_step():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D,dtype", [(64, BF), (128, FP)])
+def test_other_orders_in_memory(D, dtype):
+    """Heads first, rows far apart, an upstream gradient that is one row repeated, rows that are not aligned (copied): the bits of dense tensors."""
+    lens = [70, 130, 9]
+    T, Hq, Hk = sum(lens), 6, 3
+    q, k, v, d = (t.cuda() for t in tensors(lens, lens, Hq, Hk, D, dtype, 0, D))
+    d = d[:1].expand(T, Hq, D)
+    cu = offsets(lens).cuda()
+
+    def step(q, k, v, d):
+        f = P.sdpa_packed_train_fwd(q, k, v, cu, 0.1)
+        g = P.sdpa_packed_backward(f, d)
+        return f.o, f.stats, g.d_q, g.d_k, g.d_v
+
+    want = step(q, k, v, d.contiguous())
+    heads_first = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)
+
+    def apart(t):
+        w = torch.full((2 * t.shape[0], t.shape[1] + 2, 2 * D), NAN, dtype=dtype, device="cuda")
+        w[1::2, 1:-1, D:] = t
+        return w[1::2, 1:-1, D:]
+
+    def unaligned(t):
+        w = torch.zeros(t.numel() + 1, dtype=dtype, device="cuda")[1:].view(t.shape)
+        w.copy_(t)
+        return w
+
+    for order in (heads_first, apart, unaligned):
+        for x, y in zip(step(order(q), order(k), order(v), d), want):
+            assert torch.equal(x, y)
+        for x, y in zip(step(q, order(k), order(v), order(d.contiguous())), want):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_a_captured_recorded_step():
+    """The recorded node in a captured forward and backward (the warm-up's graph and gradients are gone by then), replayed with other values between."""
+    Hq, Hk, D, T = 6, 2, 128, 260
+    lens = [[100, 160], [1, 259]]
+    sets = [tensors([T], [T], Hq, Hk, D, FP, 0, s) for s in range(2)]
+
+    def step(q, k, v, d, cu):
+        o = P.record_sdpa_packed(q, k, v, cu, 0.1)
+        return (o.detach(), *torch.autograd.grad(o, (q, k, v), d))
+
+    eager = []
+    for s, n in zip(sets, lens):
+        q, k, v, d = (t.cuda() for t in s)
+        eager.append([t.clone() for t in step(*(t.requires_grad_() for t in (q, k, v)), d, offsets(n).cuda())])
+        del q, k, v, d
+    place = [t.cuda() for t in sets[0]]
+    leaves = [t.requires_grad_() for t in place[:3]]
+    cu = offsets(lens[0]).cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*leaves, place[3], cu)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*leaves, place[3], cu)
+    for i in (0, 1, 1, 0):
+        with torch.no_grad():
+            for t, x in zip(place, sets[i]):
+                t.copy_(x)
+        cu.copy_(offsets(lens[i]))
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(out, eager[i]):
+            assert torch.equal(x, y), i
+
+
+@pytest.mark.gpu
 def test_two_threads_on_streams_of_their_own():
     cu = offsets([200, 100]).cuda()
     sets = [[t.cuda() for t in tensors([300], [300], 4, 2, 128, BF, 0, s)] for s in range(2)]
