@@ -268,6 +268,52 @@ def test_a_captured_training_step():
         step(*(t.cuda() for t in sets[0]), offsets(lens[2]).cuda())
 
 
+# workgroups of 128 rows, with two waves to 32 rows, and of 32
+BY_FORM = [(700, 56), (500, 40), (300, 8)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H", BY_FORM)
+@pytest.mark.parametrize("D,dtype", [(64, FP), (128, BF), (256, BF)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_scores_that_rise_and_fall(T, H, D, dtype, causal):
+    """Every tile's largest score far above the one before's, in half of the heads far below: the running reference is raised on every tile, or on the first alone."""
+    q, k, v, _ = tensors([T], [T], H, H, D, dtype, 0, T + D)
+    q[:] = q[:1].abs() + 0.25                # (all queries one direction, that of the keys)
+    size = torch.linspace(0.05, 6.0, T).view(-1, 1)
+    k = (k * 0.05).double()
+    k[:, : H // 2] += (size * 1.0).unsqueeze(2)
+    k[:, H // 2:] += (size.flip(0) * 1.0).unsqueeze(2)
+    k = k.to(dtype)
+    scale = 4.0 / D
+    f = P.sdpa_packed_train_fwd(q.cuda(), k.cuda(), v.cuda(), offsets([T]).cuda(), scale, causal)
+    ref = forward(q[None], k[None], v[None], scale, -1, 0 if causal else -1, 0, [T], [0])
+    assert float(ref[1].max()) > 15
+    check_forward(f.o[None], f.stats[None], ref, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H", BY_FORM)
+@pytest.mark.parametrize("D", [64, 128])
+def test_queries_that_are_not_finite(T, H, D):
+    """A NaN or an infinity in a query: NaN in its own row, and every other row within its bounds."""
+    q, k, v, _ = tensors([T - 40, 40], [T - 40, 40], H, H, D, BF, 0, 9)
+    cu = offsets([T - 40, 40]).cuda()
+    refs = list(per_sequence([T - 40, 40], [T - 40, 40], q, k, v, True, 0.1))
+    bad = [(3, 0), (100, 1), (T - 1, H - 1), (T - 50, 2)]
+    for value in (NAN, float("inf"), -float("inf")):
+        x = q.clone()
+        for i, h in bad:
+            x[i, h, 7] = value
+        o = P.sdpa_packed(x.cuda(), k.cuda(), v.cuda(), cu, 0.1)
+        clean = P.sdpa_packed(q.cuda(), k.cuda(), v.cuda(), cu, 0.1)
+        for i, h in bad:
+            assert torch.isnan(o[i, h]).all()
+            o[i, h] = clean[i, h]
+        for rq, _, ref in refs:
+            check_forward(o[None, rq], None, ref, BF)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("D,dtype", [(64, BF), (128, FP)])
 def test_other_orders_in_memory(D, dtype):
