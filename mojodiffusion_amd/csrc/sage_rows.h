@@ -120,9 +120,14 @@ template <int SIGN> __device__ __forceinline__ void turn(const Turn& t, bool hal
         for (int i = 0; i < 4; i++) pair(y1[2 * i], y1[2 * i + 1], t.c[4 + i], t.s[4 + i]);
     }
 }
+// The sum over a group of 4, 8 or 16 lanes by moves between neighbours: the lane ^ 1, ^ 2, then the mirror image in 8 and in 16, whose four (eight) lanes hold one sum by then.
+template <int CTRL> __device__ __forceinline__ float lane_moved(float x) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true)); }
 template <int LPR> __device__ __forceinline__ float row_sum(float x) {
-#pragma unroll
-    for (int m = 1; m < LPR; m <<= 1) x += __shfl_xor(x, m);
+    static_assert(LPR == 4 || LPR == 8 || LPR == 16, "lanes of a row");
+    x += lane_moved<0xB1>(x);
+    x += lane_moved<0x4E>(x);
+    if constexpr (LPR > 4) x += lane_moved<0x141>(x);
+    if constexpr (LPR > 8) x += lane_moved<0x140>(x);
     return x;
 }
 template <int T> __device__ __forceinline__ float inv_root(float x) {
