@@ -546,9 +546,12 @@ template <int T, int D, int WAYS> __device__ __forceinline__ void packed_body(co
 #pragma unroll
             for (int i = 0; i < PIECES; i++) dma16(r.at, r.off[i], place(i));
         } else {
+            int l = lane;
+            if (D == 256) asm volatile("" : "+v"(l));                  // (its rows and columns formed here: kept over the loops, they are registers too many)
+            const typename Tiles::Pieces pieces(wave, l);
 #pragma unroll
             for (int i = 0; i < PIECES; i++) {
-                const uint32_t last = (uint32_t)(min(t * KT + tiles.pieces.row(i), span.hi) - t * KT) * r.sn + tiles.pieces.col(i, lane);
+                const uint32_t last = (uint32_t)(min(t * KT + pieces.row(i), span.hi) - t * KT) * r.sn + pieces.col(i, l);
                 dma16(r.at, t < whole ? r.off[i] : last, place(i));
             }
         }
@@ -608,9 +611,12 @@ template <int T, int D, int WAYS> __device__ __forceinline__ void packed_body(co
         walk(std::false_type{}, t, slot);
     }
     __syncthreads();                     // (no copy is in flight: the last step's wait was for all of them)
+    int none = 0;
+    asm volatile("" : "+v"(none));
+    const int behind = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));      // (the lane, formed again: kept over the loops, it went to memory, and what hangs on it)
     if constexpr (WAYS == 2) {
-        float* meet = reinterpret_cast<float*>(smem) + wave * (D / 2) * 64 + lane;
-        float* stats = reinterpret_cast<float*>(smem + L::STATS) + wave * 128 + lane;
+        float* meet = reinterpret_cast<float*>(smem) + wave * (D / 2) * 64 + behind;
+        float* stats = reinterpret_cast<float*>(smem + L::STATS) + wave * 128 + behind;
         if (way != 0) {
             stats[0] = st.ref, stats[64] = st.sum;
 #pragma unroll
@@ -625,11 +631,13 @@ template <int T, int D, int WAYS> __device__ __forceinline__ void packed_body(co
         const float f = st.ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(other - st.ref);
         st.sum = fmaf(stats[64], f, st.sum);
 #pragma unroll
-        for (int d = 0; d < D / 32; d++)
+        for (int d = 0; d < D / 32; d++) {
 #pragma unroll
             for (int i = 0; i < 16; i++) st.acc[d][i] = fmaf(meet[(d * 16 + i) * 64], f, st.acc[d][i]);
+            asm volatile("" : "+v"(st.acc[d]) : : "memory");           // (16 registers of the other part at a time: all of them together went to memory)
+        }
     }
-    if (x0 < rows) finish_rows<T, D>(a, st, smem + wave * WAYS * 64 * D, 0, kvh, x0, lane);
+    if (x0 < rows) finish_rows<T, D>(a, st, smem + wave * WAYS * 64 * D, 0, kvh, x0, behind);
 }
 constexpr int kPackedWaves(int D, int ways) { return ways == 1 ? kWindowWaves(D) : D == 64 ? 4 : 2; }
 template <int T, int D, int WAYS> __global__ __launch_bounds__(256 * WAYS, kPackedWaves(D, WAYS)) void packed_kernel(PackedArgs a, int slots) {
