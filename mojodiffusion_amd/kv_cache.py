@@ -40,12 +40,14 @@ class KvPages:
         return KvPages(codes(BLOCK, dh), codes(dh, BLOCK), scale(), scale())
 
     def dense(self, page_table, length):
-        """(k, v) F32 [length, Hk, Dh]: the values of one sequence's first `length` tokens, from its row of the page table."""
+        """(k, v) F32 [length, Hk, Dh]: the values of one sequence's first `length` tokens, from its row of the page table.  Entries that the tokens do not need are
+        not looked at; tokens whose page is not one of the cache's are NaN."""
         if page_table.dim() != 1 or not 0 <= length <= page_table.shape[0] * self.k.shape[1] * BLOCK:
             raise Error("KvPages.dense: one row of a page table that holds the tokens")
-        rows = page_table.long()
-        k = self.k.view(torch.uint8)[rows].view(self.k.dtype).float() * self.k_scale[rows][..., None, None]
-        v = self.v.view(torch.uint8)[rows].view(self.v.dtype).float() * self.v_scale[rows][..., None, None]
+        pages = page_table[:-(-length // (self.k.shape[1] * BLOCK))].long()
+        rows = pages.clamp(0, self.k.shape[0] - 1)
+        values = lambda t, scale: (t.view(torch.uint8)[rows].view(t.dtype).float() * scale[rows][..., None, None]).masked_fill_((rows != pages).view(-1, 1, 1, 1, 1), torch.nan)
+        k, v = values(self.k, self.k_scale), values(self.v, self.v_scale)
         flat = lambda t: t.flatten(0, 2)[:length]
         return flat(k.permute(0, 1, 3, 2, 4)), flat(v.permute(0, 1, 4, 2, 3))
 

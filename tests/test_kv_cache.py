@@ -62,6 +62,23 @@ def test_refusals_of_the_cache_itself():
     assert k.shape == v.shape == (40, 2, 64)
 
 
+def test_dense_looks_at_the_pages_of_its_tokens_only():
+    """A table's further entries need be no pages; one that the tokens do need and that is none gives NaN, and no page in its place."""
+    cache = C.KvPages.empty(4, 2, 64, 64, device="cpu")
+    for t in (cache.k, cache.v):
+        t.view(torch.uint8).copy_(torch.arange(t.numel()).remainder(0x77).to(torch.uint8).view(t.shape))
+    table = torch.tensor([2, 0, 99, -7, 2 ** 31 - 1], dtype=torch.int32)
+    for n in (0, 1, 64, 65, 128):
+        k, v = cache.dense(table, n)
+        assert k.shape == v.shape == (n, 2, 64)
+        for i in (0, n // 2, n - 1)[:n]:
+            at = (int(table[i // 64]), i % 64 // 32)
+            assert torch.equal(k[i], cache.k[at].float()[:, i % 32]) and torch.equal(v[i], cache.v[at].float()[..., i % 32])
+    k, v = cache.dense(table, 300)
+    for t in (k, v):
+        assert torch.isfinite(t[:128]).all() and torch.isnan(t[128:]).all()
+
+
 def test_refusals_of_attention():
     cache, ids, lens, _ = setup()
     q = torch.zeros((2, 1, 4, 64), dtype=BF)
