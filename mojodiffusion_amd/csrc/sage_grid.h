@@ -62,4 +62,13 @@ __host__ __device__ inline HeadSlot spread_item(int id, int heads, int slots) {
     return HeadSlot{item / (m * per), p % per * m + p / per};
 }
 
+// Share `id` of a list of `total` places in shares of `per`: begin .. end - 1.  Ids go beyond the last share (nothing is left for those), and their products with
+// `per` beyond 32 bits.
+struct Share { int begin, end; };
+__host__ __device__ inline Share share_of(int id, int per, int total) {
+    const long long at = (long long)id * per;
+    const int begin = at < total ? (int)at : total;
+    return Share{begin, total - begin < per ? total : begin + per};
+}
+
 }  // namespace sage

@@ -11,6 +11,7 @@
 // Blocks of all sequences and heads are one list, dealt to the workgroups in equal shares, so sequences of any lengths fill the chip; rows whose
 // blocks fall to several workgroups are left as parts in fp32 that a second launch adds up, in order: the same bits on every call.
 // Measured, bf16, 48 on 12 heads of 128: one token of 32 sequences of 2 to 16 thousand keys 171 us, 5.4 TB/s; of one with 8192 keys 13 us, in launches of 8.4 and 3.2.
+#include "sage_grid.h"
 #include "sage_kv.h"
 #include "sage_tile.h"
 #include "sage_window.h"
@@ -238,7 +239,8 @@ template <int T, int D, int COLS> __global__ __launch_bounds__(256, D == 256 ? 1
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rows = a.Sq * a.g, rblocks = (rows + ROWS - 1) / ROWS, mult = a.pool.Hk * rblocks;
     const Deal deal_ = deal(a, mult, lane);
-    const int t_begin = (int)blockIdx.x * deal_.per, t_end = min(t_begin + deal_.per, deal_.total);
+    const Share share = share_of((int)blockIdx.x, deal_.per, deal_.total);
+    const int t_begin = share.begin, t_end = share.end;
     const uint32_t k_off = (uint32_t)(((l16 >> 2) * 8 + (l16 & 3)) * D + quad * 16), v_off = (uint32_t)(l16 * kKvBlock + quad * 8);
     const KvPool& c = a.pool;
 

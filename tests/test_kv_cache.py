@@ -1,5 +1,7 @@
 """Refusals of the paged cache's calls that need no device, and its sizes."""
 import ctypes
+import os
+import subprocess
 
 import pytest
 import torch
@@ -9,6 +11,7 @@ from mojodiffusion_amd import kv_cache as C
 from mojodiffusion_amd.attention_sage import Error
 
 BF = torch.bfloat16
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mojodiffusion_amd", "csrc")
 
 
 def setup(Hk=2, D=64, page=32, B=2):
@@ -114,3 +117,35 @@ def test_sizes_of_the_c_calls():
     paged = lambda q=p, Hq=4, N=1, scale=0.1, type=0, page=32, D=64: L.mi355_sage_sdpa_paged(q, p, p, p, p, p, 4, page, p, 2, 2, p, 1, Hq, 2, N, D, type, scale, st, st, 0, 0, None, p, 1 << 20)
     assert paged(q=None) == paged(Hq=3) == paged(N=0) == paged(scale=0.0) == paged(scale=float("inf")) == -1
     assert paged(type=2) == paged(page=33) == paged(D=32) == -2
+
+
+def test_shares_of_long_lists(tmp_path):
+    """share_of: every place in one share, ids beyond the last empty, in lists of up to 2^30 places, whose ids times shares pass 32 bits (paged attention: 1024 even shares, up to 3072 ids)."""
+    src = tmp_path / "shares.cpp"
+    src.write_text('''
+#define __host__
+#define __device__
+#include "%s/sage_grid.h"
+#include <cstdio>
+using namespace sage;
+int main() {
+    const int totals[] = {1, 7, 1023, 1024, 5000, 1 << 20, (1 << 30) - 1, 1 << 30};
+    for (int total : totals) {
+        const int even = (total + 1023) / 1024, pers[] = {even, even + 1, 1 << 20, 1 << 30};
+        for (int per : pers) {
+            long long at = 0;
+            for (int id = 0; id < 3072; id++) {
+                const Share s = share_of(id, per, total);
+                if (s.begin != at || s.end < s.begin || s.end > total || s.end - s.begin > per) return 1;
+                if (s.end < total && s.end - s.begin != per) return 2;
+                at = s.end;
+            }
+            if (at != total) return 3;
+        }
+    }
+    std::puts("ok");
+}
+''' % CSRC)
+    exe = tmp_path / "shares"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover", "-o", str(exe), str(src)], check=True)
+    assert subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout == "ok\n"
