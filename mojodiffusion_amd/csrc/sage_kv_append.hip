@@ -266,7 +266,8 @@ template <int T> hipError_t launch_t(const KvAppendArgs& a, hipStream_t st) {
 
 }  // namespace
 
-bool kv_append_grid_ok(const KvAppendArgs& a) { return append_wgs(a) + query_wgs(a) <= 0x7FFFFFFF / 2; }
+// (rotate_queries numbers its groups of heads of a token, 32 to a workgroup, in 32 bits.)
+bool kv_append_grid_ok(const KvAppendArgs& a) { return append_wgs(a) + query_wgs(a) <= 0x7FFFFFFF / 2 && query_wgs(a) <= 0x7FFFFFFF / 32; }
 
 hipError_t launch_kv_append(const KvAppendArgs& args, hipStream_t st) {
     KvAppendArgs a = args;

@@ -119,6 +119,20 @@ def test_sizes_of_the_c_calls():
     assert paged(type=2) == paged(page=33) == paged(D=32) == -2
 
 
+def test_queries_of_an_append_beyond_32_bits_are_refused():
+    """2^29 rows of 8 heads are 2^31 groups of two heads, which the kernel numbers in 32 bits; (sizes and codes only: nothing runs)."""
+    if torch.cuda.is_available():
+        pytest.skip("made-up pointers: runs only where no device can be reached")
+    L, p = _lib.lib(), ctypes.c_void_p(4096)
+    st = lambda heads: (ctypes.c_int64 * 4)(0, 64, 64 * heads, 1)
+    q, out = ctypes.c_void_p(1 << 20), ctypes.c_void_p(1 << 30)
+    call = lambda rows, Hq: L.mi355_sage_kv_append(p, p, q, out, p, p, p, p, 4, 32, p, 2, 2, p, p, 1, rows, Hq, 2, 64, 0, st(2), st(2), st(Hq), st(Hq), 0, 0, 0, 0, None, None, 0, 1e-6,
+                                                   None, None, 0, 0, 0, 0, 0, None)
+    assert call(1 << 29, 8) == call(1 << 29, 7) == call((1 << 28) + 1, 16) == -2
+    for rows, Hq in ((1 << 29, 6), (1 << 28, 14), (1000, 64)):
+        assert call(rows, Hq) not in (-1, -2)        # (let through: what fails is the launch)
+
+
 def test_shares_of_long_lists(tmp_path):
     """share_of: every place in one share, ids beyond the last empty, in lists of up to 2^30 places, whose ids times shares pass 32 bits (paged attention: 1024 even shares, up to 3072 ids)."""
     src = tmp_path / "shares.cpp"
