@@ -2,8 +2,8 @@
 //
 //     S_ij = scale 2^ek(j) q_i . k_j  for the keys j up to query i's own position,  O_i = sum_j exp(S_ij - L_i) 2^ev(j) v_j,  L_i = log sum_j exp(S_ij)
 //
-// Bound by the bytes of K and V.  Codes have four significant bits, so they are operands of the inputs' type without a rounding: one instruction widens
-// two of them, and Q and the weights keep their own type.  A wave takes a block of 32 keys at a time, straight from memory into the
+// Bound by the bytes of K and V.  Codes have four significant bits, so they are operands of the inputs' type without a rounding (K's as they are, its scale goes to the scores; V's see
+// RowState): one instruction widens two of them, and Q and the weights keep their own type.  A wave takes a block of 32 keys at a time, straight from memory into the
 // registers that the matrix products read (no LDS): scores S^T = K Q^T with 16 keys as the rows, then O^T += V^T P^T over all 32.  The lane that holds the scores of
 // a query's keys 8 q .. 8 q + 7 (q = lane / 16) hands just those to the second product, because the first takes its keys in that order; V lies a
 // channel after the other, so those eight keys of a channel are eight bytes.  The next block is on its way while one is computed.
@@ -45,9 +45,6 @@ template <int T> __device__ __forceinline__ v4i widen(uint32_t lo, uint32_t hi, 
         return v4i{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, true)),
                    __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, true))};
 }
-// V in fp16 is taken halved: 65504 rounds to a code of 2^16.
-template <int T> constexpr float kVHalf = T == kBF16 ? 1.0f : 0.5f;
-
 // The four lanes of a query, 16 apart.
 __device__ __forceinline__ float max_quads(float x) {
     const v2u a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -152,19 +149,28 @@ template <int D> __device__ __forceinline__ void load_block(Block<D>& t, const u
 }
 
 // Rows of a part: COLS groups of 16 queries.
+// bf16: V's codes enter times their scale, which keeps all their bits.  fp16 has no exponents for that (below 2^-15 of its largest number a code loses bits, and a cache that
+// bf16 tensors filled may hold what fp16 cannot): there the codes enter as they are, the weights take the scale, and O has a reference of its own, of score and scale together,
+// so that what rounding takes from a weight is small against the largest of what its row adds up.
 template <int D, int COLS> struct RowState {
     v4f acc[COLS][D / 16];               // O^T: channels d * 16 + q * 4 + i
-    float ref[COLS], sum[COLS];
+    float ref[COLS], sum[COLS], vref[COLS];
     __device__ void clear() {
 #pragma unroll
         for (int n = 0; n < COLS; n++) {
 #pragma unroll
             for (int d = 0; d < D / 16; d++) acc[n][d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            ref[n] = -INFINITY;
+            ref[n] = vref[n] = -INFINITY;
             sum[n] = 0.0f;
         }
     }
+    // To another reference, in log2 units.
+    __device__ void scale_rows(int n, float f) {
+#pragma unroll
+        for (int d = 0; d < D / 16; d++) acc[n][d] *= f;
+    }
 };
+__device__ __forceinline__ float down(float from, float to) { return to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(from - to); }
 
 // What lies behind a sequence's last key may be any code.  live: how many of the lane's eight keys are the sequence's.
 template <int D> __device__ __forceinline__ void drop_values(Block<D>& t, int live) {
@@ -202,12 +208,24 @@ __device__ __forceinline__ void attend(RowState<D, COLS>& st, const v4i (&q)[COL
         for (int e = 1; e < 8; e++) top = fmaxf(top, s[n][e >> 2][e & 3]);
         top *= c;
         // (a new reference only where the old one lies more than 8 below: the weights stay under 2^8)
-        if (__any(top > st.ref[n] + 8.0f)) {
-            const float r = fmaxf(st.ref[n], max_quads(top)), f = r == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.ref[n] - r);
-            st.ref[n] = r;
-            st.sum[n] *= f;
-#pragma unroll
-            for (int d = 0; d < D / 16; d++) st.acc[n][d] *= f;
+        float mul = 1.0f;
+        if constexpr (T == kBF16) {
+            if (__any(top > st.ref[n] + 8.0f)) {
+                const float r = fmaxf(st.ref[n], max_quads(top)), f = down(st.ref[n], r);
+                st.ref[n] = r;
+                st.sum[n] *= f;
+                st.scale_rows(n, f);
+            }
+        } else {
+            const float ve = (float)((int)(__float_as_uint(vs) >> 23 & 255) - 127);
+            if (__any(top > st.ref[n] + 8.0f || top + ve > st.vref[n] + 8.0f)) {
+                const float most = max_quads(top), r = fmaxf(st.ref[n], most), w = fmaxf(st.vref[n], most + ve);
+                st.sum[n] *= down(st.ref[n], r);
+                st.scale_rows(n, down(st.vref[n], w));
+                st.ref[n] = r, st.vref[n] = w;
+            }
+            // (bounded: a weight that takes more than 2^126 is no number that fp16 shows)
+            mul = st.ref[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fminf(st.ref[n] - st.vref[n] + ve, 126.0f));
         }
         const float ref = st.ref[n] == -INFINITY ? 0.0f : st.ref[n];
         float part = 0.0f;
@@ -215,13 +233,13 @@ __device__ __forceinline__ void attend(RowState<D, COLS>& st, const v4i (&q)[COL
         for (int e = 0; e < 8; e += 2) {
             const float y = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][e & 3], c, -ref)), z = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][(e & 3) + 1], c, -ref));
             part += y + z;
-            p[n][e >> 1] = (int)pack2<T>(y, z);
+            p[n][e >> 1] = T == kBF16 ? (int)pack2<T>(y, z) : (int)pack2<T>(y * mul, z * mul);
         }
         st.sum[n] += part;
     }
 #pragma unroll
     for (int d = 0; d < D / 16; d++) {
-        const v4i v = widen<T>(t.v[d][0], t.v[d][1], vs);
+        const v4i v = widen<T>(t.v[d][0], t.v[d][1], T == kBF16 ? vs : 1.0f);
 #pragma unroll
         for (int n = 0; n < COLS; n++) st.acc[n][d] = product<T>(v, p[n], st.acc[n][d]);
     }
@@ -291,7 +309,7 @@ template <int T, int D, int COLS> __global__ __launch_bounds__(256, D == 256 ? 1
                 const int j0 = (first + wave + (i0 + i) * kWaves) * kKvBlock;
                 if (j0 > min(p_hi, len - 1)) return;
                 const float kc = a.scale * kLog2e * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), i));
-                const float vc = kVHalf<T> * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), i));
+                const float vc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), i));
                 int rel[COLS];
 #pragma unroll
                 for (int m = 0; m < COLS; m++) rel[m] = pos[m] - j0 - quad * 8;
@@ -314,6 +332,7 @@ template <int T, int D, int COLS> __global__ __launch_bounds__(256, D == 256 ? 1
         for (int m = 0; m < COLS; m++) {
             const float sum = sum_quads(st.sum[m]);
             if (quad == 0) meet_ml[wave][m * 16 + l16][0] = st.ref[m], meet_ml[wave][m * 16 + l16][1] = sum;
+            if constexpr (T == kF16) st.scale_rows(m, down(st.vref[m], st.ref[m]));
 #pragma unroll
             for (int d = 0; d < D / 16; d++) *reinterpret_cast<v4f*>(meet + (wave * ROWS + m * 16 + l16) * PR + d * 16 + quad * 4) = st.acc[m][d];
         }
@@ -334,7 +353,7 @@ template <int T, int D, int COLS> __global__ __launch_bounds__(256, D == 256 ? 1
             }
             const int i = x / a.g, hg = x - i * a.g;
             const bool blind = p0 + i < 0;
-            const float inv = whole ? weight_of(sum, blind) / kVHalf<T> : 1.0f;
+            const float inv = whole ? weight_of(sum, blind) : 1.0f;
             uint16_t* o = a.o + b * a.o_sb + ((int64_t)h * a.g + hg) * a.o_sh + i * a.o_sn;
             for (int col = tid % TPR * 4; col < D; col += TPR * 4) {
                 v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -429,7 +448,7 @@ template <int T, int D, bool SHARED> __global__ __launch_bounds__(256) void page
         }
         const int i = x / a.g, hg = x - i * a.g;
         const bool blind = len - a.Sq + i < 0;
-        const float inv = weight_of(sum, blind) / kVHalf<T>;
+        const float inv = weight_of(sum, blind);
         uint16_t* o = a.o + b * a.o_sb + ((int64_t)h * a.g + hg) * a.o_sh + i * a.o_sn + lane * N;
 #pragma unroll
         for (int e = 0; e < N; e++) y[e] = blind ? 0.0f : y[e] * inv;

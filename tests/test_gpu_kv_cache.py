@@ -464,3 +464,69 @@ def test_q_in_place_and_refusals_on_the_device():
                 lambda: C.kv_append(cache, k, v, ids, lens, cos=cos, sin=sin, q=q, q_out=q.transpose(0, 1)), lambda: C.sdpa_paged(q, cache, ids, lens, float("nan"))):
         with pytest.raises(Error):
             bad()
+
+
+def codes(g, *shape):
+    """Random codes of every size, none a NaN."""
+    return torch.randint(0, 0x7F, shape, generator=g, dtype=torch.uint8) | (torch.randint(0, 2, shape, generator=g, dtype=torch.uint8) << 7)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_one_key_gives_its_value(D, dtype):
+    """A row that sees one key is that key's value, code times scale, rounded once: at every scale that the type shows anything of."""
+    g = torch.Generator().manual_seed(D)
+    for e in (-36, -30, -24, -20, -15, -10, -3, 0, 6, 7):
+        cache = C.KvPages.empty(2, 2, D, 32)
+        for t in (cache.k, cache.v):
+            t.view(torch.uint8).copy_(codes(g, *t.shape))
+        cache.k_scale.fill_(2.0 ** -9), cache.v_scale.fill_(2.0 ** e)
+        q = torch.randn((2, 1, 6, D), generator=g).to(dtype)
+        ids = torch.tensor([[1], [0]], dtype=torch.int32).cuda()
+        o = C.sdpa_paged(q.cuda(), cache, ids, torch.tensor([1, 1]).cuda(), D ** -0.5)
+        for b in range(2):
+            want = cache.dense(ids[b], 1)[1][0].to(dtype)
+            assert torch.equal(o[b, 0], want.repeat_interleave(3, 0)), e
+
+
+def fp16_bound(ref, v, scales):
+    """The bound of check_forward with what fp16 loses of small weights as the kernel states it: a weight carries its block's scale and has an absolute step of 2^-25 of the largest
+    such product of the row, and meets a code of 448 at the most."""
+    O, L, W, A, F, E = ref
+    n = W.shape[3]
+    largest = (W * scales).amax(3).transpose(1, 2).unsqueeze(-1)
+    return 2.0 ** -11 * O.abs() + A * (1.01 * 2.0 ** -11 + n * 2.0 ** -24 + 2.1 * E.transpose(1, 2).unsqueeze(-1)) + n * 448 * 2.0 ** -25 * largest + 2.0 ** -25
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("big,small", [(12, -9), (9, -22), (-20, -30)])
+def test_fp16_queries_over_values_of_very_different_sizes(big, small):
+    """Blocks whose values fp16 cannot hold, or only below its normal range, beside others: rows that do not see them, rows that give them no weight, and rows that see nothing else."""
+    D, lens, Sq = 64, [70, 150, 40], 3
+    g = torch.Generator().manual_seed(big + 40)
+    cache, ids, _, _ = filled(lens, 2, D, 32, 4)
+    # the last block of the first two sequences (from key 64, from key 128 on), whose keys point away from the queries in the second; all of the third
+    exps = torch.full((3, 150), small, dtype=torch.float64)
+    exps[0, 64:], exps[1, 128:], exps[2] = big, big, big
+    for b, n in enumerate(lens):
+        for j in range(-(-n // 32)):
+            cache.v_scale[ids[b, j], 0] = 2.0 ** float(exps[b, j * 32])
+    q = (torch.randn((3, Sq, 4, D), generator=g).abs() + 0.5).to(FP)
+    k8 = cache.k.view(torch.uint8)
+    k8[ids[1, 4].long()] |= 0x80         # (negative codes)
+    cache.k_scale[ids[1, 4].long()] = 2.0 ** -4
+    kv = [torch.zeros((3, 150, 2, D)) for _ in range(2)]
+    for b, n in enumerate(lens):
+        for x, y in zip(kv, cache.dense(ids[b], n)):
+            x[b, :n] = y.cpu()
+    lens[0] = 66                          # (queries at 63, 64, 65: the first does not see the last block)
+    ref = forward(q, *kv, D ** -0.5, -1, 0, 0, lens, [n - Sq for n in lens])
+    scales = torch.exp2(exps)[:, None, None, :]
+    o = C.sdpa_paged(q.cuda(), cache, ids, torch.tensor(lens).cuda(), D ** -0.5).cpu().double()
+    # (65504: what is beyond it is an infinity, within the bound of it either is right)
+    bound = fp16_bound(ref, kv[1], scales)
+    sure = ref[0].abs() + bound < 65504
+    assert sure[0, 0].all() and sure[1].all() and torch.isfinite(o[sure]).all()
+    assert ((o - ref[0]).abs() <= bound)[sure].all()
+    assert (o.abs() >= 32768)[ref[0].abs() - bound > 65536].all()
