@@ -150,27 +150,29 @@ template <int D> __device__ __forceinline__ void load_block(Block<D>& t, const u
 
 // Rows of a part: COLS groups of 16 queries.
 // bf16: V's codes enter times their scale, which keeps all their bits.  fp16 has no exponents for that (below 2^-15 of its largest number a code loses bits, and a cache that
-// bf16 tensors filled may hold what fp16 cannot): there the codes enter as they are, the weights take the scale, and O has a reference of its own, of score and scale together,
-// so that what rounding takes from a weight is small against the largest of what its row adds up.
+// bf16 tensors filled may hold what fp16 cannot): there the codes enter as they are, the weights take the scale, and O is held at 2^power of the scores' reference, so that the largest
+// weight that it has met, scale included, lies near 2^7: what rounding takes from a weight is 2^-32 of that one at the most.  (fp16's numbers below 2^-14 lose bits, and its largest
+// leaves room for 7 beside the 8 that a reference may be behind.  A whole power, so that a row of one key is that key's value.)
+constexpr float kLift = 7.0f;
 template <int D, int COLS> struct RowState {
     v4f acc[COLS][D / 16];               // O^T: channels d * 16 + q * 4 + i
-    float ref[COLS], sum[COLS], vref[COLS];
+    float ref[COLS], sum[COLS];
+    int power[COLS];
     __device__ void clear() {
 #pragma unroll
         for (int n = 0; n < COLS; n++) {
 #pragma unroll
             for (int d = 0; d < D / 16; d++) acc[n][d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            ref[n] = vref[n] = -INFINITY;
+            ref[n] = -INFINITY;
             sum[n] = 0.0f;
+            power[n] = 0;
         }
     }
-    // To another reference, in log2 units.
     __device__ void scale_rows(int n, float f) {
 #pragma unroll
         for (int d = 0; d < D / 16; d++) acc[n][d] *= f;
     }
 };
-__device__ __forceinline__ float down(float from, float to) { return to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(from - to); }
 
 // What lies behind a sequence's last key may be any code.  live: how many of the lane's eight keys are the sequence's.
 template <int D> __device__ __forceinline__ void drop_values(Block<D>& t, int live) {
@@ -208,24 +210,25 @@ __device__ __forceinline__ void attend(RowState<D, COLS>& st, const v4i (&q)[COL
         for (int e = 1; e < 8; e++) top = fmaxf(top, s[n][e >> 2][e & 3]);
         top *= c;
         // (a new reference only where the old one lies more than 8 below: the weights stay under 2^8)
-        float mul = 1.0f;
+        [[maybe_unused]] int take = 0;   // power of two that the weights take
         if constexpr (T == kBF16) {
             if (__any(top > st.ref[n] + 8.0f)) {
-                const float r = fmaxf(st.ref[n], max_quads(top)), f = down(st.ref[n], r);
+                const float r = fmaxf(st.ref[n], max_quads(top)), f = r == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.ref[n] - r);
                 st.ref[n] = r;
                 st.sum[n] *= f;
                 st.scale_rows(n, f);
             }
         } else {
-            const float ve = (float)((int)(__float_as_uint(vs) >> 23 & 255) - 127);
-            if (__any(top > st.ref[n] + 8.0f || top + ve > st.vref[n] + 8.0f)) {
-                const float most = max_quads(top), r = fmaxf(st.ref[n], most), w = fmaxf(st.vref[n], most + ve);
-                st.sum[n] *= down(st.ref[n], r);
-                st.scale_rows(n, down(st.vref[n], w));
-                st.ref[n] = r, st.vref[n] = w;
+            const int ve = (int)(__float_as_uint(vs) >> 23 & 255) - 127;
+            if (__any(top > st.ref[n] + 8.0f || top + (float)(ve - st.power[n]) > st.ref[n] + (8.0f + kLift))) {
+                const float most = max_quads(top), r = fmaxf(st.ref[n], most), up = r == -INFINITY ? 0.0f : r - st.ref[n], was = (float)st.power[n];
+                const float power = r == -INFINITY ? was : fmaxf(rintf(was - up), ceilf(most - r + ((float)ve - kLift)));
+                st.ref[n] = r;
+                st.sum[n] *= __builtin_amdgcn_exp2f(-up);
+                st.scale_rows(n, __builtin_amdgcn_exp2f(was - power - up));
+                st.power[n] = (int)power;
             }
-            // (bounded: a weight that takes more than 2^126 is no number that fp16 shows)
-            mul = st.ref[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fminf(st.ref[n] - st.vref[n] + ve, 126.0f));
+            take = ve - st.power[n];
         }
         const float ref = st.ref[n] == -INFINITY ? 0.0f : st.ref[n];
         float part = 0.0f;
@@ -233,7 +236,8 @@ __device__ __forceinline__ void attend(RowState<D, COLS>& st, const v4i (&q)[COL
         for (int e = 0; e < 8; e += 2) {
             const float y = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][e & 3], c, -ref)), z = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][(e & 3) + 1], c, -ref));
             part += y + z;
-            p[n][e >> 1] = T == kBF16 ? (int)pack2<T>(y, z) : (int)pack2<T>(y * mul, z * mul);
+            if constexpr (T == kBF16) p[n][e >> 1] = (int)pack2<T>(y, z);
+            else p[n][e >> 1] = (int)pack2<T>(__builtin_amdgcn_ldexpf(y, take), __builtin_amdgcn_ldexpf(z, take));
         }
         st.sum[n] += part;
     }
@@ -332,7 +336,7 @@ template <int T, int D, int COLS> __global__ __launch_bounds__(256, D == 256 ? 1
         for (int m = 0; m < COLS; m++) {
             const float sum = sum_quads(st.sum[m]);
             if (quad == 0) meet_ml[wave][m * 16 + l16][0] = st.ref[m], meet_ml[wave][m * 16 + l16][1] = sum;
-            if constexpr (T == kF16) st.scale_rows(m, down(st.vref[m], st.ref[m]));
+            if constexpr (T == kF16) st.scale_rows(m, __builtin_amdgcn_ldexpf(1.0f, st.power[m]));
 #pragma unroll
             for (int d = 0; d < D / 16; d++) *reinterpret_cast<v4f*>(meet + (wave * ROWS + m * 16 + l16) * PR + d * 16 + quad * 4) = st.acc[m][d];
         }

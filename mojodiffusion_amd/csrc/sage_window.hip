@@ -58,10 +58,15 @@ constexpr int kFineKeys = 128;
 // of the vector instructions besides the exponentials go ([31234 rows in 6, 48 on 12 x 128] 2223 -> 2148 us, full [11696 rows in 4, 30 x 128] 629 -> 607).
 // EARLY: all fragments are requested ahead of the first product, where there are registers for it and one wave to a SIMD ([64 blocks of 128 rows, 4096 keys, 256 channels] 73 -> 70 us, 128
 // channels 47.7 -> 46.3; two waves, 128 channels: 66 -> 67).
-template <int T, int D, bool FINE, bool LATE = false, bool EARLY = false, class Mask>
+// LIFT: the reference is kept that far below the largest score (log2 units), so that weights are up to 2^LIFT larger: in fp16, whose numbers below 2^-14 lose bits and those below 2^-25
+// vanish, 7 is what its largest one leaves room for beside the 8 that a reference may be behind.  2^-32 of the largest weight is then what a weight is off by at the most, and the sum of 100000
+// of them by 2^-15 (without it, 2^-8).
+template <int T> constexpr float kPackedLift = T == kF16 ? 7.0f : 0.0f;
+template <int T, int D, bool FINE, bool LATE = false, bool EARLY = false, bool LIFTED = false, class Mask>
 __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 16], uint32_t kt, uint32_t vt, const Fragments<D>& kept,
                                             Seen what, int j0, const Mask& m, float c) {
     constexpr int KS = D / 16, DB = D / 32;
+    constexpr float LIFT = LIFTED ? kPackedLift<T> : 0.0f;
     const Fragments<D> f = D > 64 || FINE ? kept.fresh() : kept;         // (at 64 channels there is room for the addresses)
     auto key = [&](int ks) { return lds_read(kt + (f.nat ^ ((ks & 7) << 5)) + (ks >> 3) * 256); };
     auto value = [&](int j2, int d) {
@@ -103,17 +108,17 @@ __device__ __forceinline__ void attend_tile(RowState<D>& st, const v4i (&q)[D / 
             if constexpr (FINE) fine[i >> 1] = pack2<T>(rounded_off<T>(x), rounded_off<T>(y));
         }
     };
-    // A new reference only where the old one lies more than 8 below: the weights stay under 2^8, and the sums have
+    // A new reference only where the old one lies more than 8 (and LIFT) below: the weights stay under 2^8 (2^15), and the sums have
     // room for that; O is multiplied on few tiles instead of on most.  (No key so far: every weight is exp2(-inf).)
     if constexpr (LATE) {
         weights(st.ref);
-        if (__any(part[0] + part[1] > 256.0f || st.ref == -INFINITY)) {
-            st.raise(highest());
+        if (__any(part[0] + part[1] > (LIFT > 0.0f ? 32768.0f : 256.0f) || st.ref == -INFINITY)) {
+            st.raise(highest() - LIFT);
             weights(st.ref == -INFINITY ? 0.0f : st.ref);
         }
     } else {
         const float top = highest();
-        if (__any(top > st.ref + 8.0f)) st.raise(top);
+        if (__any(top > st.ref + (8.0f + LIFT))) st.raise(top - LIFT);
         weights(st.ref == -INFINITY ? 0.0f : st.ref);
     }
     st.sum += part[0] + part[1];
@@ -262,7 +267,8 @@ template <int D> struct SplitLds {
     static_assert(64 * D <= RING, "a wave's rows pass through its ring");
 };
 
-template <int T, int D, bool EARLY = false>
+// PACKED: for sequences one behind the other (attend_tile's EARLY and LIFTED).
+template <int T, int D, bool PACKED = false>
 __device__ __forceinline__ void split_body(const WindowArgs& a, uint8_t* smem, float (&meet_ml)[SplitLds<D>::NW][32][2], int b, int kvh, int x0, int item, int split) {
     using L = SplitLds<D>;
     constexpr int NW = L::NW, KT = L::KT, CPR = D / 8, RUNS = L::TILE / 1024, KS = D / 16, DB = D / 32;
@@ -330,8 +336,8 @@ __device__ __forceinline__ void split_body(const WindowArgs& a, uint8_t* smem, f
         const int j0 = span.tile(t) * KT;
         const uint32_t kt = ring + slot * L::SLOT;
         const Seen what = seen<KT>(a, p_lo, p_hi, len, j0);
-        if (D <= 128 && span.n * KT <= kFineKeys) attend_tile<T, D, D <= 128, false, EARLY>(st, q, kt, kt + L::TILE, fr, what, j0, mask, c);
-        else attend_tile<T, D, false, false, EARLY>(st, q, kt, kt + L::TILE, fr, what, j0, mask, c);
+        if (D <= 128 && span.n * KT <= kFineKeys) attend_tile<T, D, D <= 128, false, PACKED, PACKED>(st, q, kt, kt + L::TILE, fr, what, j0, mask, c);
+        else attend_tile<T, D, false, false, PACKED, PACKED>(st, q, kt, kt + L::TILE, fr, what, j0, mask, c);
         if (L::SLOTS == 2) slot ^= 1;
         else if (t + NW < t1) {
             reads_done();
@@ -591,7 +597,7 @@ template <int T, int D, int WAYS> __device__ __forceinline__ void packed_body(co
         for (; t - way < span.n; t += WAYS, slot = slot == AHEAD ? 0 : slot + 1) {
             turn(t, slot);
             const Seen what = t < all ? Seen::kAll : t < some ? Seen::kSome : Seen::kNone;
-            if (what != Seen::kNone) attend_tile<T, D, decltype(fine)::value, LATE && !decltype(fine)::value>(st, q, lds + L::keys(slot, way), lds + L::values(slot, way), fr, what, t * KT, mask, c);
+            if (what != Seen::kNone) attend_tile<T, D, decltype(fine)::value, LATE && !decltype(fine)::value, false, true>(st, q, lds + L::keys(slot, way), lds + L::values(slot, way), fr, what, t * KT, mask, c);
         }
     };
     if (D <= 128 && span.n * KT <= kFineKeys) {
@@ -602,7 +608,7 @@ template <int T, int D, int WAYS> __device__ __forceinline__ void packed_body(co
 #pragma unroll
             for (int u = 0; u < L::SLOTS; u++) {                       // (slots known ahead)
                 turn(t, u);
-                attend_tile<T, D, false, LATE>(st, q, lds + L::keys(u, way), lds + L::values(u, way), fr, Seen::kAll, t * KT, mask, c);
+                attend_tile<T, D, false, LATE, false, true>(st, q, lds + L::keys(u, way), lds + L::values(u, way), fr, Seen::kAll, t * KT, mask, c);
                 t += WAYS;
                 slot = u == AHEAD ? 0 : u + 1;
                 if (t >= all) break;

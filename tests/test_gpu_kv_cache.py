@@ -530,3 +530,25 @@ def test_fp16_queries_over_values_of_very_different_sizes(big, small):
     assert sure[0, 0].all() and sure[1].all() and torch.isfinite(o[sure]).all()
     assert ((o - ref[0]).abs() <= bound)[sure].all()
     assert (o.abs() >= 32768)[ref[0].abs() - bound > 65536].all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,Sq,Hq", [(64, 1, 2), (128, 4, 6), (256, 1, 16)])
+def test_fp16_weights_below_the_normal_range(D, Sq, Hq):
+    """One key of every block far above the others, and with a value of zero: what comes out is the sum of the others' weights, 2^-25.5 of the largest each.  Such a weight is off by 2^-32 of
+    the largest at the most."""
+    n = 1501
+    g = torch.Generator().manual_seed(D)
+    cache, ids, _, _ = filled([n], 2, D, 32, 1)
+    k, v = torch.zeros(cache.k.shape), torch.randint(64, 448, cache.v.shape, generator=g).float()
+    k[..., 0, 0], v[..., 0] = 176.0, 0.0
+    cache.k.copy_(k.to(torch.float8_e4m3fn)), cache.v.copy_(v.to(torch.float8_e4m3fn))
+    cache.k_scale.fill_(1.0), cache.v_scale.fill_(4.0)
+    q = torch.zeros((1, Sq, Hq, D), dtype=FP)
+    q[..., 0] = 25.5 * 0.6931 / 176 / 2.0 ** -6
+    kv = [x[None].cpu() for x in cache.dense(ids[0], n)]
+    ref = O, L, W, A, F, E = forward(q, *kv, 2.0 ** -6, -1, 0, 0, [n], [n - Sq])
+    assert W[..., 1].max() < 2.0 ** -25.2 * W[..., 0].min() and O.min() > 2.0 ** -12
+    bound = 2.0 ** -11 * O.abs() + A * (1.01 * 2.0 ** -11 + n * 2.0 ** -24 + 2.1 * E.transpose(1, 2).unsqueeze(-1)) + n * 448 * 2.0 ** -32 * (4 * W).amax(3).transpose(1, 2).unsqueeze(-1) + 2.0 ** -25
+    o = C.sdpa_paged(q.cuda(), cache, ids, torch.tensor([n]).cuda(), 2.0 ** -6).cpu().double()
+    assert ((o - O).abs() <= bound).all(), float(((o - O).abs() / bound).max())

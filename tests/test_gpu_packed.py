@@ -425,3 +425,25 @@ def test_a_trained_projection():
     want = x.float().T @ torch.cat((s.d_q, s.d_k, s.d_v), 1).view(90, -1).float()
     # (torch's product: bf16 operands, fp32 sums, one rounding to bf16, 2^-8, with room for a sum of 90 terms)
     assert ((w.grad.float() - want).abs() <= 2.0 ** -8 * want.abs() + 90 * 2.0 ** -23 * (x.float().abs().T @ torch.cat((s.d_q, s.d_k, s.d_v), 1).view(90, -1).float().abs())).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H", [(64, 2), (1024, 24), (1024, 56)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_fp16_weights_below_the_normal_range(T, H, D):
+    """The first keys of four tiles far above the others, and with values of zero: what comes out is the sum of 8000 weights of 2^-25.5 of the largest each, which the statistics count as well.
+    Such a weight is off by 2^-32 of the largest at the most.  (All rows alike: one of them is the reference.)  In all three forms."""
+    n = 8200
+    g = torch.Generator().manual_seed(D)
+    k, v = torch.zeros((n, 1, D)), 16 * (1 + torch.rand((n, 1, D), generator=g))
+    k[0:128:32, 0, 0], v[0:128:32] = 16.0, 0.0
+    q = torch.zeros((1, 1, D))
+    q[..., 0] = 25.5 * 0.6931 / 16 / 0.125
+    q, k, v = (t.to(FP) for t in (q, k, v))
+    O, L, W, A, F, E = forward(q[None], k[None], v[None], 0.125, -1, -1, 0, [n], [0])
+    assert W[..., 1].max() < 2.0 ** -25.2 * W[..., 0].min() and O.min() > 2.0 ** -12
+    f = P.sdpa_packed_train_fwd(q.expand(T, H, D).contiguous().cuda(), *(t.expand(n, H, D).contiguous().cuda() for t in (k, v)), offsets([T]).cuda(), 0.125, False, offsets([n]).cuda())
+    bound = 2.0 ** -11 * O.abs() + A * (1.01 * 2.0 ** -11 + n * 2.0 ** -24 + 2.1 * E.transpose(1, 2).unsqueeze(-1)) + F * 2.0 ** -32 + 2.0 ** -25
+    err = (f.o.cpu().double() - O[0]).abs()
+    assert (err <= bound[0]).all(), float((err / bound[0]).max())
+    assert ((f.stats.cpu().double() - L[0, 0, 0]).abs() <= E[0, 0, 0] + n * 2.0 ** -24).all()
