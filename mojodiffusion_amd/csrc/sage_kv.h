@@ -9,7 +9,7 @@ namespace sage {
 
 // A block is 32 tokens of a page; of one key head it is 32 * D codes of K, a token after the other, 32 * D of V, a channel after the other, and two scales.
 constexpr int kKvBlock = 32;
-// Scales are 2^e.  The least: what is smaller than 2^-109 (half of e4m3's least step, times it) becomes zero.
+// Scales are 2^e.  The least: what is no larger than 2^-110 (half of e4m3's least step, 2^-9, times it) becomes zero.
 constexpr int kKvLeast = -100;
 struct KvPool {
     uint8_t *k, *v;                              // [page, block of the page, Hk, 32, D], [.., D, 32]

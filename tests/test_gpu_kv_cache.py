@@ -552,3 +552,21 @@ def test_fp16_weights_below_the_normal_range(D, Sq, Hq):
     bound = 2.0 ** -11 * O.abs() + A * (1.01 * 2.0 ** -11 + n * 2.0 ** -24 + 2.1 * E.transpose(1, 2).unsqueeze(-1)) + n * 448 * 2.0 ** -32 * (4 * W).amax(3).transpose(1, 2).unsqueeze(-1) + 2.0 ** -25
     o = C.sdpa_paged(q.cuda(), cache, ids, torch.tensor([n]).cuda(), 2.0 ** -6).cpu().double()
     assert ((o - O).abs() <= bound).all(), float(((o - O).abs() / bound).max())
+
+
+@pytest.mark.gpu
+def test_values_around_the_least_scale():
+    """Half of e4m3's least step at the scale 2^-100 is 2^-110: that and less is zero (to the even code), more is the least step; and larger values as the least scale has them."""
+    cache = pool(1, 1, 64, 32)
+    x = torch.zeros((1, 3, 1, 64), dtype=BF)
+    sizes = [2.0 ** -112, 2.0 ** -111, 1.5 * 2.0 ** -111, 2.0 ** -110, (1 + 2.0 ** -7) * 2.0 ** -110, 1.5 * 2.0 ** -110, 2.0 ** -109, 1.5 * 2.0 ** -109, 2.5 * 2.0 ** -109, 2.0 ** -106, 2.0 ** -92]
+    x[0, 0, 0, :11], x[0, 2, 0, 11:22] = torch.tensor(sizes).to(BF), -torch.tensor(sizes).to(BF)
+    want = Cache(cache)
+    want.append(x[0].double(), x[0].double(), torch.zeros(3, 1, 64, dtype=torch.float64), [0], 0)
+    ids = torch.tensor([[0]], dtype=torch.int32).cuda()
+    C.kv_append(cache, x.cuda(), x.cuda(), ids, torch.tensor([3]).cuda())
+    want.check(cache)
+    k, v = cache.dense(ids[0], 3)
+    step = 2.0 ** -109
+    assert float(cache.k_scale[0, 0, 0]) == 2.0 ** -100 and torch.equal(k, v)
+    assert k[0, 0, :11].tolist() == [0, 0, 0, 0, step, step, step, 2 * step, 2 * step, 2.0 ** -106, 2.0 ** -92]
