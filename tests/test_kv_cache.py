@@ -119,6 +119,19 @@ def test_sizes_of_the_c_calls():
     assert paged(type=2) == paged(page=33) == paged(D=32) == -2
 
 
+def test_workspace_of_paged_attention():
+    """Two parts of 16 or 32 rows for each of at most 1024 even shares and, up to 2048 row blocks (blocks of 16 or 32 query rows of a sequence and key head), for a share more of each: the
+    most that a call takes, and about what it takes."""
+    size = _lib.lib().mi355_sage_paged_workspace_bytes
+    for B, Hq, Hk, N, D, width, page in ((32, 64, 8, 16, 128, 64, 64), (64, 64, 32, 1, 128, 64, 64), (64, 32, 32, 1, 64, 9, 32), (128, 16, 16, 1, 64, 9, 32), (129, 16, 16, 1, 64, 9, 32),
+                                         (16, 32, 8, 127, 64, 3, 64), (16, 32, 8, 128, 64, 3, 64), (16, 32, 8, 129, 64, 3, 64), (1, 1, 1, 1, 256, 1, 32), (2, 64, 64, 1, 256, 100, 32)):
+        rows = 16 if N * Hq // Hk <= 16 else 32
+        units = B * Hk * -(-N * Hq // Hk // rows)
+        shares = min(1024, -(-units * width * (page // 32) // 8)) + (units if units <= 2048 else 0)
+        assert size(B, Hq, Hk, N, D, width, page) == -(-shares * 2 * rows * (D + 2) * 4 // 256) * 256
+    assert size(16, 32, 8, 128, 64, 300, 64) == 3072 * 2 * 32 * 66 * 4 and size(16, 32, 8, 129, 64, 300, 64) == 1024 * 2 * 32 * 66 * 4
+
+
 def test_queries_of_an_append_beyond_32_bits_are_refused():
     """2^29 rows of 8 heads are 2^31 groups of two heads, which the kernel numbers in 32 bits; (sizes and codes only: nothing runs)."""
     if torch.cuda.is_available():
