@@ -62,6 +62,27 @@ __host__ __device__ inline HeadSlot spread_item(int id, int heads, int slots) {
     return HeadSlot{item / (m * per), p % per * m + p / per};
 }
 
+// Packed attention's workgroups.  kFull: 128 rows, a wave to 32, their key tiles shared; kPaired: two waves to 32 rows, even key tiles and odd; kFew: 32 rows whose waves take key tiles in
+// turn.  By the workgroups of 128 rows (the last of a sequence half full, on the average) that `rows` rows (queries times the heads that share a key head) of B sequences make on `heads` key heads, and the keys of a
+// sequence on the average (an empty sequence counts as any other): workgroups of 32 rows while one round holds them all (two to a compute unit at 64 channels, one above; two rounds
+// where causal rows leave the second one short), two waves to 32 rows while every compute unit has about one workgroup, with short walks some fewer (the XCDs' shares are not even).
+// Past 256 workgroups the others begin where the first end: with causal rows those are short, at 64 channels two fit a compute unit; else pairs would go through a second, nearly empty round.
+// Measured over sequences of one length, bf16, few / paired / full in us:
+//   64 channels, full attention of 4096 keys, 96 wgs 38 / 45 / 57, 160: 63 / 45 / 59, 256: 74 / 48 / 59, 320: 95 / 74 / 77; of 640, 95: 11 / 12 / 13, 190: 17 / 13 / 14, 255: 24 / 18 / 18;
+//   128 channels, full, 4096 keys, 64: 47 / 67 / 95, 96: 91 / 67 / 95, 256: 182 / 78 / 96, 320: 228 / 141 / 118; causal, 128: 53 / 67 / 96; 333 keys, 96: 17 / 13 / 14,
+//   192: 24 / 13 / 15, 225: 33 / 26 / 18;
+//   256 channels, full, 4096 keys, 96: 151 / 121 / 180, 256: 284 / 143 / 182; causal, 128: 82 / 121 / 180;
+// around one round, one sequence, paired / full, 256, 264 and 272 wgs of 8 heads: 64 channels, full 46 / 59, 69 / 70, 72 / 74; 128 channels, full 75 / 93, 135 / 110, 140 / 116, causal
+// 67 / 94, 67 / 94, 69 / 96 (280: 73 / 102); 256 channels, full 129 / 170, 228 / 184, 238 / 192, causal 109 / 170, 109 / 170, 113 / 175.  Two sequences, 8 heads x 128, full: 2 x 2048 (256
+// wgs) 41 / 50, 2000 + 2100 (264) 73 / 58: rows that B sequences of whole blocks make are taken for such.  (Sequences of very different lengths were not measured beyond that.)
+enum class PackedForm { kFull, kPaired, kFew };
+__host__ __device__ inline PackedForm packed_form_of(int D, bool causal, int B, long long heads, long long rows, long long keys) {
+    const long long full = rows * heads / 128, wgs = full + B * heads / 2, apart = rows % (128LL * B) == 0 ? 0 : (B - 1) * heads / 2;
+    if (full <= (D == 64 || (causal && keys >= 1024) ? 128 : 64)) return PackedForm::kFew;
+    if (D > 64 && !causal && (rows + 127) / 128 * heads + apart > 256) return PackedForm::kFull;
+    return wgs <= (keys >= 1024 ? 272 : 212) ? PackedForm::kPaired : PackedForm::kFull;
+}
+
 // Share `id` of a list of `total` places in shares of `per`: begin .. end - 1.  Ids go beyond the last share (nothing is left for those), and their products with
 // `per` beyond 32 bits.
 struct Share { int begin, end; };

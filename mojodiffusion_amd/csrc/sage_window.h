@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "sage_grid.h"
+
 namespace sage {
 
 // ---- norm and rotation of queries and keys ---------------------------------------------------------
@@ -87,9 +89,6 @@ hipError_t launch_window_bwd(const WindowBwdArgs& a, hipStream_t st);
 // ---- attention over whole sequences that lie one behind the other -------------------------------------
 // Sequence b: rows cu_q[b] .. cu_q[b + 1] - 1 of Q and O, rows cu_k[b] .. cu_k[b + 1] - 1 of K and V; its queries are the last of its positions.  Rows behind the last
 // sequence: zeros.  w: of all rows, as one sequence (B 1, lens and starts null, left, right, sinks as they are to be).
-// kFull: workgroups of 128 rows, a wave to 32, their key tiles shared; kPaired: two waves to 32 rows, even key tiles and odd; kFew: workgroups of 32 rows whose
-// waves take key tiles in turn.
-enum class PackedForm { kFull, kPaired, kFew };
 struct PackedArgs {
     WindowArgs w;
     const int32_t *cu_q, *cu_k;                  // [B + 1]

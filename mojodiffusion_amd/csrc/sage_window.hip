@@ -743,19 +743,8 @@ hipError_t launch_window(const WindowArgs& a, const WindowPlan& p, hipStream_t s
     return a.type == kBF16 ? launch_t<kBF16>(a, p, st) : launch_t<kF16>(a, p, st);
 }
 
-// By the workgroups of 128 rows (`wgs`: the last of a sequence half full), one to a compute unit up to 256, and the keys of a sequence on the average: workgroups of 32 rows while
-// one round holds them all (two to a compute unit at 64 channels, one above; two rounds where causal rows leave the second one short), two waves to 32 rows while
-// every compute unit has one workgroup at the most, with short walks some fewer (the XCDs' shares are not even).  Measured over sequences of one
-// length, bf16, few / paired / full in us:
-//   64 channels, full attention of 4096 keys, 96 wgs 38 / 45 / 57, 160: 63 / 45 / 59, 256: 74 / 48 / 59, 320: 95 / 74 / 77; of 640, 95: 11 / 12 / 13, 190: 17 / 13 / 14, 255: 24 / 18 / 18;
-//   128 channels, full, 4096 keys, 64: 47 / 67 / 95, 96: 91 / 67 / 95, 256: 182 / 78 / 96, 320: 228 / 141 / 118; causal, 128: 53 / 67 / 96; 333 keys, 96: 17 / 13 / 14,
-//   192: 24 / 13 / 15, 225: 33 / 26 / 18;
-//   256 channels, full, 4096 keys, 96: 151 / 121 / 180, 256: 284 / 143 / 182; causal, 128: 82 / 121 / 180.
 PackedForm packed_form(const PackedArgs& a) {
-    const int64_t full = (int64_t)a.rows_q * a.w.g * a.w.Hk / 128, wgs = full + (int64_t)a.B * a.w.Hk / 2, keys = a.rows_k / a.B;
-    const bool causal = a.w.right < kWindowFar;
-    if (full <= (a.w.D == 64 || (causal && keys >= 1024) ? 128 : 64)) return PackedForm::kFew;
-    return wgs <= (keys >= 1024 ? 272 : 212) ? PackedForm::kPaired : PackedForm::kFull;
+    return packed_form_of(a.w.D, a.w.right < kWindowFar, a.B, a.w.Hk, (int64_t)a.rows_q * a.w.g, a.rows_k / a.B);
 }
 bool packed_grid_ok(const PackedArgs& a) { return spread_grid(a.w.Hk, packed_slots(a, packed_rows(a))) <= 0x7FFFFFFF; }
 hipError_t launch_packed(const PackedArgs& a, hipStream_t st) { return a.w.type == kBF16 ? launch_packed_t<kBF16>(a, st) : launch_packed_t<kF16>(a, st); }

@@ -97,3 +97,34 @@ int main() {
     exe = tmp_path / "spread"
     subprocess.run(["g++", "-O1", "-std=c++17", "-o", str(exe), str(src)], check=True)
     assert subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout == "ok\n"
+
+
+def test_two_waves_to_32_rows_in_one_round_only(tmp_path):
+    """packed_form_of, full attention of one long sequence at 128 and 256 channels, where such a workgroup fills a compute unit: never with more than 256 of them; with 129 to 256, always.
+    And what the other rows of its table say: causal rows and 64 channels up to 272, few rows in workgroups of 32."""
+    src = tmp_path / "form.cpp"
+    src.write_text('''
+#define __host__
+#define __device__
+#include "%s/sage_grid.h"
+#include <cstdio>
+using namespace sage;
+int main() {
+    for (int D = 64; D <= 256; D *= 2)
+        for (int heads = 1; heads <= 40; heads++)
+            for (int rows = 1024; rows <= 9000; rows += 31) {
+                const int wgs = (rows + 127) / 128 * heads;
+                const PackedForm full = packed_form_of(D, false, 1, heads, rows, rows), causal = packed_form_of(D, true, 1, heads, rows, rows);
+                if (D > 64 && wgs > 256 && full == PackedForm::kPaired) return std::printf("%%d channels, %%d rows, %%d heads: %%d workgroups\\n", D, rows, heads, wgs), 1;
+                if (wgs > 128 + heads && wgs <= 256 && full != PackedForm::kPaired) return 2;
+                if (wgs > 128 + heads && wgs <= 272 - heads && causal != PackedForm::kPaired) return 3;
+                if ((wgs > 272 + heads && (causal != PackedForm::kFull || full != PackedForm::kFull)) || (wgs <= 64 && (causal != PackedForm::kFew || full != PackedForm::kFew))) return 4;
+            }
+    // two sequences: rows that whole blocks may make, and others, which make a workgroup more for every head
+    if (packed_form_of(128, false, 2, 8, 4096, 2048) != PackedForm::kPaired || packed_form_of(128, false, 2, 8, 4090, 2045) != PackedForm::kFull) return 5;
+    std::puts("ok");
+}
+''' % CSRC)
+    exe = tmp_path / "form"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-o", str(exe), str(src)], check=True)
+    assert subprocess.run([str(exe)], capture_output=True, text=True).stdout == "ok\n"
