@@ -570,3 +570,19 @@ def test_values_around_the_least_scale():
     step = 2.0 ** -109
     assert float(cache.k_scale[0, 0, 0]) == 2.0 ** -100 and torch.equal(k, v)
     assert k[0, 0, :11].tolist() == [0, 0, 0, 0, step, step, step, 2 * step, 2 * step, 2.0 ** -106, 2.0 ** -92]
+
+
+CHUNKS = [
+    # some hundred query tokens of every sequence (a prompt's chunk over its cache): row blocks by the hundred, and more than are given shares of their own; more queries than keys
+    ([700, 333, 90], 333, 12, 3, 128, BF, 64),
+    ([1200], 500, 6, 2, 64, FP, 32),
+    ([300, 40], 257, 4, 1, 256, BF, 128),
+    ([400, 390, 600, 17], 400, 64, 8, 64, BF, 64),
+    ([900, 512], 512, 6, 6, 128, FP, 64),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,Sq,Hq,Hk,D,dtype,page", CHUNKS)
+def test_attention_of_a_chunk_over_the_cache(lens, Sq, Hq, Hk, D, dtype, page):
+    test_attention_over_the_cache(lens, Sq, Hq, Hk, D, dtype, page)

@@ -447,3 +447,20 @@ def test_fp16_weights_below_the_normal_range(T, H, D):
     err = (f.o.cpu().double() - O[0]).abs()
     assert (err <= bound[0]).all(), float((err / bound[0]).max())
     assert ((f.stats.cpu().double() - L[0, 0, 0]).abs() <= E[0, 0, 0] + n * 2.0 ** -24).all()
+
+
+PADDED = [
+    # a batch of fixed B whose last, first or other sequences are empty: gradients in parts (keys' pairs and rows' key tiles), two waves to 32 rows
+    ([3000, 0, 0, 0, 0], None, 1, 1, 64, BF, True, 0),
+    ([0, 2200, 0, 700, 0], None, 4, 2, 128, FP, False, 3),
+    ([0, 0, 1500], None, 12, 12, 128, BF, True, 0),
+    ([0, 1500, 0], [0, 1700, 0], 12, 12, 64, FP, False, 2),
+    ([0] * 63 + [900], None, 2, 1, 64, BF, True, 1),
+    ([900] + [0] * 80, None, 3, 3, 128, FP, True, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nk,Hq,Hk,D,dtype,causal,tail", PADDED)
+def test_packed_with_empty_sequences(nq, nk, Hq, Hk, D, dtype, causal, tail):
+    test_packed(nq, nk, Hq, Hk, D, dtype, causal, tail)
