@@ -90,7 +90,7 @@ __device__ __forceinline__ int wave_scan(int x) {
 }
 
 // The list of blocks: sequence after sequence, in each head after head, row block after row block, block after block.
-// The share of a workgroup: all of them evenly, eight at the least (two to a wave; 16 from 96 rows on, 32 from 192: fewer parts where the chip is full without them), and at the least half the root of the longest sequence's
+// The share of a workgroup: all of them evenly, eight at the least (two to a wave; 16 from 96 row blocks on, 32 from 192: fewer parts where the chip is full without them), and at the least half the root of the longest sequence's
 // blocks, since the second launch's time grows with the parts as the shares shrink.  Where shares are small (up to 32) a workgroup that had the
 // end of one row's blocks and the beginning of another's would go through the chain of latencies twice, and all would wait for it: there every row's blocks are
 // divided into shares of their own, of 8, 16 or 32.
@@ -498,7 +498,16 @@ int64_t paged_tiles(const PagedArgs& a) {
     const int64_t rblocks = ((int64_t)a.Sq * a.g + paged_rows(a) - 1) / paged_rows(a);
     return (int64_t)a.B * a.pool.Hk * rblocks * std::max<int64_t>(1, (int64_t)a.pool.width << a.pool.sub);
 }
-// Workgroups for even shares, and how many more shares there may be where every row has its own (one for each row block of a head; with more than 2048 of them: even shares).
+// Workgroups for even shares, and how many more shares there may be where every row has its own: one for each row block (of a sequence and key head), up to 2048 of them; more row blocks go by even
+// shares, whose parts take no more workspace as those grow.  (Own / even shares, us, 64 channels, rows of 100, 300, 1000 keys: 2048 row blocks 12 / 23, 18 / 24, 46 / 47; 2064: 13 / 26, 20 / 25,
+// 49 / 50; 4096: 25 / 29, 35 / 36, 120 / 102; 8192: 58 / 43, 79 / 74, 205 / 204.  So the border bounds the workspace, and short rows just past it pay for that.)
+// Blocks of a share at the least, 8 / 16 / 32, us, 128 channels, rows of 500, 1000, 2000 keys:
+//    48 row blocks 10.1 / 7.4 / 7.4, 10.6 / 11.6 /  9.9, 12.0 / 12.0 / 14.1;   88: 10.3 / 7.4 / 7.4, 12.4 / 11.9 / 10.1, 17.2 / 15.9 / 15.7;
+//   108 row blocks 10.4 / 7.4 / 7.4, 12.6 / 12.1 / 10.5, 19.2 / 17.7 / 16.3;  180: 12.1 / 7.5 / 7.6, 17.7 / 16.4 / 11.6, 23.9 / 23.8 / 22.6;
+//   204 row blocks 12.4 / 7.7 / 7.9, 19.4 / 16.5 / 12.4, 27.1 / 27.2 / 24.0;  6000 keys: the same within 3 %.
+// Rows of one share gain the most, since nothing is added up; few rows of some thousand keys are those that a larger least costs.
+// The host knows the table's width, not the lengths: the second launch is left out only where a row of the table holds no more than one share (paged_whole).  With a table for 16384 tokens
+// 32 sequences of 500 keys, 48 on 12 heads x 128, take 15.4 us for 12.6, 20 of 300, 40 on 10 x 64, 9.0 for 5.3.
 void paged_plan(PagedArgs* a) {
     a->wgs = (int)std::min<int64_t>(1024, std::max<int64_t>(1, (paged_tiles(*a) + 7) / 8));
     const int64_t units = (int64_t)a->B * a->pool.Hk * (((int64_t)a->Sq * a->g + paged_rows(*a) - 1) / paged_rows(*a));

@@ -919,8 +919,9 @@ void packed_bwd_plan(PackedBwdArgs* a) {
     while (n > 1 && n * n > pairs) n--;
     a->chunks = (int)n;
     // Rows whose walk over the keys would take longer than the chip's average (four or two workgroups to a compute unit): their key tiles dealt out likewise, to no more
-    // than half the places, since two rounds gain nothing ([1292 rows, 30 x 64] in two parts 88 -> 103 us).  A step of [8000 rows, 1 x 64] 244 -> 120, [4000, 4 on 1 x 128] 221 -> 162,
-    // [2048, 8 x 128] 134 -> 112.
+    // than half the places, since two rounds gain nothing ([1292 rows, 30 x 64] in two parts 88 -> 103 us), and to eight workgroups at the most.  A step with up to 1 / 4 / 8 / 16 of them, us:
+    // [8000 rows, 1 x 64] 242 / 122 / 114 / 114, [4000, 1 x 64] 131 / 72 / 64 / 65, full [4096, 2 x 64] 136 / 92 / 95 / 94, [4000, 4 on 1 x 128] 192 / 149 / 149 / 149, [2048, 8 x 128] 120 / 105 / 105 / 105.
+    // (All of it by averages over B, which counts empty sequences: [8000 rows, 1 x 64] with 63 of them behind it is dealt to one workgroup, 239 us.)
     const int64_t tiles = (a->p.rows_k / std::max(a->p.B, 1) + 31) / 32, row_blocks = (a->p.rows_q * a->w.w.g + kRowsWg - 1) / kRowsWg * heads, places = a->w.w.D == 64 ? 1024 : 512;
     const int64_t load = (row_blocks * tiles + blocks * heads * pairs) / (a->w.w.right < kWindowFar ? 2 : 1) / places;
     a->q_chunks = (int)std::max<int64_t>(1, std::min({tiles / std::max<int64_t>(load, 8), tiles / 8, places / 2 / row_blocks, (int64_t)8}));
