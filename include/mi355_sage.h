@@ -586,6 +586,7 @@ int mi355_sage_sdpa_packed_bwd(
  * root mean square (eps inside the root) times k_gain [D] if that is not NULL, then rotated by the row of rope_cos / rope_sin that
  * their position names, as in mi355_sage_qk_norm_rope (rot 0: not at all; a position outside the tables: NaN); V's go as they are.  Q (may be NULL) [B,Hq,N,D] or [1,Hq,N,D] likewise, with q_gain, to Q_out,
  * which may be Q itself and must otherwise overlap nothing that is read; rows of Q that belong to no sequence come out as zeros.
+ * B N rows (with cu_seqlens: N) up to 2^29, and times half the query heads, rounded up, below 2^31.
  * Tokens at positions below zero or beyond the table, or whose page is not in [0, pages), are not stored.  Rows of a block behind the last token keep
  * what they hold.  Blocks that a call appends to must belong to one sequence each (pages that sequences share must be full).  The same
  * call again leaves the same cache.  One launch; no workspace. */

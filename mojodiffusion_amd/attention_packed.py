@@ -93,7 +93,7 @@ def sdpa_packed(q, k, v, cu_seqlens, scale, causal=True, cu_seqlens_k=None):
 
 
 def sdpa_packed_train_fwd(q, k, v, cu_seqlens, scale, causal=True, cu_seqlens_k=None):
-    """sdpa_packed for a training step: the output with what the backward needs."""
+    """sdpa_packed for a training step: the output with what the backward needs (Dh 64 or 128; at 256 the statistics are what is had of it, no backward takes it)."""
     o, rest, stats, q, k, v, cu, cu_k = _forward("sdpa_packed_train_fwd", q, k, v, cu_seqlens, cu_seqlens_k, scale, causal, True)
     return SdpaPackedFwd(o, rest, stats, q, k, v, cu, cu_k, float(scale), bool(causal))
 

@@ -7,15 +7,16 @@
 // S^T = K Q^T lands with the row as the lane's column, which is the operand layout of O^T += V^T P^T, so the
 // probabilities go from registers into the next product; V^T comes from the row-major tile by the transposing LDS read.
 // Scores, reference, sum and O are fp32; P is rounded to the inputs' type as a matrix operand (an error of at most
-// half a step of each weight, unbiased over the keys), the sum is taken over the unrounded values.
+// half a step of each weight, unbiased over the keys; fp16 weights below its normal range: 2^-25 of the largest, sequences
+// one behind the other 2^-32, see attend_tile), the sum is taken over the unrounded values.
 //
 // Which keys a workgroup walks follows from its rows' positions: the tiles of the first `sinks` keys, then those from the first
 // row's left edge to the last row's right edge.  Tiles that every row of a wave sees whole take no mask; a wave leaves out tiles that
 // none of its rows sees.  Rows of a tile that no row of the workgroup sees are not read at all (another key's row stands
 // in), so whatever lies there, or behind a sequence's end, cannot reach a result.
 //
-// The same for whole sequences that lie one behind the other (packed_body).  Measured, bf16: [31234 rows in 6 sequences, 48 on 12 heads x 128] causal 2069 us, 1.11 PFLOP/s;
-// full [11696 rows in 4, 30 x 128] 584 us, 1.02.
+// The same for whole sequences that lie one behind the other (packed_body).  Measured, bf16: [31234 rows in 6 sequences, 48 on 12 heads x 128] causal 2050 to 2140 us by card, 1.12 to
+// 1.08 PFLOP/s; full [11696 rows in 4, 30 x 128] 584 to 606 us, 1.02 to 0.98.
 #include "sage_grid.h"
 #include "sage_window_common.h"
 
